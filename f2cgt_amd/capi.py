@@ -12,7 +12,7 @@ from ctypes import c_char_p, c_int, c_int64, c_void_p
 
 from . import capi_path
 
-DT_U8, DT_I8, DT_I16, DT_I32, DT_I64, DT_F16, DT_F32, DT_F64 = range(8)
+DT_U8, DT_I8, DT_I16, DT_I32, DT_I64, DT_F16, DT_F32, DT_F64, DT_BF16 = range(9)
 METRIC_L2, METRIC_COSINE = 0, 1
 
 P, I, L = c_void_p, c_int, c_int64
@@ -60,6 +60,13 @@ SIGNATURES = {
     "f2cgt_sage_linear_ahead": ([L, L, L, L], c_int),
     "f2cgt_sage_linear_grad_workspace_bytes": ([L, L, L, L], c_int64),
     "f2cgt_sage_linear_grad": ([P, P, P, P, P, P, P, P, L, L, L, L, L, P], c_int),
+    "f2cgt_quantize_rows": ([P, I, L, P, L, P, L, L, P], c_int),
+    "f2cgt_int8_linear": ([P, L, P, P, L, P, P, P, I, L, L, L, I, P], c_int),
+    "f2cgt_quantized_linear_workspace_bytes": ([L, L, L], c_int64),
+    "f2cgt_quantized_linear": ([P, I, L, P, L, P, P, P, P, L, L, L, L, I, P], c_int),
+    "f2cgt_muon_workspace_bytes": ([L, L, L], c_int64),
+    "f2cgt_orthogonalize": ([P, I, P, L, L, L, I, P, P, L, P], c_int),
+    "f2cgt_muon_step": ([P, I, P, I, P, L, L, L, ctypes.c_float, ctypes.c_float, ctypes.c_float, I, I, P, P, L, P], c_int),
     "f2cgt_kmeans_update_static": ([P, P, P, P, P, P, I, ctypes.c_float, L, L, L, P], c_int),
 }
 
@@ -127,7 +134,7 @@ def _tag(t):
     import torch
     return {torch.uint8: DT_U8, torch.int8: DT_I8, torch.int16: DT_I16, torch.int32: DT_I32,
             torch.int64: DT_I64, torch.float16: DT_F16, torch.float32: DT_F32,
-            torch.float64: DT_F64}[t.dtype]
+            torch.float64: DT_F64, torch.bfloat16: DT_BF16}[t.dtype]
 
 
 def _stream():

@@ -21,6 +21,8 @@
 #include <string>
 #include <vector>
 
+#include <array>
+
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -1191,6 +1193,201 @@ bool vq_encode_slices(torch::Tensor x, torch::Tensor codebooks, torch::Tensor ou
   return true;
 }
 
+// ---- dense layers in 8 bits ------------------------------------------------------------------------------
+int dense_tag(torch::ScalarType type, const char* name) {
+  if (type == torch::kFloat32) return F2CGT_DT_F32;
+  if (type == torch::kFloat16) return F2CGT_DT_F16;
+  TORCH_CHECK(type == torch::kBFloat16, name, " must be float32, float16 or bfloat16, not ", type);
+  return F2CGT_DT_BF16;
+}
+
+void undifferentiated(const torch::Tensor& t, const char* op) {
+  TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), op, " is not differentiated: call it under torch.no_grad()");
+}
+
+// Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart or rows overlap.
+torch::Tensor value_rows(const torch::Tensor& x, const char* name) {
+  TORCH_CHECK(x.defined() && x.device().is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(x.dim() >= 1, name, " must have rows");
+  auto rows = x.dim() == 2 ? x : x.reshape({x.size(-1) ? x.numel() / x.size(-1) : x.numel(), x.size(-1)});
+  const bool plain = (rows.size(1) <= 1 || rows.stride(1) == 1) && (rows.size(0) <= 1 || rows.stride(0) >= rows.size(1));
+  return plain ? rows : rows.contiguous();
+}
+int64_t row_step(const torch::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// New int8 rows that start at multiples of 16 bytes: a view of [rows, k] in whole pieces.
+torch::Tensor room_for_codes(int64_t rows, int64_t k, const torch::Tensor& like) {
+  return torch::empty({rows, (k + 15) / 16 * 16}, like.options().dtype(torch::kInt8)).narrow(1, 0, k);
+}
+
+// The same of codes that a caller gives: themselves, or a copy where they are not laid out so.
+torch::Tensor code_rows(const torch::Tensor& codes, const char* name) {
+  TORCH_CHECK(codes.defined() && codes.device().is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == torch::kInt8, name, " must be int8 [rows, columns]");
+  const int64_t step = codes.stride(0);
+  if ((codes.size(1) <= 1 || codes.stride(1) == 1) && step % 16 == 0 && step >= codes.size(1) &&
+      reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0)
+    return codes;
+  auto room = room_for_codes(codes.size(0), codes.size(1), codes);
+  room.copy_(codes);
+  return room;
+}
+
+torch::Tensor scales_of(const torch::Tensor& scales, const torch::Tensor& codes, const char* name) {
+  auto s = beside(scales, codes, name);
+  TORCH_CHECK(s.scalar_type() == torch::kFloat32 && s.dim() == 1 && s.size(0) == codes.size(0), name,
+              " must be float32 with a value for each of the ", codes.size(0), " rows of codes");
+  return s;
+}
+
+torch::Tensor bias_of(const c10::optional<torch::Tensor>& bias, const torch::Tensor& weight) {
+  if (!bias.has_value()) return torch::Tensor();
+  auto b = beside(*bias, weight, "bias");
+  TORCH_CHECK(b.scalar_type() == torch::kFloat32 && b.dim() == 1 && b.size(0) == weight.size(0), "bias must be float32 [",
+              weight.size(0), "]");
+  return b;
+}
+
+// -> (codes int8 [..., k], scales fp32 [...]) of the rows of x (the last dimension).
+std::tuple<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
+  auto rows = value_rows(x, "x");
+  const int tag = dense_tag(rows.scalar_type(), "x");
+  undifferentiated(x, "quantize_rows");
+  c10::DeviceGuard guard(rows.device());
+  const int64_t m = rows.size(0), k = rows.size(1);
+  auto codes = room_for_codes(m, k, rows);
+  auto scales = empty_f32({m}, rows);
+  check_rc(f2cgt_quantize_rows(rows.data_ptr(), tag, row_step(rows), codes.data_ptr<int8_t>(), (k + 15) / 16 * 16,
+                               scales.data_ptr<float>(), m, k, current_stream()),
+           "quantize_rows");
+  if (x.dim() == 2) return {codes, scales};
+  auto lead = x.sizes().vec();
+  auto shape = lead;
+  lead.pop_back();
+  return {codes.view(shape), scales.view(lead)};
+}
+
+torch::Tensor int8_linear(const torch::Tensor& codes_in, const torch::Tensor& scales_in, const torch::Tensor& weight_in,
+                          const torch::Tensor& weight_scales_in, const c10::optional<torch::Tensor>& bias_in, bool relu,
+                          torch::ScalarType dtype) {
+  const int tag = dense_tag(dtype, "dtype");
+  auto codes = code_rows(codes_in, "codes"), weight = code_rows(weight_in, "weight_codes");
+  TORCH_CHECK(codes.device() == weight.device(), "codes are on ", codes.device(), ", the weights on ", weight.device());
+  TORCH_CHECK(codes.size(1) == weight.size(1), "codes have ", codes.size(1), " columns, the weights ", weight.size(1));
+  auto scales = scales_of(scales_in, codes, "scales"), weight_scales = scales_of(weight_scales_in, weight, "weight_scales");
+  auto bias = bias_of(bias_in, weight);
+  c10::DeviceGuard guard(codes.device());
+  const int64_t m = codes.size(0), n = weight.size(0), k = codes.size(1);
+  auto out = torch::empty({m, n}, codes.options().dtype(dtype));
+  check_rc(f2cgt_int8_linear(codes.data_ptr<int8_t>(), codes.stride(0), scales.data_ptr<float>(), weight.data_ptr<int8_t>(),
+                             weight.stride(0), weight_scales.data_ptr<float>(), bias.defined() ? bias.data_ptr<float>() : nullptr,
+                             out.data_ptr(), tag, m, n, k, relu ? 1 : 0, current_stream()),
+           "int8_linear");
+  return out;
+}
+
+// x [..., k] floating -> [..., n] of the same type.
+torch::Tensor quantized_linear(const torch::Tensor& x, const torch::Tensor& weight_in, const torch::Tensor& weight_scales_in,
+                               const c10::optional<torch::Tensor>& bias_in, bool relu) {
+  auto rows = value_rows(x, "x");
+  const int tag = dense_tag(rows.scalar_type(), "x");
+  undifferentiated(x, "quantized_linear");
+  auto weight = code_rows(weight_in, "weight_codes");
+  TORCH_CHECK(rows.device() == weight.device(), "x is on ", rows.device(), ", the weights on ", weight.device());
+  TORCH_CHECK(rows.size(1) == weight.size(1), "x has ", rows.size(1), " columns, the weights ", weight.size(1));
+  auto weight_scales = scales_of(weight_scales_in, weight, "weight_scales");
+  auto bias = bias_of(bias_in, weight);
+  c10::DeviceGuard guard(rows.device());
+  const int64_t m = rows.size(0), n = weight.size(0), k = rows.size(1);
+  auto out = torch::empty({m, n}, rows.options());
+  const int64_t bytes = f2cgt_quantized_linear_workspace_bytes(m, n, k);
+  torch::Tensor ws;
+  if (bytes > 0) ws = torch::empty({bytes}, rows.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_quantized_linear(rows.data_ptr(), tag, row_step(rows), weight.data_ptr<int8_t>(), weight.stride(0),
+                                  weight_scales.data_ptr<float>(), bias.defined() ? bias.data_ptr<float>() : nullptr,
+                                  out.data_ptr(), bytes > 0 ? ws.data_ptr() : nullptr, bytes, m, n, k, relu ? 1 : 0,
+                                  current_stream()),
+           "quantized_linear");
+  if (x.dim() == 2) return out;
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  return out.view(shape);
+}
+
+// ---- the optimiser's step for dense weights ----------------------------------------------------------------
+// update [..., rows, cols] -> its matrices made orthogonal, of the same shape and type.
+torch::Tensor orthogonalize(const torch::Tensor& update, int64_t steps, const std::array<double, 3>& coefficients) {
+  TORCH_CHECK(update.defined() && update.device().is_cuda(), "update must be a GPU tensor");
+  TORCH_CHECK(update.dim() >= 2, "update must be a matrix or a batch of them");
+  TORCH_CHECK(steps >= 1 && steps <= 100, "orthogonalize: from one to 100 steps");
+  const int tag = dense_tag(update.scalar_type(), "update");
+  undifferentiated(update, "orthogonalize");
+  c10::DeviceGuard guard(update.device());
+  auto u = update.contiguous();
+  auto out = torch::empty(u.sizes(), u.options());
+  const int64_t rows = u.size(-2), cols = u.size(-1), count = u.numel() ? u.numel() / (rows * cols) : 0;
+  const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
+  const int64_t bytes = f2cgt_muon_workspace_bytes(count, rows, cols);
+  auto ws = torch::empty({bytes}, u.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_orthogonalize(u.data_ptr(), tag, out.data_ptr(), count, rows, cols, (int)steps, c,
+                               bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+           "orthogonalize");
+  return out;
+}
+
+// One step of weights of one shape, in place; momenta too.
+void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torch::Tensor>& grads,
+               const std::vector<torch::Tensor>& momenta, double step_size, double decay, double momentum, bool nesterov,
+               int64_t steps, const std::array<double, 3>& coefficients) {
+  const size_t count = weights.size();
+  TORCH_CHECK(grads.size() == count && momenta.size() == count, "muon_step: lists of different lengths");
+  TORCH_CHECK(steps >= 1 && steps <= 100, "muon_step: from one to 100 steps");
+  if (count == 0) return;
+  const auto& like = weights[0];
+  TORCH_CHECK(like.defined() && like.device().is_cuda() && like.dim() == 2, "muon_step: weights must be matrices on the GPU");
+  const int weight_tag = dense_tag(like.scalar_type(), "weights"), grad_tag = dense_tag(grads[0].scalar_type(), "grads");
+  std::vector<torch::Tensor> w(count), g(count), v(count);
+  std::vector<void*> wp(count);
+  std::vector<const void*> gp(count);
+  std::vector<float*> vp(count);
+  c10::DeviceGuard guard(like.device());
+  for (size_t i = 0; i < count; ++i) {
+    TORCH_CHECK(weights[i].defined() && weights[i].device() == like.device() && weights[i].scalar_type() == like.scalar_type() &&
+                    weights[i].sizes() == like.sizes(), "muon_step: weights of one shape, type and device only");
+    TORCH_CHECK(grads[i].defined() && grads[i].layout() == torch::kStrided && grads[i].device() == like.device() &&
+                    grads[i].scalar_type() == grads[0].scalar_type() && grads[i].sizes() == like.sizes(),
+                "muon_step: gradients of the weights' shape and device, and of one type, only");
+    TORCH_CHECK(momenta[i].defined() && momenta[i].device() == like.device() && momenta[i].scalar_type() == torch::kFloat32 &&
+                    momenta[i].sizes() == like.sizes(), "muon_step: momenta must be float32 of the weights' shape and device");
+    w[i] = weights[i].contiguous();
+    g[i] = grads[i].contiguous();
+    v[i] = momenta[i].contiguous();
+    wp[i] = w[i].data_ptr();
+    gp[i] = g[i].data_ptr();
+    vp[i] = v[i].data_ptr<float>();
+  }
+  {
+    std::vector<const void*> all;
+    for (size_t i = 0; i < count && like.numel(); ++i) { all.push_back(weights[i].data_ptr()); all.push_back(momenta[i].data_ptr()); }
+    std::sort(all.begin(), all.end());
+    TORCH_CHECK(std::adjacent_find(all.begin(), all.end()) == all.end(), "muon_step: a weight or a momentum is listed twice");
+  }
+  const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
+  const int64_t bytes = f2cgt_muon_workspace_bytes((int64_t)count, like.size(0), like.size(1));
+  auto ws = torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_muon_step(wp.data(), weight_tag, gp.data(), grad_tag, vp.data(), (int64_t)count, like.size(0), like.size(1),
+                           (float)step_size, (float)decay, (float)momentum, nesterov ? 1 : 0, (int)steps, c,
+                           bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+           "muon_step");
+  torch::NoGradGuard no_grad;
+  for (size_t i = 0; i < count; ++i) {
+    for (auto both : {std::make_pair(weights[i], w[i]), std::make_pair(momenta[i], v[i])}) {
+      if (both.first.data_ptr() != both.second.data_ptr()) both.first.copy_(both.second);       // (counts the change itself)
+      else if (!both.first.is_inference()) both.first.unsafeGetTensorImpl()->bump_version();
+    }
+  }
+}
+
 }  // namespace
 
 // Output store policy of the SQ aggregation operators: "auto" (by output size), "stream"
@@ -1264,6 +1461,16 @@ PYBIND11_MODULE(F2CGTLib, m) {
       .def("kmeans_slices_fit", &kmeans_slices_fit, py::arg("x"), py::arg("keep"), py::arg("centers"), py::arg("metric"),
            py::arg("rule"), py::arg("tol"), py::arg("growth"), py::arg("max_iter"), py::arg("check_every"),
            py::arg("bad_row") = py::none(), py::arg("rescale") = false)
+      .def("quantize_rows", &quantize_rows, py::arg("x"))
+      .def("int8_linear", &int8_linear, py::arg("codes"), py::arg("scales"), py::arg("weight_codes"), py::arg("weight_scales"),
+           py::arg("bias") = py::none(), py::arg("relu") = false, py::arg("dtype") = torch::ScalarType(torch::kFloat32))
+      .def("quantized_linear", &quantized_linear, py::arg("x"), py::arg("weight_codes"), py::arg("weight_scales"),
+           py::arg("bias") = py::none(), py::arg("relu") = false)
+      .def("orthogonalize", &orthogonalize, py::arg("update"), py::arg("steps") = 5,
+           py::arg("coefficients") = std::array<double, 3>{3.4445, -4.7750, 2.0315})
+      .def("muon_step", &muon_step, py::arg("weights"), py::arg("grads"), py::arg("momenta"), py::arg("step_size"),
+           py::arg("decay") = 0.0, py::arg("momentum") = 0.95, py::arg("nesterov") = true, py::arg("steps") = 5,
+           py::arg("coefficients") = std::array<double, 3>{3.4445, -4.7750, 2.0315})
       .def("set_store_mode", &set_store_mode, py::arg("mode"));
   py::class_<PendingFlag, std::shared_ptr<PendingFlag>>(m, "PendingFlag").def("wait", &PendingFlag::wait);
   py::class_<KMeans>(m, "KMeans")

@@ -744,3 +744,111 @@ class MySAGEConv(nn.Module):
         if self.norm is not None:
             rst = self.norm(rst)
         return rst
+
+
+# ---- training and serving the dense weights ----------------------------------------------------------
+class Muon(torch.optim.Optimizer):
+    """Optimiser of weight matrices: momentum, the update made orthogonal by Newton-Schulz products, decoupled weight decay.
+    Weights of one shape and type take their step together (`muon_step`).
+
+    `scale` is what the orthogonal update (singular values near one) is multiplied with besides `lr`: "spectral" is
+    sqrt(max(1, rows / cols)), "rms" is 0.2 sqrt(max(rows, cols)), which gives the entries of any shape the size that an
+    Adam step's have.  Only matrices on the GPU; biases and the like belong to another optimiser.  Momenta are kept in float32
+    whatever the weights' type."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, scale="spectral",
+                 coefficients=(3.4445, -4.7750, 2.0315)):
+        if not lr >= 0.0:
+            raise ValueError("lr must not be negative")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("momentum must be in [0, 1)")
+        if not weight_decay >= 0.0:
+            raise ValueError("weight_decay must not be negative")
+        if scale not in ("spectral", "rms"):
+            raise ValueError("scale must be 'spectral' or 'rms'")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      scale=scale, coefficients=tuple(coefficients)))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError("Muon trains matrices only (got a parameter of shape %s)" % (tuple(p.shape),))
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (the base class casts states to their parameters' type)
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], saved["params"]):
+                held = state_dict["state"].get(key, {}).get("momentum")
+                if held is not None:
+                    self.state[p]["momentum"] = held.detach().to(device=p.device, dtype=torch.float32, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            alike = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if "momentum" not in self.state[p]:
+                    self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                alike.setdefault((p.shape, p.dtype, p.device, p.grad.dtype), []).append(p)
+            for (shape, _, _, _), members in alike.items():
+                rows, cols = shape
+                if rows == 0 or cols == 0:
+                    continue
+                size = math.sqrt(max(1.0, rows / cols)) if group["scale"] == "spectral" else 0.2 * math.sqrt(max(rows, cols))
+                _capi().muon_step(members, [p.grad for p in members], [self.state[p]["momentum"] for p in members],
+                                  group["lr"] * size, group["lr"] * group["weight_decay"], group["momentum"],
+                                  group["nesterov"], group["steps"], group["coefficients"])
+        return loss
+
+
+class Int8Linear(nn.Module):
+    """An `nn.Linear` for inference with 8-bit weights, a scale per output, and inputs coded row by row within the call
+    (`quantized_linear`); for any floating type of input.  `Int8Linear(linear)` codes the layer's weight where it lies."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        with torch.no_grad():
+            codes, scales = _capi().quantize_rows(linear.weight)
+            # rows in whole 16-byte pieces, as the product takes them without a copy; zeros behind a row's end
+            whole = torch.zeros((codes.shape[0], (codes.shape[1] + 15) // 16 * 16), dtype=torch.int8, device=codes.device)
+            whole[:, :codes.shape[1]] = codes
+        self.register_buffer("weight_codes", whole)
+        self.register_buffer("weight_scales", scales)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float().clone())
+
+    def _apply(self, fn, recurse=True):
+        # scales and bias stay float32 under .half() and the like
+        kept = {name: getattr(self, name) for name in ("weight_scales", "bias")}
+        super()._apply(fn, recurse)
+        for name, held in kept.items():
+            moved = getattr(self, name)
+            if moved is not None and moved.dtype != torch.float32:
+                setattr(self, name, held.to(moved.device))
+        return self
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, bias=%s" % (self.in_features, self.out_features, self.bias is not None)
+
+    def forward(self, x):
+        return _capi().quantized_linear(x, self.weight_codes[:, :self.in_features], self.weight_scales, self.bias)
+
+
+def int8_layers(module):
+    """`module` for serving: every plain `nn.Linear` below it replaced by an `Int8Linear` of its weights, in place.  A
+    `MySAGEConv` then makes its dense part in 8 bits."""
+    for name, child in list(module.named_children()):
+        if _plain_linear(child):
+            setattr(module, name, Int8Linear(child))
+        else:
+            int8_layers(child)
+    return module

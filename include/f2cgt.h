@@ -35,7 +35,8 @@ enum {
   F2CGT_DT_I64 = 4,
   F2CGT_DT_F16 = 5,
   F2CGT_DT_F32 = 6,
-  F2CGT_DT_F64 = 7
+  F2CGT_DT_F64 = 7,
+  F2CGT_DT_BF16 = 8         /* the dense operators at the end of this file only */
 };
 
 enum {
@@ -386,6 +387,56 @@ int f2cgt_sage_linear_grad(const float* grad, const float* out, const float* x0,
 #define F2CGT_SAGE_STEP 2
 #define F2CGT_SAGE_GRAD 4
 int f2cgt_sage_linear_ahead(int64_t m, int64_t n, int64_t k0, int64_t k1);
+
+/* ---- dense layers in 8 bits ------------------------------------------------------ */
+
+/* No counterpart in the reference, whose layers are fp32 (examples/conv.py:68-76).  Types of floating values: F2CGT_DT_F32,
+ * F2CGT_DT_F16, F2CGT_DT_BF16.
+ *
+ * f2cgt_quantize_rows: x [m, k], row r starting ld values after row r - 1 -> codes int8 [m, k], rows code_stride bytes apart,
+ * and scales fp32 [m]:  scale = max(max |x_rj|, 1e-30) * fl(1/127), code = rint(fl(x_rj * fl(1 / scale))) within +-127,
+ * in fp32.  A row with a NaN or an infinity has that as its scale and zeros for the codes that are no numbers.
+ *
+ * f2cgt_int8_linear: out [m, n] (dense, out_dtype) = (codes weight^T) * (scales_i weight_scales_j) + bias_j, through
+ * max(., 0) where relu is nonzero (a NaN stays one); weight int8 [n, k], bias fp32 [n] or NULL.  The sums are exact whole
+ * numbers; k <= 131071.  Rows of codes and of weights start at multiples of 16 bytes (buffers and strides); what lies
+ * between a row's k bytes and the next row is not used.  No columns: the bias alone.
+ *
+ * f2cgt_quantized_linear: f2cgt_quantize_rows and f2cgt_int8_linear in one call, out of x's type; a row of x that holds
+ * a NaN or an infinity gives a row of NaN.  workspace: f2cgt_quantized_linear_workspace_bytes, 16-byte aligned, contents
+ * irrelevant. */
+int f2cgt_quantize_rows(const void* x, int dtype, int64_t ld, int8_t* codes, int64_t code_stride, float* scales, int64_t m,
+                        int64_t k, void* stream);
+int f2cgt_int8_linear(const int8_t* codes, int64_t code_stride, const float* scales, const int8_t* weight,
+                      int64_t weight_stride, const float* weight_scales, const float* bias, void* out, int out_dtype,
+                      int64_t m, int64_t n, int64_t k, int relu, void* stream);
+int64_t f2cgt_quantized_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, const int8_t* weight, int64_t weight_stride,
+                           const float* weight_scales, const float* bias, void* out, void* workspace, int64_t workspace_bytes,
+                           int64_t m, int64_t n, int64_t k, int relu, void* stream);
+
+/* ---- the optimiser's step for dense weights ---------------------------------------- */
+
+/* No counterpart in the reference (its trainers call torch's optimisers).
+ *
+ * f2cgt_orthogonalize: every matrix of update [count, rows, cols] (dense) -> out, of the same shape and type (it may be
+ * the same buffer):  X = U / (|U|_F + 1e-7), its shorter side as rows, then `steps` times (1 to 100)
+ * G = X X^T, X = a X + (b G + c G G) X, coefficients (host) a, b, c.  Refused (F2CGT_E_UNSUPPORTED): coefficients that lead
+ * singular values from [0, 1] beyond 2.5 or multiply them with more than 7.5 in some step; more than 65536 rows or columns.
+ * A NaN or an infinity in a matrix makes it NaN.  Sums and norm are fp32 and fp64, products of 22 bits and more.
+ *
+ * f2cgt_muon_step: lists (host) of `count` dense matrices [rows, cols] on the device, per matrix
+ *   held = momentum held + (1 - momentum) grad;  u = nesterov ? momentum held + (1 - momentum) grad : held
+ *   weight = (1 - decay) weight - step_size orthogonalize(u)
+ * in place; momenta fp32, weights and gradients of any type above.
+ *
+ * workspace (both): f2cgt_muon_workspace_bytes, 256-byte aligned, contents irrelevant. */
+int64_t f2cgt_muon_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
+int f2cgt_orthogonalize(const void* update, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps,
+                        const float* coefficients, void* workspace, int64_t workspace_bytes, void* stream);
+int f2cgt_muon_step(void* const* weights, int weight_dtype, const void* const* grads, int grad_dtype, float* const* momenta,
+                    int64_t count, int64_t rows, int64_t cols, float step_size, float decay, float momentum, int nesterov,
+                    int steps, const float* coefficients, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
