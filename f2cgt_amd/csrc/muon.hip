@@ -1,7 +1,7 @@
 // An update made orthogonal by Newton-Schulz products, and the optimiser's step around it.
 //
 //   X = U / (|U|_F + 1e-7), its shorter side as rows;  then `steps` times
-//   G = X X^T,  P = a I + b G + c G G,  X = P X
+//   G = X X^T,  P = b G + c G G,  X = a X + P X
 //
 // which takes every singular value s of X through s (a + b s^2 + c s^4) and leaves the vectors alone.  What small singular
 // values there are grow by a factor a in each step (480 in five), and so does what rounding adds to them: operands of
@@ -45,6 +45,7 @@ struct MuonArgs {
   char* g;                                     // [count][r] lines of G
   char* p;                                     // of P
   float a, b, c;
+  int whole;                                   // rows of the results start at multiples of four values
 };
 
 // The update's value i: the gradient, or what the momentum makes of it (held: after this step's change).
@@ -123,85 +124,558 @@ __global__ __launch_bounds__(256) void muon_split_kernel(MuonArgs a) {
   }
 }
 
-// G (square false) from X, or P (square true) from G: the tiles on and below the diagonal, each written on both sides of it.
+// ---- strips of finished tiles: 32 rows and WN columns of sums in LDS, in lanes' turns of eight neighbours -----------------
+__device__ __forceinline__ void eight_of(const char* row, int64_t c, float (&v)[8]) {
+  const char* line = row + (c >> 5) * kLine + 2 * (c & 31);
+  const halfx8 hi = *reinterpret_cast<const halfx8*>(line), lo = *reinterpret_cast<const halfx8*>(line + 64);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
+}
+__device__ __forceinline__ void put_eight(char* row, int64_t c, const float (&v)[8]) {
+  halfx8 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    hi[e] = (_Float16)v[e];
+    lo[e] = (_Float16)(v[e] - (float)hi[e]);
+  }
+  char* line = row + (c >> 5) * kLine + 2 * (c & 31);
+  *reinterpret_cast<halfx8*>(line) = hi;
+  *reinterpret_cast<halfx8*>(line + 64) = lo;
+}
+
+// change(row, col, v): eight neighbours of a row; then put(row, col, v) with them, and turned(row, col, v) with eight neighbours of
+// a column from `row` on.  Rows and columns are whole eights, and may lie beyond the matrix.
+template <int WN, class Change, class Turned>
+__device__ __forceinline__ void strip_passes(float* strip, int64_t row0, int64_t col0, int lane, bool both, const Change& change,
+                                             const Turned& turned) {
+  constexpr int kLd = WN + 4, kAcross = WN / 8, kRows = kWave / kAcross;
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int r = i * kRows + lane / kAcross, c = 8 * (lane % kAcross);
+    fltx4* at = reinterpret_cast<fltx4*>(strip + r * kLd + c);
+    const fltx4 a = at[0], b = at[1];
+    float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    change(row0 + r, col0 + c, v);
+    if (both) {
+      at[0] = fltx4{v[0], v[1], v[2], v[3]};
+      at[1] = fltx4{v[4], v[5], v[6], v[7]};
+    }
+  }
+  if (!both) return;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < WN / 16; ++i) {
+    const int c = i * 16 + lane / 4, r = 8 * (lane % 4);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = strip[(r + e) * kLd + c];
+    turned(row0 + r, col0 + c, v);
+  }
+}
+
+// G from X, or P = b G + c G G from G (g not null): the tiles on and below the diagonal, each written on both sides of it.
 template <int WN>
 struct SymmetricEpilogue {
   const MuonArgs& a;
   char* out;
-  const char* g;                               // null for G
+  const char* g;
   bool mirror;
-  __device__ __forceinline__ void operator()(const float* strip, int64_t row0, int64_t col0, int lane) const {
+  __device__ __forceinline__ void operator()(float* strip, int64_t row0, int64_t col0, int lane) const {
     const int64_t line = a.s.short_line(), r = a.s.r, padded = (r + 31) & ~31ll;
-    for (int i = lane; i < 32 * WN; i += kWave) {
-      const int64_t row = row0 + i / WN, col = col0 + i % WN;
-      if (row < padded && col < padded) {
-        float v = strip[(i / WN) * (WN + 4) + i % WN] * (1.f / kScale);
-        if (g != nullptr) {
-          const int64_t er = row < r ? row : r - 1, ec = col < r ? col : r - 1;
-          const char* e = g + er * line + (ec >> 5) * kLine + 2 * (ec & 31);
-          const float gv = (float)*reinterpret_cast<const _Float16*>(e) + (float)*reinterpret_cast<const _Float16*>(e + 64);
-          v = a.b * gv + a.c * v + (row == col ? a.a * kScale : 0.f);
-        }
-        if (row >= r || col >= r) v = 0.f;
-        if (row < r) put_split(out + row * line, col, v);
-        if (mirror && col < r) put_split(out + col * line, row, v);
-      }
-    }
+    strip_passes<WN>(strip, row0, col0, lane, mirror,
+        [&](int64_t row, int64_t col, float (&v)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= 1.f / kScale;
+          if (row < r && col < padded) {
+            if (g != nullptr) {
+              float gv[8];
+              eight_of(g + row * line, col, gv);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = a.b * gv[e] + a.c * v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e >= r) v[e] = 0.f;
+            put_eight(out + row * line, col, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          }
+        },
+        [&](int64_t row, int64_t col, const float (&v)[8]) {
+          if (col < r && row < padded) put_eight(out + col * line, row, v);
+        });
   }
 };
 
-template <bool SQUARE>
-__global__ __launch_bounds__(256) void muon_symmetric_kernel(MuonArgs a) {
-  typedef TileProduct<SplitOp, 64, 64, 32, 32> Tile;
-  __shared__ __attribute__((aligned(128))) char lds[Tile::kLds];
-  int i = 0, left = blockIdx.x;                // tile (i, j), j <= i, in the order of rows
-  while (left > i) left -= ++i;
-  const int64_t z = blockIdx.z, row0 = 64ll * i, col0 = 64ll * left;
+template <bool SQUARE, int B, int W, int WJ>
+__global__ __launch_bounds__((B / W) * (B / WJ) * kWave) void muon_symmetric_kernel(MuonArgs a) {
+  typedef TileProduct<SplitOp, B, B, W, WJ, 2> Tile;
+  __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
+  // tile (i, j), j <= i, in the order of rows
+  int i = (int)((sqrtf(8.f * (float)blockIdx.x + 1.f) - 1.f) * 0.5f);
+  while ((i + 1) * (i + 2) / 2 <= (int)blockIdx.x) ++i;
+  while (i * (i + 1) / 2 > (int)blockIdx.x) --i;
+  const int64_t z = blockIdx.z, row0 = (int64_t)B * i, col0 = (int64_t)B * ((int)blockIdx.x - i * (i + 1) / 2);
   const Shape& s = a.s;
   char* g = a.g + z * s.r * s.short_line();
   char* p = a.p + z * s.r * s.short_line();
   const Lines from = SQUARE ? Lines{g, s.short_line(), s.r, s.short_line()}
                             : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line()};
-  Tile::run(lds, from, from, row0, col0, SymmetricEpilogue<32>{a, SQUARE ? p : g, SQUARE ? g : nullptr, row0 != col0});
+  Tile::run({lds0, lds1}, from, from, row0, col0, SymmetricEpilogue<WJ>{a, SQUARE ? p : g, SQUARE ? g : nullptr, row0 != col0});
 }
 
-// X = P X in planes, both ways round, or the last one into the caller's matrix.
+// X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  (a X from its own planes: with a in
+// P's diagonal, which is rounded to 22 bits there, errors were half as much again.)
 template <int WN>
 struct UpdateEpilogue {
   const MuonArgs& a;
   int64_t z;
   char* xt;                                    // null: the last one
-  __device__ __forceinline__ void operator()(const float* strip, int64_t row0, int64_t col0, int lane) const {
+  __device__ __forceinline__ void operator()(float* strip, int64_t row0, int64_t col0, int lane) const {
     const Shape& s = a.s;
     const int64_t padded_r = (s.r + 31) & ~31ll, padded_l = (s.l + 31) & ~31ll;
-    for (int i = lane; i < 32 * WN; i += kWave) {
-      const int64_t row = row0 + i / WN, col = col0 + i % WN;
-      if (row >= padded_r || col >= padded_l) continue;
-      float v = strip[(i / WN) * (WN + 4) + i % WN] * (1.f / kScale);
-      const bool in = row < s.r && col < s.l;
-      if (xt != nullptr) {
-        if (!in) v = 0.f;
-        if (row < s.r) put_split(a.x + (z * s.r + row) * s.long_line(), col, v);
-        if (col < s.l) put_split(xt + (z * s.l + col) * s.short_line(), row, v);
-      } else if (in) {
-        v *= 1.f / kScale;
-        const int64_t at = s.turned ? col * s.cols + row : row * s.cols + col;
-        void* w = a.at.out[z];
-        if (a.keep != 0.f) v = a.keep * load_value(w, a.out_dtype, at) - a.size * v;
-        store_value(w, a.out_dtype, at, v);
+    const bool last = xt == nullptr;
+    strip_passes<WN>(strip, row0, col0, lane, !last || s.turned,
+        [&](int64_t row, int64_t col, float (&v)[8]) {
+          if (row < s.r && col < padded_l) {
+            char* x = a.x + (z * s.r + row) * s.long_line();
+            float xv[8];
+            eight_of(x, col, xv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = col + e < s.l ? a.a * xv[e] + v[e] * (1.f / kScale) : 0.f;
+            if (!last) put_eight(x, col, v);
+            else if (!s.turned) result(row, col, s.l, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          }
+        },
+        [&](int64_t row, int64_t col, const float (&v)[8]) {
+          if (col >= s.l || row >= padded_r) return;
+          if (!last) put_eight(xt + (z * s.l + col) * s.short_line(), row, v);
+          else result(col, row, s.r, v);
+        });
+  }
+  // Eight neighbours of a row of the caller's matrix, of rows of `end` values.
+  __device__ __forceinline__ void result(int64_t row, int64_t col, int64_t end, const float (&v)[8]) const {
+    void* w = a.at.out[z];
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const int64_t at = row * end + col + e;
+      if (a.whole && col + e < end) {
+        fltx4 o;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = v[e + d] * (1.f / kScale);
+        if (a.keep != 0.f) {
+          const fltx4 before = load_four(w, a.out_dtype, at);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] = a.keep * before[d] - a.size * o[d];
+        }
+        store_four(w, a.out_dtype, at, o);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          if (col + e + d < end) {
+            float o = v[e + d] * (1.f / kScale);
+            if (a.keep != 0.f) o = a.keep * load_value(w, a.out_dtype, at + d) - a.size * o;
+            store_value(w, a.out_dtype, at + d, o);
+          }
       }
     }
   }
 };
 
-__global__ __launch_bounds__(256) void muon_update_kernel(MuonArgs a, int from, int last) {
-  typedef TileProduct<SplitOp, 64, 64, 32, 32> Tile;
-  __shared__ __attribute__((aligned(128))) char lds[Tile::kLds];
+template <int BM, int BN, int WM, int WN, int DEEP>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
+  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2> Tile;
+  __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   const int64_t z = blockIdx.z;
+  uint32_t i, j;
+  tile_of(blockIdx.x, (uint32_t)ceil_div(s.r, BM), (uint32_t)ceil_div(s.l, BN), DEEP, i, j);
   const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, s.short_line()};
   const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, s.short_line()};
-  Tile::run(lds, p, x, 64ll * blockIdx.x, 64ll * blockIdx.y, UpdateEpilogue<32>{a, z, last ? nullptr : a.xt[1 - from]});
+  Tile::run({lds0, lds1}, p, x, (int64_t)BM * i, (int64_t)BN * j, UpdateEpilogue<WN>{a, z, last ? nullptr : a.xt[1 - from]});
+}
+
+template <bool SQUARE, int B, int W, int WJ>
+void launch_symmetric(const MuonArgs& a, int64_t n, hipStream_t st) {
+  const int64_t tiles = ceil_div(a.s.r, B);
+  muon_symmetric_kernel<SQUARE, B, W, WJ><<<dim3((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n), (B / W) * (B / WJ) * kWave, 0, st>>>(a);
+}
+
+template <int BM, int BN, int WM, int WN, int DEEP>
+void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
+  muon_update_kernel<BM, BN, WM, WN, DEEP><<<dim3((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n),
+                                             (BM / WM) * (BN / WN) * kWave, 0, st>>>(a, from, last);
+}
+
+void symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
+  const int64_t tiles = ceil_div(a.s.r, 128);
+  if (n * tiles * (tiles + 1) / 2 >= num_cus()) {
+    if (square) launch_symmetric<true, 128, 64, 64>(a, n, st);
+    else launch_symmetric<false, 128, 64, 64>(a, n, st);
+  } else {
+    if (square) launch_symmetric<true, 64, 32, 32>(a, n, st);
+    else launch_symmetric<false, 64, 32, 32>(a, n, st);
+  }
+}
+
+void update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
+  const int64_t large = n * ceil_div(a.s.r, 256) * ceil_div(a.s.l, 256), middle = n * ceil_div(a.s.r, 128) * ceil_div(a.s.l, 128);
+  if (large >= num_cus()) launch_update<256, 256, 128, 64, 4>(a, n, from, last, st);
+  else if (middle >= num_cus()) launch_update<128, 128, 64, 64, 8>(a, n, from, last, st);
+  else launch_update<64, 64, 32, 32, 8>(a, n, from, last, st);
+}
+
+// ---- small matrices: a workgroup each, from the update to the result in one launch --------------------------------------
+// X stays in registers, in fp32: a wave has the 32-column strips wave, wave + 8, ... as the matrix instructions leave their sums
+// (a lane: one column, of eight rows its side's four).  That is also what they take as a second operand, if the first
+// one's columns are in the same order; so P X needs no X in LDS.
+constexpr int kOneWaves = 8;
+
+// Row v of a lane's sixteen values of a 32 x 32 tile.
+__device__ __forceinline__ int tile_row(int v, int side) { return 8 * (v / 4) + 4 * side + v % 4; }
+
+// Where a lane's sixteen values of tile (i, column tile c) lie in the caller's matrix: those outside it have the place of one
+// inside.
+struct TilePlaces {
+  int from, down, rows;                                    // of its column; from a row to the next; rows from its first one on
+  bool column;
+  __device__ __forceinline__ TilePlaces(const Shape& m, int i, int c) {
+    const int lane = threadIdx.x & (kWave - 1), col = 32 * c + (lane & 31), row = 32 * i + 4 * (lane >> 5);
+    down = m.turned ? 1 : (int)m.cols;
+    column = col < (int)m.l;
+    rows = (int)m.r - row;
+    from = (column ? col : (int)m.l - 1) * (m.turned ? (int)m.cols : 1) + row * down;
+  }
+  __device__ __forceinline__ bool in(int v) const { return column && tile_row(v, 0) < rows; }
+  __device__ __forceinline__ int at(int v) const { return from + (tile_row(v, 0) < rows ? tile_row(v, 0) : rows - 1) * down; }
+};
+
+template <typename T>
+__device__ __forceinline__ fltx16 load_tile(const void* m, const TilePlaces& p) {
+  fltx16 x;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) x[v] = (float)static_cast<const T*>(m)[p.at(v)];
+  return x;
+}
+__device__ __forceinline__ fltx16 load_tile(const void* m, int dtype, const TilePlaces& p) {
+  if (dtype == F2CGT_DT_F32) return load_tile<float>(m, p);
+  if (dtype == F2CGT_DT_F16) return load_tile<_Float16>(m, p);
+  return load_tile<__bf16>(m, p);
+}
+template <typename T>
+__device__ __forceinline__ void store_tile(void* m, const TilePlaces& p, const fltx16& x) {
+#pragma unroll
+  for (int v = 0; v < 16; ++v)
+    if (p.in(v)) static_cast<T*>(m)[p.at(v)] = (T)x[v];
+}
+
+// Strips of the update, of length `to` (momenta kept).
+template <int RT, int S>
+__device__ __forceinline__ void load_strips(const MuonArgs& a, int64_t z, double* s_sum, float to, fltx16 (&x)[S][RT]) {
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
+  double sum = 0.;
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const TilePlaces p(a.s, i, wave + kOneWaves * s);
+      fltx16 o = load_tile(a.at.u[z], a.u_dtype, p);
+      if (a.at.held[z] != nullptr) {
+        fltx16 h = load_tile<float>(a.at.held[z], p);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          h[v] = a.momentum * h[v] + (1.f - a.momentum) * o[v];
+          o[v] = update_of(a, o[v], h[v]);
+        }
+        store_tile<float>(a.at.held[z], p, h);
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        if (!p.in(v)) o[v] = 0.f;
+        sum += (double)o[v] * (double)o[v];
+      }
+      x[s][i] = o;
+    }
+#pragma unroll
+  for (int by = 32; by > 0; by /= 2) sum += __shfl_xor(sum, by);
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  double all = 0.;
+#pragma unroll
+  for (int i = 0; i < kOneWaves; ++i) all += s_sum[i];
+  const float scale = (float)((double)to / (sqrt(all) + 1e-7));
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[s][i][v] *= scale;
+}
+
+template <int RT, int S>
+__device__ __forceinline__ void store_strips(const MuonArgs& a, int64_t z, float by, const fltx16 (&x)[S][RT]) {
+  const int wave = threadIdx.x / kWave;
+  void* w = a.at.out[z];
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const TilePlaces p(a.s, i, wave + kOneWaves * s);
+      fltx16 o;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[v] = x[s][i][v] * by;
+      if (a.keep != 0.f) {
+        const fltx16 before = load_tile(w, a.out_dtype, p);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[v] = a.keep * before[v] - a.size * o[v];
+      }
+      if (a.out_dtype == F2CGT_DT_F32) store_tile<float>(w, p, o);
+      else if (a.out_dtype == F2CGT_DT_F16) store_tile<_Float16>(w, p, o);
+      else store_tile<__bf16>(w, p, o);
+    }
+}
+
+// Up to 32 rows, all in fp32 (32 x 32 x 2 instructions): a product of this size is latency, not rate.
+template <int S>
+__global__ __launch_bounds__(kOneWaves * kWave) void muon_narrow_kernel(MuonArgs a, int steps) {
+  constexpr int kRow = 32 + 4;                             // floats of a row of 32 in LDS
+  __shared__ double s_sum[kOneWaves];
+  __shared__ __attribute__((aligned(16))) float s_x[kOneWaves][S][32][kRow], s_g[kOneWaves][32][kRow], s_p[32][kRow];
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave, at = lane & 31, side = lane >> 5;
+  const int64_t z = blockIdx.x;
+  fltx16 x[S][1];
+  load_strips<1, S>(a, z, s_sum, 1.f, x);
+  for (int step = 0; step < steps; ++step) {
+    // G: each wave the part of its own columns, in the order of a lane's reads
+    fltx16 g;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) g[v] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s_x[wave][s][tile_row(v, side)][at] = x[s][0][v];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const fltx4 k = *reinterpret_cast<const fltx4*>(&s_x[wave][s][at][8 * q + 4 * side]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], k[e], g, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s_g[wave][tile_row(v, side)][at] = g[v];
+    __syncthreads();
+    for (int i = t; i < 1024; i += kOneWaves * kWave) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kOneWaves; ++w) sum += s_g[w][i / 32][i % 32];
+      s_p[i / 32][i % 32] = sum;                           // (G, until it is P)
+    }
+    __syncthreads();
+    if (wave == 0) {
+      fltx16 square;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) square[v] = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const fltx4 k = *reinterpret_cast<const fltx4*>(&s_p[at][8 * q + 4 * side]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) square = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], k[e], square, 0, 0, 0);
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) square[v] = a.b * s_p[tile_row(v, side)][at] + a.c * square[v];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s_p[tile_row(v, side)][at] = square[v];
+    }
+    __syncthreads();
+    fltx16 sum[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sum[s][v] = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const fltx4 k = *reinterpret_cast<const fltx4*>(&s_p[at][8 * q + 4 * side]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int s = 0; s < S; ++s) sum[s] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], x[s][0][4 * q + e], sum[s], 0, 0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[s][0][v] = a.a * x[s][0][v] + sum[s][v];
+    // (s_p is written again behind the next step's first barrier, s_g in front of it: read before this step's second)
+  }
+  store_strips<1, S>(a, z, 1.f, x);
+}
+
+// Four neighbours of a row of 32 as planes in a line of LDS, from piece `piece`, half `half` on.
+__device__ __forceinline__ void put_four(char* lds, int line, int piece, int half, const float (&v)[4]) {
+  halfx4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = (_Float16)v[e];
+    lo[e] = (_Float16)(v[e] - (float)hi[e]);
+  }
+  *reinterpret_cast<halfx4*>(lds + piece_at(line, piece) + 8 * half) = hi;
+  *reinterpret_cast<halfx4*>(lds + piece_at(line, piece + 4) + 8 * half) = lo;
+}
+
+// From 33 to 32 RT rows: products of planes.  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
+// P's, of 32 RT rows by RT column tiles each, in the same place.
+template <int RT, int S>
+__global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a, int steps) {
+  constexpr int kRows = 32 * RT, kTile = kRows * kLine;    // a column tile
+  constexpr int kTiles = S * kOneWaves > 2 * RT ? S * kOneWaves : 2 * RT;
+  constexpr int TJ = (RT + 1) / 2;                         // column tiles of a wave, in products of square matrices
+  __shared__ double s_sum[kOneWaves];
+  __shared__ __attribute__((aligned(128))) char lds[kTiles * kTile];
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave), at = lane & 31, side = lane >> 5;
+  const int64_t z = blockIdx.x;
+  const int columns = (int)ceil_div(a.s.l, 32);
+  char* gl = lds;
+  char* pl = lds + RT * kTile;
+  fltx16 x[S][RT];
+  load_strips<RT, S>(a, z, s_sum, kScale, x);
+  // tiles (i, j0 ...) of square products
+  const int i0 = wave / 2, j0 = (wave & 1) * TJ;
+  const bool squares = i0 < RT;
+  // rows i of a times rows j of b, column tiles [0, n)
+  auto product = [&](const char* of, int n, fltx16 (&sum)[TJ]) {
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sum[j][v] = 0.f;
+    for (int c = 0; c < n; ++c) {
+      const char* tile = of + c * kTile;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        intx4 fa[2], fb[TJ][2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          fa[p] = *reinterpret_cast<const intx4*>(tile + piece_at(32 * i0 + at, 4 * p + 2 * g + side));
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) {
+            const int jj = j0 + j < RT ? j0 + j : RT - 1;
+            fb[j][p] = *reinterpret_cast<const intx4*>(tile + piece_at(32 * jj + at, 4 * p + 2 * g + side));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) SplitOp::mma(sum[j], fa, fb[j]);
+      }
+    }
+  };
+  for (int step = 0; step < steps; ++step) {
+    // X's lines: a lane has a column
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int c = wave + kOneWaves * s;
+      if (c < columns) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const _Float16 hi = (_Float16)x[s][i][v], lo = (_Float16)(x[s][i][v] - (float)hi);
+            const int row = 32 * i + tile_row(v, side);
+            *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, at / 8) + 2 * (at % 8)) = hi;
+            *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, 4 + at / 8) + 2 * (at % 8)) = lo;
+          }
+      }
+    }
+    __syncthreads();
+    fltx16 sum[TJ];
+    if (squares) product(lds, columns, sum);
+    __syncthreads();
+    // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
+    if (squares) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        if (j0 + j < RT) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float v[4] = {sum[j][4 * q] / kScale, sum[j][4 * q + 1] / kScale, sum[j][4 * q + 2] / kScale, sum[j][4 * q + 3] / kScale};
+            put_four(gl + i0 * kTile, 32 * (j0 + j) + at, q, side, v);
+          }
+        }
+    }
+    __syncthreads();
+    if (squares) {
+      product(gl, RT, sum);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        if (j0 + j < RT) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const char* g = gl + i0 * kTile;
+            const int row = 32 * (j0 + j) + at;
+            const halfx4 hi = *reinterpret_cast<const halfx4*>(g + piece_at(row, q) + 8 * side);
+            const halfx4 lo = *reinterpret_cast<const halfx4*>(g + piece_at(row, q + 4) + 8 * side);
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = a.b * ((float)hi[e] + (float)lo[e]) + a.c * (sum[j][4 * q + e] / kScale);
+            // columns in the order in which a lane of x has its rows: 4 side ... of each eight
+            put_four(pl + i0 * kTile, row, 2 * (q / 2) + side, q & 1, v);
+          }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (wave + kOneWaves * s >= columns) continue;
+      fltx16 next[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) next[i][v] = 0.f;
+#pragma unroll
+      for (int c = 0; c < RT; ++c)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          halfx8 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            hi[e] = (_Float16)x[s][c][8 * g + e];
+            lo[e] = (_Float16)(x[s][c][8 * g + e] - (float)hi[e]);
+          }
+          const intx4 fb[2] = {__builtin_bit_cast(intx4, hi), __builtin_bit_cast(intx4, lo)};
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            intx4 fa[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              fa[p] = *reinterpret_cast<const intx4*>(pl + c * kTile + piece_at(32 * i + at, 4 * p + 2 * g + side));
+            SplitOp::mma(next[i], fa, fb);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[s][i][v] = a.a * x[s][i][v] + next[i][v] / kScale;
+    }
+    __syncthreads();
+  }
+  store_strips<RT, S>(a, z, 1.f / kScale, x);
+}
+
+// Whether a workgroup takes a matrix, and takes it.
+bool one_launch(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
+  const int64_t rt = ceil_div(a.s.r, 32), s = ceil_div(ceil_div(a.s.l, 32), kOneWaves);
+  const unsigned grid = (unsigned)n, block = kOneWaves * kWave;
+  if (rt == 1 && s == 1) muon_narrow_kernel<1><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 1 && s == 2) muon_narrow_kernel<2><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 2 && s == 1) muon_one_kernel<2, 1><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 2 && s == 2) muon_one_kernel<2, 2><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 3 && s == 1) muon_one_kernel<3, 1><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 4 && s == 1) muon_one_kernel<4, 1><<<grid, block, 0, st>>>(a, steps);
+  else return false;
+  return true;
 }
 
 Shape shape_of(int64_t rows, int64_t cols) {
@@ -269,19 +743,23 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
   a.p = take(group * s.r * s.short_line());
   for (int64_t first = 0; first < count; first += group) {
     const int64_t n = count - first < group ? count - first : group;
+    a.whole = cols % 4 == 0;
     for (int64_t i = 0; i < n; ++i) {
       a.at.u[i] = u_step ? static_cast<const char*>(u[0]) + (first + i) * u_step * type_size(a.u_dtype) : u[first + i];
       a.at.out[i] = u_step ? static_cast<char*>(out[0]) + (first + i) * u_step * type_size(a.out_dtype) : out[first + i];
       a.at.held[i] = held != nullptr ? held[first + i] : nullptr;
+      a.whole = a.whole && aligned(a.at.out[i], 4 * type_size(a.out_dtype));
+    }
+    if (one_launch(a, n, steps, st)) {
+      if (int rc = launch_status(what)) return rc;
+      continue;
     }
     muon_norm_kernel<<<dim3((unsigned)a.parts, (unsigned)n), 256, 0, st>>>(a);
     muon_split_kernel<<<dim3((unsigned)ceil_div(rows, 32), (unsigned)ceil_div(cols, 32), (unsigned)n), 256, 0, st>>>(a);
-    const int64_t tiles = ceil_div(s.r, 64);
     for (int step = 0; step < steps; ++step) {
-      const dim3 lower((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n);
-      muon_symmetric_kernel<false><<<lower, 256, 0, st>>>(a);
-      muon_symmetric_kernel<true><<<lower, 256, 0, st>>>(a);
-      muon_update_kernel<<<dim3((unsigned)tiles, (unsigned)ceil_div(s.l, 64), (unsigned)n), 256, 0, st>>>(a, step & 1, step == steps - 1);
+      symmetric(a, n, false, st);
+      symmetric(a, n, true, st);
+      update(a, n, step & 1, step == steps - 1, st);
     }
     if (int rc = launch_status(what)) return rc;
   }

@@ -17,7 +17,8 @@ typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLine = 128;                 // bytes of a row that a step of the main loop takes
 
-// Rows of one operand: row r at base + r * stride (a multiple of 16), `bytes` of it are summed over.
+// Rows of one operand: row r at base + r * stride (a multiple of 16), `bytes` of it are summed over.  The 16-byte piece with a
+// row's last byte is read as a whole.
 struct Lines {
   const char* base;
   int64_t stride;
@@ -29,6 +30,7 @@ struct Lines {
 struct Int8Op {
   typedef intx16 Acc;
   static constexpr int kGroups = 4, kParts = 1;
+  static constexpr bool kTrim = true;        // a row may end within a line
   static __device__ __forceinline__ int chunk(int group, int) { return 2 * group; }
   static __device__ __forceinline__ void mma(Acc& acc, const intx4 (&p)[1], const intx4 (&q)[1]) {
     acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(p[0], q[0], acc, 0, 0, 0);
@@ -40,6 +42,7 @@ struct Int8Op {
 struct SplitOp {
   typedef fltx16 Acc;
   static constexpr int kGroups = 2, kParts = 2;
+  static constexpr bool kTrim = false;       // rows are whole lines
   static __device__ __forceinline__ int chunk(int group, int part) { return 4 * part + 2 * group; }
   static __device__ __forceinline__ void mma(Acc& acc, const intx4 (&p)[2], const intx4 (&q)[2]) {
     const halfx8 p0 = __builtin_bit_cast(halfx8, p[0]), p1 = __builtin_bit_cast(halfx8, p[1]);
@@ -50,59 +53,86 @@ struct SplitOp {
   }
 };
 
-// 16 bytes of row r from byte k0 on, zeros behind the operand's end.  Rows beyond the last one repeat it (what they give is not kept).
-__device__ __forceinline__ intx4 line_piece(const Lines& x, int64_t r, int64_t k0) {
-  const char* p = x.base + (r < x.rows ? r : x.rows - 1) * x.stride + k0;
-  intx4 v = {0, 0, 0, 0};
-  if (k0 + 16 <= x.bytes) {
-    v = *reinterpret_cast<const intx4*>(p);
-  } else if (k0 < x.bytes) {
-    const int left = (int)(x.bytes - k0);
-#pragma unroll
-    for (int i = 0; i < 15; ++i)
-      if (i < left) v[i >> 2] |= (int)(uint8_t)p[i] << (8 * (i & 3));
-  }
-  return v;
-}
-
-// A piece's place in LDS: rows of 128 bytes, the eight pieces of a row in another order in each of eight rows, so that the
-// lanes of a read, which take the same piece of consecutive rows, spread over the banks.
-__device__ __forceinline__ int piece_at(int r, int c) { return r * kLine + ((c ^ (r & 7)) << 4); }
+// A piece's place in LDS: rows of 128 bytes, the eight pieces of a row in another order in each of eight pairs of rows (64 banks
+// hold two rows), so that the lanes of a read, which take the same piece of consecutive rows, spread over the banks.
+__device__ __forceinline__ int piece_at(int r, int c) { return r * kLine + ((c ^ (r >> 1 & 7)) << 4); }
 
 // A sum as a word of LDS.  (By value: a bit cast of a vector's element itself takes the vector's first one.)
 __device__ __forceinline__ float word_of(float v) { return v; }
 __device__ __forceinline__ float word_of(int v) { return __builtin_bit_cast(float, v); }
 
-template <class Op, int BM, int BN, int WM, int WN>
+// Waits until at most `loads` of this wave's copies into LDS are under way and its reads of LDS are done.
+template <int loads>
+__device__ __forceinline__ void wait_copies() {
+  __builtin_amdgcn_s_waitcnt((loads & 15) | (loads >> 4) << 14 | 7 << 4 | 0 << 8);
+}
+
+// The pieces of a tile go from memory into LDS without a stop in registers, STAGES - 1 steps ahead of the one that is
+// multiplied; a step costs one barrier.  The stages are LDS arrays of their own (Buffers), which is how the compiler knows that a
+// read of one need not wait for the copies into the others.
+template <class Op, int BM, int BN, int WM, int WN, int STAGES>
 struct TileProduct {
   static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = kWaves * kWave;
   static constexpr int TI = WM / 32, TJ = WN / 32;
   static constexpr int kLd = WN + 4;                                   // floats of a strip's row in LDS
   static constexpr int kStrip = 32 * kLd * 4;
-  static constexpr int kStage = (BM + BN) * kLine;
-  static constexpr int kLds = kStage > kWaves * kStrip ? kStage : kWaves * kStrip;
+  static constexpr int kStage = (BM + BN) * kLine;                     // bytes of a stage, and of a buffer
+  static constexpr int kPieces = (BM + BN) * 8 / kThreads;             // copies of a thread in a step
+  static_assert((BM + BN) * 8 % kThreads == 0 && BM * 8 % kThreads == 0, "whole pieces per thread");
+  static constexpr int kStripsPerStage = kStage / kStrip;
+  static_assert(kStripsPerStage * STAGES >= kWaves, "a strip per wave");
   typedef typename Op::Acc Acc;
+  typedef char* Buffers[STAGES];
 
   // Rows [row0, row0 + BM) of a against rows [col0, col0 + BN) of b.  epilogue(strip, row, col, lane): strip [32][kLd] holds
   // the sums of 32 rows from `row` on and WN columns from `col` on.
   template <class Epilogue>
-  static __device__ __forceinline__ void run(char* lds, const Lines& a, const Lines& b, int64_t row0, int64_t col0, const Epilogue& epilogue) {
+  static __device__ __forceinline__ void run(const Buffers& lds, const Lines& a, const Lines& b, int64_t row0, int64_t col0,
+                                             const Epilogue& epilogue) {
     const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int wi = (wave % (BM / WM)) * WM, wj = (wave / (BM / WM)) * WN;
-    constexpr int PA = BM * 8 / kThreads, PB = BN * 8 / kThreads;
-    static_assert(BM * 8 % kThreads == 0 && BN * 8 % kThreads == 0, "whole pieces per thread");
-    intx4 va[PA], vb[PB];
-    auto load = [&](int64_t k0) {
+    const int at = lane & 31, side = lane >> 5;
+    const int steps = (int)((a.bytes + kLine - 1) / kLine);
+    const int left = (int)(a.bytes - (int64_t)(steps - 1) * kLine);     // bytes of the last step
+
+    // Thread t copies the pieces of places t + i kThreads: place q holds, of row q / 8, piece (q % 8) ^ (row / 2 % 8), and the rows
+    // of a thread are whole sixteens apart: the same piece of each.  Rows beyond the operand's end repeat its last one: what they give
+    // is not kept.  Offsets are 32 bits from a tile's first row (strides are below 2^23 here).
+    const int piece = ((t & 7) ^ (t >> 4 & 7)) << 4;
+    static_assert(kThreads % 128 == 0, "rows of a thread sixteen apart");
+    const char* base_a = a.base + row0 * a.stride;
+    const char* base_b = b.base + col0 * b.stride;
+    uint32_t from[kPieces];
 #pragma unroll
-      for (int i = 0; i < PA; ++i) {
-        const int q = t + i * kThreads;
-        va[i] = line_piece(a, row0 + (q >> 3), k0 + 16 * (q & 7));
-      }
+    for (int i = 0; i < kPieces; ++i) {
+      const bool first = i * kThreads < BM * 8;
+      const int r = (t + i * kThreads) / 8 - (first ? 0 : BM);
+      const int64_t rows = first ? a.rows - row0 : b.rows - col0;
+      from[i] = (uint32_t)(r < rows ? r : (int)rows - 1) * (uint32_t)(first ? a.stride : b.stride) + piece;
+    }
+    auto copy = [&](char* to, int step) {
+      // (pieces of the last step that begin behind the end: the row's first one of this step, which is made zero below)
+      const int back = step == steps - 1 && piece >= left ? piece : 0;
+      const char* pa = base_a + (int64_t)step * kLine;
+      const char* pb = base_b + (int64_t)step * kLine;
 #pragma unroll
-      for (int i = 0; i < PB; ++i) {
-        const int q = t + i * kThreads;
-        vb[i] = line_piece(b, col0 + (q >> 3), k0 + 16 * (q & 7));
+      for (int i = 0; i < kPieces; ++i)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)((i * kThreads < BM * 8 ? pa : pb) + (from[i] - back)),
+            (__attribute__((address_space(3))) void*)(to + (wave * kWave + i * kThreads) * 16), 16, 0, 0);
+    };
+    // The first operand's bytes behind the end made zero, by the thread that copied them (the second's then do not count).
+    auto trim = [&](char* stage) {
+      const int in = left - piece;
+      intx4 mask;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mask[e] = in >= 4 * e + 4 ? -1 : in <= 4 * e ? 0 : (1 << (8 * (in - 4 * e))) - 1;
+#pragma unroll
+      for (int i = 0; i * kThreads < BM * 8; ++i) {
+        intx4* at_piece = reinterpret_cast<intx4*>(stage + (t + i * kThreads) * 16);
+        *at_piece &= mask;
       }
+      __builtin_amdgcn_s_waitcnt(63 | 3 << 14 | 7 << 4 | 0 << 8);      // (LDS only)
     };
     Acc acc[TI][TJ];
 #pragma unroll
@@ -111,42 +141,62 @@ struct TileProduct {
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-    const int at = lane & 31, side = lane >> 5;
-    load(0);
-    for (int64_t k0 = 0; k0 < a.bytes; k0 += kLine) {
-#pragma unroll
-      for (int i = 0; i < PA; ++i) {
-        const int q = t + i * kThreads;
-        *reinterpret_cast<intx4*>(lds + piece_at(q >> 3, q & 7)) = va[i];
-      }
-#pragma unroll
-      for (int i = 0; i < PB; ++i) {
-        const int q = t + i * kThreads;
-        *reinterpret_cast<intx4*>(lds + BM * kLine + piece_at(q >> 3, q & 7)) = vb[i];
-      }
-      __syncthreads();
-      if (k0 + kLine < a.bytes) load(k0 + kLine);
-#pragma unroll
-      for (int g = 0; g < Op::kGroups; ++g) {
-        intx4 fa[TI][Op::kParts], fb[TJ][Op::kParts];
+    // Products of a stage, a group's operands read while the group before is multiplied.
+    auto multiply = [&](const char* stage) {
+      intx4 fa[2][TI][Op::kParts], fb[2][TJ][Op::kParts];
+      auto read = [&](int g) {
 #pragma unroll
         for (int p = 0; p < Op::kParts; ++p) {
 #pragma unroll
-          for (int i = 0; i < TI; ++i)
-            fa[i][p] = *reinterpret_cast<const intx4*>(lds + piece_at(wi + 32 * i + at, Op::chunk(g, p) + side));
-#pragma unroll
           for (int j = 0; j < TJ; ++j)
-            fb[j][p] = *reinterpret_cast<const intx4*>(lds + BM * kLine + piece_at(wj + 32 * j + at, Op::chunk(g, p) + side));
+            fb[g & 1][j][p] = *reinterpret_cast<const intx4*>(stage + BM * kLine + piece_at(wj + 32 * j + at, Op::chunk(g, p) + side));
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            fa[g & 1][i][p] = *reinterpret_cast<const intx4*>(stage + piece_at(wi + 32 * i + at, Op::chunk(g, p) + side));
         }
+      };
+      read(0);
+#pragma unroll
+      for (int g = 0; g < Op::kGroups; ++g) {
+        if (g + 1 < Op::kGroups) read(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < TI; ++i)
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) Op::mma(acc[i][j], fb[j], fa[i]);
+          for (int j = 0; j < TJ; ++j) Op::mma(acc[i][j], fb[g & 1][j], fa[g & 1][i]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __syncthreads();
+    };
+    if (steps > 0) {
+      // Step `step` from stage s: its copies are done when only those of the STAGES - 2 steps behind it are under way; then
+      // all waves have them, and nobody reads the stage of the step before any more, which the next copies overwrite.  (There
+      // are always as many copies under way: behind the last step it is copied again, into a stage that nobody reads.)
+      auto held = [&](int step) { return step < steps ? step : steps - 1; };
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; ++s) copy(lds[s], held(s));
+      int step = 0;
+      while (true) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+          wait_copies<(STAGES - 2) * kPieces>();
+          if (Op::kTrim && left < kLine && step == steps - 1) trim(lds[s]);
+          __builtin_amdgcn_s_barrier();
+          copy(lds[(s + STAGES - 1) % STAGES], held(step + STAGES - 1));
+          __builtin_amdgcn_sched_barrier(0);             // (the compiler would sink them to the step's end)
+          multiply(lds[s]);
+          if (++step == steps) goto done;
+        }
+      }
     }
+  done:
+    wait_copies<0>();
+    __builtin_amdgcn_s_barrier();
     // The columns' operand came first: a lane holds, of one row, four columns after four.
-    float* strip = reinterpret_cast<float*>(lds + wave * kStrip);
+    char* mine = nullptr;
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+      if (wave / kStripsPerStage == s) mine = lds[s] + (wave % kStripsPerStage) * kStrip;
+    float* strip = reinterpret_cast<float*>(mine);
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
 #pragma unroll
@@ -165,6 +215,17 @@ struct TileProduct {
   }
 };
 
+// Workgroup `id` of tiles_m x tiles_n: neighbours in time share operands.  Workgroups go round the eight XCDs, each with an L2
+// of its own, so an XCD gets one run of the tiles' order, which goes down `deep` tiles before it goes to the next column.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t deep, uint32_t& i, uint32_t& j) {
+  const uint32_t all = tiles_m * tiles_n, xcd = id & 7, share = all >> 3, more = all & 7;
+  const uint32_t at = xcd * share + (xcd < more ? xcd : more) + (id >> 3);
+  const uint32_t band = at / (deep * tiles_n), first = band * deep, in = at - band * deep * tiles_n;
+  const uint32_t rows = tiles_m - first < deep ? tiles_m - first : deep;
+  j = in / rows;
+  i = first + in - j * rows;
+}
+
 // ---- values of the types that the dense operators take ---------------------------------------------------
 __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i) {
   if (dtype == F2CGT_DT_F32) return static_cast<const float*>(p)[i];
@@ -175,6 +236,19 @@ __device__ __forceinline__ void store_value(void* p, int dtype, int64_t i, float
   if (dtype == F2CGT_DT_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == F2CGT_DT_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
   else static_cast<__bf16*>(p)[i] = (__bf16)v;
+}
+// Four neighbours at once, at an address that is a multiple of four values.
+__device__ __forceinline__ void store_four(void* p, int dtype, int64_t i, const fltx4& v) {
+  typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+  if (dtype == F2CGT_DT_F32) *reinterpret_cast<fltx4*>(static_cast<float*>(p) + i) = v;
+  else if (dtype == F2CGT_DT_F16) *reinterpret_cast<halfx4*>(static_cast<_Float16*>(p) + i) = __builtin_convertvector(v, halfx4);
+  else *reinterpret_cast<bf4*>(static_cast<__bf16*>(p) + i) = __builtin_convertvector(v, bf4);
+}
+__device__ __forceinline__ fltx4 load_four(const void* p, int dtype, int64_t i) {
+  typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+  if (dtype == F2CGT_DT_F32) return *reinterpret_cast<const fltx4*>(static_cast<const float*>(p) + i);
+  if (dtype == F2CGT_DT_F16) return __builtin_convertvector(*reinterpret_cast<const halfx4*>(static_cast<const _Float16*>(p) + i), fltx4);
+  return __builtin_convertvector(*reinterpret_cast<const bf4*>(static_cast<const __bf16*>(p) + i), fltx4);
 }
 inline bool dense_type(int dtype) { return dtype == F2CGT_DT_F32 || dtype == F2CGT_DT_F16 || dtype == F2CGT_DT_BF16; }
 inline int type_size(int dtype) { return dtype == F2CGT_DT_F32 ? 4 : 2; }
