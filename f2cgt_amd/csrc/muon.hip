@@ -350,15 +350,28 @@ struct TilePlaces {
     rows = (int)m.r - row;
     from = (column ? col : (int)m.l - 1) * (m.turned ? (int)m.cols : 1) + row * down;
   }
+  __device__ __forceinline__ bool whole(int q) const { return 8 * q + 4 <= rows; }       // rows of values 4 q to 4 q + 3
   __device__ __forceinline__ bool in(int v) const { return column && tile_row(v, 0) < rows; }
   __device__ __forceinline__ int at(int v) const { return from + (tile_row(v, 0) < rows ? tile_row(v, 0) : rows - 1) * down; }
 };
 
+// (four neighbours in memory at once where the columns of X are the caller's rows)
 template <typename T>
 __device__ __forceinline__ fltx16 load_tile(const void* m, const TilePlaces& p) {
+  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   fltx16 x;
 #pragma unroll
-  for (int v = 0; v < 16; ++v) x[v] = (float)static_cast<const T*>(m)[p.at(v)];
+  for (int q = 0; q < 4; ++q) {
+    const T* from = static_cast<const T*>(m) + p.at(4 * q);
+    if (p.down == 1 && p.whole(q)) {
+      const four o = *reinterpret_cast<const four*>(from);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * q + e] = (float)o[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * q + e] = (float)static_cast<const T*>(m)[p.at(4 * q + e)];
+    }
+  }
   return x;
 }
 __device__ __forceinline__ fltx16 load_tile(const void* m, int dtype, const TilePlaces& p) {
@@ -368,9 +381,21 @@ __device__ __forceinline__ fltx16 load_tile(const void* m, int dtype, const Tile
 }
 template <typename T>
 __device__ __forceinline__ void store_tile(void* m, const TilePlaces& p, const fltx16& x) {
+  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 #pragma unroll
-  for (int v = 0; v < 16; ++v)
-    if (p.in(v)) static_cast<T*>(m)[p.at(v)] = (T)x[v];
+  for (int q = 0; q < 4; ++q) {
+    if (p.down == 1 && p.whole(q)) {
+      if (!p.column) continue;
+      four o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (T)x[4 * q + e];
+      *reinterpret_cast<four*>(static_cast<T*>(m) + p.at(4 * q)) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (p.in(4 * q + e)) static_cast<T*>(m)[p.at(4 * q + e)] = (T)x[4 * q + e];
+    }
+  }
 }
 
 // Strips of the update, of length `to` (momenta kept).
@@ -445,7 +470,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_narrow_kernel(MuonArgs
   constexpr int kRow = 32 + 4;                             // floats of a row of 32 in LDS
   __shared__ double s_sum[kOneWaves];
   __shared__ __attribute__((aligned(16))) float s_x[kOneWaves][S][32][kRow], s_g[kOneWaves][32][kRow], s_p[32][kRow];
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave, at = lane & 31, side = lane >> 5;
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave), at = lane & 31, side = lane >> 5;
   const int64_t z = blockIdx.x;
   fltx16 x[S][1];
   load_strips<1, S>(a, z, s_sum, 1.f, x);
@@ -456,6 +481,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_narrow_kernel(MuonArgs
     for (int v = 0; v < 16; ++v) g[v] = 0.f;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
+      if (32 * (wave + kOneWaves * s) >= a.s.l) break;
 #pragma unroll
       for (int v = 0; v < 16; ++v) s_x[wave][s][tile_row(v, side)][at] = x[s][0][v];
       __builtin_amdgcn_wave_barrier();
@@ -504,7 +530,8 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_narrow_kernel(MuonArgs
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int s = 0; s < S; ++s) sum[s] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], x[s][0][4 * q + e], sum[s], 0, 0, 0);
+        for (int s = 0; s < S; ++s)
+          if (32 * (wave + kOneWaves * s) < a.s.l) sum[s] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], x[s][0][4 * q + e], sum[s], 0, 0, 0);
     }
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -536,7 +563,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   constexpr int TJ = (RT + 1) / 2;                         // column tiles of a wave, in products of square matrices
   __shared__ double s_sum[kOneWaves];
   __shared__ __attribute__((aligned(128))) char lds[kTiles * kTile];
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave), at = lane & 31, side = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t z = blockIdx.x;
   const int columns = (int)ceil_div(a.s.l, 32);
   char* gl = lds;
@@ -547,7 +574,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   const int i0 = wave / 2, j0 = (wave & 1) * TJ;
   const bool squares = i0 < RT;
   // rows i of a times rows j of b, column tiles [0, n)
-  auto product = [&](const char* of, int n, fltx16 (&sum)[TJ]) {
+  auto product = [&](const char* of, int n, int at, int side, fltx16 (&sum)[TJ]) {
 #pragma unroll
     for (int j = 0; j < TJ; ++j)
 #pragma unroll
@@ -567,11 +594,17 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
           }
         }
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) SplitOp::mma(sum[j], fa, fb[j]);
+        for (int m = 0; m < SplitOp::kTerms; ++m)
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) SplitOp::mma(sum[j], m, fa, fb[j]);
       }
     }
   };
   for (int step = 0; step < steps; ++step) {
+    // (places in LDS are made anew in each step: kept across all of it they are more than the registers hold)
+    int lane_of = (int)threadIdx.x & (kWave - 1);
+    asm volatile("" : "+v"(lane_of));
+    const int at = lane_of & 31, side = lane_of >> 5;
     // X's lines: a lane has a column
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -590,7 +623,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     }
     __syncthreads();
     fltx16 sum[TJ];
-    if (squares) product(lds, columns, sum);
+    if (squares) product(lds, columns, at, side, sum);
     __syncthreads();
     // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
     if (squares) {
@@ -606,7 +639,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     }
     __syncthreads();
     if (squares) {
-      product(gl, RT, sum);
+      product(gl, RT, at, side, sum);
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
         if (j0 + j < RT) {
@@ -644,14 +677,16 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
             lo[e] = (_Float16)(x[s][c][8 * g + e] - (float)hi[e]);
           }
           const intx4 fb[2] = {__builtin_bit_cast(intx4, hi), __builtin_bit_cast(intx4, lo)};
+          intx4 fa[RT][2];
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            intx4 fa[2];
+          for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
-              fa[p] = *reinterpret_cast<const intx4*>(pl + c * kTile + piece_at(32 * i + at, 4 * p + 2 * g + side));
-            SplitOp::mma(next[i], fa, fb);
-          }
+              fa[i][p] = *reinterpret_cast<const intx4*>(pl + c * kTile + piece_at(32 * i + at, 4 * p + 2 * g + side));
+#pragma unroll
+          for (int m = 0; m < SplitOp::kTerms; ++m)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) SplitOp::mma(next[i], m, fa[i], fb);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -664,7 +699,12 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   store_strips<RT, S>(a, z, 1.f / kScale, x);
 }
 
-// Whether a workgroup takes a matrix, and takes it.
+// Whether a workgroup takes a matrix; and takes them.
+bool one_workgroup(const Shape& m) {
+  const int64_t rt = ceil_div(m.r, 32), s = ceil_div(ceil_div(m.l, 32), kOneWaves);
+  return (rt <= 2 && s <= 2) || (rt <= 4 && s == 1);
+}
+
 bool one_launch(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
   const int64_t rt = ceil_div(a.s.r, 32), s = ceil_div(ceil_div(a.s.l, 32), kOneWaves);
   const unsigned grid = (unsigned)n, block = kOneWaves * kWave;
@@ -693,13 +733,14 @@ int64_t whole(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
 // Matrices that go through a set of launches together: enough for the chip's workgroups twice, so that the planes of
 // those under way are not more than that takes.
 int64_t group_of(int64_t count, int64_t rows, int64_t cols) {
-  const int64_t tiles = ceil_div(rows, 64) * ceil_div(cols, 64), want = ceil_div(2048, tiles);
+  const int64_t tiles = ceil_div(rows, 64) * ceil_div(cols, 64), want = one_workgroup(shape_of(rows, cols)) ? kGroup : ceil_div(2048, tiles);
   const int64_t most = want < kGroup ? want : kGroup;
   return count < most ? count : most;
 }
 
 int64_t workspace_of(int64_t count, int64_t rows, int64_t cols) {
   const Shape s = shape_of(rows, cols);
+  if (one_workgroup(s)) return 0;
   const int64_t n = group_of(count, rows, cols);
   return whole(n * parts_of(rows, cols) * 8) + whole(n * s.r * s.long_line()) + 2 * whole(n * s.l * s.short_line()) +
          2 * whole(n * s.r * s.short_line());
@@ -710,17 +751,21 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
   F2CGT_REQUIRE(rows <= 65536 && cols <= 65536, F2CGT_E_UNSUPPORTED, "%s: at most 65536 rows and columns", what);
   F2CGT_REQUIRE(steps >= 1 && steps <= 100, F2CGT_E_INVALID, "%s: from one to 100 steps", what);
   F2CGT_REQUIRE(coefficients != nullptr, F2CGT_E_INVALID, "%s: null coefficients", what);
-  // How far singular values from [0, 1] get, step by step, and what they are multiplied with.
+  // How far singular values from [0, reach] get in a step, and what they are multiplied with: p(t) = a + b t + c t^2 of their
+  // squares, and x p(x^2), at the ends and where a derivative is zero.
   const double a = coefficients[0], b = coefficients[1], c = coefficients[2];
   double reach = 1.;
   for (int s = 0; s < steps; ++s) {
+    const double end = 1.002 * reach * reach, root = 9. * b * b - 20. * a * c;
+    const double at[5] = {0., end, c != 0. ? -b / (2. * c) : 0., c != 0. && root >= 0. ? (-3. * b + sqrt(root)) / (10. * c) : b != 0. ? -a / (3. * b) : 0.,
+                          c != 0. && root >= 0. ? (-3. * b - sqrt(root)) / (10. * c) : 0.};
     double next = 0.;
-    for (int i = 0; i <= 4096; ++i) {
-      const double x = 1.001 * reach * i / 4096, p = a + b * x * x + c * x * x * x * x;
-      F2CGT_REQUIRE(p > -kMost && p < kMost, F2CGT_E_UNSUPPORTED, "%s: these coefficients lead out of the range of the products", what);
-      next = fabs(x * p) > next ? fabs(x * p) : next;
+    for (double t : at) {
+      if (!(t >= 0. && t <= end) && t == t) continue;
+      const double p = a + b * t + c * t * t, x = sqrt(t) * fabs(p);
+      F2CGT_REQUIRE(p > -kMost && p < kMost && x < 2.5, F2CGT_E_UNSUPPORTED, "%s: these coefficients lead out of the range of the products", what);
+      next = x > next ? x : next;
     }
-    F2CGT_REQUIRE(next < 2.5, F2CGT_E_UNSUPPORTED, "%s: these coefficients lead out of the range of the products", what);
     reach = next;
   }
   return 0;
@@ -734,7 +779,7 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
   a.a = coefficients[0]; a.b = coefficients[1]; a.c = coefficients[2];
   const int64_t group = group_of(count, rows, cols);
   char* at = static_cast<char*>(workspace);
-  auto take = [&](int64_t bytes) { char* p = at; at += whole(bytes); return p; };
+  auto take = [&](int64_t bytes) { char* p = at; at = p != nullptr ? p + whole(bytes) : p; return p; };
   a.partial = reinterpret_cast<double*>(take(group * a.parts * 8));
   a.x = take(group * s.r * s.long_line());
   a.xt[0] = take(group * s.l * s.short_line());
@@ -784,7 +829,8 @@ extern "C" int f2cgt_orthogonalize(const void* update, int dtype, void* out, int
   if (count == 0 || rows == 0 || cols == 0) return 0;
   F2CGT_REQUIRE(update && out && aligned(update, type_size(dtype)) && aligned(out, type_size(dtype)), F2CGT_E_INVALID,
                 "%s: null or misaligned buffer", what);
-  F2CGT_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= workspace_of(count, rows, cols), F2CGT_E_INVALID,
+  const int64_t bytes = workspace_of(count, rows, cols);
+  F2CGT_REQUIRE(bytes == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= bytes), F2CGT_E_INVALID,
                 "%s: workspace too small or misaligned", what);
   MuonArgs a{};
   a.u_dtype = a.out_dtype = dtype;
@@ -806,7 +852,8 @@ extern "C" int f2cgt_muon_step(void* const* weights, int weight_dtype, const voi
     F2CGT_REQUIRE(weights[i] && grads[i] && momenta[i] && aligned(weights[i], type_size(weight_dtype)) &&
                       aligned(grads[i], type_size(grad_dtype)) && aligned(momenta[i], 4),
                   F2CGT_E_INVALID, "%s: null or misaligned buffer", what);
-  F2CGT_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= workspace_of(count, rows, cols), F2CGT_E_INVALID,
+  const int64_t bytes = workspace_of(count, rows, cols);
+  F2CGT_REQUIRE(bytes == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= bytes), F2CGT_E_INVALID,
                 "%s: workspace too small or misaligned", what);
   MuonArgs a{};
   a.u_dtype = grad_dtype;

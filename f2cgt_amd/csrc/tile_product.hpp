@@ -32,7 +32,8 @@ struct Int8Op {
   static constexpr int kGroups = 4, kParts = 1;
   static constexpr bool kTrim = true;        // a row may end within a line
   static __device__ __forceinline__ int chunk(int group, int) { return 2 * group; }
-  static __device__ __forceinline__ void mma(Acc& acc, const intx4 (&p)[1], const intx4 (&q)[1]) {
+  static constexpr int kTerms = 1;
+  static __device__ __forceinline__ void mma(Acc& acc, int, const intx4 (&p)[1], const intx4 (&q)[1]) {
     acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(p[0], q[0], acc, 0, 0, 0);
   }
 };
@@ -44,12 +45,10 @@ struct SplitOp {
   static constexpr int kGroups = 2, kParts = 2;
   static constexpr bool kTrim = false;       // rows are whole lines
   static __device__ __forceinline__ int chunk(int group, int part) { return 4 * part + 2 * group; }
-  static __device__ __forceinline__ void mma(Acc& acc, const intx4 (&p)[2], const intx4 (&q)[2]) {
-    const halfx8 p0 = __builtin_bit_cast(halfx8, p[0]), p1 = __builtin_bit_cast(halfx8, p[1]);
-    const halfx8 q0 = __builtin_bit_cast(halfx8, q[0]), q1 = __builtin_bit_cast(halfx8, q[1]);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p1, q0, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p0, q1, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p0, q0, acc, 0, 0, 0);
+  static constexpr int kTerms = 3;             // (one after the other over all tiles: in a row on one they wait for each other)
+  static __device__ __forceinline__ void mma(Acc& acc, int term, const intx4 (&p)[2], const intx4 (&q)[2]) {
+    const halfx8 a = __builtin_bit_cast(halfx8, p[term == 0 ? 1 : 0]), b = __builtin_bit_cast(halfx8, q[term == 1 ? 1 : 0]);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
   }
 };
 
@@ -161,9 +160,11 @@ struct TileProduct {
         if (g + 1 < Op::kGroups) read(g + 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < TI; ++i)
+        for (int m = 0; m < Op::kTerms; ++m)
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) Op::mma(acc[i][j], fb[g & 1][j], fa[g & 1][i]);
+          for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) Op::mma(acc[i][j], m, fb[g & 1][j], fa[g & 1][i]);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
