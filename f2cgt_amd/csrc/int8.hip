@@ -151,6 +151,7 @@ struct LinearEpilogue {
   const LinearArgs& a;
   __device__ __forceinline__ void operator()(const float* strip, int64_t row0, int64_t col0, int lane) const {
     constexpr int kAcross = WN / 4, kRows = kWave / kAcross;        // lanes along a row, rows at a time
+    static_assert(kWave % kAcross == 0, "whole rows at a time");
     const int c = 4 * (lane % kAcross);
     const int64_t col = col0 + c;
     const int in = a.n - col < 4 ? (int)(a.n - col) : 4;
@@ -186,27 +187,24 @@ struct LinearEpilogue {
   }
 };
 
-template <int BM, int BN, int WM, int WN, int STAGES, int DEEP>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * kWave) void int8_linear_kernel(LinearArgs a) {
-  typedef TileProduct<Int8Op, BM, BN, WM, WN, STAGES> Tile;
+template <int BM, int BN, int WM, int WN, int STAGES, int GROUPS, int DEEP>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void int8_linear_kernel(LinearArgs a) {
+  typedef TileProduct<Int8Op, BM, BN, WM, WN, STAGES, GROUPS> Tile;
   uint32_t i, j;
   tile_of(blockIdx.x, (uint32_t)ceil_div(a.m, BM), (uint32_t)ceil_div(a.n, BN), DEEP, i, j);
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   if constexpr (STAGES == 2) {
     Tile::run({lds0, lds1}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});
-  } else if constexpr (STAGES == 3) {
-    __shared__ __attribute__((aligned(128))) char lds2[Tile::kStage];
-    Tile::run({lds0, lds1, lds2}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});
   } else {
     __shared__ __attribute__((aligned(128))) char lds2[Tile::kStage], lds3[Tile::kStage];
     Tile::run({lds0, lds1, lds2, lds3}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});
   }
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int DEEP>
+template <int BM, int BN, int WM, int WN, int STAGES, int GROUPS, int DEEP>
 void launch_linear(const LinearArgs& a, hipStream_t st) {
-  int8_linear_kernel<BM, BN, WM, WN, STAGES, DEEP>
-      <<<(unsigned)(ceil_div(a.m, BM) * ceil_div(a.n, BN)), (BM / WM) * (BN / WN) * kWave, 0, st>>>(a);
+  int8_linear_kernel<BM, BN, WM, WN, STAGES, GROUPS, DEEP>
+      <<<(unsigned)(ceil_div(a.m, BM) * ceil_div(a.n, BN)), (BM / WM) * (BN / WN) * GROUPS * kWave, 0, st>>>(a);
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------
@@ -408,8 +406,9 @@ void launch_few(const LinearArgs& a, hipStream_t st) {
 //     6.1 and 4.8
 //   of few tokens 16 or 8 waves: 1 x 4096 -> 4096 5.4 and 6.2, 1 x 128 -> 256 4.2 and 3.7, 24 x 4096 -> 4096 7.5 and 8.7, but
 //     48 rows 16.2 and 11.5 (registers); 32 outputs a workgroup or 16: 16 x 2048 -> 16384 8.8 and 10.7, 16 x 4096 -> 4096 8.4 and 7.8
-//   64 x 64 tiles in four stages, 64 x 128 or 128 x 128 in two: 256 x 4096 -> 4096 13.7, 20.6, 24.1; 2048 x 2048 -> 2048 21, 16.3,
-//     17.2; 4099 x 4096 -> 4096 134, 102, 96; 60001 x 602 -> 128 26, 18.5, 17.1
+//   64 x 64 tiles by four groups of waves or by two, 64 x 128 or 128 x 128 tiles: 256 x 4096 -> 4096 12.8, 14.3, 20.6, 24.0;
+//     33 x 4096 -> 16384 15.8, 15.2, 21.2, 23.4; 490 x 1135 -> 9698 40, 26.7, 20.3, 21.2; 2048 x 2048 -> 2048 31, 20.5, 15.7,
+//     17.0; 60001 x 602 -> 128, the last two 18.5 and 17.1; 4099 x 4096 -> 4096 102 and 96
 //   128 x 128 or 256 x 256: 8192 x 8192 -> 8192 586 and 509, 4099 x 4096 -> 4096 (272 large tiles for 256 CUs) 96 and 124
 int linear(const char* what, LinearArgs a, hipStream_t st) {
   if (a.m == 0 || a.n == 0) return 0;
@@ -430,10 +429,11 @@ int linear(const char* what, LinearArgs a, hipStream_t st) {
   const int64_t large = ceil_div(m, 256) * ceil_div(n, 256), middle = ceil_div(m, 128) * ceil_div(n, 128);
   const int64_t small = ceil_div(m, 64) * ceil_div(n, 128);
   // a round of large tiles is as long as 3.5 rounds of middle ones
-  if (k >= 1024 && large >= cus && 7 * ceil_div(large, cus) * cus <= 2 * middle) launch_linear<256, 256, 128, 64, 2, 4>(a, st);
-  else if (2 * middle >= 3 * cus) launch_linear<128, 128, 64, 32, 2, 8>(a, st);
-  else if (small >= cus) launch_linear<64, 128, 32, 32, 2, 8>(a, st);
-  else launch_linear<64, 64, 32, 32, 4, 8>(a, st);
+  if (k >= 1024 && large >= cus && 7 * ceil_div(large, cus) * cus <= 2 * middle) launch_linear<256, 256, 128, 64, 2, 1, 4>(a, st);
+  else if (2 * middle >= 3 * cus) launch_linear<128, 128, 64, 32, 2, 1, 8>(a, st);
+  else if (small >= cus) launch_linear<64, 128, 32, 32, 2, 1, 8>(a, st);
+  else if (ceil_div(m, 64) * ceil_div(n, 64) > cus) launch_linear<64, 64, 32, 32, 2, 2, 8>(a, st);
+  else launch_linear<64, 64, 32, 32, 2, 4, 8>(a, st);
   return launch_status(what);
 }
 

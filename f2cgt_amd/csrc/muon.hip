@@ -148,10 +148,11 @@ __device__ __forceinline__ void put_eight(char* row, int64_t c, const float (&v)
 template <int WN, class Change, class Turned>
 __device__ __forceinline__ void strip_passes(float* strip, int64_t row0, int64_t col0, int lane, bool both, const Change& change,
                                              const Turned& turned) {
-  constexpr int kLd = WN + 4, kAcross = WN / 8, kRows = kWave / kAcross;
+  constexpr int kLd = WN + 4, kAcross = WN / 8;
+  static_assert(32 * kAcross % kWave == 0, "whole turns of the lanes");
 #pragma unroll
-  for (int i = 0; i < 32 / kRows; ++i) {
-    const int r = i * kRows + lane / kAcross, c = 8 * (lane % kAcross);
+  for (int i = 0; i < 32 * kAcross / kWave; ++i) {
+    const int r = (i * kWave + lane) / kAcross, c = 8 * ((i * kWave + lane) % kAcross);
     fltx4* at = reinterpret_cast<fltx4*>(strip + r * kLd + c);
     const fltx4 a = at[0], b = at[1];
     float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -208,9 +209,9 @@ struct SymmetricEpilogue {
   }
 };
 
-template <bool SQUARE, int B, int W, int WJ>
-__global__ __launch_bounds__((B / W) * (B / WJ) * kWave) void muon_symmetric_kernel(MuonArgs a) {
-  typedef TileProduct<SplitOp, B, B, W, WJ, 2> Tile;
+template <bool SQUARE, int B, int W, int WJ, int GROUPS>
+__global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symmetric_kernel(MuonArgs a) {
+  typedef TileProduct<SplitOp, B, B, W, WJ, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   // tile (i, j), j <= i, in the order of rows
   int i = (int)((sqrtf(8.f * (float)blockIdx.x + 1.f) - 1.f) * 0.5f);
@@ -286,9 +287,9 @@ struct UpdateEpilogue {
   }
 };
 
-template <int BM, int BN, int WM, int WN, int DEEP>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
-  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2> Tile;
+template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
+  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   const int64_t z = blockIdx.z;
@@ -299,34 +300,57 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * kWave) void muon_update_ker
   Tile::run({lds0, lds1}, p, x, (int64_t)BM * i, (int64_t)BN * j, UpdateEpilogue<WN>{a, z, last ? nullptr : a.xt[1 - from]});
 }
 
-template <bool SQUARE, int B, int W, int WJ>
+template <bool SQUARE, int B, int W, int WJ, int GROUPS>
 void launch_symmetric(const MuonArgs& a, int64_t n, hipStream_t st) {
   const int64_t tiles = ceil_div(a.s.r, B);
-  muon_symmetric_kernel<SQUARE, B, W, WJ><<<dim3((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n), (B / W) * (B / WJ) * kWave, 0, st>>>(a);
+  muon_symmetric_kernel<SQUARE, B, W, WJ, GROUPS>
+      <<<dim3((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n), (B / W) * (B / WJ) * GROUPS * kWave, 0, st>>>(a);
 }
 
-template <int BM, int BN, int WM, int WN, int DEEP>
+template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
-  muon_update_kernel<BM, BN, WM, WN, DEEP><<<dim3((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n),
-                                             (BM / WM) * (BN / WN) * kWave, 0, st>>>(a, from, last);
+  muon_update_kernel<BM, BN, WM, WN, GROUPS, DEEP><<<dim3((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n),
+                                                     (BM / WM) * (BN / WN) * GROUPS * kWave, 0, st>>>(a, from, last);
+}
+
+// Which tiles.  Time of a step of 32 summed columns, us, by tiles per CU:
+//   128 x 128 in eight waves, two workgroups a CU: one tile 0.67-0.75, two 0.93, so 0.93 for each pair and 0.67 for a last one
+//   192 x 192 in four waves (symmetric products): 1.33 each;  64 x 128 in eight waves (updates), three a CU: 0.30 each
+//   64 x 64: 0.47 for one, 0.28 each for many; with four groups of waves 0.31 for one
+// Gram products of 1000 x 2051: 64 x 64 30.6, in four groups 20.0, 128 x 128 44; 2048 x 2048: 33.8, 55.8 and 43; 3000 x 3000: 112, 144
+// and 88, 192 x 192 128; 4096 x 4096: 300, 349, 222 and 171 (253 tiles for 256 CUs).  Updates: 1000 x 2051: 64 x 64 20.9, 64 x 128 23.5,
+// 128 x 128 26.7; 2048 x 2048: 52, 42, 48; 3000 x 3000: 160, 130, 142; 4096 x 4096: 361, 280, 238, 256 x 256 299.
+int64_t pairs_cost(int64_t tiles, int64_t cus) {
+  const int64_t left = tiles % (2 * cus);
+  return 93 * (tiles / (2 * cus)) + (left == 0 ? 0 : left <= cus ? 67 : 93);
 }
 
 void symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
-  const int64_t tiles = ceil_div(a.s.r, 128);
-  if (n * tiles * (tiles + 1) / 2 >= num_cus()) {
-    if (square) launch_symmetric<true, 128, 64, 64>(a, n, st);
-    else launch_symmetric<false, 128, 64, 64>(a, n, st);
+  auto tiles = [&](int64_t b) { return n * ceil_div(a.s.r, b) * (ceil_div(a.s.r, b) + 1) / 2; };
+  const int64_t cus = num_cus();
+  if (tiles(128) >= cus) {
+    if (133 * ceil_div(tiles(192), cus) < pairs_cost(tiles(128), cus)) {
+      if (square) launch_symmetric<true, 192, 96, 96, 1>(a, n, st);
+      else launch_symmetric<false, 192, 96, 96, 1>(a, n, st);
+    } else {
+      if (square) launch_symmetric<true, 128, 64, 32, 1>(a, n, st);
+      else launch_symmetric<false, 128, 64, 32, 1>(a, n, st);
+    }
+  } else if (tiles(64) <= cus) {
+    if (square) launch_symmetric<true, 64, 32, 32, 4>(a, n, st);
+    else launch_symmetric<false, 64, 32, 32, 4>(a, n, st);
   } else {
-    if (square) launch_symmetric<true, 64, 32, 32>(a, n, st);
-    else launch_symmetric<false, 64, 32, 32>(a, n, st);
+    if (square) launch_symmetric<true, 64, 32, 32, 1>(a, n, st);
+    else launch_symmetric<false, 64, 32, 32, 1>(a, n, st);
   }
 }
 
 void update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
-  const int64_t large = n * ceil_div(a.s.r, 256) * ceil_div(a.s.l, 256), middle = n * ceil_div(a.s.r, 128) * ceil_div(a.s.l, 128);
-  if (large >= num_cus()) launch_update<256, 256, 128, 64, 4>(a, n, from, last, st);
-  else if (middle >= num_cus()) launch_update<128, 128, 64, 64, 8>(a, n, from, last, st);
-  else launch_update<64, 64, 32, 32, 8>(a, n, from, last, st);
+  const int64_t cus = num_cus(), middle = n * ceil_div(a.s.r, 128) * ceil_div(a.s.l, 128);
+  const int64_t flat = n * ceil_div(a.s.r, 64) * ceil_div(a.s.l, 128);
+  if (2 * flat <= 3 * cus) launch_update<64, 64, 32, 32, 1, 8>(a, n, from, last, st);
+  else if (30 * ceil_div(flat, cus) <= pairs_cost(middle, cus)) launch_update<64, 128, 32, 32, 1, 8>(a, n, from, last, st);
+  else launch_update<128, 128, 64, 32, 1, 8>(a, n, from, last, st);
 }
 
 // ---- small matrices: a workgroup each, from the update to the result in one launch --------------------------------------

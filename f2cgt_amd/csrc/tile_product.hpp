@@ -59,6 +59,8 @@ __device__ __forceinline__ int piece_at(int r, int c) { return r * kLine + ((c ^
 // A sum as a word of LDS.  (By value: a bit cast of a vector's element itself takes the vector's first one.)
 __device__ __forceinline__ float word_of(float v) { return v; }
 __device__ __forceinline__ float word_of(int v) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ void add_word(fltx16& sums, int i, float word) { sums[i] += word; }
+__device__ __forceinline__ void add_word(intx16& sums, int i, float word) { sums[i] += __builtin_bit_cast(int, word); }
 
 // Waits until at most `loads` of this wave's copies into LDS are under way and its reads of LDS are done.
 template <int loads>
@@ -69,17 +71,22 @@ __device__ __forceinline__ void wait_copies() {
 // The pieces of a tile go from memory into LDS without a stop in registers, STAGES - 1 steps ahead of the one that is
 // multiplied; a step costs one barrier.  The stages are LDS arrays of their own (Buffers), which is how the compiler knows that a
 // read of one need not wait for the copies into the others.
-template <class Op, int BM, int BN, int WM, int WN, int STAGES>
+//
+// GROUPS > 1: groups of waves take the steps in turn, each into its own part of the stages, and add their sums in the end: for
+// tiles that are fewer than the chip's CUs.
+template <class Op, int BM, int BN, int WM, int WN, int STAGES, int GROUPS = 1>
 struct TileProduct {
-  static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = kWaves * kWave;
+  static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = kWaves * kWave;      // of a group
+  static constexpr int kBlock = kThreads * GROUPS;
   static constexpr int TI = WM / 32, TJ = WN / 32;
   static constexpr int kLd = WN + 4;                                   // floats of a strip's row in LDS
   static constexpr int kStrip = 32 * kLd * 4;
-  static constexpr int kStage = (BM + BN) * kLine;                     // bytes of a stage, and of a buffer
+  static constexpr int kPart = (BM + BN) * kLine;                      // bytes of a group's stage
+  static constexpr int kStage = GROUPS * kPart;                        // of a buffer
   static constexpr int kPieces = (BM + BN) * 8 / kThreads;             // copies of a thread in a step
   static_assert((BM + BN) * 8 % kThreads == 0 && BM * 8 % kThreads == 0, "whole pieces per thread");
   static constexpr int kStripsPerStage = kStage / kStrip;
-  static_assert(kStripsPerStage * STAGES >= kWaves, "a strip per wave");
+  static_assert(kStripsPerStage * STAGES >= kWaves * GROUPS, "a strip per wave");
   typedef typename Op::Acc Acc;
   typedef char* Buffers[STAGES];
 
@@ -88,7 +95,8 @@ struct TileProduct {
   template <class Epilogue>
   static __device__ __forceinline__ void run(const Buffers& lds, const Lines& a, const Lines& b, int64_t row0, int64_t col0,
                                              const Epilogue& epilogue) {
-    const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+    const int t = threadIdx.x - group * kThreads, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int wi = (wave % (BM / WM)) * WM, wj = (wave / (BM / WM)) * WN;
     const int at = lane & 31, side = lane >> 5;
     const int steps = (int)((a.bytes + kLine - 1) / kLine);
@@ -173,19 +181,21 @@ struct TileProduct {
       // all waves have them, and nobody reads the stage of the step before any more, which the next copies overwrite.  (There
       // are always as many copies under way: behind the last step it is copied again, into a stage that nobody reads.)
       auto held = [&](int step) { return step < steps ? step : steps - 1; };
+      const int part = group * kPart;
 #pragma unroll
-      for (int s = 0; s < STAGES - 1; ++s) copy(lds[s], held(s));
-      int step = 0;
+      for (int s = 0; s < STAGES - 1; ++s) copy(lds[s] + part, held(s * GROUPS + group));
+      int step = group;
       while (true) {
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) {
           wait_copies<(STAGES - 2) * kPieces>();
-          if (Op::kTrim && left < kLine && step == steps - 1) trim(lds[s]);
+          if (Op::kTrim && left < kLine && step == steps - 1) trim(lds[s] + part);
           __builtin_amdgcn_s_barrier();
-          copy(lds[(s + STAGES - 1) % STAGES], held(step + STAGES - 1));
+          copy(lds[(s + STAGES - 1) % STAGES] + part, held(step + (STAGES - 1) * GROUPS));
           __builtin_amdgcn_sched_barrier(0);             // (the compiler would sink them to the step's end)
-          multiply(lds[s]);
-          if (++step == steps) goto done;
+          if (GROUPS == 1 || step < steps) multiply(lds[s] + part);
+          step += GROUPS;
+          if (step - group >= steps) goto done;
         }
       }
     }
@@ -193,22 +203,49 @@ struct TileProduct {
     wait_copies<0>();
     __builtin_amdgcn_s_barrier();
     // The columns' operand came first: a lane holds, of one row, four columns after four.
-    char* mine = nullptr;
+    auto strip_of = [&](int of) {
+      const int n = of * kWaves + wave;
+      char* at_stage = nullptr;
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s)
-      if (wave / kStripsPerStage == s) mine = lds[s] + (wave % kStripsPerStage) * kStrip;
-    float* strip = reinterpret_cast<float*>(mine);
+      for (int s = 0; s < STAGES; ++s)
+        if (n / kStripsPerStage == s) at_stage = lds[s] + (n % kStripsPerStage) * kStrip;
+      return reinterpret_cast<float*>(at_stage);
+    };
+    float* strip = strip_of(group);
+    auto place = [&](float* of, int j, int q) { return reinterpret_cast<fltx4*>(of + at * kLd + 32 * j + 8 * q + 4 * side); };
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
+      if (GROUPS > 1 && i > 0) __syncthreads();
+      if (GROUPS == 1 || group > 0) {
 #pragma unroll
-      for (int j = 0; j < TJ; ++j)
+        for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          fltx4 v;
+          for (int q = 0; q < 4; ++q) {
+            fltx4 v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = word_of(acc[i][j][4 * q + e]);
-          *reinterpret_cast<fltx4*>(strip + at * kLd + 32 * j + 8 * q + 4 * side) = v;
-        }
+            for (int e = 0; e < 4; ++e) v[e] = word_of(acc[i][j][4 * q + e]);
+            *place(strip, j, q) = v;
+          }
+      }
+      if constexpr (GROUPS > 1) {
+        __syncthreads();
+        if (group > 0) continue;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int o = 1; o < GROUPS; ++o) {
+              const fltx4 v = *place(strip_of(o), j, q);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) add_word(acc[i][j], 4 * q + e, v[e]);
+            }
+            fltx4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = word_of(acc[i][j][4 * q + e]);
+            *place(strip, j, q) = v;
+          }
+      }
       __builtin_amdgcn_wave_barrier();
       epilogue(strip, row0 + wi + 32 * i, col0 + wj, lane);
       __builtin_amdgcn_wave_barrier();

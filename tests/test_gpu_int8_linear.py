@@ -55,7 +55,8 @@ def test_products_against_whole_numbers(m, k, n, dtype):
         _check(out, *_want(codes, scales, weight, weight_scales, bias, relu), dtype)
 
 
-@pytest.mark.parametrize("m,k,n", [(2048, 512, 2048), (4096, 1024, 768), (2500, 700, 1111), (8192, 128, 256), (777, 5000, 4000)])
+@pytest.mark.parametrize("m,k,n", [(2048, 512, 2048), (4096, 1024, 768), (2500, 700, 1111), (8192, 128, 256), (777, 5000, 4000),
+                                   (4096, 1030, 4096), (4095, 1100, 4093), (8300, 1024, 4100)])
 def test_large_products_are_the_whole_numbers(m, k, n):
     # unit scales: every sum below 2^24 is given as it is
     lib = f2cgt_amd.load()

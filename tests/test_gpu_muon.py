@@ -73,6 +73,27 @@ def test_larger_matrices(rows, cols):
     _check(lib.orthogonalize(u.bfloat16()), u.bfloat16(), torch.bfloat16)
 
 
+@pytest.mark.parametrize("rows,cols", [(3970, 4100), (4333, 4000)])
+def test_the_largest_tiles(rows, cols):
+    # (both references on the device: float64 products of this size take the host minutes)
+    lib = f2cgt_amd.load()
+    u = _update(rows, cols, "low", _gen(rows))
+
+    def iterate(dtype):
+        a, b, c = COEFFICIENTS
+        x = u.to(dtype) if rows <= cols else u.t().to(dtype).contiguous()
+        x = x / (x.norm() + 1e-7)
+        for _ in range(5):
+            gram = torch.mm(x, x.t())
+            x = a * x + torch.mm(b * gram + c * torch.mm(gram, gram), x)
+        return x if rows <= cols else x.t()
+
+    want, single = iterate(torch.float64), iterate(torch.float32)
+    got = lib.orthogonalize(u)
+    bound = 4 * float((single.double() - want).norm()) + (2.0 ** -21 + HALF[torch.float32]) * float(want.norm())
+    assert float((got.double() - want).norm()) <= bound
+
+
 @pytest.mark.parametrize("count,rows,cols", [(1, 20, 30), (3, 128, 128), (5, 64, 96), (70, 33, 17), (130, 8, 8), (3, 200, 300), (2, 400, 150)])
 def test_a_batch_is_its_matrices(count, rows, cols):
     lib = f2cgt_amd.load()
