@@ -45,6 +45,10 @@ struct MuonArgs {
   char* g;                                     // [count][r] lines of G
   char* p;                                     // of P
   float a, b, c;
+  // A result in bf16: its own rounding is 1.65e-3 of it (in the norm; in fp16 it is 2e-4, too little for this).  G of the hi planes alone in all steps and the last
+  // product of theirs make it 1.7e-3 to 2.0e-3, and 23 of 30 instructions are left of a square matrix; G G or an earlier
+  // update from them 2.5e-3 and more.
+  __host__ __device__ bool few() const { return out_dtype == F2CGT_DT_BF16; }
   int whole;                                   // rows of the results start at multiples of four values
 };
 
@@ -209,9 +213,9 @@ struct SymmetricEpilogue {
   }
 };
 
-template <bool SQUARE, int B, int W, int WJ, int GROUPS>
+template <class Op, bool SQUARE, int B, int W, int WJ, int GROUPS>
 __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symmetric_kernel(MuonArgs a) {
-  typedef TileProduct<SplitOp, B, B, W, WJ, 2, GROUPS> Tile;
+  typedef TileProduct<Op, B, B, W, WJ, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   // tile (i, j), j <= i, in the order of rows
   int i = (int)((sqrtf(8.f * (float)blockIdx.x + 1.f) - 1.f) * 0.5f);
@@ -222,7 +226,7 @@ __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symm
   char* g = a.g + z * s.r * s.short_line();
   char* p = a.p + z * s.r * s.short_line();
   const Lines from = SQUARE ? Lines{g, s.short_line(), s.r, s.short_line()}
-                            : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line()};
+                            : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line() * kLine / Op::kFrom};
   Tile::run({lds0, lds1}, from, from, row0, col0, SymmetricEpilogue<WJ>{a, SQUARE ? p : g, SQUARE ? g : nullptr, row0 != col0});
 }
 
@@ -287,30 +291,36 @@ struct UpdateEpilogue {
   }
 };
 
-template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
+template <class Op, int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
-  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2, GROUPS> Tile;
+  typedef TileProduct<Op, BM, BN, WM, WN, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   const int64_t z = blockIdx.z;
   uint32_t i, j;
   tile_of(blockIdx.x, (uint32_t)ceil_div(s.r, BM), (uint32_t)ceil_div(s.l, BN), DEEP, i, j);
-  const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, s.short_line()};
-  const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, s.short_line()};
+  const int64_t bytes = s.short_line() * kLine / Op::kFrom;
+  const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, bytes};
+  const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, bytes};
   Tile::run({lds0, lds1}, p, x, (int64_t)BM * i, (int64_t)BN * j, UpdateEpilogue<WN>{a, z, last ? nullptr : a.xt[1 - from]});
 }
 
-template <bool SQUARE, int B, int W, int WJ, int GROUPS>
-void launch_symmetric(const MuonArgs& a, int64_t n, hipStream_t st) {
+template <int B, int W, int WJ, int GROUPS>
+void launch_symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
   const int64_t tiles = ceil_div(a.s.r, B);
-  muon_symmetric_kernel<SQUARE, B, W, WJ, GROUPS>
-      <<<dim3((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n), (B / W) * (B / WJ) * GROUPS * kWave, 0, st>>>(a);
+  const dim3 grid((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n);
+  constexpr int kBlock = (B / W) * (B / WJ) * GROUPS * kWave;
+  if (square) muon_symmetric_kernel<SplitOp, true, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
+  else if (a.few()) muon_symmetric_kernel<HiOp, false, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
+  else muon_symmetric_kernel<SplitOp, false, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
 }
 
 template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
-  muon_update_kernel<BM, BN, WM, WN, GROUPS, DEEP><<<dim3((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n),
-                                                     (BM / WM) * (BN / WN) * GROUPS * kWave, 0, st>>>(a, from, last);
+  const dim3 grid((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n);
+  constexpr int kBlock = (BM / WM) * (BN / WN) * GROUPS * kWave;
+  if (last && a.few()) muon_update_kernel<HiOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
+  else muon_update_kernel<SplitOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
 }
 
 // Which tiles.  Time of a step of 32 summed columns, us, by tiles per CU:
@@ -330,18 +340,14 @@ void symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
   const int64_t cus = num_cus();
   if (tiles(128) >= cus) {
     if (133 * ceil_div(tiles(192), cus) < pairs_cost(tiles(128), cus)) {
-      if (square) launch_symmetric<true, 192, 96, 96, 1>(a, n, st);
-      else launch_symmetric<false, 192, 96, 96, 1>(a, n, st);
+      launch_symmetric<192, 96, 96, 1>(a, n, square, st);
     } else {
-      if (square) launch_symmetric<true, 128, 64, 32, 1>(a, n, st);
-      else launch_symmetric<false, 128, 64, 32, 1>(a, n, st);
+      launch_symmetric<128, 64, 32, 1>(a, n, square, st);
     }
   } else if (tiles(64) <= cus) {
-    if (square) launch_symmetric<true, 64, 32, 32, 4>(a, n, st);
-    else launch_symmetric<false, 64, 32, 32, 4>(a, n, st);
+    launch_symmetric<64, 32, 32, 4>(a, n, square, st);
   } else {
-    if (square) launch_symmetric<true, 64, 32, 32, 1>(a, n, st);
-    else launch_symmetric<false, 64, 32, 32, 1>(a, n, st);
+    launch_symmetric<64, 32, 32, 1>(a, n, square, st);
   }
 }
 
