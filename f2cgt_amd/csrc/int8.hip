@@ -191,7 +191,7 @@ template <int BM, int BN, int WM, int WN, int STAGES, int GROUPS, int DEEP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void int8_linear_kernel(LinearArgs a) {
   typedef TileProduct<Int8Op, BM, BN, WM, WN, STAGES, GROUPS> Tile;
   uint32_t i, j;
-  tile_of(blockIdx.x, (uint32_t)ceil_div(a.m, BM), (uint32_t)ceil_div(a.n, BN), DEEP, i, j);
+  tile_of(place_of(blockIdx.x, gridDim.x), (uint32_t)ceil_div(a.m, BM), (uint32_t)ceil_div(a.n, BN), DEEP, i, j);
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   if constexpr (STAGES == 2) {
     Tile::run({lds0, lds1}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});

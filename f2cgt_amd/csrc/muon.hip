@@ -57,20 +57,54 @@ __device__ __forceinline__ float update_of(const MuonArgs& a, float grad, float 
   return a.nesterov ? a.momentum * held + (1.f - a.momentum) * grad : held;
 }
 
+// Four neighbours of memory, wherever they start, and fewer at its end.
+template <typename T>
+__device__ __forceinline__ fltx4 load_up_to_four(const void* p, int64_t i, int64_t end) {
+  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  fltx4 v = {0.f, 0.f, 0.f, 0.f};
+  if (i + 4 <= end) {
+    const four o = *reinterpret_cast<const four*>(static_cast<const T*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)o[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < end) v[e] = (float)static_cast<const T*>(p)[i + e];
+  }
+  return v;
+}
+__device__ __forceinline__ fltx4 load_up_to_four(const void* p, int dtype, int64_t i, int64_t end) {
+  if (dtype == F2CGT_DT_F32) return load_up_to_four<float>(p, i, end);
+  if (dtype == F2CGT_DT_F16) return load_up_to_four<_Float16>(p, i, end);
+  return load_up_to_four<__bf16>(p, i, end);
+}
+
 // Momenta, and the sum of squares of the updates by parts, in 64 bits (a square of an fp32 number may be none).
 __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
-  const int64_t count = a.s.rows * a.s.cols, z = blockIdx.y;
+  constexpr int U = 4;
+  const int64_t count = a.s.rows * a.s.cols, z = blockIdx.y, step = (int64_t)gridDim.x * 1024;
   const void* u = a.at.u[z];
   float* held = a.at.held[z];
   double sum = 0.;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-    float v = load_value(u, a.u_dtype, i);
-    if (held != nullptr) {
-      const float h = a.momentum * held[i] + (1.f - a.momentum) * v;
-      held[i] = h;
-      v = update_of(a, v, h);
+  for (int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x * 4; i0 < count; i0 += U * step) {
+    fltx4 v[U], h[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      v[k] = load_up_to_four(u, a.u_dtype, i0 + k * step, count);
+      if (held != nullptr) h[k] = load_up_to_four<float>(held, i0 + k * step, count);
     }
-    sum += (double)v * (double)v;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (held != nullptr) {
+          h[k][e] = a.momentum * h[k][e] + (1.f - a.momentum) * v[k][e];
+          const int64_t i = i0 + k * step + e;
+          if (i < count) held[i] = h[k][e];
+          v[k][e] = update_of(a, v[k][e], h[k][e]);
+        }
+        sum += (double)v[k][e] * (double)v[k][e];
+      }
   }
   __shared__ double s_sum[4];
 #pragma unroll
@@ -78,54 +112,6 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
   if ((threadIdx.x & (kWave - 1)) == 0) s_sum[threadIdx.x / kWave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) a.partial[z * a.parts + blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-}
-
-__device__ __forceinline__ void put_split(char* row, int64_t c, float v) {
-  const _Float16 hi = (_Float16)v;
-  const _Float16 lo = (_Float16)(v - (float)hi);
-  char* line = row + (c >> 5) * kLine + 2 * (c & 31);
-  *reinterpret_cast<_Float16*>(line) = hi;
-  *reinterpret_cast<_Float16*>(line + 64) = lo;
-}
-
-// The update of length one in planes, both ways round: a 32 x 32 tile of the caller's matrix per workgroup.
-__global__ __launch_bounds__(256) void muon_split_kernel(MuonArgs a) {
-  __shared__ double s_sum[4];
-  __shared__ float s_tile[32][33];
-  const int t = threadIdx.x;
-  const int64_t z = blockIdx.z;
-  double sum = 0.;
-  for (int i = t; i < a.parts; i += 256) sum += a.partial[z * a.parts + i];
-#pragma unroll
-  for (int by = 32; by > 0; by /= 2) sum += __shfl_xor(sum, by);
-  if ((t & (kWave - 1)) == 0) s_sum[t / kWave] = sum;
-  __syncthreads();
-  const double norm = sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
-  const float scale = (float)(kScale / (norm + 1e-7));
-  const int64_t row0 = (int64_t)blockIdx.x * 32, col0 = (int64_t)blockIdx.y * 32;
-  const void* u = a.at.u[z];
-  const float* held = a.at.held[z];
-  for (int i = t; i < 1024; i += 256) {
-    const int64_t row = row0 + i / 32, col = col0 + i % 32;
-    float v = 0.f;
-    if (row < a.s.rows && col < a.s.cols) {
-      const int64_t at = row * a.s.cols + col;
-      v = load_value(u, a.u_dtype, at);
-      if (held != nullptr) v = update_of(a, v, held[at]);
-      v *= scale;
-    }
-    s_tile[i / 32][i % 32] = v;
-  }
-  __syncthreads();
-  // the caller's rows are X's, or X^T's
-  char* along = a.s.turned ? a.xt[0] + z * a.s.l * a.s.short_line() : a.x + z * a.s.r * a.s.long_line();
-  char* across = a.s.turned ? a.x + z * a.s.r * a.s.long_line() : a.xt[0] + z * a.s.l * a.s.short_line();
-  const int64_t along_line = a.s.turned ? a.s.short_line() : a.s.long_line();
-  const int64_t across_line = a.s.turned ? a.s.long_line() : a.s.short_line();
-  for (int i = t; i < 1024; i += 256) {
-    if (row0 + i / 32 < a.s.rows) put_split(along + (row0 + i / 32) * along_line, col0 + i % 32, s_tile[i / 32][i % 32]);
-    if (col0 + i / 32 < a.s.cols) put_split(across + (col0 + i / 32) * across_line, row0 + i % 32, s_tile[i % 32][i / 32]);
-  }
 }
 
 // ---- strips of finished tiles: 32 rows and WN columns of sums in LDS, in lanes' turns of eight neighbours -----------------
@@ -145,6 +131,59 @@ __device__ __forceinline__ void put_eight(char* row, int64_t c, const float (&v)
   char* line = row + (c >> 5) * kLine + 2 * (c & 31);
   *reinterpret_cast<halfx8*>(line) = hi;
   *reinterpret_cast<halfx8*>(line + 64) = lo;
+}
+
+// The update of length kScale in planes, both ways round: a 64 x 64 tile of the caller's matrix per workgroup.
+__global__ __launch_bounds__(256) void muon_split_kernel(MuonArgs a) {
+  __shared__ double s_sum[4];
+  __shared__ float s_tile[64][65];
+  const int t = threadIdx.x;
+  const int64_t z = blockIdx.z, rows = a.s.rows, cols = a.s.cols;
+  const int64_t row0 = (int64_t)blockIdx.x * 64, col0 = (int64_t)blockIdx.y * 64;
+  const void* u = a.at.u[z];
+  const float* held = a.at.held[z];
+  fltx4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + t / 16 + 16 * i, col = col0 + 4 * (t % 16), end = row < rows ? (row + 1) * cols : 0;
+    const int64_t from = col < cols ? row * cols + col : end;
+    v[i] = load_up_to_four(u, a.u_dtype, from, end);
+    if (held != nullptr) {
+      const fltx4 h = load_up_to_four<float>(held, from, end);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = update_of(a, v[i][e], h[e]);
+    }
+  }
+  double sum = 0.;
+  for (int i = t; i < a.parts; i += 256) sum += a.partial[z * a.parts + i];
+#pragma unroll
+  for (int by = 32; by > 0; by /= 2) sum += __shfl_xor(sum, by);
+  if ((t & (kWave - 1)) == 0) s_sum[t / kWave] = sum;
+  __syncthreads();
+  const double norm = sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
+  const float scale = (float)(kScale / (norm + 1e-7));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_tile[t / 16 + 16 * i][4 * (t % 16) + e] = v[i][e] * scale;
+  __syncthreads();
+  // the caller's rows are X's, or X^T's
+  char* along = a.s.turned ? a.xt[0] + z * a.s.l * a.s.short_line() : a.x + z * a.s.r * a.s.long_line();
+  char* across = a.s.turned ? a.x + z * a.s.r * a.s.long_line() : a.xt[0] + z * a.s.l * a.s.short_line();
+  const int64_t along_line = a.s.turned ? a.s.short_line() : a.s.long_line();
+  const int64_t across_line = a.s.turned ? a.s.long_line() : a.s.short_line();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = t / 8 + 32 * i, c = 8 * (t % 8);
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = s_tile[r][c + e];
+      y[e] = s_tile[c + e][r];
+    }
+    if (row0 + r < rows && (col0 + c) / 32 * 32 < cols) put_eight(along + (row0 + r) * along_line, col0 + c, x);
+    if (col0 + r < cols && (row0 + c) / 32 * 32 < rows) put_eight(across + (col0 + r) * across_line, row0 + c, y);
+  }
 }
 
 // change(row, col, v): eight neighbours of a row; then put(row, col, v) with them, and turned(row, col, v) with eight neighbours of
@@ -213,15 +252,14 @@ struct SymmetricEpilogue {
   }
 };
 
-template <class Op, bool SQUARE, int B, int W, int WJ, int GROUPS>
+template <class Op, bool SQUARE, int B, int W, int WJ, int GROUPS, int DEEP>
 __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symmetric_kernel(MuonArgs a) {
   typedef TileProduct<Op, B, B, W, WJ, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
-  // tile (i, j), j <= i, in the order of rows
-  int i = (int)((sqrtf(8.f * (float)blockIdx.x + 1.f) - 1.f) * 0.5f);
-  while ((i + 1) * (i + 2) / 2 <= (int)blockIdx.x) ++i;
-  while (i * (i + 1) / 2 > (int)blockIdx.x) --i;
-  const int64_t z = blockIdx.z, row0 = (int64_t)B * i, col0 = (int64_t)B * ((int)blockIdx.x - i * (i + 1) / 2);
+  const uint32_t tiles = (uint32_t)ceil_div(a.s.r, B), each = tiles * (tiles + 1) / 2, at = place_of(blockIdx.x, gridDim.x);
+  uint32_t i, j;
+  lower_tile_of(at % each, tiles, DEEP, i, j);
+  const int64_t z = at / each, row0 = (int64_t)B * i, col0 = (int64_t)B * j;
   const Shape& s = a.s;
   char* g = a.g + z * s.r * s.short_line();
   char* p = a.p + z * s.r * s.short_line();
@@ -296,40 +334,42 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void muon_u
   typedef TileProduct<Op, BM, BN, WM, WN, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
-  const int64_t z = blockIdx.z;
+  const uint32_t tiles_r = (uint32_t)ceil_div(s.r, BM), tiles_l = (uint32_t)ceil_div(s.l, BN), at = place_of(blockIdx.x, gridDim.x);
   uint32_t i, j;
-  tile_of(blockIdx.x, (uint32_t)ceil_div(s.r, BM), (uint32_t)ceil_div(s.l, BN), DEEP, i, j);
+  tile_of(at % (tiles_r * tiles_l), tiles_r, tiles_l, DEEP, i, j);
+  const int64_t z = at / (tiles_r * tiles_l);
   const int64_t bytes = s.short_line() * kLine / Op::kFrom;
   const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, bytes};
   const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, bytes};
   Tile::run({lds0, lds1}, p, x, (int64_t)BM * i, (int64_t)BN * j, UpdateEpilogue<WN>{a, z, last ? nullptr : a.xt[1 - from]});
 }
 
-template <int B, int W, int WJ, int GROUPS>
+template <int B, int W, int WJ, int GROUPS, int DEEP>
 void launch_symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
   const int64_t tiles = ceil_div(a.s.r, B);
-  const dim3 grid((unsigned)(tiles * (tiles + 1) / 2), 1, (unsigned)n);
+  const unsigned grid = (unsigned)(n * tiles * (tiles + 1) / 2);
   constexpr int kBlock = (B / W) * (B / WJ) * GROUPS * kWave;
-  if (square) muon_symmetric_kernel<SplitOp, true, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
-  else if (a.few()) muon_symmetric_kernel<HiOp, false, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
-  else muon_symmetric_kernel<SplitOp, false, B, W, WJ, GROUPS><<<grid, kBlock, 0, st>>>(a);
+  if (square) muon_symmetric_kernel<SplitOp, true, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
+  else if (a.few()) muon_symmetric_kernel<HiOp, false, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
+  else muon_symmetric_kernel<SplitOp, false, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
 }
 
 template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
-  const dim3 grid((unsigned)(ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN)), 1, (unsigned)n);
+  const unsigned grid = (unsigned)(n * ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN));
   constexpr int kBlock = (BM / WM) * (BN / WN) * GROUPS * kWave;
   if (last && a.few()) muon_update_kernel<HiOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
   else muon_update_kernel<SplitOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
 }
 
-// Which tiles.  Time of a step of 32 summed columns, us, by tiles per CU:
-//   128 x 128 in eight waves, two workgroups a CU: one tile 0.67-0.75, two 0.93, so 0.93 for each pair and 0.67 for a last one
-//   192 x 192 in four waves (symmetric products): 1.33 each;  64 x 128 in eight waves (updates), three a CU: 0.30 each
-//   64 x 64: 0.47 for one, 0.28 each for many; with four groups of waves 0.31 for one
-// Gram products of 1000 x 2051: 64 x 64 30.6, in four groups 20.0, 128 x 128 44; 2048 x 2048: 33.8, 55.8 and 43; 3000 x 3000: 112, 144
-// and 88, 192 x 192 128; 4096 x 4096: 300, 349, 222 and 171 (253 tiles for 256 CUs).  Updates: 1000 x 2051: 64 x 64 20.9, 64 x 128 23.5,
-// 128 x 128 26.7; 2048 x 2048: 52, 42, 48; 3000 x 3000: 160, 130, 142; 4096 x 4096: 361, 280, 238, 256 x 256 299.
+// Which tiles.  Time of a step of 32 summed columns, in 10 ns, by tiles per CU, and steps' worth of a tile's begin and end:
+//   128 x 128 in eight waves, two workgroups a CU: one tile 67, two 93, so 93 for each pair and 67 for a last one; 6 steps
+//   192 x 192 in four waves (symmetric products): 133 each; 8 steps.  64 x 128 in eight waves (updates), three a CU: 30 each
+//   64 x 64: 47 for one, 22 each for many; 2 steps.  With four groups of waves 31 for one
+// us of Gram products of 1000 x 2051: 64 x 64 30, in four groups 19.5, 128 x 128 42; 2048 x 2048: 34, 54, 42; eight of 1000 x 700: 18, 27, 24;
+// 3000 x 3000: 97, 128, 86, 192 x 192 128; 4096 x 4096: 195, 262, 169, 168 (528 and 253 tiles; of the hi planes 215, 224, 125, 88).
+// Updates: 1000 x 2051: 64 x 64 20.8, 64 x 128 23.5, 128 x 128 27.1; 2048 x 2048: 50, 43, 49; 3000 x 3000: 160, 130, 142;
+// 4096 x 4096: 349, 284, 237, 256 x 256 299.
 int64_t pairs_cost(int64_t tiles, int64_t cus) {
   const int64_t left = tiles % (2 * cus);
   return 93 * (tiles / (2 * cus)) + (left == 0 ? 0 : left <= cus ? 67 : 93);
@@ -337,18 +377,13 @@ int64_t pairs_cost(int64_t tiles, int64_t cus) {
 
 void symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st) {
   auto tiles = [&](int64_t b) { return n * ceil_div(a.s.r, b) * (ceil_div(a.s.r, b) + 1) / 2; };
-  const int64_t cus = num_cus();
-  if (tiles(128) >= cus) {
-    if (133 * ceil_div(tiles(192), cus) < pairs_cost(tiles(128), cus)) {
-      launch_symmetric<192, 96, 96, 1>(a, n, square, st);
-    } else {
-      launch_symmetric<128, 64, 32, 1>(a, n, square, st);
-    }
-  } else if (tiles(64) <= cus) {
-    launch_symmetric<64, 32, 32, 4>(a, n, square, st);
-  } else {
-    launch_symmetric<64, 32, 32, 1>(a, n, square, st);
-  }
+  const int64_t cus = num_cus(), steps = ceil_div(square ? a.s.r : a.s.l, 32);
+  const int64_t small = (steps + 2) * 22 * tiles(64) / cus;
+  const int64_t middle = (steps + 6) * pairs_cost(tiles(128), cus), large = (steps + 8) * 133 * ceil_div(tiles(192), cus);
+  if (tiles(64) <= cus) launch_symmetric<64, 32, 32, 4, 8>(a, n, square, st);
+  else if (tiles(128) < cus || (small < middle && small < large)) launch_symmetric<64, 32, 32, 1, 8>(a, n, square, st);
+  else if (middle <= large) launch_symmetric<128, 64, 32, 1, 8>(a, n, square, st);
+  else launch_symmetric<192, 96, 96, 1, 6>(a, n, square, st);
 }
 
 void update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
@@ -755,7 +790,7 @@ Shape shape_of(int64_t rows, int64_t cols) {
 
 int64_t parts_of(int64_t rows, int64_t cols) {
   const int64_t n = ceil_div(rows * cols, 4096);
-  return n < 256 ? n : 256;
+  return n < 1024 ? n : 1024;
 }
 
 int64_t whole(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
@@ -830,7 +865,7 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
       continue;
     }
     muon_norm_kernel<<<dim3((unsigned)a.parts, (unsigned)n), 256, 0, st>>>(a);
-    muon_split_kernel<<<dim3((unsigned)ceil_div(rows, 32), (unsigned)ceil_div(cols, 32), (unsigned)n), 256, 0, st>>>(a);
+    muon_split_kernel<<<dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64), (unsigned)n), 256, 0, st>>>(a);
     for (int step = 0; step < steps; ++step) {
       symmetric(a, n, false, st);
       symmetric(a, n, true, st);

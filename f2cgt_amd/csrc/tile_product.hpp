@@ -271,15 +271,40 @@ struct TileProduct {
   }
 };
 
-// Workgroup `id` of tiles_m x tiles_n: neighbours in time share operands.  Workgroups go round the eight XCDs, each with an L2
-// of its own, so an XCD gets one run of the tiles' order, which goes down `deep` tiles before it goes to the next column.
-__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t deep, uint32_t& i, uint32_t& j) {
-  const uint32_t all = tiles_m * tiles_n, xcd = id & 7, share = all >> 3, more = all & 7;
-  const uint32_t at = xcd * share + (xcd < more ? xcd : more) + (id >> 3);
+// Neighbours in time share operands: workgroups go round the eight XCDs, each with an L2 of its own, so an XCD gets one run of the
+// tiles' order.  Workgroup `id` of `all` -> its place in that order.
+__device__ __forceinline__ uint32_t place_of(uint32_t id, uint32_t all) {
+  const uint32_t xcd = id & 7, share = all >> 3, more = all & 7;
+  return xcd * share + (xcd < more ? xcd : more) + (id >> 3);
+}
+// Place `at` among tiles_m x tiles_n, which are gone through in bands of `deep` rows, a band column by column.
+__device__ __forceinline__ void tile_of(uint32_t at, uint32_t tiles_m, uint32_t tiles_n, uint32_t deep, uint32_t& i, uint32_t& j) {
   const uint32_t band = at / (deep * tiles_n), first = band * deep, in = at - band * deep * tiles_n;
   const uint32_t rows = tiles_m - first < deep ? tiles_m - first : deep;
   j = in / rows;
   i = first + in - j * rows;
+}
+// The same of the tiles on and below the diagonal of `tiles` rows.
+__device__ __forceinline__ void lower_tile_of(uint32_t at, uint32_t tiles, uint32_t deep, uint32_t& i, uint32_t& j) {
+  uint32_t first = 0;
+  while (true) {
+    const uint32_t rows = tiles - first < deep ? tiles - first : deep, square = rows * first, all = square + rows * (rows + 1) / 2;
+    if (at < square) {
+      j = at / rows;
+      i = first + at - j * rows;
+      return;
+    }
+    if (at < all) {
+      at -= square;
+      i = 0;
+      while (at > i) at -= ++i;
+      j = first + at;
+      i += first;
+      return;
+    }
+    at -= all;
+    first += rows;
+  }
 }
 
 // ---- values of the types that the dense operators take ---------------------------------------------------
