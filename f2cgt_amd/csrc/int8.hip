@@ -18,103 +18,132 @@ struct QuantizeArgs {
   int64_t m, k, ld, stride;
 };
 
-__device__ __forceinline__ float scale_of(float most) { return (most < kLeast ? kLeast : most) * (1.f / 127.f); }
+// Magnitudes are compared as the whole numbers of their bits: the order is the same, and a NaN is above infinity and stays.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
-__device__ __forceinline__ int code_of(float x, float inverse) {
-  const float q = rintf(x * inverse);
-  return q != q ? 0 : (int)fminf(fmaxf(q, -127.f), 127.f);
-}
-
-// V neighbours of a row, wherever it starts (memory takes 16 bytes at any address).
-template <typename X>
-struct Piece {
-  static constexpr int kEach = 16 / sizeof(X);
-  typedef X Values __attribute__((ext_vector_type(kEach), aligned(sizeof(X))));
-  typedef int8_t Codes __attribute__((ext_vector_type(kEach), aligned(1)));
+// What the codes of a row are made with, from its largest magnitude.
+struct RowCode {
+  float scale, inverse;
+  uint32_t keep;                             // no bit where a NaN is among the row's values: its codes are zero
+  __device__ __forceinline__ explicit RowCode(uint32_t bits) {
+    const float most = __builtin_bit_cast(float, bits);
+    scale = (most < kLeast ? kLeast : most) * (1.f / 127.f);
+    inverse = 1.f / scale;
+    keep = most == most ? ~0u : 0u;
+  }
+  // rint(x * inverse) in the low byte.  Adding 3 * 2^22 rounds to a whole number in the place of the last bit.  No magnitude
+  // is above 127: x <= most, and three roundings on the way are not half a code.  (Infinities: inverse 0, inf * 0 is the NaN without payload.)
+  __device__ __forceinline__ uint32_t operator()(float x) const { return __builtin_bit_cast(uint32_t, x * inverse + 12582912.f); }
+  __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const {
+    const uint32_t low = __builtin_amdgcn_perm((*this)(b), (*this)(a), 0x0c0c0400), high = __builtin_amdgcn_perm((*this)(d), (*this)(c), 0x04000c0c);
+    return (low | high) & keep;
+  }
 };
 
 template <typename X>
-__device__ __forceinline__ void load_piece(const X* row, int64_t c, int64_t k, float (&v)[16 / sizeof(X)]) {
-  constexpr int V = 16 / sizeof(X);
-  if (c + V <= k) {
-    const typename Piece<X>::Values p = *reinterpret_cast<const typename Piece<X>::Values*>(row + c);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (float)p[e];
-  } else {
+constexpr int piece_values() { return 16 / sizeof(X); }
+
+// V neighbours of a row of k values from column c on, wherever they start in memory (which takes 16 bytes at any address): zeros
+// for those behind the row's end, but for a piece that begins there others of the row.  `last`: behind this row is
+// nothing that may be read.  One load without a branch around it, so that a caller's loads are under way together.
+template <typename X, int V>
+__device__ __forceinline__ void load_piece(const X* row, int64_t c, int64_t k, bool last, float (&v)[V]) {
+  typedef X values __attribute__((ext_vector_type(V), aligned(sizeof(X))));
+  if (k < V) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = c + e < k ? (float)row[c + e] : 0.f;
+    return;
+  }
+  const int64_t from = c < k ? c : 0;
+  const bool over = last && from + V > k;
+  const values p = *reinterpret_cast<const values*>(row + (over ? k - V : from));
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = (float)p[e];
+  if (k % V != 0) {
+    if (over) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = from + e < k ? (float)row[from + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = from + e < k ? v[e] : 0.f;
   }
 }
 
 template <int V>
-__device__ __forceinline__ float largest(const float (&v)[V], float most) {
+__device__ __forceinline__ uint32_t largest(const float (&v)[V], uint32_t most) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float o = fabsf(v[e]);
-    most = o > most || o != o ? o : most;    // a NaN stays
-  }
+  for (int e = 0; e < V; ++e) most = larger(most, magnitude(v[e]));
   return most;
 }
+
+// A piece's codes, four in a word.
+template <int V>
+struct Words {
+  uint32_t w[V / 4] = {};
+  __device__ __forceinline__ Words() {}
+  __device__ __forceinline__ Words(const RowCode& code, const float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) w[i] = code.four(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  }
+};
 
 // A row per LANES lanes (16, 64, or 256: a workgroup), read once: up to HELD pieces of 16 bytes a lane stay in registers, what is
 // beyond them is read again for the codes.
 template <typename X, int LANES, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
-  constexpr int V = Piece<X>::kEach;
+  constexpr int V = piece_values<X>();
   const int t = threadIdx.x, lane = t % LANES;
-  __shared__ float s_most[4];
+  __shared__ uint32_t s_most[4];
   for (int64_t r0 = (int64_t)blockIdx.x * (256 / LANES); r0 < a.m; r0 += (int64_t)gridDim.x * (256 / LANES)) {
     const int64_t r = r0 + t / LANES, rr = r < a.m ? r : a.m - 1;
+    const bool last = rr == a.m - 1;
     const X* x = static_cast<const X*>(a.x) + rr * a.ld;
     float v[HELD][V];
-    float most = 0.f;
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) load_piece<X>(x, (int64_t)(lane + i * LANES) * V, a.k, v[i]);
+    for (int i = 0; i < HELD; ++i) load_piece<X, V>(x, (int64_t)(lane + i * LANES) * V, a.k, last, v[i]);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) most = largest<V>(v[i], most);
     for (int64_t c = (int64_t)(lane + HELD * LANES) * V; c < a.k; c += LANES * V) {
       float w[V];
-      load_piece<X>(x, c, a.k, w);
+      load_piece<X, V>(x, c, a.k, last, w);
       most = largest<V>(w, most);
     }
 #pragma unroll
-    for (int by = 1; by < (LANES < kWave ? LANES : kWave); by *= 2) {
-      const float o = __shfl_xor(most, by);
-      most = o > most || o != o ? o : most;
-    }
+    for (int by = 1; by < (LANES < kWave ? LANES : kWave); by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
     if (LANES > kWave) {
       __syncthreads();                         // (of the row before)
       if (t % kWave == 0) s_most[t / kWave] = most;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float o = s_most[i];
-        most = o > most || o != o ? o : most;
-      }
+      for (int i = 0; i < 4; ++i) most = larger(most, s_most[i]);
     }
-    const float scale = scale_of(most), inverse = 1.f / scale;
+    const RowCode code(most);
     if (r >= a.m) continue;
     int8_t* codes = a.codes + r * a.stride;
     auto put = [&](int64_t c, const float (&w)[V]) {
+      const Words<V> q(code, w);
       if (c + V <= a.k) {
-        typename Piece<X>::Codes q;
+        typedef uint32_t words __attribute__((ext_vector_type(V / 4), aligned(1)));
+        words o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) q[e] = (int8_t)code_of(w[e], inverse);
-        *reinterpret_cast<typename Piece<X>::Codes*>(codes + c) = q;
+        for (int e = 0; e < V / 4; ++e) o[e] = q.w[e];
+        *reinterpret_cast<words*>(codes + c) = o;
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (c + e < a.k) codes[c + e] = (int8_t)code_of(w[e], inverse);
+          if (c + e < a.k) codes[c + e] = (int8_t)(q.w[e / 4] >> (8 * (e % 4)));
       }
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i) put((int64_t)(lane + i * LANES) * V, v[i]);
     for (int64_t c = (int64_t)(lane + HELD * LANES) * V; c < a.k; c += LANES * V) {
       float w[V];
-      load_piece<X>(x, c, a.k, w);
+      load_piece<X, V>(x, c, a.k, last, w);
       put(c, w);
     }
-    if (lane == 0) a.scales[r] = scale;
+    if (lane == 0) a.scales[r] = code.scale;
   }
 }
 
@@ -126,7 +155,7 @@ void launch_quantize(const QuantizeArgs& a, hipStream_t st) {
 
 template <typename X>
 void quantize(const QuantizeArgs& a, hipStream_t st) {
-  const int64_t pieces = ceil_div(a.k, Piece<X>::kEach);
+  const int64_t pieces = ceil_div(a.k, piece_values<X>());
   const bool spread = a.m <= 2048 && pieces > 64;
   if (!spread && pieces <= 32) launch_quantize<X, 16, 2>(a, st);
   else if (!spread && pieces <= 64) launch_quantize<X, 16, 4>(a, st);
@@ -146,42 +175,62 @@ struct LinearArgs {
   int dtype, relu, whole;                      // whole: rows of the output start at multiples of four values
 };
 
+// scales: of the tokens from row `from` on.
 template <int WN>
 struct LinearEpilogue {
   const LinearArgs& a;
+  const float* scales;
+  int64_t from;
   __device__ __forceinline__ void operator()(const float* strip, int64_t row0, int64_t col0, int lane) const {
+    if (a.dtype == F2CGT_DT_F32) put<float>(strip, row0, col0, lane);
+    else if (a.dtype == F2CGT_DT_F16) put<_Float16>(strip, row0, col0, lane);
+    else put<__bf16>(strip, row0, col0, lane);
+  }
+  template <typename T>
+  __device__ __forceinline__ void put(const float* strip, int64_t row0, int64_t col0, int lane) const {
+    typedef T four __attribute__((ext_vector_type(4)));
     constexpr int kAcross = WN / 4, kRows = kWave / kAcross;        // lanes along a row, rows at a time
     static_assert(kWave % kAcross == 0, "whole rows at a time");
-    const int c = 4 * (lane % kAcross);
+    const int c = 4 * (lane % kAcross), r0 = lane / kAcross;
     const int64_t col = col0 + c;
-    const int in = a.n - col < 4 ? (int)(a.n - col) : 4;
-    fltx4 scale = {0.f, 0.f, 0.f, 0.f}, bias = scale;
+    const int in = a.n - col < 4 ? (int)(a.n - col) : 4, rows = a.m - row0 < 32 ? (int)(a.m - row0) : 32;
+    if (in <= 0) return;
+    const float least = a.relu ? 0.f : -__builtin_inff();           // (a NaN stays one)
+    fltx4 scale, bias = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < in) {
-        scale[e] = a.w_scales[col + e];
-        if (a.bias != nullptr) bias[e] = a.bias[col + e];
-      }
+    for (int e = 0; e < 4; ++e) scale[e] = a.w_scales[e < in ? col + e : col];
+    if (a.bias != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 32 / kRows; ++i) {
-      const int r = i * kRows + lane / kAcross;
-      const int64_t row = row0 + r;
-      if (row >= a.m || in <= 0) continue;
+      for (int e = 0; e < 4; ++e) bias[e] = a.bias[e < in ? col + e : col];
+    }
+    const float* by = scales + (row0 - from);
+    T* out = static_cast<T*>(a.out) + row0 * a.n + col;
+    auto values = [&](int r) {
       const intx4 sum = *reinterpret_cast<const intx4*>(strip + r * (WN + 4) + c);
-      const float by = a.x_scales[row];
+      const float of = by[r < rows ? r : rows - 1];
       fltx4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = (float)sum[e] * (by * scale[e]);
-        if (a.bias != nullptr) v[e] += bias[e];
-        if (a.relu && v[e] <= 0.f) v[e] = 0.f;                      // (a NaN stays one)
+        v[e] = (float)sum[e] * (of * scale[e]) + bias[e];
+        v[e] = v[e] <= least ? least : v[e];
       }
-      if (a.whole) {
-        store_four(a.out, a.dtype, row * a.n + col, v);
-      } else {
+      return v;
+    };
+    if (a.whole) {
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int r = i * kRows + r0;
+        const four v = __builtin_convertvector(values(r), four);
+        if (r < rows) *reinterpret_cast<four*>(out + r * a.n) = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int r = i * kRows + r0;
+        const four v = __builtin_convertvector(values(r), four);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (e < in) store_value(a.out, a.dtype, row * a.n + col + e, v[e]);
+          if (r < rows && e < in) out[r * a.n + e] = v[e];
       }
     }
   }
@@ -194,10 +243,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void int8_l
   tile_of(place_of(blockIdx.x, gridDim.x), (uint32_t)ceil_div(a.m, BM), (uint32_t)ceil_div(a.n, BN), DEEP, i, j);
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   if constexpr (STAGES == 2) {
-    Tile::run({lds0, lds1}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});
+    Tile::run({lds0, lds1}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a, a.x_scales, 0});
   } else {
     __shared__ __attribute__((aligned(128))) char lds2[Tile::kStage], lds3[Tile::kStage];
-    Tile::run({lds0, lds1, lds2, lds3}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a});
+    Tile::run({lds0, lds1, lds2, lds3}, a.x, a.w, (int64_t)i * BM, (int64_t)j * BN, LinearEpilogue<WN>{a, a.x_scales, 0});
   }
 }
 
@@ -205,6 +254,91 @@ template <int BM, int BN, int WM, int WN, int STAGES, int GROUPS, int DEEP>
 void launch_linear(const LinearArgs& a, hipStream_t st) {
   int8_linear_kernel<BM, BN, WM, WN, STAGES, GROUPS, DEEP>
       <<<(unsigned)(ceil_div(a.m, BM) * ceil_div(a.n, BN)), (BM / WM) * (BN / WN) * GROUPS * kWave, 0, st>>>(a);
+}
+
+// ---- rows of few columns, coded where they are multiplied ------------------------------------------------------
+// Floating rows of up to 128 L columns: a workgroup codes 64 of them into LDS (16 lanes a row, as quantize_rows_kernel) while the
+// weights of its 128 outputs are copied there, and multiplies.  The codes never go through memory.
+template <typename X, int L>
+__global__ __launch_bounds__(256) void int8_rows_kernel(LinearArgs a, int64_t ld) {
+  constexpr int V = piece_values<X>(), kHeldPieces = 128 * L / (16 * V), kM = 64, kN = 128;
+  constexpr int kStripBytes = 32 * (64 + 4) * 4, kCodes = L * (kM + kN) * kLine;
+  __shared__ __attribute__((aligned(128))) char lds[kCodes > 4 * kStripBytes ? kCodes : 4 * kStripBytes];
+  __shared__ float s_scale[kM];
+  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int at = lane & 31, side = lane >> 5;
+  const uint32_t tiles = (uint32_t)ceil_div(a.n, kN), place = place_of(blockIdx.x, gridDim.x);
+  const int64_t row0 = (int64_t)(place / tiles) * kM, col0 = (int64_t)(place % tiles) * kN, k = a.w.bytes;
+  char* lds_w = lds + L * kM * kLine;
+  // weights: thread t's pieces lie sixteen rows and more apart; those behind a row's end are the row's first one (the codes are zero)
+  const int piece = ((t & 7) ^ (t >> 4 & 7)) << 4;
+#pragma unroll
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int i = 0; i < kN / 32; ++i) {
+      const int64_t r = col0 + t / 8 + 32 * i, c = l * kLine + piece;
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(a.w.base + (r < a.n ? r : a.n - 1) * a.w.stride + (c < k ? c : 0)),
+          (__attribute__((address_space(3))) void*)(lds_w + l * kN * kLine + (wave * kWave + i * 256) * 16), 16, 0, 0);
+    }
+  const int turn = lane & 15;
+  float v[4][kHeldPieces][V];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t r = row0 + 16 * wave + 4 * p + lane / 16;
+    const X* x = reinterpret_cast<const X*>(a.x.base) + (r < a.m ? r : a.m - 1) * ld;
+#pragma unroll
+    for (int i = 0; i < kHeldPieces; ++i) load_piece<X, V>(x, (turn + 16 * i) * V, k, r >= a.m - 1, v[p][i]);
+  }
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kHeldPieces; ++i) most = largest<V>(v[p][i], most);
+#pragma unroll
+    for (int by = 1; by < 16; by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
+    const RowCode code(most);
+    const int r = 16 * wave + 4 * p + lane / 16;
+    if (turn == 0) s_scale[r] = code.scale;
+#pragma unroll
+    for (int i = 0; i < kHeldPieces; ++i) {
+      const int c = (turn + 16 * i) * V;
+      Words<V> q(code, v[p][i]);
+      if (c >= k) q = Words<V>();
+      *reinterpret_cast<Words<V>*>(lds + c / kLine * kM * kLine + piece_at(r, c % kLine / 16) + c % 16) = q;
+    }
+  }
+  __syncthreads();
+  const int wi = 32 * (wave & 1), wj = 64 * (wave >> 1);
+  intx16 acc[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0;
+#pragma unroll
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const intx4 fa = *reinterpret_cast<const intx4*>(lds + l * kM * kLine + piece_at(wi + at, 2 * g + side));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const intx4 fb = *reinterpret_cast<const intx4*>(lds_w + l * kN * kLine + piece_at(wj + 32 * j + at, 2 * g + side));
+        acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb, fa, acc[j], 0, 0, 0);
+      }
+    }
+  __syncthreads();
+  float* strip = reinterpret_cast<float*>(lds + wave * kStripBytes);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      fltx4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = word_of(acc[j][4 * q + e]);
+      *reinterpret_cast<fltx4*>(strip + at * 68 + 32 * j + 8 * q + 4 * side) = o;
+    }
+  __builtin_amdgcn_wave_barrier();
+  LinearEpilogue<64>{a, s_scale, row0}(strip, row0 + wi, col0 + wj, lane);
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------
@@ -234,7 +368,8 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
   const int at = lane & 15, part = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), k = a.x.bytes;
   const int blocks = (int)ceil_div(k, 64);
-  __shared__ float s_most[WAVES], s_scale[MT * 16];
+  __shared__ uint32_t s_most[WAVES];
+  __shared__ float s_scale[MT * 16];
   __shared__ __attribute__((aligned(16))) int s_sum[WAVES][NT][MT * 16][20];
   extern __shared__ __attribute__((aligned(16))) char s_codes[];        // (floating rows: [m][fused_row(k)])
   const char* w[NT];
@@ -275,47 +410,28 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
     const int share = WAVES / (int)a.m, row = wave / share, sub = wave - row * share;
     const bool mine = row < a.m;
     const int64_t line = fused_row(k);
-    typedef X four __attribute__((ext_vector_type(4), aligned(sizeof(X))));
     const X* from = reinterpret_cast<const X*>(a.x.base) + (mine ? row : 0) * f.ld;
     float v[kHeld][4];
-    float most = 0.f;
+    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int64_t c = 4ll * (sub * kWave + lane + i * share * kWave);
-      if (c + 4 <= k) {
-        const four p = *reinterpret_cast<const four*>(from + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = (float)p[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = c + e < k ? (float)from[c + e] : 0.f;
-      }
+      load_piece<X, 4>(from, c, k, !mine || row == a.m - 1, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) most = largest<4>(v[i], most);
 #pragma unroll
-    for (int by = 1; by < kWave; by *= 2) {
-      const float o = __shfl_xor(most, by);
-      most = o > most || o != o ? o : most;
-    }
+    for (int by = 1; by < kWave; by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
     if (lane == 0) s_most[wave] = most;
     __syncthreads();
     if (mine) {
-      for (int i = 0; i < share; ++i) {
-        const float o = s_most[row * share + i];
-        most = o > most || o != o ? o : most;
-      }
-      const float scale = scale_of(most), inverse = 1.f / scale;
-      if (sub == 0 && lane == 0) s_scale[row] = scale;
+      for (int i = 0; i < share; ++i) most = larger(most, s_most[row * share + i]);
+      const RowCode code(most);
+      if (sub == 0 && lane == 0) s_scale[row] = code.scale;
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         const int64_t c = 4ll * (sub * kWave + lane + i * share * kWave);
-        if (c < line) {
-          int word = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) word |= (code_of(v[i][e], inverse) & 255) << (8 * e);
-          *reinterpret_cast<int*>(s_codes + row * line + c) = word;       // (zeros behind the row's end)
-        }
+        if (c < line) *reinterpret_cast<uint32_t*>(s_codes + row * line + c) = c < k ? code.four(v[i][0], v[i][1], v[i][2], v[i][3]) : 0u;
       }
     }
     __syncthreads();
@@ -379,6 +495,18 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
 bool fused(int64_t m, int64_t k) {
   if (m < 1 || m > 16 || m * fused_row(k) > kFusedBytes) return false;
   return ceil_div(fused_row(k), 4 * kWave * (kFusedWaves / m)) <= kHeld;
+}
+
+// Whether rows of few columns are coded where they are multiplied, once for every 128 outputs.  us, so and by two launches:
+// 1024 x 128 -> 256 6.3 and 8.6, 20 000 x 100 -> 47 9.1 and 11.1, 250 000 x 100 -> 128 51 and 57, bf16 36 and 62,
+// 250 000 x 128 -> 256 84 and 98, 30 000 x 128 -> 512 20 and 23; but 30 000 x 250 -> 512 37 and 29, 100 000 x 200 -> 1024 188 and 140.
+bool rows_fused(int64_t m, int64_t n, int64_t k) { return k <= 256 && n * ceil_div(k, kLine) <= 512 && ceil_div(m, 64) * 4 < (1ll << 24); }
+
+template <typename X>
+void launch_rows(const FewArgs& f, hipStream_t st) {
+  const unsigned grid = (unsigned)(ceil_div(f.l.m, 64) * ceil_div(f.l.n, 128));
+  if (f.l.w.bytes <= kLine) int8_rows_kernel<X, 1><<<grid, 256, 0, st>>>(f.l, f.ld);
+  else int8_rows_kernel<X, 2><<<grid, 256, 0, st>>>(f.l, f.ld);
 }
 
 template <typename X>
@@ -486,7 +614,7 @@ extern "C" int f2cgt_int8_linear(const int8_t* codes, int64_t code_stride, const
 
 // The codes of the tokens, then their scales.
 extern "C" int64_t f2cgt_quantized_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k < 0 || fused(m, k)) return 0;
+  if (m <= 0 || n <= 0 || k < 0 || fused(m, k) || rows_fused(m, n, k)) return 0;
   return m * code_row(k) + 4 * m;
 }
 
@@ -501,12 +629,19 @@ extern "C" int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, cons
   F2CGT_REQUIRE(weight_scales && out && (k == 0 || x), F2CGT_E_INVALID, "%s: null buffer", what);
   F2CGT_REQUIRE(aligned(out, type_size(dtype)) && aligned(x, type_size(dtype)), F2CGT_E_INVALID, "%s: misaligned rows", what);
   if (int rc = check_codes(what, weight, weight_stride, k, "weights")) return rc;
+  const FewArgs f{{{static_cast<const char*>(x), 0, m, k}, {reinterpret_cast<const char*>(weight), weight_stride, n, k}, nullptr,
+                   weight_scales, bias, out, m, n, dtype, relu, n % 4 == 0 && aligned(out, 4 * type_size(dtype))}, ld};
+  hipStream_t st = as_stream(stream);
   if (fused(m, k)) {
-    const FewArgs f{{{static_cast<const char*>(x), 0, m, k}, {reinterpret_cast<const char*>(weight), weight_stride, n, k}, nullptr,
-                     weight_scales, bias, out, m, n, dtype, relu, 0}, ld};
-    if (dtype == F2CGT_DT_F32) launch_fused<float>(f, as_stream(stream));
-    else if (dtype == F2CGT_DT_F16) launch_fused<_Float16>(f, as_stream(stream));
-    else launch_fused<__bf16>(f, as_stream(stream));
+    if (dtype == F2CGT_DT_F32) launch_fused<float>(f, st);
+    else if (dtype == F2CGT_DT_F16) launch_fused<_Float16>(f, st);
+    else launch_fused<__bf16>(f, st);
+    return launch_status(what);
+  }
+  if (rows_fused(m, n, k)) {
+    if (dtype == F2CGT_DT_F32) launch_rows<float>(f, st);
+    else if (dtype == F2CGT_DT_F16) launch_rows<_Float16>(f, st);
+    else launch_rows<__bf16>(f, st);
     return launch_status(what);
   }
   F2CGT_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= f2cgt_quantized_linear_workspace_bytes(m, n, k),
@@ -516,5 +651,5 @@ extern "C" int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, cons
   if (int rc = f2cgt_quantize_rows(x, dtype, ld, codes, code_row(k), scales, m, k, stream)) return rc;
   LinearArgs a{{reinterpret_cast<const char*>(codes), code_row(k), m, k}, {reinterpret_cast<const char*>(weight), weight_stride, n, k},
                scales, weight_scales, bias, out, m, n, dtype, relu, 0};
-  return linear(what, a, as_stream(stream));
+  return linear(what, a, st);
 }
