@@ -44,6 +44,7 @@ struct MuonArgs {
   char* xt[2];                                 // [count][l] lines of X^T
   char* g;                                     // [count][r] lines of G
   char* p;                                     // of P
+  float* sums;                                 // of parts of Gram products
   float a, b, c;
   // A result in bf16: its own rounding is 1.65e-3 of it (in the norm; in fp16 it is 2e-4, too little for this).  G of the hi planes alone in all steps and the last
   // product of theirs make it 1.7e-3 to 2.0e-3, and 23 of 30 instructions are left of a square matrix; G G or an earlier
@@ -266,6 +267,69 @@ __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symm
   const Lines from = SQUARE ? Lines{g, s.short_line(), s.r, s.short_line()}
                             : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line() * kLine / Op::kFrom};
   Tile::run({lds0, lds1}, from, from, row0, col0, SymmetricEpilogue<WJ>{a, SQUARE ? p : g, SQUARE ? g : nullptr, row0 != col0});
+}
+
+// G of a long X with few rows: its columns in `splits` parts for as many workgroups of a tile, whose sums of 64 x 64 go to memory...
+struct PartEpilogue {
+  float* sums;
+  __device__ __forceinline__ void operator()(float* strip, int64_t row, int64_t col, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 8, c = 4 * (lane % 8);
+      *reinterpret_cast<fltx4*>(sums + (row + r) * 64 + col + c) = *reinterpret_cast<const fltx4*>(strip + r * 36 + c);
+    }
+  }
+};
+
+template <class Op>
+__global__ __launch_bounds__(1024) void muon_gram_part_kernel(MuonArgs a, int splits) {
+  typedef TileProduct<Op, 64, 64, 32, 32, 2, 4> Tile;
+  __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
+  const Shape& s = a.s;
+  // the parts of a tile go to different XCDs, tiles of a part to the same
+  const uint32_t tiles = (uint32_t)ceil_div(s.r, 64), each = tiles * (tiles + 1) / 2, all = gridDim.x / splits, at = place_of(blockIdx.x, gridDim.x);
+  const uint32_t part = at / all, tile = at % all;
+  uint32_t i, j;
+  lower_tile_of(tile % each, tiles, 8, i, j);
+  const int64_t z = tile / each, bytes = s.long_line() * kLine / Op::kFrom, steps = ceil_div(bytes, kLine);
+  const int64_t first = steps * part / splits, end = steps * (part + 1) / splits;
+  const char* x = a.x + z * s.r * s.long_line() + first * Op::kFrom;
+  const int64_t here = (end * kLine < bytes ? end * kLine : bytes) - first * kLine;
+  const Lines row_lines{x + 64 * i * s.long_line(), s.long_line(), s.r - 64 * i, here};
+  const Lines col_lines{x + 64 * j * s.long_line(), s.long_line(), s.r - 64 * j, here};
+  Tile::run({lds0, lds1}, row_lines, col_lines, 0, 0, PartEpilogue{a.sums + ((int64_t)tile * splits + part) * 4096});
+}
+
+// ... and are added, in their order, a quarter of a tile per wave.
+__global__ __launch_bounds__(256) void muon_gram_add_kernel(MuonArgs a, int splits) {
+  __shared__ __attribute__((aligned(16))) float s_strip[4][32 * 36];
+  const Shape& s = a.s;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, wi = 32 * (wave >> 1), wj = 32 * (wave & 1);
+  const uint32_t tiles = (uint32_t)ceil_div(s.r, 64), each = tiles * (tiles + 1) / 2, tile = blockIdx.x;
+  uint32_t i, j;
+  lower_tile_of(tile % each, tiles, 8, i, j);
+  const int64_t z = tile / each;
+  const float* sums = a.sums + (int64_t)tile * splits * 4096 + wi * 64 + wj;
+  fltx4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = fltx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < splits; ++p)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += *reinterpret_cast<const fltx4*>(sums + p * 4096 + (k * 8 + lane / 8) * 64 + 4 * (lane % 8));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) *reinterpret_cast<fltx4*>(&s_strip[wave][(k * 8 + lane / 8) * 36 + 4 * (lane % 8)]) = v[k];
+  __builtin_amdgcn_wave_barrier();
+  SymmetricEpilogue<32>{a, a.g + z * s.r * s.short_line(), nullptr, i != j}(s_strip[wave], 64 * i + wi, 64 * j + wj, lane);
+}
+
+// How many parts: as many as make a workgroup per CU, of eight steps at least, where that saves more than the addition costs (4 us; a
+// step 0.28).  99 x 2721: 24 us in one part.  1 where it does not.
+int gram_splits(int64_t n, const Shape& s, bool few) {
+  const int64_t tiles = n * ceil_div(s.r, 64) * (ceil_div(s.r, 64) + 1) / 2, steps = ceil_div(s.l, few ? 64 : 32), cus = num_cus();
+  int64_t splits = cus / tiles;
+  if (splits > steps / 8) splits = steps / 8;
+  return splits >= 2 && steps - steps / splits >= 20 ? (int)splits : 1;
 }
 
 // X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  (a X from its own planes: with a in
@@ -808,7 +872,7 @@ int64_t workspace_of(int64_t count, int64_t rows, int64_t cols) {
   if (one_workgroup(s)) return 0;
   const int64_t n = group_of(count, rows, cols);
   return whole(n * parts_of(rows, cols) * 8) + whole(n * s.r * s.long_line()) + 2 * whole(n * s.l * s.short_line()) +
-         2 * whole(n * s.r * s.short_line());
+         2 * whole(n * s.r * s.short_line()) + (int64_t)num_cus() * 4096 * 4;
 }
 
 int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int steps, const float* coefficients) {
@@ -851,6 +915,7 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
   a.xt[1] = take(group * s.l * s.short_line());
   a.g = take(group * s.r * s.short_line());
   a.p = take(group * s.r * s.short_line());
+  a.sums = reinterpret_cast<float*>(take((int64_t)num_cus() * 4096 * 4));
   for (int64_t first = 0; first < count; first += group) {
     const int64_t n = count - first < group ? count - first : group;
     a.whole = cols % 4 == 0;
@@ -864,10 +929,18 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
       if (int rc = launch_status(what)) return rc;
       continue;
     }
+    const int splits = gram_splits(n, s, a.few());
     muon_norm_kernel<<<dim3((unsigned)a.parts, (unsigned)n), 256, 0, st>>>(a);
     muon_split_kernel<<<dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64), (unsigned)n), 256, 0, st>>>(a);
     for (int step = 0; step < steps; ++step) {
-      symmetric(a, n, false, st);
+      if (splits > 1) {
+        const unsigned tiles = (unsigned)(n * ceil_div(s.r, 64) * (ceil_div(s.r, 64) + 1) / 2);
+        if (a.few()) muon_gram_part_kernel<HiOp><<<tiles * splits, 1024, 0, st>>>(a, splits);
+        else muon_gram_part_kernel<SplitOp><<<tiles * splits, 1024, 0, st>>>(a, splits);
+        muon_gram_add_kernel<<<tiles, 256, 0, st>>>(a, splits);
+      } else {
+        symmetric(a, n, false, st);
+      }
       symmetric(a, n, true, st);
       update(a, n, step & 1, step == steps - 1, st);
     }
