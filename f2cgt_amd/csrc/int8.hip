@@ -48,32 +48,32 @@ constexpr int piece_values() { return 16 / sizeof(X); }
 // for those behind the row's end, but for a piece that begins there others of the row.  `last`: behind this row is
 // nothing that may be read.  One load without a branch around it, so that a caller's loads are under way together.
 template <typename X, int V>
-__device__ __forceinline__ void load_piece(const X* row, int64_t c, int64_t k, bool last, float (&v)[V]) {
+__device__ __forceinline__ void load_piece(const X* row, int64_t c, int64_t k, bool last, X (&v)[V]) {
   typedef X values __attribute__((ext_vector_type(V), aligned(sizeof(X))));
   if (k < V) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = c + e < k ? (float)row[c + e] : 0.f;
+    for (int e = 0; e < V; ++e) v[e] = c + e < k ? row[c + e] : (X)0.f;
     return;
   }
   const int64_t from = c < k ? c : 0;
   const bool over = last && from + V > k;
   const values p = *reinterpret_cast<const values*>(row + (over ? k - V : from));
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = (float)p[e];
+  for (int e = 0; e < V; ++e) v[e] = p[e];
   if (k % V != 0) {
     if (over) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = from + e < k ? (float)row[from + e] : 0.f;
+      for (int e = 0; e < V; ++e) v[e] = from + e < k ? row[from + e] : (X)0.f;
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = from + e < k ? v[e] : 0.f;
+    for (int e = 0; e < V; ++e) v[e] = from + e < k ? v[e] : (X)0.f;
   }
 }
 
-template <int V>
-__device__ __forceinline__ uint32_t largest(const float (&v)[V], uint32_t most) {
+template <typename X, int V>
+__device__ __forceinline__ uint32_t largest(const X (&v)[V], uint32_t most) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) most = larger(most, magnitude(v[e]));
+  for (int e = 0; e < V; ++e) most = larger(most, magnitude((float)v[e]));
   return most;
 }
 
@@ -82,9 +82,10 @@ template <int V>
 struct Words {
   uint32_t w[V / 4] = {};
   __device__ __forceinline__ Words() {}
-  __device__ __forceinline__ Words(const RowCode& code, const float (&v)[V]) {
+  template <typename X>
+  __device__ __forceinline__ Words(const RowCode& code, const X (&v)[V]) {
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) w[i] = code.four(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    for (int i = 0; i < V / 4; ++i) w[i] = code.four((float)v[4 * i], (float)v[4 * i + 1], (float)v[4 * i + 2], (float)v[4 * i + 3]);
   }
 };
 
@@ -99,16 +100,19 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
     const int64_t r = r0 + t / LANES, rr = r < a.m ? r : a.m - 1;
     const bool last = rr == a.m - 1;
     const X* x = static_cast<const X*>(a.x) + rr * a.ld;
-    float v[HELD][V];
+    X v[HELD][V];
     uint32_t most = 0;
+    auto any = [&](int i) { return i == 0 || i * LANES * V < a.k; };         // (for all lanes)
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) load_piece<X, V>(x, (int64_t)(lane + i * LANES) * V, a.k, last, v[i]);
+    for (int i = 0; i < HELD; ++i)
+      if (any(i)) load_piece<X, V>(x, (int64_t)(lane + i * LANES) * V, a.k, last, v[i]);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) most = largest<V>(v[i], most);
+    for (int i = 0; i < HELD; ++i)
+      if (any(i)) most = largest(v[i], most);
     for (int64_t c = (int64_t)(lane + HELD * LANES) * V; c < a.k; c += LANES * V) {
-      float w[V];
+      X w[V];
       load_piece<X, V>(x, c, a.k, last, w);
-      most = largest<V>(w, most);
+      most = largest(w, most);
     }
 #pragma unroll
     for (int by = 1; by < (LANES < kWave ? LANES : kWave); by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
@@ -122,7 +126,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
     const RowCode code(most);
     if (r >= a.m) continue;
     int8_t* codes = a.codes + r * a.stride;
-    auto put = [&](int64_t c, const float (&w)[V]) {
+    auto put = [&](int64_t c, const X (&w)[V]) {
       const Words<V> q(code, w);
       if (c + V <= a.k) {
         typedef uint32_t words __attribute__((ext_vector_type(V / 4), aligned(1)));
@@ -137,9 +141,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
       }
     };
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) put((int64_t)(lane + i * LANES) * V, v[i]);
+    for (int i = 0; i < HELD; ++i)
+      if (any(i)) put((int64_t)(lane + i * LANES) * V, v[i]);
     for (int64_t c = (int64_t)(lane + HELD * LANES) * V; c < a.k; c += LANES * V) {
-      float w[V];
+      X w[V];
       load_piece<X, V>(x, c, a.k, last, w);
       put(c, w);
     }
@@ -153,16 +158,20 @@ void launch_quantize(const QuantizeArgs& a, hipStream_t st) {
   quantize_rows_kernel<X, LANES, HELD><<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 256, 0, st>>>(a);
 }
 
+// As few lanes a row as hold it, but enough waves.  us at 250 000 x 128 fp32 by 16 lanes 25 (6.4 TB/s), by 64 68; 60 000 x 602 by 16 34, by 64 36;
+// 16 384 x 1024 by 64 13.5, by 16 22; 4099 x 4096 by 256 14, by 64 22; 4096 x 602 by 64 4.8, by 16 5.9; 33 rows of 4096 by 256 3.8,
+// by 64 7.3.  Rows of 16 bits, eight values a piece, hold less: the instructions of pieces that are not there, or not whole, cost more than
+// reading those beyond again (60 000 x 602 by 16 lanes 25, eight pieces held 36; 4099 x 4096 by 64 10.9, by 256 11.2, four held 17;
+// 16 384 x 8192 by 256 80, by 64 106).
 template <typename X>
 void quantize(const QuantizeArgs& a, hipStream_t st) {
+  constexpr bool kWide = sizeof(X) == 4;
   const int64_t pieces = ceil_div(a.k, piece_values<X>());
-  const bool spread = a.m <= 2048 && pieces > 64;
-  if (!spread && pieces <= 32) launch_quantize<X, 16, 2>(a, st);
-  else if (!spread && pieces <= 64) launch_quantize<X, 16, 4>(a, st);
-  else if (!spread && pieces <= 256) launch_quantize<X, 64, 4>(a, st);
-  else if (!spread && pieces <= 512) launch_quantize<X, 64, 8>(a, st);
-  else if (pieces <= 512) launch_quantize<X, 256, 2>(a, st);
-  else launch_quantize<X, 256, 8>(a, st);
+  if (pieces <= 32) launch_quantize<X, 16, 2>(a, st);
+  else if (pieces <= 128 && a.m > 8192) launch_quantize<X, 16, kWide ? 8 : 2>(a, st);
+  else if (pieces <= (kWide ? 256 : 512) && (pieces <= 128 || a.m > 1024)) launch_quantize<X, 64, kWide ? 4 : 2>(a, st);
+  else if (pieces <= 1024) launch_quantize<X, 256, kWide ? 4 : 2>(a, st);
+  else launch_quantize<X, 256, kWide ? 8 : 2>(a, st);
 }
 
 struct LinearArgs {
@@ -282,7 +291,7 @@ __global__ __launch_bounds__(256) void int8_rows_kernel(LinearArgs a, int64_t ld
           (__attribute__((address_space(3))) void*)(lds_w + l * kN * kLine + (wave * kWave + i * 256) * 16), 16, 0, 0);
     }
   const int turn = lane & 15;
-  float v[4][kHeldPieces][V];
+  X v[4][kHeldPieces][V];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int64_t r = row0 + 16 * wave + 4 * p + lane / 16;
@@ -294,7 +303,7 @@ __global__ __launch_bounds__(256) void int8_rows_kernel(LinearArgs a, int64_t ld
   for (int p = 0; p < 4; ++p) {
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < kHeldPieces; ++i) most = largest<V>(v[p][i], most);
+    for (int i = 0; i < kHeldPieces; ++i) most = largest(v[p][i], most);
 #pragma unroll
     for (int by = 1; by < 16; by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
     const RowCode code(most);
@@ -402,24 +411,30 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
       for (int i = 0; i < MT; ++i) next_x[u][i] = *reinterpret_cast<const intx4*>(x[i] + (c < k ? c : 0));
     }
   };
-  if (blocks > 0) load_w(wave);
   if constexpr (kCoded) {
-    if (blocks > 0) load_x(wave);
+    if (blocks > 0) {
+      load_w(wave);
+      load_x(wave);
+    }
   } else {
     // waves in a row's share: `share`; this one is number `sub` of row `row`
     const int share = WAVES / (int)a.m, row = wave / share, sub = wave - row * share;
     const bool mine = row < a.m;
     const int64_t line = fused_row(k);
     const X* from = reinterpret_cast<const X*>(a.x.base) + (mine ? row : 0) * f.ld;
-    float v[kHeld][4];
+    X v[kHeld][4];
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const int64_t c = 4ll * (sub * kWave + lane + i * share * kWave);
-      load_piece<X, 4>(from, c, k, !mine || row == a.m - 1, v[i]);
+      if (i == 0 || 4ll * i * share * kWave < line) load_piece<X, 4>(from, c, k, !mine || row == a.m - 1, v[i]);
+      else v[i][0] = v[i][1] = v[i][2] = v[i][3] = (X)0.f;
     }
+    __builtin_amdgcn_sched_barrier(0);           // (loads come back in their order: the tokens before the weights)
+    if (blocks > 0) load_w(wave);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) most = largest<4>(v[i], most);
+    for (int i = 0; i < kHeld; ++i) most = largest(v[i], most);
 #pragma unroll
     for (int by = 1; by < kWave; by *= 2) most = larger(most, (uint32_t)__shfl_xor((int)most, by));
     if (lane == 0) s_most[wave] = most;
@@ -431,7 +446,7 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         const int64_t c = 4ll * (sub * kWave + lane + i * share * kWave);
-        if (c < line) *reinterpret_cast<uint32_t*>(s_codes + row * line + c) = c < k ? code.four(v[i][0], v[i][1], v[i][2], v[i][3]) : 0u;
+        if (c < line) *reinterpret_cast<uint32_t*>(s_codes + row * line + c) = c < k ? code.four((float)v[i][0], (float)v[i][1], (float)v[i][2], (float)v[i][3]) : 0u;
       }
     }
     __syncthreads();
@@ -491,9 +506,10 @@ __global__ __launch_bounds__(WAVES * kWave) void int8_few_kernel(FewArgs f) {
   }
 }
 
-// Whether floating rows are coded by the product's own workgroups.
-bool fused(int64_t m, int64_t k) {
-  if (m < 1 || m > 16 || m * fused_row(k) > kFusedBytes) return false;
+// Whether floating rows are coded by the product's own workgroups.  us, so and by two launches: 1 x 4096 -> 4096 7.2 and 9.1,
+// 8 x 4096 -> 4096 9.1 and 9.8, 16 x 1000 -> 300 6.1 and 8.1; but 1 x 4096 -> 16384 23 and 18.6 (a thousand workgroups code).
+bool fused(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || m > 16 || n >= 8192 || m * fused_row(k) > kFusedBytes) return false;
   return ceil_div(fused_row(k), 4 * kWave * (kFusedWaves / m)) <= kHeld;
 }
 
@@ -554,6 +570,23 @@ int linear(const char* what, LinearArgs a, hipStream_t st) {
   }
   a.whole = n % 4 == 0 && aligned(a.out, 4 * type_size(a.dtype));
   F2CGT_REQUIRE(ceil_div(m, 64) * ceil_div(n, 64) < (1ll << 24), F2CGT_E_UNSUPPORTED, "%s: too many tiles", what);
+  // A few rows behind the last whole 128: where they begin another round of tiles, they go to the kernel for few tokens
+  // (4099 x 4096 -> 4096: 96 us in one launch, 75 in two).  A step of a round of tiles is 0.7 us, that kernel reads 4e6 codes a us.
+  const int64_t rest = m % 128;
+  if (rest > 0 && rest <= 16 && m > 128) {
+    auto rounds = [&](int64_t rows) { return ceil_div(ceil_div(rows, 128) * ceil_div(n, 128), cus); };
+    if (rounds(m) > rounds(m - rest) && ceil_div(k, kLine) * 0.7 > 4. + n * k / 4e6) {
+      LinearArgs tail = a;
+      const int64_t done = m - rest;
+      tail.x.base += done * a.x.stride;
+      tail.x.rows = tail.m = rest;
+      tail.x_scales += done;
+      tail.out = static_cast<char*>(a.out) + done * n * type_size(a.dtype);
+      a.x.rows = a.m = done;
+      if (int rc = linear(what, tail, st)) return rc;
+      return linear(what, a, st);
+    }
+  }
   const int64_t large = ceil_div(m, 256) * ceil_div(n, 256), middle = ceil_div(m, 128) * ceil_div(n, 128);
   const int64_t small = ceil_div(m, 64) * ceil_div(n, 128);
   // a round of large tiles is as long as 3.5 rounds of middle ones
@@ -614,7 +647,7 @@ extern "C" int f2cgt_int8_linear(const int8_t* codes, int64_t code_stride, const
 
 // The codes of the tokens, then their scales.
 extern "C" int64_t f2cgt_quantized_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k < 0 || fused(m, k) || rows_fused(m, n, k)) return 0;
+  if (m <= 0 || n <= 0 || k < 0 || fused(m, n, k) || rows_fused(m, n, k)) return 0;
   return m * code_row(k) + 4 * m;
 }
 
@@ -632,7 +665,7 @@ extern "C" int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, cons
   const FewArgs f{{{static_cast<const char*>(x), 0, m, k}, {reinterpret_cast<const char*>(weight), weight_stride, n, k}, nullptr,
                    weight_scales, bias, out, m, n, dtype, relu, n % 4 == 0 && aligned(out, 4 * type_size(dtype))}, ld};
   hipStream_t st = as_stream(stream);
-  if (fused(m, k)) {
+  if (fused(m, n, k)) {
     if (dtype == F2CGT_DT_F32) launch_fused<float>(f, st);
     else if (dtype == F2CGT_DT_F16) launch_fused<_Float16>(f, st);
     else launch_fused<__bf16>(f, st);

@@ -683,9 +683,9 @@ __device__ __forceinline__ void put_four(char* lds, int line, int piece, int hal
   *reinterpret_cast<halfx4*>(lds + piece_at(line, piece + 4) + 8 * half) = lo;
 }
 
-// From 33 to 32 RT rows: products of planes.  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
+// From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
 // P's, of 32 RT rows by RT column tiles each, in the same place.
-template <int RT, int S>
+template <int RT, int S, bool FEW>
 __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a, int steps) {
   constexpr int kRows = 32 * RT, kTile = kRows * kLine;    // a column tile
   constexpr int kTiles = S * kOneWaves > 2 * RT ? S * kOneWaves : 2 * RT;
@@ -703,7 +703,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   const int i0 = wave / 2, j0 = (wave & 1) * TJ;
   const bool squares = i0 < RT;
   // rows i of a times rows j of b, column tiles [0, n)
-  auto product = [&](const char* of, int n, int at, int side, fltx16 (&sum)[TJ]) {
+  auto product = [&](const char* of, int n, int at, int side, bool hi, fltx16 (&sum)[TJ]) {
 #pragma unroll
     for (int j = 0; j < TJ; ++j)
 #pragma unroll
@@ -715,6 +715,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
         intx4 fa[2], fb[TJ][2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
+          if (hi && p == 1) break;
           fa[p] = *reinterpret_cast<const intx4*>(tile + piece_at(32 * i0 + at, 4 * p + 2 * g + side));
 #pragma unroll
           for (int j = 0; j < TJ; ++j) {
@@ -723,9 +724,11 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
           }
         }
 #pragma unroll
-        for (int m = 0; m < SplitOp::kTerms; ++m)
+        for (int m = 0; m < SplitOp::kTerms; ++m) {
+          if (hi && m < SplitOp::kTerms - 1) continue;       // (the last term is the one of both hi planes)
 #pragma unroll
           for (int j = 0; j < TJ; ++j) SplitOp::mma(sum[j], m, fa, fb[j]);
+        }
       }
     }
   };
@@ -746,13 +749,13 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
             const _Float16 hi = (_Float16)x[s][i][v], lo = (_Float16)(x[s][i][v] - (float)hi);
             const int row = 32 * i + tile_row(v, side);
             *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, at / 8) + 2 * (at % 8)) = hi;
-            *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, 4 + at / 8) + 2 * (at % 8)) = lo;
+            if (!FEW) *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, 4 + at / 8) + 2 * (at % 8)) = lo;
           }
       }
     }
     __syncthreads();
     fltx16 sum[TJ];
-    if (squares) product(lds, columns, at, side, sum);
+    if (squares) product(lds, columns, at, side, FEW, sum);
     __syncthreads();
     // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
     if (squares) {
@@ -768,7 +771,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     }
     __syncthreads();
     if (squares) {
-      product(gl, RT, at, side, sum);
+      product(gl, RT, at, side, false, sum);
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
         if (j0 + j < RT) {
@@ -834,15 +837,21 @@ bool one_workgroup(const Shape& m) {
   return (rt <= 2 && s <= 2) || (rt <= 4 && s == 1);
 }
 
+template <int RT, int S>
+void launch_one(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
+  if (a.few()) muon_one_kernel<RT, S, true><<<(unsigned)n, kOneWaves * kWave, 0, st>>>(a, steps);
+  else muon_one_kernel<RT, S, false><<<(unsigned)n, kOneWaves * kWave, 0, st>>>(a, steps);
+}
+
 bool one_launch(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
   const int64_t rt = ceil_div(a.s.r, 32), s = ceil_div(ceil_div(a.s.l, 32), kOneWaves);
   const unsigned grid = (unsigned)n, block = kOneWaves * kWave;
   if (rt == 1 && s == 1) muon_narrow_kernel<1><<<grid, block, 0, st>>>(a, steps);
   else if (rt == 1 && s == 2) muon_narrow_kernel<2><<<grid, block, 0, st>>>(a, steps);
-  else if (rt == 2 && s == 1) muon_one_kernel<2, 1><<<grid, block, 0, st>>>(a, steps);
-  else if (rt == 2 && s == 2) muon_one_kernel<2, 2><<<grid, block, 0, st>>>(a, steps);
-  else if (rt == 3 && s == 1) muon_one_kernel<3, 1><<<grid, block, 0, st>>>(a, steps);
-  else if (rt == 4 && s == 1) muon_one_kernel<4, 1><<<grid, block, 0, st>>>(a, steps);
+  else if (rt == 2 && s == 1) launch_one<2, 1>(a, n, steps, st);
+  else if (rt == 2 && s == 2) launch_one<2, 2>(a, n, steps, st);
+  else if (rt == 3 && s == 1) launch_one<3, 1>(a, n, steps, st);
+  else if (rt == 4 && s == 1) launch_one<4, 1>(a, n, steps, st);
   else return false;
   return true;
 }
