@@ -1224,8 +1224,10 @@ torch::Tensor room_for_codes(int64_t rows, int64_t k, const torch::Tensor& like)
 torch::Tensor code_rows(const torch::Tensor& codes, const char* name) {
   TORCH_CHECK(codes.defined() && codes.device().is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == torch::kInt8, name, " must be int8 [rows, columns]");
-  const int64_t step = codes.stride(0);
-  if ((codes.size(1) <= 1 || codes.stride(1) == 1) && step % 16 == 0 && step >= codes.size(1) &&
+  const int64_t step = codes.stride(0), whole = (codes.size(1) + 15) / 16 * 16;
+  // (the kernels read whole pieces, the last row's last one too)
+  const bool inside = codes.size(0) == 0 || codes.storage_offset() + (codes.size(0) - 1) * step + whole <= (int64_t)codes.storage().nbytes();
+  if ((codes.size(1) <= 1 || codes.stride(1) == 1) && step % 16 == 0 && step >= codes.size(1) && step < (1 << 23) && inside &&
       reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0)
     return codes;
   auto room = room_for_codes(codes.size(0), codes.size(1), codes);

@@ -516,7 +516,7 @@ bool fused(int64_t m, int64_t n, int64_t k) {
 // Whether rows of few columns are coded where they are multiplied, once for every 128 outputs.  us, so and by two launches:
 // 1024 x 128 -> 256 6.3 and 8.6, 20 000 x 100 -> 47 9.1 and 11.1, 250 000 x 100 -> 128 51 and 57, bf16 36 and 62,
 // 250 000 x 128 -> 256 84 and 98, 30 000 x 128 -> 512 20 and 23; but 30 000 x 250 -> 512 37 and 29, 100 000 x 200 -> 1024 188 and 140.
-bool rows_fused(int64_t m, int64_t n, int64_t k) { return k <= 256 && n * ceil_div(k, kLine) <= 512 && ceil_div(m, 64) * 4 < (1ll << 24); }
+bool rows_fused(int64_t m, int64_t n, int64_t k) { return k <= 256 && n * ceil_div(k, kLine) <= 512 && ceil_div(m, 64) * ceil_div(n, 128) < (1ll << 24); }
 
 template <typename X>
 void launch_rows(const FewArgs& f, hipStream_t st) {
@@ -569,7 +569,6 @@ int linear(const char* what, LinearArgs a, hipStream_t st) {
     return launch_status(what);
   }
   a.whole = n % 4 == 0 && aligned(a.out, 4 * type_size(a.dtype));
-  F2CGT_REQUIRE(ceil_div(m, 64) * ceil_div(n, 64) < (1ll << 24), F2CGT_E_UNSUPPORTED, "%s: too many tiles", what);
   // A few rows behind the last whole 128: where they begin another round of tiles, they go to the kernel for few tokens
   // (4099 x 4096 -> 4096: 96 us in one launch, 75 in two).  A step of a round of tiles is 0.7 us, that kernel reads 4e6 codes a us.
   const int64_t rest = m % 128;
@@ -589,6 +588,7 @@ int linear(const char* what, LinearArgs a, hipStream_t st) {
   }
   const int64_t large = ceil_div(m, 256) * ceil_div(n, 256), middle = ceil_div(m, 128) * ceil_div(n, 128);
   const int64_t small = ceil_div(m, 64) * ceil_div(n, 128);
+  F2CGT_REQUIRE(middle < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many tiles", what);     // (a launch has 2^32 threads at most)
   // a round of large tiles is as long as 3.5 rounds of middle ones
   if (k >= 1024 && large >= cus && 7 * ceil_div(large, cus) * cus <= 2 * middle) launch_linear<256, 256, 128, 64, 2, 1, 4>(a, st);
   else if (2 * middle >= 3 * cus) launch_linear<128, 128, 64, 32, 2, 1, 8>(a, st);
@@ -601,8 +601,8 @@ int linear(const char* what, LinearArgs a, hipStream_t st) {
 int check_codes(const char* what, const int8_t* codes, int64_t stride, int64_t k, const char* name) {
   if (k == 0) return 0;
   F2CGT_REQUIRE(codes != nullptr, F2CGT_E_INVALID, "%s: null buffer", what);
-  F2CGT_REQUIRE(stride % 16 == 0 && stride >= k && aligned(codes, 16), F2CGT_E_UNSUPPORTED,
-                "%s: rows of %s must start at multiples of 16 bytes and not overlap", what, name);
+  F2CGT_REQUIRE(stride % 16 == 0 && stride >= k && stride < (1ll << 23) && aligned(codes, 16), F2CGT_E_UNSUPPORTED,
+                "%s: rows of %s must start at multiples of 16 bytes, less than 2^23 apart, and not overlap", what, name);
   return 0;
 }
 

@@ -399,8 +399,9 @@ int f2cgt_sage_linear_ahead(int64_t m, int64_t n, int64_t k0, int64_t k1);
  *
  * f2cgt_int8_linear: out [m, n] (dense, out_dtype) = (codes weight^T) * (scales_i weight_scales_j) + bias_j, through
  * max(., 0) where relu is nonzero (a NaN stays one); weight int8 [n, k], bias fp32 [n] or NULL.  The sums are exact whole
- * numbers; k <= 131071.  Rows of codes and of weights start at multiples of 16 bytes (buffers and strides); what lies
- * between a row's k bytes and the next row is not used.  No columns: the bias alone.
+ * numbers; k <= 131071.  Rows of codes and of weights start at multiples of 16 bytes (buffers and strides, which are below 2^23);
+ * what lies behind a row's k bytes does not matter, but the 16-byte piece with its last one must be readable, the last row's
+ * too.  No columns: the bias alone.
  *
  * f2cgt_quantized_linear: f2cgt_quantize_rows and f2cgt_int8_linear in one call, out of x's type; a row of x that holds
  * a NaN or an infinity gives a row of NaN.  workspace: f2cgt_quantized_linear_workspace_bytes, 16-byte aligned, contents

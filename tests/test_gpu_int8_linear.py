@@ -94,6 +94,11 @@ def test_layouts_of_codes():
     for other in (packed, columns, shifted, twice[::2, :50]):
         assert torch.equal(lib.int8_linear(other, scales, weight, weight_scales), want)
     assert torch.equal(lib.int8_linear(codes, scales, weight.clone(memory_format=torch.contiguous_format), weight_scales), want)
+    ends = torch.zeros(36 * 64 + 50, dtype=torch.int8, device="cuda").as_strided((37, 50), (64, 1))      # nothing behind its last row
+    apart = torch.zeros(36 * (1 << 23) + 64, dtype=torch.int8, device="cuda").as_strided((37, 50), (1 << 23, 1))
+    for other in (ends, apart):
+        other.copy_(codes)
+        assert torch.equal(lib.int8_linear(other, scales, weight, weight_scales), want)
     same = codes[:1].expand(37, 50)                                     # one row again and again
     assert torch.equal(lib.int8_linear(same, scales, weight, weight_scales),
                        lib.int8_linear(same.contiguous(), scales, weight, weight_scales))

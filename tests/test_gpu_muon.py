@@ -49,7 +49,8 @@ def _check(got, u, dtype, steps=5, coefficients=COEFFICIENTS):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 40), (16, 16), (31, 33), (32, 32), (33, 31), (47, 256), (64, 64), (65, 65), (64, 200), (100, 128),
-          (128, 128), (128, 256), (256, 128), (129, 130), (200, 77), (256, 256), (300, 1000), (1000, 70), (513, 511), (600, 600)]
+          (128, 128), (128, 256), (256, 128), (129, 130), (200, 77), (256, 256), (300, 1000), (1000, 70), (513, 511), (600, 600),
+          (20, 4000), (99, 2721), (2100, 64), (200, 1800)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
@@ -181,6 +182,26 @@ def test_layouts_of_lists_and_versions():
     with pytest.raises(RuntimeError):                                   # the weight that was kept has changed since
         product.backward()
     lib.muon_step([], [], [], 0.1)
+
+
+@pytest.mark.parametrize("rows,cols", [(30, 40), (100, 128), (70, 3000), (300, 500)])
+def test_replayed_in_a_graph(rows, cols):
+    lib = f2cgt_amd.load()
+    g = _gen(rows)
+    w, d, v = (torch.randn((rows, cols), generator=g, device="cuda") for _ in range(3))
+    lib.muon_step([w], [d], [v], 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lib.muon_step([w], [d], [v], 0.1)
+    for _ in range(3):
+        d.copy_(torch.randn((rows, cols), generator=g, device="cuda"))
+        want_w, want_v = w.clone(), v.clone()
+        lib.muon_step([want_w], [d], [want_v], 0.1)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, want_w) and torch.equal(v, want_v)
 
 
 def test_what_is_refused():
