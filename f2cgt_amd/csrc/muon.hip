@@ -81,8 +81,10 @@ __device__ __forceinline__ fltx4 load_up_to_four(const void* p, int dtype, int64
 }
 
 // Momenta, and the sum of squares of the updates by parts, in 64 bits (a square of an fp32 number may be none).
+template <bool HELD>
 __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
-  constexpr int U = 4;
+  typedef fltx4 unaligned4 __attribute__((aligned(4)));
+  constexpr int U = HELD ? 4 : 8;
   const int64_t count = a.s.rows * a.s.cols, z = blockIdx.y, step = (int64_t)gridDim.x * 1024;
   const void* u = a.at.u[z];
   float* held = a.at.held[z];
@@ -92,20 +94,27 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       v[k] = load_up_to_four(u, a.u_dtype, i0 + k * step, count);
-      if (held != nullptr) h[k] = load_up_to_four<float>(held, i0 + k * step, count);
+      if (HELD) h[k] = load_up_to_four<float>(held, i0 + k * step, count);
     }
 #pragma unroll
-    for (int k = 0; k < U; ++k)
+    for (int k = 0; k < U; ++k) {
+      if (HELD) {
+        const int64_t i = i0 + k * step;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (held != nullptr) {
-          h[k][e] = a.momentum * h[k][e] + (1.f - a.momentum) * v[k][e];
-          const int64_t i = i0 + k * step + e;
-          if (i < count) held[i] = h[k][e];
-          v[k][e] = update_of(a, v[k][e], h[k][e]);
+        for (int e = 0; e < 4; ++e) h[k][e] = a.momentum * h[k][e] + (1.f - a.momentum) * v[k][e];
+        if (i + 4 <= count) {
+          *reinterpret_cast<unaligned4*>(held + i) = h[k];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < count) held[i + e] = h[k][e];
         }
-        sum += (double)v[k][e] * (double)v[k][e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = update_of(a, v[k][e], h[k][e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += (double)v[k][e] * (double)v[k][e];
+    }
   }
   __shared__ double s_sum[4];
 #pragma unroll
@@ -939,7 +948,9 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
       continue;
     }
     const int splits = gram_splits(n, s, a.few());
-    muon_norm_kernel<<<dim3((unsigned)a.parts, (unsigned)n), 256, 0, st>>>(a);
+    const dim3 parts((unsigned)a.parts, (unsigned)n);
+    if (held != nullptr) muon_norm_kernel<true><<<parts, 256, 0, st>>>(a);
+    else muon_norm_kernel<false><<<parts, 256, 0, st>>>(a);
     muon_split_kernel<<<dim3((unsigned)ceil_div(rows, 64), (unsigned)ceil_div(cols, 64), (unsigned)n), 256, 0, st>>>(a);
     for (int step = 0; step < steps; ++step) {
       if (splits > 1) {
