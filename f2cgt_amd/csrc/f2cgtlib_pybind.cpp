@@ -1209,7 +1209,9 @@ void undifferentiated(const torch::Tensor& t, const char* op) {
 torch::Tensor value_rows(const torch::Tensor& x, const char* name) {
   TORCH_CHECK(x.defined() && x.device().is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(x.dim() >= 1, name, " must have rows");
-  auto rows = x.dim() == 2 ? x : x.reshape({x.size(-1) ? x.numel() / x.size(-1) : x.numel(), x.size(-1)});
+  int64_t count = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) count *= x.size(d);
+  auto rows = x.dim() == 2 ? x : x.reshape({count, x.size(-1)});
   const bool plain = (rows.size(1) <= 1 || rows.stride(1) == 1) && (rows.size(0) <= 1 || rows.stride(0) >= rows.size(1));
   return plain ? rows : rows.contiguous();
 }

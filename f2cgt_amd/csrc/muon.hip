@@ -80,7 +80,8 @@ __device__ __forceinline__ fltx4 load_up_to_four(const void* p, int dtype, int64
   return load_up_to_four<__bf16>(p, i, end);
 }
 
-// Momenta, and the sum of squares of the updates by parts, in 64 bits (a square of an fp32 number may be none).
+// Momenta, and the sum of squares of the updates by parts, in 64 bits (a square of an fp32 number may be none).  Bound by memory:
+// four bf16 gradients of 2048 x 512 and their momenta, 42 MB, 9.1 us (4.6 TB/s).
 template <bool HELD>
 __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
   typedef fltx4 unaligned4 __attribute__((aligned(4)));
@@ -143,7 +144,8 @@ __device__ __forceinline__ void put_eight(char* row, int64_t c, const float (&v)
   *reinterpret_cast<halfx8*>(line + 64) = lo;
 }
 
-// The update of length kScale in planes, both ways round: a 64 x 64 tile of the caller's matrix per workgroup.
+// The update of length kScale in planes, both ways round: a 64 x 64 tile of the caller's matrix per workgroup.  Bound by memory, at
+// 4096 x 4096 in bf16 168 MB in 34 to 41 us, and by a launch and two round trips at 1000 x 2051 (9.8 us).
 __global__ __launch_bounds__(256) void muon_split_kernel(MuonArgs a) {
   __shared__ double s_sum[4];
   __shared__ float s_tile[64][65];
@@ -228,6 +230,9 @@ __device__ __forceinline__ void strip_passes(float* strip, int64_t row0, int64_t
 }
 
 // G from X, or P = b G + c G G from G (g not null): the tiles on and below the diagonal, each written on both sides of it.
+// At 4096 x 4096, where the card's power bounds them, G of hi planes takes 88 us, P of both planes 180: 0.78 and 1.15e15 executed
+// operations a second.  At 1000 x 2051 there are 136 tiles of 64 x 64 for 256 CUs, each of whose LDS is read and written for
+// most of the time (19.5 and 10.5 us); larger tiles leave more of the chip without one, and a third or fourth stage gained nothing.
 template <int WN>
 struct SymmetricEpilogue {
   const MuonArgs& a;
@@ -341,7 +346,8 @@ int gram_splits(int64_t n, const Shape& s, bool few) {
   return splits >= 2 && steps - steps / splits >= 20 ? (int)splits : 1;
 }
 
-// X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  (a X from its own planes: with a in
+// X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  At 4096 x 4096 300 us, 1.37e15 executed
+// operations a second, what the library's fp16 product of 8192 x 8192 x 8192 reaches when it runs as long (1.32e15); 22 us at 1000 x 2051.  (a X from its own planes: with a in
 // P's diagonal, which is rounded to 22 bits there, errors were half as much again.)
 template <int WN>
 struct UpdateEpilogue {
@@ -692,6 +698,10 @@ __device__ __forceinline__ void put_four(char* lds, int line, int piece, int hal
   *reinterpret_cast<halfx4*>(lds + piece_at(line, piece + 4) + 8 * half) = lo;
 }
 
+// 48 of 128 x 128 in bf16 47 us, two of 256 x 128 in fp32 83: a CU's matrix instructions are busy for 29 % of it, the rest is
+// reads and writes of LDS and the waits between three products a step that need each other.  Tiles over the whole chip would
+// be seventeen launches, 4 us and more each.
+//
 // From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
 // P's, of 32 RT rows by RT column tiles each, in the same place.
 template <int RT, int S, bool FEW>

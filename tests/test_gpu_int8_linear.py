@@ -272,3 +272,14 @@ def test_layer_of_eight_bits():
         half = served.half()
         assert half.weight_scales.dtype == torch.float32 and torch.equal(half(x), got)
         assert half(x.bfloat16()).dtype == torch.bfloat16
+
+
+def test_leading_dimensions_without_columns():
+    lib = f2cgt_amd.load()
+    w = torch.empty((5, 0), dtype=torch.int8, device="cuda")
+    ws, bias = torch.ones(5, device="cuda"), torch.arange(5.0, device="cuda")
+    x = torch.empty((2, 3, 0), device="cuda")
+    assert torch.equal(lib.quantized_linear(x, w, ws, bias), bias.expand(2, 3, 5))
+    codes, scales = lib.quantize_rows(x)
+    assert codes.shape == (2, 3, 0) and scales.shape == (2, 3)
+    assert lib.quantized_linear(torch.empty((2, 0, 0), device="cuda"), w, ws, bias).shape == (2, 0, 5)
