@@ -125,19 +125,30 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
   if (threadIdx.x == 0) a.partial[z * a.parts + blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
 }
 
+// ---- planes ----------------------------------------------------------------------------------------------------------------
+// v = hi + lo: a rounding, the exact rest rounded, and their sum.  The two ones are hidden from the compiler, so that it takes the
+// instruction that multiplies and adds fp16 and fp32 numbers and does not convert them first (two instructions a value instead of
+// three, one instead of three for the sum; same results: 48 of 128 x 128 46.8 -> 42.9 us, with G kept in registers for P).
+__device__ __forceinline__ float hidden(float one) {
+  asm("" : "+s"(one));
+  return one;
+}
+__device__ __forceinline__ _Float16 rest_of(float v, _Float16 hi) { return (_Float16)__builtin_fmaf((float)hi, hidden(-1.f), v); }
+__device__ __forceinline__ float sum_of(_Float16 hi, _Float16 lo) { return __builtin_fmaf((float)hi, hidden(1.f), (float)lo); }
+
 // ---- strips of finished tiles: 32 rows and WN columns of sums in LDS, in lanes' turns of eight neighbours -----------------
 __device__ __forceinline__ void eight_of(const char* row, int64_t c, float (&v)[8]) {
   const char* line = row + (c >> 5) * kLine + 2 * (c & 31);
   const halfx8 hi = *reinterpret_cast<const halfx8*>(line), lo = *reinterpret_cast<const halfx8*>(line + 64);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
+  for (int e = 0; e < 8; ++e) v[e] = sum_of(hi[e], lo[e]);
 }
 __device__ __forceinline__ void put_eight(char* row, int64_t c, const float (&v)[8]) {
   halfx8 hi, lo;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     hi[e] = (_Float16)v[e];
-    lo[e] = (_Float16)(v[e] - (float)hi[e]);
+    lo[e] = rest_of(v[e], hi[e]);
   }
   char* line = row + (c >> 5) * kLine + 2 * (c & 31);
   *reinterpret_cast<halfx8*>(line) = hi;
@@ -243,14 +254,15 @@ struct SymmetricEpilogue {
     const int64_t line = a.s.short_line(), r = a.s.r, padded = (r + 31) & ~31ll;
     strip_passes<WN>(strip, row0, col0, lane, mirror,
         [&](int64_t row, int64_t col, float (&v)[8]) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= 1.f / kScale;
           if (row < r && col < padded) {
             if (g != nullptr) {
               float gv[8];
               eight_of(g + row * line, col, gv);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = a.b * gv[e] + a.c * v[e];
+              for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(a.c * (1.f / kScale), v[e], a.b * gv[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] *= 1.f / kScale;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -365,7 +377,7 @@ struct UpdateEpilogue {
             float xv[8];
             eight_of(x, col, xv);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = col + e < s.l ? a.a * xv[e] + v[e] * (1.f / kScale) : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = col + e < s.l ? __builtin_fmaf(v[e], 1.f / kScale, a.a * xv[e]) : 0.f;
             if (!last) put_eight(x, col, v);
             else if (!s.turned) result(row, col, s.l, v);
           } else {
@@ -692,13 +704,13 @@ __device__ __forceinline__ void put_four(char* lds, int line, int piece, int hal
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     hi[e] = (_Float16)v[e];
-    lo[e] = (_Float16)(v[e] - (float)hi[e]);
+    lo[e] = rest_of(v[e], hi[e]);
   }
   *reinterpret_cast<halfx4*>(lds + piece_at(line, piece) + 8 * half) = hi;
   *reinterpret_cast<halfx4*>(lds + piece_at(line, piece + 4) + 8 * half) = lo;
 }
 
-// 48 of 128 x 128 in bf16 47 us, two of 256 x 128 in fp32 83: a CU's matrix instructions are busy for 29 % of it, the rest is
+// 48 of 128 x 128 in bf16 43 us, two of 256 x 128 in fp32 79: a CU's matrix instructions are busy for 29 % of it, the rest is
 // reads and writes of LDS and the waits between three products a step that need each other.  Tiles over the whole chip would
 // be seventeen launches, 4 us and more each.
 //
@@ -765,7 +777,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const _Float16 hi = (_Float16)x[s][i][v], lo = (_Float16)(x[s][i][v] - (float)hi);
+            const _Float16 hi = (_Float16)x[s][i][v], lo = rest_of(x[s][i][v], hi);
             const int row = 32 * i + tile_row(v, side);
             *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, at / 8) + 2 * (at % 8)) = hi;
             if (!FEW) *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, 4 + at / 8) + 2 * (at % 8)) = lo;
@@ -773,8 +785,8 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
       }
     }
     __syncthreads();
-    fltx16 sum[TJ];
-    if (squares) product(lds, columns, at, side, FEW, sum);
+    fltx16 gram[TJ];                                       // (and P is made from these, not from their planes)
+    if (squares) product(lds, columns, at, side, FEW, gram);
     __syncthreads();
     // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
     if (squares) {
@@ -783,28 +795,27 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
         if (j0 + j < RT) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float v[4] = {sum[j][4 * q] / kScale, sum[j][4 * q + 1] / kScale, sum[j][4 * q + 2] / kScale, sum[j][4 * q + 3] / kScale};
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = gram[j][4 * q + e] *= 1.f / kScale;
             put_four(gl + i0 * kTile, 32 * (j0 + j) + at, q, side, v);
           }
         }
     }
     __syncthreads();
     if (squares) {
+      fltx16 sum[TJ];
       product(gl, RT, at, side, false, sum);
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
         if (j0 + j < RT) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const char* g = gl + i0 * kTile;
-            const int row = 32 * (j0 + j) + at;
-            const halfx4 hi = *reinterpret_cast<const halfx4*>(g + piece_at(row, q) + 8 * side);
-            const halfx4 lo = *reinterpret_cast<const halfx4*>(g + piece_at(row, q + 4) + 8 * side);
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = a.b * ((float)hi[e] + (float)lo[e]) + a.c * (sum[j][4 * q + e] / kScale);
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(sum[j][4 * q + e], a.c * (1.f / kScale), a.b * gram[j][4 * q + e]);
             // columns in the order in which a lane of x has its rows: 4 side ... of each eight
-            put_four(pl + i0 * kTile, row, 2 * (q / 2) + side, q & 1, v);
+            put_four(pl + i0 * kTile, 32 * (j0 + j) + at, 2 * (q / 2) + side, q & 1, v);
           }
         }
     }
@@ -825,7 +836,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             hi[e] = (_Float16)x[s][c][8 * g + e];
-            lo[e] = (_Float16)(x[s][c][8 * g + e] - (float)hi[e]);
+            lo[e] = rest_of(x[s][c][8 * g + e], hi[e]);
           }
           const intx4 fb[2] = {__builtin_bit_cast(intx4, hi), __builtin_bit_cast(intx4, lo)};
           intx4 fa[RT][2];
@@ -843,7 +854,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) x[s][i][v] = a.a * x[s][i][v] + next[i][v] / kScale;
+        for (int v = 0; v < 16; ++v) x[s][i][v] = __builtin_fmaf(next[i][v], 1.f / kScale, a.a * x[s][i][v]);
     }
     __syncthreads();
   }
