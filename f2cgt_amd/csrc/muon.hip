@@ -710,8 +710,16 @@ __device__ __forceinline__ void put_four(char* lds, int line, int piece, int hal
   *reinterpret_cast<halfx4*>(lds + piece_at(line, piece + 4) + 8 * half) = lo;
 }
 
-// 48 of 128 x 128 in bf16 43 us, two of 256 x 128 in fp32 79: a CU's matrix instructions are busy for 29 % of it, the rest is
-// reads and writes of LDS and the waits between three products a step that need each other.  Tiles over the whole chip would
+// Two rows of a lane's column -> two columns of a row, an even lane's first, an odd one's second (turn: the bytes to take).
+__device__ __forceinline__ uint32_t beside(halfx2 rows, uint32_t turn) {
+  const uint32_t own = __builtin_bit_cast(uint32_t, rows);
+  const uint32_t next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xF, 0xF, true);      // (of lane ^ 1)
+  return __builtin_amdgcn_perm(next, own, turn);
+}
+
+// 48 of 128 x 128 in bf16 41 us, two of 256 x 128 in fp32 74.  Of a step's 27 thousand clocks in the latter G takes 7500 and its planes
+// 2200, P 5300, the update 8100 and the writing of X's lines 4100 (6000 value by value instead of by pairs); 15 400 of them issue matrix instructions on each SIMD,
+// the rest is the splitting of values, reads and writes of LDS, and the waits between three products that need each other.  Tiles over the whole chip would
 // be seventeen launches, 4 us and more each.
 //
 // From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
@@ -768,20 +776,39 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     int lane_of = (int)threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane_of));
     const int at = lane_of & 31, side = lane_of >> 5;
-    // X's lines: a lane has a column
+    // X's lines: a lane has a column; of two rows each, neighbours exchange one
+    const uint32_t turn = at & 1 ? 0x03020706 : 0x05040100;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int c = wave + kOneWaves * s;
       if (c < columns) {
+        // (piece_at of row 8 q + 4 side + 2 e + (at & 1), which is piece at / 8 of the hi plane for one parity of q and of the lo
+        // plane for the other)
+        char* place[2][2];
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int odd = 0; odd < 2; ++odd)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const _Float16 hi = (_Float16)x[s][i][v], lo = rest_of(x[s][i][v], hi);
-            const int row = 32 * i + tile_row(v, side);
-            *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, at / 8) + 2 * (at % 8)) = hi;
-            if (!FEW) *reinterpret_cast<_Float16*>(lds + c * kTile + piece_at(row, 4 + at / 8) + 2 * (at % 8)) = lo;
-          }
+          for (int e = 0; e < 2; ++e)
+            place[odd][e] = lds + c * kTile + (4 * side + (at & 1)) * kLine + ((at / 8 ^ (4 * odd + 2 * side + e)) << 4) + 2 * (at & 6);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              halfx2 hi, lo;
+#pragma unroll
+              for (int d = 0; d < 2; ++d) {
+                const float v = x[s][i][4 * q + 2 * e + d];
+                hi[d] = (_Float16)v;
+                lo[d] = rest_of(v, hi[d]);
+              }
+              const int down = (32 * i + 8 * q + 2 * e) * kLine;
+              *reinterpret_cast<uint32_t*>(place[q & 1][e] + down) = beside(hi, turn);
+              if (!FEW) *reinterpret_cast<uint32_t*>(place[~q & 1][e] + down) = beside(lo, turn);
+            }
+          __builtin_amdgcn_sched_barrier(0);                 // (so that no more values are under way than registers)
+        }
       }
     }
     __syncthreads();
@@ -823,6 +850,11 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if (wave + kOneWaves * s >= columns) continue;
+      // (X's planes are made once for its lines and once here: kept in between, both are more than the registers hold)
+      if constexpr (RT == 4 && !FEW) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(x[s][i]));
+      }
       fltx16 next[RT];
 #pragma unroll
       for (int i = 0; i < RT; ++i)

@@ -13,6 +13,7 @@ typedef int intx16 __attribute__((ext_vector_type(16)));
 typedef float fltx4 __attribute__((ext_vector_type(4)));
 typedef float fltx16 __attribute__((ext_vector_type(16)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLine = 128;                 // bytes of a row that a step of the main loop takes
