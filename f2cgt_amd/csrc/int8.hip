@@ -517,7 +517,8 @@ bool fused(int64_t m, int64_t n, int64_t k) {
 // Whether rows of few columns are coded where they are multiplied, once for every 128 outputs.  us, so and by two launches:
 // 1024 x 128 -> 256 6.3 and 8.6, 20 000 x 100 -> 47 9.1 and 11.1, 250 000 x 100 -> 128 51 and 57, bf16 36 and 62,
 // 250 000 x 128 -> 256 84 and 98, 30 000 x 128 -> 512 20 and 23; but 30 000 x 250 -> 512 37 and 29, 100 000 x 200 -> 1024 188 and 140.
-bool rows_fused(int64_t m, int64_t n, int64_t k) { return k <= 256 && n * ceil_div(k, kLine) <= 512 && ceil_div(m, 64) * ceil_div(n, 128) < (1ll << 24); }
+// (Without columns there may be no weights to copy.)
+bool rows_fused(int64_t m, int64_t n, int64_t k) { return k >= 1 && k <= 256 && n * ceil_div(k, kLine) <= 512 && ceil_div(m, 64) * ceil_div(n, 128) < (1ll << 24); }
 
 template <typename X>
 void launch_rows(const FewArgs& f, hipStream_t st) {

@@ -37,7 +37,7 @@ struct MuonArgs {
   Matrices at;
   Shape s;
   int u_dtype, out_dtype, nesterov;
-  float momentum, keep, size;                  // weights: keep * w - size * o; results: keep 0, size -1
+  float momentum, keep, size;                  // weights: keep * w - size * o; results: keep 0
   double* partial;                             // [count][parts]
   int parts;
   char* x;                                     // [count][r] lines of X

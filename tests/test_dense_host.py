@@ -46,6 +46,9 @@ def test_rows_and_products_in_8_bits():
     assert b"workspace" in lib.f2cgt_last_error()
     assert lib.f2cgt_quantized_linear_workspace_bytes(1, 4096, 4096) == 0                # coded where it is multiplied
     assert lib.f2cgt_quantized_linear_workspace_bytes(0, 4096, 4096) == 0
+    # without columns there is nothing to code in the product's workgroups: the weights' buffer may be null
+    assert lib.f2cgt_quantized_linear_workspace_bytes(100, 300, 128) == 0
+    assert lib.f2cgt_quantized_linear_workspace_bytes(100, 300, 0) == 400
 
 
 def test_orthogonalised_updates():

@@ -283,3 +283,15 @@ def test_leading_dimensions_without_columns():
     codes, scales = lib.quantize_rows(x)
     assert codes.shape == (2, 3, 0) and scales.shape == (2, 3)
     assert lib.quantized_linear(torch.empty((2, 0, 0), device="cuda"), w, ws, bias).shape == (2, 0, 5)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 48, 70, 128, 700])
+def test_no_columns(rows):
+    lib = f2cgt_amd.load()
+    w = torch.empty((300, 0), dtype=torch.int8, device="cuda")
+    ws, bias = torch.ones(300, device="cuda"), torch.arange(-5.0, 295.0, device="cuda")
+    want = bias.clamp(min=0).expand(rows, 300)
+    x = torch.empty((rows, 0), device="cuda")
+    assert torch.equal(lib.quantized_linear(x, w, ws, bias, relu=True), want)
+    assert torch.equal(lib.int8_linear(torch.empty((rows, 0), dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda"), w,
+                                       ws, bias, True), want)
