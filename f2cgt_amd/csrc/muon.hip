@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
 // ---- planes ----------------------------------------------------------------------------------------------------------------
 // v = hi + lo: a rounding, the exact rest rounded, and their sum.  The two ones are hidden from the compiler, so that it takes the
 // instruction that multiplies and adds fp16 and fp32 numbers and does not convert them first (two instructions a value instead of
-// three, one instead of three for the sum; same results: 48 of 128 x 128 46.8 -> 42.9 us, with G kept in registers for P).
+// three, one instead of three for the sum; same results: 48 of 128 x 128 46.8 -> 42.9 us then, with G kept in registers for P).
 __device__ __forceinline__ float hidden(float one) {
   asm("" : "+s"(one));
   return one;
@@ -717,13 +717,14 @@ __device__ __forceinline__ uint32_t beside(halfx2 rows, uint32_t turn) {
   return __builtin_amdgcn_perm(next, own, turn);
 }
 
-// 48 of 128 x 128 in bf16 41 us, two of 256 x 128 in fp32 74.  Of a step's 27 thousand clocks in the latter G takes 7500 and its planes
+// 48 of 128 x 128 in bf16 40.5 us, two of 256 x 128 in fp32 74.  Of a step's 27 thousand clocks in the latter G takes 7500 and its planes
 // 2200, P 5300, the update 8100 and the writing of X's lines 4100 (6000 value by value instead of by pairs); 15 400 of them issue matrix instructions on each SIMD,
 // the rest is the splitting of values, reads and writes of LDS, and the waits between three products that need each other.  Tiles over the whole chip would
 // be seventeen launches, 4 us and more each.
 //
-// From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32 after the other, while G is made; then G's and
-// P's, of 32 RT rows by RT column tiles each, in the same place.
+// From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32
+// after the other, while G is made; then G's and P's, of 32 RT rows by RT column tiles each, in the same place.  Where there is
+// room G's lie behind X's, and no wave waits for the others' products before it writes its part.
 template <int RT, int S, bool FEW>
 __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a, int steps) {
   constexpr int kRows = 32 * RT, kTile = kRows * kLine;    // a column tile
@@ -734,8 +735,9 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t z = blockIdx.x;
   const int columns = (int)ceil_div(a.s.l, 32);
-  char* gl = lds;
-  char* pl = lds + RT * kTile;
+  const bool apart = columns + RT <= kTiles;
+  char* gl = lds + (apart ? columns : 0) * kTile;
+  char* pl = lds + (apart ? 0 : RT) * kTile;
   fltx16 x[S][RT];
   load_strips<RT, S>(a, z, s_sum, kScale, x);
   // tiles (i, j0 ...) of square products
@@ -814,7 +816,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     __syncthreads();
     fltx16 gram[TJ];                                       // (and P is made from these, not from their planes)
     if (squares) product(lds, columns, at, side, FEW, gram);
-    __syncthreads();
+    if (!apart) __syncthreads();
     // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
     if (squares) {
 #pragma unroll
