@@ -295,3 +295,29 @@ def test_no_columns(rows):
     assert torch.equal(lib.quantized_linear(x, w, ws, bias, relu=True), want)
     assert torch.equal(lib.int8_linear(torch.empty((rows, 0), dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda"), w,
                                        ws, bias, True), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(20_000_000, 96, 112), (270_000, 320, 8192)])
+def test_results_of_more_than_2_31_values(m, k, n):
+    """The last rows, far beyond 32-bit offsets, are what a call of those rows alone gives."""
+    lib = f2cgt_amd.load()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    weight, weight_scales = lib.quantize_rows(torch.randn((n, k), generator=g, device="cuda"))
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    x[-333:] = torch.randn((333, k), generator=g, device="cuda").bfloat16()
+    out = lib.quantized_linear(x, weight, weight_scales)
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-333:], lib.quantized_linear(x[-333:].clone(), weight, weight_scales))
+    assert not out[:1000].any() and not out[m // 2:m // 2 + 1000].any()
+
+
+def test_rows_of_more_than_2_31_values():
+    lib = f2cgt_amd.load()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    m, k = 1_100_000, 2000
+    x = torch.ones((m, k), dtype=torch.float16, device="cuda")
+    x[-50:] = torch.randn((50, k), generator=g, device="cuda").half()
+    codes, scales = lib.quantize_rows(x)
+    tail, tail_scales = lib.quantize_rows(x[-50:].clone())
+    assert torch.equal(codes[-50:], tail) and torch.equal(scales[-50:], tail_scales)
+    assert bool((codes[:-50] == 127).all())

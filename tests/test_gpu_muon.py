@@ -262,3 +262,19 @@ def test_train_and_serve():
     full, few, equal, losses = train_and_serve.run(nodes=5000, steps=30)
     assert float(losses[-5:].mean()) < 0.5 * float(losses[0])
     assert full > 0.8 and few > full - 0.02 and equal > 0.95
+
+
+@pytest.mark.parametrize("rows,cols", [(33, 40), (100, 128), (128, 256), (90, 2800), (700, 650)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_special_values_in_every_form(rows, cols, dtype):
+    lib = f2cgt_amd.load()
+    u = torch.randn((2, rows, cols), generator=_gen(rows), device="cuda").to(dtype)
+    assert bool((lib.orthogonalize(torch.zeros_like(u)) == 0).all())
+    alone = lib.orthogonalize(u[:1])
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        v = u.clone()
+        v[1, rows - 1, cols - 1] = bad
+        got = lib.orthogonalize(v)
+        assert bool(got[1].isnan().all()) and bool(got[0].isfinite().all())
+        off = float((got[0].double() - alone[0].double()).norm() / alone[0].double().norm())
+        assert off <= 2.0 ** -18 + 2 * HALF[dtype] * (2 if dtype == torch.bfloat16 else 1)     # (a batch may be tiled otherwise)
