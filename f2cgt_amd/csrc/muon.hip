@@ -7,6 +7,8 @@
 // values there are grow by a factor a in each step (480 in five), and so does what rounding adds to them: operands of
 // eleven bits leave 2 to 4 % of error in updates of low rank, so all operands are two fp16 planes (tile_product.hpp), 22 bits
 // and more, with fp32 sums; the result is as near to float64 as fp32 products are, at three fp16 instructions per product.
+// That holds for bf16 results too: Gram products of the hi planes alone add 1e-3 where roundings average out, but 5e-3 to an update
+// whose entries have few different values, and 3.6e-2 in ten steps of steep coefficients.
 //
 // Planes hold kScale times their number: entries of an n x n matrix of norm one are about 1 / n, too near to the least
 // fp16 numbers for a second plane; all numbers stay below 65504 / kScale (the entry points refuse coefficients that would not).
@@ -46,10 +48,6 @@ struct MuonArgs {
   char* p;                                     // of P
   float* sums;                                 // of parts of Gram products
   float a, b, c;
-  // A result in bf16: its own rounding is 1.65e-3 of it (in the norm; in fp16 it is 2e-4, too little for this).  G of the hi planes alone in all steps and the last
-  // product of theirs make it 1.7e-3 to 2.0e-3, and 23 of 30 instructions are left of a square matrix; G G or an earlier
-  // update from them 2.5e-3 and more.
-  __host__ __device__ bool few() const { return out_dtype == F2CGT_DT_BF16; }
   int whole;                                   // rows of the results start at multiples of four values
 };
 
@@ -241,8 +239,7 @@ __device__ __forceinline__ void strip_passes(float* strip, int64_t row0, int64_t
 }
 
 // G from X, or P = b G + c G G from G (g not null): the tiles on and below the diagonal, each written on both sides of it.
-// At 4096 x 4096, where the card's power bounds them, G of hi planes takes 88 us, P of both planes 180: 0.78 and 1.15e15 executed
-// operations a second.  At 1000 x 2051 there are 136 tiles of 64 x 64 for 256 CUs, each of whose LDS is read and written for
+// At 4096 x 4096, where the card's power bounds them, G and P take 180 us each: 1.15e15 executed operations a second.  At 1000 x 2051 there are 136 tiles of 64 x 64 for 256 CUs, each of whose LDS is read and written for
 // most of the time (19.5 and 10.5 us); larger tiles leave more of the chip without one, and a third or fourth stage gained nothing.
 template <int WN>
 struct SymmetricEpilogue {
@@ -279,9 +276,9 @@ struct SymmetricEpilogue {
   }
 };
 
-template <class Op, bool SQUARE, int B, int W, int WJ, int GROUPS, int DEEP>
+template <bool SQUARE, int B, int W, int WJ, int GROUPS, int DEEP>
 __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symmetric_kernel(MuonArgs a) {
-  typedef TileProduct<Op, B, B, W, WJ, 2, GROUPS> Tile;
+  typedef TileProduct<SplitOp, B, B, W, WJ, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const uint32_t tiles = (uint32_t)ceil_div(a.s.r, B), each = tiles * (tiles + 1) / 2, at = place_of(blockIdx.x, gridDim.x);
   uint32_t i, j;
@@ -291,7 +288,7 @@ __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symm
   char* g = a.g + z * s.r * s.short_line();
   char* p = a.p + z * s.r * s.short_line();
   const Lines from = SQUARE ? Lines{g, s.short_line(), s.r, s.short_line()}
-                            : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line() * kLine / Op::kFrom};
+                            : Lines{a.x + z * s.r * s.long_line(), s.long_line(), s.r, s.long_line()};
   Tile::run({lds0, lds1}, from, from, row0, col0, SymmetricEpilogue<WJ>{a, SQUARE ? p : g, SQUARE ? g : nullptr, row0 != col0});
 }
 
@@ -307,9 +304,8 @@ struct PartEpilogue {
   }
 };
 
-template <class Op>
 __global__ __launch_bounds__(1024) void muon_gram_part_kernel(MuonArgs a, int splits) {
-  typedef TileProduct<Op, 64, 64, 32, 32, 2, 4> Tile;
+  typedef TileProduct<SplitOp, 64, 64, 32, 32, 2, 4> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   // the parts of a tile go to different XCDs, tiles of a part to the same
@@ -317,10 +313,10 @@ __global__ __launch_bounds__(1024) void muon_gram_part_kernel(MuonArgs a, int sp
   const uint32_t part = at / all, tile = at % all;
   uint32_t i, j;
   lower_tile_of(tile % each, tiles, 8, i, j);
-  const int64_t z = tile / each, bytes = s.long_line() * kLine / Op::kFrom, steps = ceil_div(bytes, kLine);
+  const int64_t z = tile / each, steps = s.long_line() / kLine;
   const int64_t first = steps * part / splits, end = steps * (part + 1) / splits;
-  const char* x = a.x + z * s.r * s.long_line() + first * Op::kFrom;
-  const int64_t here = (end * kLine < bytes ? end * kLine : bytes) - first * kLine;
+  const char* x = a.x + z * s.r * s.long_line() + first * kLine;
+  const int64_t here = (end - first) * kLine;
   const Lines row_lines{x + 64 * i * s.long_line(), s.long_line(), s.r - 64 * i, here};
   const Lines col_lines{x + 64 * j * s.long_line(), s.long_line(), s.r - 64 * j, here};
   Tile::run({lds0, lds1}, row_lines, col_lines, 0, 0, PartEpilogue{a.sums + ((int64_t)tile * splits + part) * 4096});
@@ -351,8 +347,8 @@ __global__ __launch_bounds__(256) void muon_gram_add_kernel(MuonArgs a, int spli
 
 // How many parts: as many as make a workgroup per CU, of eight steps at least, where that saves more than the addition costs (4 us; a
 // step 0.28).  99 x 2721: 24 us in one part.  1 where it does not.
-int gram_splits(int64_t n, const Shape& s, bool few) {
-  const int64_t tiles = n * ceil_div(s.r, 64) * (ceil_div(s.r, 64) + 1) / 2, steps = ceil_div(s.l, few ? 64 : 32), cus = num_cus();
+int gram_splits(int64_t n, const Shape& s) {
+  const int64_t tiles = n * ceil_div(s.r, 64) * (ceil_div(s.r, 64) + 1) / 2, steps = ceil_div(s.l, 32), cus = num_cus();
   int64_t splits = cus / tiles;
   if (splits > steps / 8) splits = steps / 8;
   return splits >= 2 && steps - steps / splits >= 20 ? (int)splits : 1;
@@ -420,18 +416,17 @@ struct UpdateEpilogue {
   }
 };
 
-template <class Op, int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
+template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
-  typedef TileProduct<Op, BM, BN, WM, WN, 2, GROUPS> Tile;
+  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   const uint32_t tiles_r = (uint32_t)ceil_div(s.r, BM), tiles_l = (uint32_t)ceil_div(s.l, BN), at = place_of(blockIdx.x, gridDim.x);
   uint32_t i, j;
   tile_of(at % (tiles_r * tiles_l), tiles_r, tiles_l, DEEP, i, j);
   const int64_t z = at / (tiles_r * tiles_l);
-  const int64_t bytes = s.short_line() * kLine / Op::kFrom;
-  const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, bytes};
-  const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, bytes};
+  const Lines p{a.p + z * s.r * s.short_line(), s.short_line(), s.r, s.short_line()};
+  const Lines x{a.xt[from] + z * s.l * s.short_line(), s.short_line(), s.l, s.short_line()};
   Tile::run({lds0, lds1}, p, x, (int64_t)BM * i, (int64_t)BN * j, UpdateEpilogue<WN>{a, z, last ? nullptr : a.xt[1 - from]});
 }
 
@@ -440,17 +435,14 @@ void launch_symmetric(const MuonArgs& a, int64_t n, bool square, hipStream_t st)
   const int64_t tiles = ceil_div(a.s.r, B);
   const unsigned grid = (unsigned)(n * tiles * (tiles + 1) / 2);
   constexpr int kBlock = (B / W) * (B / WJ) * GROUPS * kWave;
-  if (square) muon_symmetric_kernel<SplitOp, true, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
-  else if (a.few()) muon_symmetric_kernel<HiOp, false, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
-  else muon_symmetric_kernel<SplitOp, false, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
+  if (square) muon_symmetric_kernel<true, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
+  else muon_symmetric_kernel<false, B, W, WJ, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a);
 }
 
 template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t st) {
   const unsigned grid = (unsigned)(n * ceil_div(a.s.r, BM) * ceil_div(a.s.l, BN));
-  constexpr int kBlock = (BM / WM) * (BN / WN) * GROUPS * kWave;
-  if (last && a.few()) muon_update_kernel<HiOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
-  else muon_update_kernel<SplitOp, BM, BN, WM, WN, GROUPS, DEEP><<<grid, kBlock, 0, st>>>(a, from, last);
+  muon_update_kernel<BM, BN, WM, WN, GROUPS, DEEP><<<grid, (BM / WM) * (BN / WN) * GROUPS * kWave, 0, st>>>(a, from, last);
 }
 
 // Which tiles.  Time of a step of 32 summed columns, in 10 ns, by tiles per CU, and steps' worth of a tile's begin and end:
@@ -458,7 +450,7 @@ void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t
 //   192 x 192 in four waves (symmetric products): 133 each; 8 steps.  64 x 128 in eight waves (updates), three a CU: 30 each
 //   64 x 64: 47 for one, 22 each for many; 2 steps.  With four groups of waves 31 for one
 // us of Gram products of 1000 x 2051: 64 x 64 30, in four groups 19.5, 128 x 128 42; 2048 x 2048: 34, 54, 42; eight of 1000 x 700: 18, 27, 24;
-// 3000 x 3000: 97, 128, 86, 192 x 192 128; 4096 x 4096: 195, 262, 169, 168 (528 and 253 tiles; of the hi planes 215, 224, 125, 88).
+// 3000 x 3000: 97, 128, 86, 192 x 192 128; 4096 x 4096: 195, 262, 169, 168 (528 and 253 tiles).
 // Updates: 1000 x 2051: 64 x 64 20.8, 64 x 128 23.5, 128 x 128 27.1; 2048 x 2048: 50, 43, 49; 3000 x 3000: 160, 130, 142;
 // 4096 x 4096: 349, 284, 237, 256 x 256 299.
 int64_t pairs_cost(int64_t tiles, int64_t cus) {
@@ -722,10 +714,10 @@ __device__ __forceinline__ uint32_t beside(halfx2 rows, uint32_t turn) {
 // the rest is the splitting of values, reads and writes of LDS, and the waits between three products that need each other.  Tiles over the whole chip would
 // be seventeen launches, 4 us and more each.
 //
-// From 33 to 32 RT rows: products of planes (FEW: MuonArgs::few, G from the hi planes).  LDS: X's lines, a column tile of 32
+// From 33 to 32 RT rows: products of planes.  LDS: X's lines, a column tile of 32
 // after the other, while G is made; then G's and P's, of 32 RT rows by RT column tiles each, in the same place.  Where there is
 // room G's lie behind X's, and no wave waits for the others' products before it writes its part.
-template <int RT, int S, bool FEW>
+template <int RT, int S>
 __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a, int steps) {
   constexpr int kRows = 32 * RT, kTile = kRows * kLine;    // a column tile
   constexpr int kTiles = S * kOneWaves > 2 * RT ? S * kOneWaves : 2 * RT;
@@ -744,7 +736,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
   const int i0 = wave / 2, j0 = (wave & 1) * TJ;
   const bool squares = i0 < RT;
   // rows i of a times rows j of b, column tiles [0, n)
-  auto product = [&](const char* of, int n, int at, int side, bool hi, fltx16 (&sum)[TJ]) {
+  auto product = [&](const char* of, int n, int at, int side, fltx16 (&sum)[TJ]) {
 #pragma unroll
     for (int j = 0; j < TJ; ++j)
 #pragma unroll
@@ -756,7 +748,6 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
         intx4 fa[2], fb[TJ][2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          if (hi && p == 1) break;
           fa[p] = *reinterpret_cast<const intx4*>(tile + piece_at(32 * i0 + at, 4 * p + 2 * g + side));
 #pragma unroll
           for (int j = 0; j < TJ; ++j) {
@@ -766,7 +757,6 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
         }
 #pragma unroll
         for (int m = 0; m < SplitOp::kTerms; ++m) {
-          if (hi && m < SplitOp::kTerms - 1) continue;       // (the last term is the one of both hi planes)
 #pragma unroll
           for (int j = 0; j < TJ; ++j) SplitOp::mma(sum[j], m, fa, fb[j]);
         }
@@ -807,7 +797,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
               }
               const int down = (32 * i + 8 * q + 2 * e) * kLine;
               *reinterpret_cast<uint32_t*>(place[q & 1][e] + down) = beside(hi, turn);
-              if (!FEW) *reinterpret_cast<uint32_t*>(place[~q & 1][e] + down) = beside(lo, turn);
+              *reinterpret_cast<uint32_t*>(place[~q & 1][e] + down) = beside(lo, turn);
             }
           __builtin_amdgcn_sched_barrier(0);                 // (so that no more values are under way than registers)
         }
@@ -815,7 +805,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     }
     __syncthreads();
     fltx16 gram[TJ];                                       // (and P is made from these, not from their planes)
-    if (squares) product(lds, columns, at, side, FEW, gram);
+    if (squares) product(lds, columns, at, side, gram);
     if (!apart) __syncthreads();
     // A lane has, of tile (i, j), column j's `at` and four rows after four; G is symmetric: four neighbours of row `at`.
     if (squares) {
@@ -834,7 +824,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     __syncthreads();
     if (squares) {
       fltx16 sum[TJ];
-      product(gl, RT, at, side, false, sum);
+      product(gl, RT, at, side, sum);
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
         if (j0 + j < RT) {
@@ -853,7 +843,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
     for (int s = 0; s < S; ++s) {
       if (wave + kOneWaves * s >= columns) continue;
       // (X's planes are made once for its lines and once here: kept in between, both are more than the registers hold)
-      if constexpr (RT == 4 && !FEW) {
+      if constexpr (RT == 4) {
 #pragma unroll
         for (int i = 0; i < RT; ++i) asm volatile("" : "+v"(x[s][i]));
       }
@@ -903,8 +893,7 @@ bool one_workgroup(const Shape& m) {
 
 template <int RT, int S>
 void launch_one(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
-  if (a.few()) muon_one_kernel<RT, S, true><<<(unsigned)n, kOneWaves * kWave, 0, st>>>(a, steps);
-  else muon_one_kernel<RT, S, false><<<(unsigned)n, kOneWaves * kWave, 0, st>>>(a, steps);
+  muon_one_kernel<RT, S><<<(unsigned)n, kOneWaves * kWave, 0, st>>>(a, steps);
 }
 
 bool one_launch(const MuonArgs& a, int64_t n, int steps, hipStream_t st) {
@@ -1002,7 +991,7 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
       if (int rc = launch_status(what)) return rc;
       continue;
     }
-    const int splits = gram_splits(n, s, a.few());
+    const int splits = gram_splits(n, s);
     const dim3 parts((unsigned)a.parts, (unsigned)n);
     if (held != nullptr) muon_norm_kernel<true><<<parts, 256, 0, st>>>(a);
     else muon_norm_kernel<false><<<parts, 256, 0, st>>>(a);
@@ -1010,8 +999,7 @@ int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t 
     for (int step = 0; step < steps; ++step) {
       if (splits > 1) {
         const unsigned tiles = (unsigned)(n * ceil_div(s.r, 64) * (ceil_div(s.r, 64) + 1) / 2);
-        if (a.few()) muon_gram_part_kernel<HiOp><<<tiles * splits, 1024, 0, st>>>(a, splits);
-        else muon_gram_part_kernel<SplitOp><<<tiles * splits, 1024, 0, st>>>(a, splits);
+        muon_gram_part_kernel<<<tiles * splits, 1024, 0, st>>>(a, splits);
         muon_gram_add_kernel<<<tiles, 256, 0, st>>>(a, splits);
       } else {
         symmetric(a, n, false, st);

@@ -18,7 +18,7 @@ typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLine = 128;                 // bytes of a row that a step of the main loop takes
 
-// Rows of one operand: row r at base + r * stride (a multiple of 16), `bytes` of it are summed over (of the hi planes: of those).
+// Rows of one operand: row r at base + r * stride (a multiple of 16), `bytes` of it are summed over.
 // The 16-byte piece with a row's last byte is read as a whole.
 struct Lines {
   const char* base;
@@ -30,8 +30,6 @@ struct Lines {
 // 8-bit codes: a group is one 32 x 32 x 32 instruction over 32 codes.
 struct Int8Op {
   typedef intx16 Acc;
-  static constexpr int kFrom = kLine;          // bytes of a row in memory that become a line of a step
-  static __device__ __forceinline__ int source(int at) { return at; }
   static constexpr int kGroups = 4, kParts = 1;
   static constexpr bool kTrim = true;        // a row may end within a line
   static __device__ __forceinline__ int chunk(int group, int) { return 2 * group; }
@@ -45,8 +43,6 @@ struct Int8Op {
 // first): a group is three 32 x 32 x 16 instructions over 16 numbers.
 struct SplitOp {
   typedef fltx16 Acc;
-  static constexpr int kFrom = kLine;
-  static __device__ __forceinline__ int source(int at) { return at; }
   static constexpr int kGroups = 2, kParts = 2;
   static constexpr bool kTrim = false;       // rows are whole lines
   static __device__ __forceinline__ int chunk(int group, int part) { return 4 * part + 2 * group; }
@@ -54,20 +50,6 @@ struct SplitOp {
   static __device__ __forceinline__ void mma(Acc& acc, int term, const intx4 (&p)[2], const intx4 (&q)[2]) {
     const halfx8 a = __builtin_bit_cast(halfx8, p[term == 0 ? 1 : 0]), b = __builtin_bit_cast(halfx8, q[term == 1 ? 1 : 0]);
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
-  }
-};
-
-// The hi planes alone, of 64 numbers in a step: the first halves of two lines.
-struct HiOp {
-  typedef fltx16 Acc;
-  static constexpr int kFrom = 2 * kLine;
-  static __device__ __forceinline__ int source(int at) { return (at >> 6) * kLine + (at & 63); }
-  static constexpr int kGroups = 4, kParts = 1;
-  static constexpr bool kTrim = true;          // (an odd number of lines)
-  static __device__ __forceinline__ int chunk(int group, int) { return 2 * group; }
-  static constexpr int kTerms = 1;
-  static __device__ __forceinline__ void mma(Acc& acc, int, const intx4 (&p)[1], const intx4 (&q)[1]) {
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, p[0]), __builtin_bit_cast(halfx8, q[0]), acc, 0, 0, 0);
   }
 };
 
@@ -138,13 +120,13 @@ struct TileProduct {
       const bool first = i * kThreads < BM * 8;
       const int r = (t + i * kThreads) / 8 - (first ? 0 : BM);
       const int64_t rows = first ? a.rows - row0 : b.rows - col0;
-      from[i] = (uint32_t)(r < rows ? r : (int)rows - 1) * (uint32_t)(first ? a.stride : b.stride) + Op::source(piece);
+      from[i] = (uint32_t)(r < rows ? r : (int)rows - 1) * (uint32_t)(first ? a.stride : b.stride) + piece;
     }
     auto copy = [&](char* to, int step) {
       // (pieces of the last step that begin behind the end: the row's first one of this step, which is made zero below)
-      const int back = step == steps - 1 && piece >= left ? Op::source(piece) : 0;
-      const char* pa = base_a + (int64_t)step * Op::kFrom;
-      const char* pb = base_b + (int64_t)step * Op::kFrom;
+      const int back = step == steps - 1 && piece >= left ? piece : 0;
+      const char* pa = base_a + (int64_t)step * kLine;
+      const char* pb = base_b + (int64_t)step * kLine;
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
         __builtin_amdgcn_global_load_lds(

@@ -424,8 +424,8 @@ int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, const int8_t* w
  * the same buffer):  X = U / (|U|_F + 1e-7), its shorter side as rows, then `steps` times (1 to 100)
  * G = X X^T, X = a X + (b G + c G G) X, coefficients (host) a, b, c.  Refused (F2CGT_E_UNSUPPORTED): coefficients that lead
  * singular values from [0, 1] beyond 2.5 or multiply them with more than 7.5 in some step; more than 65536 rows or columns.
- * A NaN or an infinity in a matrix makes it NaN.  Sums and norm are fp32 and fp64, products of 22 bits and more, with results
- * in bf16 some of eleven (their own rounding, 1.65e-3 of the norm, becomes 1.7e-3 to 2.0e-3).  X is held to 1e-11 in absolute
+ * A NaN or an infinity in a matrix makes it NaN.  Sums and norm are fp32 and fp64, products of 22 bits and more whatever the
+ * result's type.  X is held to 1e-11 in absolute
  * terms at first, which shows where |U|_F is below 1e-11 and X, for the 1e-7, nearly zero.
  *
  * f2cgt_muon_step: lists (host) of `count` dense matrices [rows, cols] on the device, per matrix
