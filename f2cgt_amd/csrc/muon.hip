@@ -11,14 +11,15 @@
 // whose entries have few different values, and 3.6e-2 in ten steps of steep coefficients.
 //
 // Planes hold kScale times their number: entries of an n x n matrix of norm one are about 1 / n, too near to the least
-// fp16 numbers for a second plane; all numbers stay below 65504 / kScale (the entry points refuse coefficients that would not).
+// fp16 numbers for a second plane; all numbers stay below 65504 / kScale (the entry points refuse coefficients that would not).  P's eigenvalues are
+// b t + c t^2, which may be twice what the whole polynomial is: its planes hold half as much where they have to.
 #include "tile_product.hpp"
 
 namespace f2cgt {
 namespace {
 
 constexpr float kScale = 8192.f;
-constexpr double kMost = 7.5;                  // of the polynomial's values and of what it multiplies
+constexpr double kMost = 7.5;                  // of the polynomial's values; of P's before its planes hold half
 constexpr int kGroup = 64;                     // matrices that one set of launches takes
 
 // Several matrices of one shape; `rows` and `cols` as the caller has them, r <= l the sides as the products have them.
@@ -48,6 +49,7 @@ struct MuonArgs {
   char* p;                                     // of P
   float* sums;                                 // of parts of Gram products
   float a, b, c;
+  float plane_b, plane_c, back;                // what makes P's planes of G's and of the sums of G G, and numbers of the sums of P X
   int whole;                                   // rows of the results start at multiples of four values
 };
 
@@ -256,7 +258,7 @@ struct SymmetricEpilogue {
               float gv[8];
               eight_of(g + row * line, col, gv);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(a.c * (1.f / kScale), v[e], a.b * gv[e]);
+              for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(a.plane_c, v[e], a.plane_b * gv[e]);
             } else {
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] *= 1.f / kScale;
@@ -373,7 +375,7 @@ struct UpdateEpilogue {
             float xv[8];
             eight_of(x, col, xv);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = col + e < s.l ? __builtin_fmaf(v[e], 1.f / kScale, a.a * xv[e]) : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = col + e < s.l ? __builtin_fmaf(v[e], a.back, a.a * xv[e]) : 0.f;
             if (!last) put_eight(x, col, v);
             else if (!s.turned) result(row, col, s.l, v);
           } else {
@@ -832,7 +834,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
           for (int q = 0; q < 4; ++q) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(sum[j][4 * q + e], a.c * (1.f / kScale), a.b * gram[j][4 * q + e]);
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(sum[j][4 * q + e], a.plane_c, a.plane_b * gram[j][4 * q + e]);
             // columns in the order in which a lane of x has its rows: 4 side ... of each eight
             put_four(pl + i0 * kTile, 32 * (j0 + j) + at, 2 * (q / 2) + side, q & 1, v);
           }
@@ -878,7 +880,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void muon_one_kernel(MuonArgs a,
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) x[s][i][v] = __builtin_fmaf(next[i][v], 1.f / kScale, a.a * x[s][i][v]);
+        for (int v = 0; v < 16; ++v) x[s][i][v] = __builtin_fmaf(next[i][v], a.back, a.a * x[s][i][v]);
     }
     __syncthreads();
   }
@@ -937,7 +939,8 @@ int64_t workspace_of(int64_t count, int64_t rows, int64_t cols) {
          2 * whole(n * s.r * s.short_line()) + (int64_t)num_cus() * 4096 * 4;
 }
 
-int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int steps, const float* coefficients) {
+// most_p: what P's eigenvalues stay below.
+int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int steps, const float* coefficients, double& most_p) {
   F2CGT_REQUIRE(count >= 0 && rows >= 0 && cols >= 0, F2CGT_E_INVALID, "%s: sizes must not be negative", what);
   F2CGT_REQUIRE(rows <= 65536 && cols <= 65536, F2CGT_E_UNSUPPORTED, "%s: at most 65536 rows and columns", what);
   F2CGT_REQUIRE(steps >= 1 && steps <= 100, F2CGT_E_INVALID, "%s: from one to 100 steps", what);
@@ -946,6 +949,7 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
   // squares, and x p(x^2), at the ends and where a derivative is zero.
   const double a = coefficients[0], b = coefficients[1], c = coefficients[2];
   double reach = 1.;
+  most_p = 0.;
   for (int s = 0; s < steps; ++s) {
     const double end = 1.002 * reach * reach, root = 9. * b * b - 20. * a * c;
     const double at[5] = {0., end, c != 0. ? -b / (2. * c) : 0., c != 0. && root >= 0. ? (-3. * b + sqrt(root)) / (10. * c) : b != 0. ? -a / (3. * b) : 0.,
@@ -956,6 +960,7 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
       const double p = a + b * t + c * t * t, x = sqrt(t) * fabs(p);
       F2CGT_REQUIRE(p > -kMost && p < kMost && x < 2.5, F2CGT_E_UNSUPPORTED, "%s: these coefficients lead out of the range of the products", what);
       next = x > next ? x : next;
+      most_p = fabs(p - a) > most_p ? fabs(p - a) : most_p;
     }
     reach = next;
   }
@@ -963,11 +968,13 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
 }
 
 int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t cols, int steps, const float* coefficients,
-             void* const* out, const void* const* u, float* const* held, int64_t u_step, void* workspace, hipStream_t st) {
+             double most_p, void* const* out, const void* const* u, float* const* held, int64_t u_step, void* workspace, hipStream_t st) {
   a.s = shape_of(rows, cols);
   const Shape& s = a.s;
   a.parts = (int)parts_of(rows, cols);
   a.a = coefficients[0]; a.b = coefficients[1]; a.c = coefficients[2];
+  const float fit = most_p < kMost ? 1.f : 0.5f;           // (a and a + b t + c t^2 are below kMost: most_p is below twice that)
+  a.plane_b = a.b * fit; a.plane_c = a.c * fit * (1.f / kScale); a.back = 1.f / (kScale * fit);
   const int64_t group = group_of(count, rows, cols);
   char* at = static_cast<char*>(workspace);
   auto take = [&](int64_t bytes) { char* p = at; at = p != nullptr ? p + whole(bytes) : p; return p; };
@@ -1025,7 +1032,8 @@ extern "C" int64_t f2cgt_muon_workspace_bytes(int64_t count, int64_t rows, int64
 extern "C" int f2cgt_orthogonalize(const void* update, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps,
                                    const float* coefficients, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "orthogonalize";
-  if (int rc = check_muon(what, count, rows, cols, steps, coefficients)) return rc;
+  double most_p;
+  if (int rc = check_muon(what, count, rows, cols, steps, coefficients, most_p)) return rc;
   F2CGT_REQUIRE(dense_type(dtype), F2CGT_E_UNSUPPORTED, "%s: fp32, fp16 or bf16 only", what);
   if (count == 0 || rows == 0 || cols == 0) return 0;
   F2CGT_REQUIRE(update && out && aligned(update, type_size(dtype)) && aligned(out, type_size(dtype)), F2CGT_E_INVALID,
@@ -1038,14 +1046,15 @@ extern "C" int f2cgt_orthogonalize(const void* update, int dtype, void* out, int
   a.keep = 0.f;
   void* outs[1] = {out};
   const void* ins[1] = {update};
-  return run_muon(what, a, count, rows, cols, steps, coefficients, outs, ins, nullptr, rows * cols, workspace, as_stream(stream));
+  return run_muon(what, a, count, rows, cols, steps, coefficients, most_p, outs, ins, nullptr, rows * cols, workspace, as_stream(stream));
 }
 
 extern "C" int f2cgt_muon_step(void* const* weights, int weight_dtype, const void* const* grads, int grad_dtype, float* const* momenta,
                                int64_t count, int64_t rows, int64_t cols, float step_size, float decay, float momentum, int nesterov,
                                int steps, const float* coefficients, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "muon_step";
-  if (int rc = check_muon(what, count, rows, cols, steps, coefficients)) return rc;
+  double most_p;
+  if (int rc = check_muon(what, count, rows, cols, steps, coefficients, most_p)) return rc;
   F2CGT_REQUIRE(dense_type(weight_dtype) && dense_type(grad_dtype), F2CGT_E_UNSUPPORTED, "%s: fp32, fp16 or bf16 only", what);
   if (count == 0 || rows == 0 || cols == 0) return 0;
   F2CGT_REQUIRE(weights && grads && momenta, F2CGT_E_INVALID, "%s: null list", what);
@@ -1065,5 +1074,5 @@ extern "C" int f2cgt_muon_step(void* const* weights, int weight_dtype, const voi
   a.size = step_size;
   F2CGT_REQUIRE(a.keep > 0.f && a.keep <= 1.f && momentum >= 0.f && momentum < 1.f, F2CGT_E_INVALID,
                 "%s: decay must be in [0, 1), momentum too", what);
-  return run_muon(what, a, count, rows, cols, steps, coefficients, weights, grads, momenta, 0, workspace, as_stream(stream));
+  return run_muon(what, a, count, rows, cols, steps, coefficients, most_p, weights, grads, momenta, 0, workspace, as_stream(stream));
 }
