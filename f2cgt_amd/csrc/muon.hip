@@ -952,8 +952,9 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
   most_p = 0.;
   for (int s = 0; s < steps; ++s) {
     const double end = 1.002 * reach * reach, root = 9. * b * b - 20. * a * c;
-    const double at[5] = {0., end, c != 0. ? -b / (2. * c) : 0., c != 0. && root >= 0. ? (-3. * b + sqrt(root)) / (10. * c) : b != 0. ? -a / (3. * b) : 0.,
-                          c != 0. && root >= 0. ? (-3. * b - sqrt(root)) / (10. * c) : 0.};
+    // the derivative a + 3 b t + 5 c t^2 of x p(x^2) is zero at q / 5 c and a / q: no difference of near numbers, whatever c is
+    const double q = -0.5 * (3. * b + copysign(sqrt(root), b));
+    const double at[5] = {0., end, c != 0. ? -b / (2. * c) : 0., root >= 0. && c != 0. ? q / (5. * c) : 0., root >= 0. && q != 0. ? a / q : 0.};
     double next = 0.;
     for (double t : at) {
       if (!(t >= 0. && t <= end) && t == t) continue;
