@@ -317,6 +317,7 @@ __global__ __launch_bounds__(256) void int8_rows_kernel(LinearArgs a, int64_t ld
       *reinterpret_cast<Words<V>*>(lds + c / kLine * kM * kLine + piece_at(r, c % kLine / 16) + c % 16) = q;
     }
   }
+  wait_copies<0>();                            // (the weights: a barrier alone does not wait for copies into LDS)
   __syncthreads();
   const int wi = 32 * (wave & 1), wj = 64 * (wave >> 1);
   intx16 acc[2];
