@@ -1201,8 +1201,11 @@ int dense_tag(torch::ScalarType type, const char* name) {
   return F2CGT_DT_BF16;
 }
 
-void undifferentiated(const torch::Tensor& t, const char* op) {
-  TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), op, " is not differentiated: call it under torch.no_grad()");
+// For each tensor that a result would have a gradient by; an undefined one is none that was given.
+void undifferentiated(const char* op, std::initializer_list<torch::Tensor> tensors) {
+  for (const auto& t : tensors)
+    TORCH_CHECK(!(t.defined() && c10::GradMode::is_enabled() && t.requires_grad()), op,
+                " is not differentiated: call it under torch.no_grad()");
 }
 
 // Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart or rows overlap.
@@ -1256,7 +1259,7 @@ torch::Tensor bias_of(const c10::optional<torch::Tensor>& bias, const torch::Ten
 std::tuple<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
   auto rows = value_rows(x, "x");
   const int tag = dense_tag(rows.scalar_type(), "x");
-  undifferentiated(x, "quantize_rows");
+  undifferentiated("quantize_rows", {x});
   c10::DeviceGuard guard(rows.device());
   const int64_t m = rows.size(0), k = rows.size(1);
   auto codes = room_for_codes(m, k, rows);
@@ -1275,6 +1278,7 @@ torch::Tensor int8_linear(const torch::Tensor& codes_in, const torch::Tensor& sc
                           const torch::Tensor& weight_scales_in, const c10::optional<torch::Tensor>& bias_in, bool relu,
                           torch::ScalarType dtype) {
   const int tag = dense_tag(dtype, "dtype");
+  undifferentiated("int8_linear", {scales_in, weight_scales_in, bias_in.value_or(torch::Tensor())});
   auto codes = code_rows(codes_in, "codes"), weight = code_rows(weight_in, "weight_codes");
   TORCH_CHECK(codes.device() == weight.device(), "codes are on ", codes.device(), ", the weights on ", weight.device());
   TORCH_CHECK(codes.size(1) == weight.size(1), "codes have ", codes.size(1), " columns, the weights ", weight.size(1));
@@ -1295,7 +1299,7 @@ torch::Tensor quantized_linear(const torch::Tensor& x, const torch::Tensor& weig
                                const c10::optional<torch::Tensor>& bias_in, bool relu) {
   auto rows = value_rows(x, "x");
   const int tag = dense_tag(rows.scalar_type(), "x");
-  undifferentiated(x, "quantized_linear");
+  undifferentiated("quantized_linear", {x, weight_scales_in, bias_in.value_or(torch::Tensor())});
   auto weight = code_rows(weight_in, "weight_codes");
   TORCH_CHECK(rows.device() == weight.device(), "x is on ", rows.device(), ", the weights on ", weight.device());
   TORCH_CHECK(rows.size(1) == weight.size(1), "x has ", rows.size(1), " columns, the weights ", weight.size(1));
@@ -1325,7 +1329,7 @@ torch::Tensor orthogonalize(const torch::Tensor& update, int64_t steps, const st
   TORCH_CHECK(update.dim() >= 2, "update must be a matrix or a batch of them");
   TORCH_CHECK(steps >= 1 && steps <= 100, "orthogonalize: from one to 100 steps");
   const int tag = dense_tag(update.scalar_type(), "update");
-  undifferentiated(update, "orthogonalize");
+  undifferentiated("orthogonalize", {update});
   c10::DeviceGuard guard(update.device());
   auto u = update.contiguous();
   auto out = torch::empty(u.sizes(), u.options());

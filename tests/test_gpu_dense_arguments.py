@@ -1,0 +1,36 @@
+"""What the dense operators do with tensors that are more than their values: differentiated ones, lazily negated ones, ones that share memory."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+if torch.cuda.is_available():
+    import f2cgt_amd
+
+pytestmark = pytest.mark.gpu
+
+
+def _dense(seed=0):
+    """x, weight codes and scales, bias, codes of x and their scales."""
+    lib = f2cgt_amd.load()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((5, 40), generator=g, device="cuda")
+    weight, weight_scales = lib.quantize_rows(torch.randn((7, 40), generator=g, device="cuda"))
+    bias = torch.randn((7,), generator=g, device="cuda")
+    return (lib, x, weight, weight_scales, bias) + tuple(lib.quantize_rows(x))
+
+
+def test_scales_and_biases_that_require_gradients():
+    lib, x, weight, weight_scales, bias, codes, scales = _dense()
+    want = lib.quantized_linear(x, weight, weight_scales, bias)
+    leaf = lambda t: t.clone().requires_grad_()     # noqa: E731
+    for call in (lambda: lib.quantized_linear(x, weight, leaf(weight_scales)), lambda: lib.quantized_linear(x, weight, weight_scales, leaf(bias)),
+                 lambda: lib.int8_linear(codes, leaf(scales), weight, weight_scales), lambda: lib.int8_linear(codes, scales, weight, leaf(weight_scales)),
+                 lambda: lib.int8_linear(codes, scales, weight, weight_scales, leaf(bias)),
+                 lambda: lib.int8_linear(codes, scales, weight, weight_scales, torch.nn.Linear(40, 7, device="cuda").bias)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.no_grad():
+        assert torch.equal(lib.quantized_linear(leaf(x), weight, leaf(weight_scales), leaf(bias)), want)
+        assert torch.equal(lib.int8_linear(codes, leaf(scales), weight, leaf(weight_scales), leaf(bias)), want)
