@@ -1201,11 +1201,19 @@ int dense_tag(torch::ScalarType type, const char* name) {
   return F2CGT_DT_BF16;
 }
 
+// Forward-mode tangents, which torch.no_grad() does not turn off.
+void without_tangent(const char* op, const torch::Tensor& t) {
+  TORCH_CHECK(!(t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), op,
+              " is not differentiated: a forward-mode tangent of its arguments would be lost (torch.autograd.forward_ad.unpack_dual(x).primal)");
+}
+
 // For each tensor that a result would have a gradient by; an undefined one is none that was given.
 void undifferentiated(const char* op, std::initializer_list<torch::Tensor> tensors) {
-  for (const auto& t : tensors)
+  for (const auto& t : tensors) {
     TORCH_CHECK(!(t.defined() && c10::GradMode::is_enabled() && t.requires_grad()), op,
                 " is not differentiated: call it under torch.no_grad()");
+    without_tangent(op, t);
+  }
 }
 
 // Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart or rows overlap.
@@ -1367,6 +1375,7 @@ void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torc
                 "muon_step: gradients of the weights' shape and device, and of one type, only");
     TORCH_CHECK(momenta[i].defined() && momenta[i].device() == like.device() && momenta[i].scalar_type() == torch::kFloat32 &&
                     momenta[i].sizes() == like.sizes(), "muon_step: momenta must be float32 of the weights' shape and device");
+    for (const auto& t : {weights[i], grads[i], momenta[i]}) without_tangent("muon_step", t);
     w[i] = weights[i].contiguous();
     g[i] = grads[i].contiguous();
     v[i] = momenta[i].contiguous();

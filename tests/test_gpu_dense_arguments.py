@@ -34,3 +34,26 @@ def test_scales_and_biases_that_require_gradients():
     with torch.no_grad():
         assert torch.equal(lib.quantized_linear(leaf(x), weight, leaf(weight_scales), leaf(bias)), want)
         assert torch.equal(lib.int8_linear(codes, leaf(scales), weight, leaf(weight_scales), leaf(bias)), want)
+
+
+def test_forward_tangents():
+    import torch.autograd.forward_ad as forward
+    lib, x, weight, weight_scales, bias, codes, scales = _dense()
+    want = lib.quantized_linear(x, weight, weight_scales, bias)
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))       # noqa: E731
+        for call in (lambda: lib.quantize_rows(dual(x)), lambda: lib.quantized_linear(dual(x), weight, weight_scales, bias),
+                     lambda: lib.quantized_linear(x, weight, weight_scales, dual(bias)), lambda: lib.int8_linear(codes, dual(scales), weight, weight_scales),
+                     lambda: lib.int8_linear(codes, scales, weight, dual(weight_scales)), lambda: lib.orthogonalize(dual(x)),
+                     lambda: lib.muon_step([x.clone()], [dual(x)], [x.clone()], 0.1), lambda: lib.muon_step([dual(x.clone())], [x], [x.clone()], 0.1)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        held = dual(x)
+        assert torch.equal(lib.quantized_linear(forward.unpack_dual(held).primal, weight, weight_scales, bias), want)
+        with forward._set_fwd_grad_enabled(False):
+            assert torch.equal(lib.quantized_linear(held, weight, weight_scales, bias), want)
+    assert torch.equal(lib.quantized_linear(held, weight, weight_scales, bias), want)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: lib.quantized_linear(v, weight, weight_scales, bias), (x,), (x,))
