@@ -1216,13 +1216,14 @@ void undifferentiated(const char* op, std::initializer_list<torch::Tensor> tenso
   }
 }
 
-// Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart or rows overlap.
+// Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart, rows overlap or x is
+// a lazily negated view, which holds the values' opposites (here and below: contiguous() keeps it one).
 torch::Tensor value_rows(const torch::Tensor& x, const char* name) {
   TORCH_CHECK(x.defined() && x.device().is_cuda(), name, " must be a GPU tensor");
   TORCH_CHECK(x.dim() >= 1, name, " must have rows");
   int64_t count = 1;
   for (int64_t d = 0; d + 1 < x.dim(); ++d) count *= x.size(d);
-  auto rows = x.dim() == 2 ? x : x.reshape({count, x.size(-1)});
+  auto rows = (x.dim() == 2 ? x : x.reshape({count, x.size(-1)})).resolve_neg();
   const bool plain = (rows.size(1) <= 1 || rows.stride(1) == 1) && (rows.size(0) <= 1 || rows.stride(0) >= rows.size(1));
   return plain ? rows : rows.contiguous();
 }
@@ -1234,8 +1235,9 @@ torch::Tensor room_for_codes(int64_t rows, int64_t k, const torch::Tensor& like)
 }
 
 // The same of codes that a caller gives: themselves, or a copy where they are not laid out so.
-torch::Tensor code_rows(const torch::Tensor& codes, const char* name) {
-  TORCH_CHECK(codes.defined() && codes.device().is_cuda(), name, " must be a GPU tensor");
+torch::Tensor code_rows(const torch::Tensor& codes_in, const char* name) {
+  TORCH_CHECK(codes_in.defined() && codes_in.device().is_cuda(), name, " must be a GPU tensor");
+  const auto codes = codes_in.resolve_neg();
   TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == torch::kInt8, name, " must be int8 [rows, columns]");
   const int64_t step = codes.stride(0), whole = (codes.size(1) + 15) / 16 * 16;
   // (the kernels read whole pieces, the last row's last one too)
@@ -1249,7 +1251,7 @@ torch::Tensor code_rows(const torch::Tensor& codes, const char* name) {
 }
 
 torch::Tensor scales_of(const torch::Tensor& scales, const torch::Tensor& codes, const char* name) {
-  auto s = beside(scales, codes, name);
+  auto s = beside(scales.defined() ? scales.resolve_neg() : scales, codes, name);
   TORCH_CHECK(s.scalar_type() == torch::kFloat32 && s.dim() == 1 && s.size(0) == codes.size(0), name,
               " must be float32 with a value for each of the ", codes.size(0), " rows of codes");
   return s;
@@ -1257,7 +1259,7 @@ torch::Tensor scales_of(const torch::Tensor& scales, const torch::Tensor& codes,
 
 torch::Tensor bias_of(const c10::optional<torch::Tensor>& bias, const torch::Tensor& weight) {
   if (!bias.has_value()) return torch::Tensor();
-  auto b = beside(*bias, weight, "bias");
+  auto b = beside(bias->defined() ? bias->resolve_neg() : *bias, weight, "bias");
   TORCH_CHECK(b.scalar_type() == torch::kFloat32 && b.dim() == 1 && b.size(0) == weight.size(0), "bias must be float32 [",
               weight.size(0), "]");
   return b;
@@ -1339,7 +1341,7 @@ torch::Tensor orthogonalize(const torch::Tensor& update, int64_t steps, const st
   const int tag = dense_tag(update.scalar_type(), "update");
   undifferentiated("orthogonalize", {update});
   c10::DeviceGuard guard(update.device());
-  auto u = update.contiguous();
+  auto u = update.resolve_neg().contiguous();
   auto out = torch::empty(u.sizes(), u.options());
   const int64_t rows = u.size(-2), cols = u.size(-1), count = u.numel() ? u.numel() / (rows * cols) : 0;
   const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
@@ -1376,9 +1378,9 @@ void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torc
     TORCH_CHECK(momenta[i].defined() && momenta[i].device() == like.device() && momenta[i].scalar_type() == torch::kFloat32 &&
                     momenta[i].sizes() == like.sizes(), "muon_step: momenta must be float32 of the weights' shape and device");
     for (const auto& t : {weights[i], grads[i], momenta[i]}) without_tangent("muon_step", t);
-    w[i] = weights[i].contiguous();
-    g[i] = grads[i].contiguous();
-    v[i] = momenta[i].contiguous();
+    w[i] = weights[i].resolve_neg().contiguous();
+    g[i] = grads[i].resolve_neg().contiguous();
+    v[i] = momenta[i].resolve_neg().contiguous();
     wp[i] = w[i].data_ptr();
     gp[i] = g[i].data_ptr();
     vp[i] = v[i].data_ptr<float>();

@@ -57,3 +57,22 @@ def test_forward_tangents():
     assert torch.equal(lib.quantized_linear(held, weight, weight_scales, bias), want)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda v: lib.quantized_linear(v, weight, weight_scales, bias), (x,), (x,))
+
+
+def test_lazily_negated_views():
+    lib, x, weight, weight_scales, bias, codes, scales = _dense()
+    lazy = lambda t: torch._neg_view((-t).contiguous())      # noqa: E731
+    assert lazy(x).is_neg() and torch.equal(lazy(x), x)
+    want = lib.quantized_linear(x, weight, weight_scales, bias)
+    for a, b, c in ((lazy(x), weight_scales, bias), (x, lazy(weight_scales), bias), (x, weight_scales, lazy(bias)),
+                    (lazy(x.t().contiguous()).t(), weight_scales, bias), (lazy(x.reshape(5, 1, 40)).reshape(5, 40), weight_scales, bias)):
+        assert torch.equal(lib.quantized_linear(a, weight, b, c), want)
+    assert torch.equal(lib.int8_linear(lazy(codes), lazy(scales), lazy(weight), weight_scales, bias), want)
+    assert torch.equal(lib.quantize_rows(lazy(x))[0], codes)
+    assert torch.equal(lib.orthogonalize(lazy(x)), lib.orthogonalize(x))
+    w, d, v = x.clone(), x.flip(0).contiguous(), 0.1 * x.roll(1, 1)
+    want_w, want_v = w.clone(), v.clone()
+    lib.muon_step([want_w], [d], [want_v], 0.1)
+    held_w, held_v = lazy(w), lazy(v)
+    lib.muon_step([held_w], [lazy(d)], [held_v], 0.1)
+    assert held_w.is_neg() and torch.equal(held_w, want_w) and torch.equal(held_v, want_v)
