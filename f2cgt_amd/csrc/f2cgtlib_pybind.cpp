@@ -23,6 +23,7 @@
 
 #include <array>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/autocast_mode.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -1353,6 +1354,69 @@ torch::Tensor orthogonalize(const torch::Tensor& update, int64_t steps, const st
   return out;
 }
 
+// A matrix's elements in memory: rows of `inner` elements, `step` bytes apart, at multiples of `stride` from `from` on.
+struct Places {
+  int64_t from, rows, stride, inner, step, size;
+  explicit Places(const torch::Tensor& t) : from((int64_t)reinterpret_cast<intptr_t>(t.data_ptr())), size((int64_t)t.element_size()) {
+    const int out = t.stride(0) >= t.stride(1) ? 0 : 1;
+    rows = t.size(out); stride = t.stride(out) * size;
+    inner = t.size(1 - out); step = t.stride(1 - out) * size;
+    if (rows == 1) stride = 0;
+    if (inner == 1) step = 0;
+  }
+  int64_t row_bytes() const { return (inner - 1) * step + size; }
+  int64_t end() const { return from + (rows - 1) * stride + row_bytes(); }
+};
+
+// Whether a row of b that begins `apart` bytes behind one of a shares elements with it; rows whose elements lie in between each
+// other's do not.  (Where steps differ, rows that only just reach each other count as sharing.)
+bool rows_share(const Places& a, const Places& b, int64_t apart) {
+  if (apart >= a.row_bytes() || -apart >= b.row_bytes()) return false;
+  int64_t by = a.step, rest = b.step;
+  while (rest != 0) { const int64_t more = by % rest; by = rest; rest = more; }      // the steps' greatest common divisor
+  if (by == 0) return true;                                                          // (of single elements)
+  const int64_t phase = (apart % by + by) % by;
+  return phase < a.size || phase > by - b.size;
+}
+
+// Whether two matrices share elements.  (Those whose rows reach into the next one count as sharing whatever is between their ends.)
+bool share_memory(const Places& a, const Places& b) {
+  if (a.from >= b.end() || b.from >= a.end()) return false;
+  for (const Places* p : {&a, &b})
+    if (p->rows > 1 && p->stride < p->row_bytes()) return true;
+  const int64_t apart = b.from - a.from;
+  if (a.rows > 1 && a.stride == b.stride) {                // each row of one meets the same two of the other
+    const int64_t next = (apart >= 0 ? apart : apart - a.stride + 1) / a.stride;
+    for (int64_t q = next; q <= next + 1; ++q)
+      if (q < a.rows && q > -b.rows && rows_share(a, b, apart - q * a.stride)) return true;
+    return false;
+  }
+  for (int64_t i = 0; i < a.rows; ++i) {
+    const int64_t to = apart - i * a.stride;               // from this row to b's first
+    int64_t k = to + b.row_bytes() > 0 || b.rows == 1 ? 0 : -(to + b.row_bytes()) / b.stride + 1;
+    for (; k < b.rows && to + k * b.stride < a.row_bytes(); ++k)
+      if (rows_share(a, b, to + k * b.stride)) return true;
+  }
+  return false;
+}
+
+// What is written shares no memory with anything else of the lists.
+void check_apart(const std::vector<torch::Tensor>& weights, const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>& momenta) {
+  std::vector<std::pair<Places, bool>> all;                // (whether it is written)
+  for (size_t i = 0; i < weights.size(); ++i) {
+    at::assert_no_internal_overlap(weights[i]);
+    at::assert_no_internal_overlap(momenta[i]);
+    all.emplace_back(Places(weights[i]), true);
+    all.emplace_back(Places(momenta[i]), true);
+    all.emplace_back(Places(grads[i]), false);
+  }
+  std::sort(all.begin(), all.end(), [](const auto& a, const auto& b) { return a.first.from < b.first.from; });
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t j = i + 1; j < all.size() && all[j].first.from < all[i].first.end(); ++j)
+      TORCH_CHECK(!(all[i].second || all[j].second) || !share_memory(all[i].first, all[j].first),
+                  "muon_step: a weight or a momentum shares memory with another tensor of the step");
+}
+
 // One step of weights of one shape, in place; momenta too.
 void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torch::Tensor>& grads,
                const std::vector<torch::Tensor>& momenta, double step_size, double decay, double momentum, bool nesterov,
@@ -1385,12 +1449,7 @@ void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torc
     gp[i] = g[i].data_ptr();
     vp[i] = v[i].data_ptr<float>();
   }
-  {
-    std::vector<const void*> all;
-    for (size_t i = 0; i < count && like.numel(); ++i) { all.push_back(weights[i].data_ptr()); all.push_back(momenta[i].data_ptr()); }
-    std::sort(all.begin(), all.end());
-    TORCH_CHECK(std::adjacent_find(all.begin(), all.end()) == all.end(), "muon_step: a weight or a momentum is listed twice");
-  }
+  if (like.numel() > 0) check_apart(weights, grads, momenta);
   const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
   const int64_t bytes = f2cgt_muon_workspace_bytes((int64_t)count, like.size(0), like.size(1));
   auto ws = torch::empty({bytes}, like.options().dtype(torch::kUInt8));

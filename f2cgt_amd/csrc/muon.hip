@@ -15,6 +15,10 @@
 // b t + c t^2, which may be twice what the whole polynomial is: its planes hold half as much where they have to.
 #include "tile_product.hpp"
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 namespace f2cgt {
 namespace {
 
@@ -968,6 +972,32 @@ int check_muon(const char* what, int64_t count, int64_t rows, int64_t cols, int 
   return 0;
 }
 
+// Whether what a step writes shares no memory with anything else of its lists (of dense matrices of `values`).
+int check_apart(const char* what, void* const* weights, int weight_size, const void* const* grads, int grad_size, float* const* momenta,
+                int64_t count, int64_t values) {
+  struct Range { uintptr_t from, end; bool written; };
+  std::unique_ptr<Range[]> all(new (std::nothrow) Range[3 * count]);
+  F2CGT_REQUIRE(all != nullptr, F2CGT_E_INVALID, "%s: out of host memory", what);
+  auto put = [&](int64_t i, const void* p, int size, bool written) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+    all[i] = Range{from, from + (uintptr_t)(values * size), written};
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    put(3 * i, weights[i], weight_size, true);
+    put(3 * i + 1, grads[i], grad_size, false);
+    put(3 * i + 2, momenta[i], 4, true);
+  }
+  std::sort(all.get(), all.get() + 3 * count, [](const Range& x, const Range& y) { return x.from < y.from; });
+  uintptr_t end = 0, written_end = 0;                      // of those before
+  for (int64_t i = 0; i < 3 * count; ++i) {
+    const Range& r = all[i];
+    F2CGT_REQUIRE(r.from >= (r.written ? end : written_end), F2CGT_E_INVALID, "%s: a weight or a momentum shares memory with another matrix", what);
+    end = std::max(end, r.end);
+    if (r.written) written_end = std::max(written_end, r.end);
+  }
+  return 0;
+}
+
 int run_muon(const char* what, MuonArgs a, int64_t count, int64_t rows, int64_t cols, int steps, const float* coefficients,
              double most_p, void* const* out, const void* const* u, float* const* held, int64_t u_step, void* workspace, hipStream_t st) {
   a.s = shape_of(rows, cols);
@@ -1063,6 +1093,7 @@ extern "C" int f2cgt_muon_step(void* const* weights, int weight_dtype, const voi
     F2CGT_REQUIRE(weights[i] && grads[i] && momenta[i] && aligned(weights[i], type_size(weight_dtype)) &&
                       aligned(grads[i], type_size(grad_dtype)) && aligned(momenta[i], 4),
                   F2CGT_E_INVALID, "%s: null or misaligned buffer", what);
+  if (int rc = check_apart(what, weights, type_size(weight_dtype), grads, type_size(grad_dtype), momenta, count, rows * cols)) return rc;
   const int64_t bytes = workspace_of(count, rows, cols);
   F2CGT_REQUIRE(bytes == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= bytes), F2CGT_E_INVALID,
                 "%s: workspace too small or misaligned", what);

@@ -431,7 +431,8 @@ int f2cgt_quantized_linear(const void* x, int dtype, int64_t ld, const int8_t* w
  * f2cgt_muon_step: lists (host) of `count` dense matrices [rows, cols] on the device, per matrix
  *   held = momentum held + (1 - momentum) grad;  u = nesterov ? momentum held + (1 - momentum) grad : held
  *   weight = (1 - decay) weight - step_size orthogonalize(u)
- * in place; momenta fp32, weights and gradients of any type above.
+ * in place; momenta fp32, weights and gradients of any type above.  Weights and momenta share no memory with anything else of
+ * the lists (gradients may, with each other).
  *
  * workspace (both): f2cgt_muon_workspace_bytes, 256-byte aligned, contents irrelevant. */
 int64_t f2cgt_muon_workspace_bytes(int64_t count, int64_t rows, int64_t cols);

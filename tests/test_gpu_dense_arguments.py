@@ -76,3 +76,44 @@ def test_lazily_negated_views():
     held_w, held_v = lazy(w), lazy(v)
     lib.muon_step([held_w], [lazy(d)], [held_v], 0.1)
     assert held_w.is_neg() and torch.equal(held_w, want_w) and torch.equal(held_v, want_v)
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 30), (200, 300)])
+def test_steps_of_views_into_one_buffer(rows, cols):
+    """Views whose elements lie in between each other's take their step, those that share some are refused before anything is written."""
+    lib = f2cgt_amd.load()
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")       # noqa: E731
+    wide = rand(rows, 4 * cols)
+    views = [wide[:, i * cols:(i + 1) * cols] for i in range(4)]
+    d = rand(rows, cols)
+    want = [v.clone() for v in views]
+    lib.muon_step(want[:2], [d, d], want[2:], 0.1)
+    lib.muon_step(views[:2], [d, d], views[2:], 0.1)
+    assert all(torch.equal(a, b) for a, b in zip(views, want))
+    deep = rand(rows, cols, 3)                              # every third element
+    want = [deep[..., i].clone() for i in range(3)]
+    lib.muon_step([want[0]], [want[1]], [want[2]], 0.1)
+    lib.muon_step([deep[..., 0]], [deep[..., 1]], [deep[..., 2]], 0.1)
+    assert torch.equal(deep[..., 0], want[0]) and torch.equal(deep[..., 2], want[2])
+    turned = rand(2 * cols, rows)
+    want = [turned[:cols].t().clone(), turned[cols:].t().clone()]
+    lib.muon_step([want[0]], [d], [want[1]], 0.1)
+    lib.muon_step([turned[:cols].t()], [d], [turned[cols:].t()], 0.1)
+    assert torch.equal(turned[:cols].t(), want[0])
+
+    flat = rand(2 * rows * cols)
+    one, two = flat[:rows * cols].view(rows, cols), flat[rows * cols:].view(rows, cols)
+    late = flat[rows * cols - 1:2 * rows * cols - 1].view(rows, cols)
+    square = rand(rows, rows)
+    v = rand(rows, cols)
+    half = v.view(torch.bfloat16)[:, :cols]                 # (NaNs among them)
+    bits = lambda t: t.contiguous().view(torch.uint8)       # noqa: E731
+    for w, grads, held in (([one], [v], [v]), ([one], [one], [v]), ([one], [late], [v]), ([one], [v], [late]), ([one, late], [d, d], [v, d.clone()]),
+                           ([wide[:, :cols]], [v], [wide[:, cols - 1:2 * cols - 1]]), ([square], [square.clone()], [square.t()]),
+                           ([half], [half.clone()], [v]), ([one[:1].expand(rows, cols)], [v], [two]), ([one], [v], [two[:1].expand(rows, cols)])):
+        before = [t.clone() for t in w + grads + held]
+        with pytest.raises(RuntimeError):
+            lib.muon_step(w, grads, held, 0.1)
+        assert all(torch.equal(bits(t), bits(b)) for t, b in zip(w + grads + held, before))
+    lib.muon_step([one], [v[:1].expand(rows, cols)], [two], 0.1)
