@@ -15,6 +15,7 @@ Everything numerical happens in `F2CGTLib` (f2cgt_amd.load()); this module only 
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -747,6 +748,9 @@ class MySAGEConv(nn.Module):
 
 
 # ---- training and serving the dense weights ----------------------------------------------------------
+_DENSE_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
 class Muon(torch.optim.Optimizer):
     """Optimiser of weight matrices: momentum, the update made orthogonal by Newton-Schulz products, decoupled weight decay.
     Weights of one shape and type take their step together (`muon_step`).
@@ -758,23 +762,44 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, scale="spectral",
                  coefficients=(3.4445, -4.7750, 2.0315)):
-        if not lr >= 0.0:
+        defaults = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, scale=scale,
+                        coefficients=tuple(coefficients))
+        self._check_options(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check_options(group):
+        from . import capi as c_abi
+        if not group["lr"] >= 0.0:
             raise ValueError("lr must not be negative")
-        if not 0.0 <= momentum < 1.0:
+        if not 0.0 <= group["momentum"] < 1.0:
             raise ValueError("momentum must be in [0, 1)")
-        if not weight_decay >= 0.0:
+        if not group["weight_decay"] >= 0.0:
             raise ValueError("weight_decay must not be negative")
-        if scale not in ("spectral", "rms"):
+        if not group["lr"] * group["weight_decay"] < 1.0:
+            raise ValueError("lr * weight_decay must be below 1")
+        if group["scale"] not in ("spectral", "rms"):
             raise ValueError("scale must be 'spectral' or 'rms'")
-        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
-                                      scale=scale, coefficients=tuple(coefficients)))
+        if len(group["coefficients"]) != 3:
+            raise ValueError("coefficients must be three numbers")
+        # (a call for no matrix: the library's own check of steps and coefficients)
+        if c_abi.lib().f2cgt_orthogonalize(None, c_abi.DT_F32, None, 0, 0, 0, int(group["steps"]), (ctypes.c_float * 3)(*group["coefficients"]),
+                                           None, 0, None):
+            raise ValueError(c_abi.lib().f2cgt_last_error().decode())
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() != 2:
-                self.param_groups.pop()
-                raise ValueError("Muon trains matrices only (got a parameter of shape %s)" % (tuple(p.shape),))
+        group = self.param_groups[-1]
+        try:
+            self._check_options(group)
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError("Muon trains matrices only (got a parameter of shape %s)" % (tuple(p.shape),))
+                if p.dtype not in _DENSE_TYPES:
+                    raise ValueError("Muon trains float32, float16 and bfloat16 only (got %s)" % p.dtype)
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -791,6 +816,12 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:                  # before any of them takes its step: options may have changed since
+            self._check_options(group)
+            for p in group["params"]:
+                if p.grad is not None and (not p.is_cuda or p.grad.layout != torch.strided or p.grad.dtype not in _DENSE_TYPES):
+                    raise ValueError("Muon takes dense gradients of float32, float16 or bfloat16 on the GPU only (got %s %s on %s)" %
+                                     (p.grad.layout, p.grad.dtype, p.device))
         for group in self.param_groups:
             alike = {}
             for p in group["params"]:
