@@ -556,6 +556,7 @@ void launch_few(const LinearArgs& a, hipStream_t st) {
 //   64 x 64 tiles by four groups of waves or by two, 64 x 128 or 128 x 128 tiles: 256 x 4096 -> 4096 12.8, 14.3, 20.6, 24.0;
 //     33 x 4096 -> 16384 15.8, 15.2, 21.2, 23.4; 490 x 1135 -> 9698 40, 26.7, 20.3, 21.2; 2048 x 2048 -> 2048 31, 20.5, 15.7,
 //     17.0; 60001 x 602 -> 128, the last two 18.5 and 17.1; 4099 x 4096 -> 4096 102 and 96
+//   (tests/test_gpu_dense_forms.py and test_gpu_int8_linear.py have a shape for each)
 //   128 x 128 or 256 x 256: 8192 x 8192 -> 8192 586 and 509, 4099 x 4096 -> 4096 (272 large tiles for 256 CUs) 96 and 124
 int linear(const char* what, LinearArgs a, hipStream_t st) {
   if (a.m == 0 || a.n == 0) return 0;

@@ -458,7 +458,7 @@ void launch_update(const MuonArgs& a, int64_t n, int from, int last, hipStream_t
 // us of Gram products of 1000 x 2051: 64 x 64 30, in four groups 19.5, 128 x 128 42; 2048 x 2048: 34, 54, 42; eight of 1000 x 700: 18, 27, 24;
 // 3000 x 3000: 97, 128, 86, 192 x 192 128; 4096 x 4096: 195, 262, 169, 168 (528 and 253 tiles).
 // Updates: 1000 x 2051: 64 x 64 20.8, 64 x 128 23.5, 128 x 128 27.1; 2048 x 2048: 50, 43, 49; 3000 x 3000: 160, 130, 142;
-// 4096 x 4096: 349, 284, 237, 256 x 256 299.
+// 4096 x 4096: 349, 284, 237, 256 x 256 299.  (tests/test_gpu_dense_forms.py and test_gpu_muon.py have a shape for each.)
 int64_t pairs_cost(int64_t tiles, int64_t cus) {
   const int64_t left = tiles % (2 * cus);
   return 93 * (tiles / (2 * cus)) + (left == 0 ? 0 : left <= cus ? 67 : 93);

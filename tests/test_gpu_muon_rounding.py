@@ -24,10 +24,10 @@ def _two_planes(x):
     return (hi.double() + (x - hi).half().double()) / 4096
 
 
-def _iterate(u, steps, coefficients, operand=lambda x: x, dtype=torch.float64):
-    """The definition in `dtype`, on the host; `operand` is done to what goes into a product."""
+def _iterate(u, steps, coefficients, operand=lambda x: x, dtype=torch.float64, where="cpu"):
+    """The definition in `dtype`; `operand` is done to what goes into a product."""
     a, b, c = coefficients
-    x = u.detach().cpu().to(dtype)
+    x = u.detach().to(where).to(dtype)
     turned = x.shape[0] > x.shape[1]
     x = x.t() if turned else x
     x = x / (x.norm() + 1e-7)
@@ -39,19 +39,19 @@ def _iterate(u, steps, coefficients, operand=lambda x: x, dtype=torch.float64):
     return x.t() if turned else x
 
 
-def check(got, u, steps=5, coefficients=DEFAULT):
+def check(got, u, steps=5, coefficients=DEFAULT, where="cpu"):
     """Operands of two planes cost `far`, and as much for the products' fourth part, which is left out.  Each product's fp32 sum is
     off too, and later steps multiply that as they do in a float32 evaluation, which adds its own; four times its distance
     `single` is what the other tests of these results take: E = 2 far + 4 single + 2^-20 of the norm.  A rounded y is as near to
     `want` as the rounded `want`, but for 2 |y - want|, value by value (it is rounded otherwise only where `want` is as near to the
     middle of two neighbours): E twice beside the result's own rounding."""
-    want = _iterate(u, steps, coefficients)
+    want = _iterate(u, steps, coefficients, where=where)
     norm = float(want.norm())
-    far = float((_iterate(u, steps, coefficients, _two_planes) - want).norm())
-    single = float((_iterate(u, steps, coefficients, dtype=torch.float32).double() - want).norm())
+    far = float((_iterate(u, steps, coefficients, _two_planes, where=where) - want).norm())
+    single = float((_iterate(u, steps, coefficients, dtype=torch.float32, where=where).double() - want).norm())
     error = 2 * far + 4 * single + 2.0 ** -20 * norm
     own = float((want.to(got.dtype).double() - want).norm())
-    off = float((got.cpu().double() - want).norm())
+    off = float((got.to(where).double() - want).norm())
     assert off <= own + 2 * error, (off / norm, own / norm, error / norm)
 
 
