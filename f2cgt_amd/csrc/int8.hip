@@ -251,7 +251,7 @@ struct LinearEpilogue {
 // multiply, but there are enough of them for fewer rows: 60 001 x 602 -> 128 in 17 us, 4.1 TB/s of the codes, which is its bound.
 template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void int8_linear_kernel(LinearArgs a) {
-  typedef TileProduct<Int8Op, BM, BN, WM, WN, 2, GROUPS> Tile;
+  typedef TileProduct<Int8Op, BM, BN, WM, WN, GROUPS> Tile;
   uint32_t i, j;
   tile_of(place_of(blockIdx.x, gridDim.x), (uint32_t)ceil_div(a.m, BM), (uint32_t)ceil_div(a.n, BN), DEEP, i, j);
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256) void int8_rows_kernel(LinearArgs a, int64_t ld
       *reinterpret_cast<Words<V>*>(lds + c / kLine * kM * kLine + piece_at(r, c % kLine / 16) + c % 16) = q;
     }
   }
-  wait_copies<0>();                            // (the weights: a barrier alone does not wait for copies into LDS)
+  wait_copies();                            // (the weights: a barrier alone does not wait for copies into LDS)
   __syncthreads();
   const int wi = 32 * (wave & 1), wj = 64 * (wave >> 1);
   intx16 acc[2];

@@ -284,7 +284,7 @@ struct SymmetricEpilogue {
 
 template <bool SQUARE, int B, int W, int WJ, int GROUPS, int DEEP>
 __global__ __launch_bounds__((B / W) * (B / WJ) * GROUPS * kWave) void muon_symmetric_kernel(MuonArgs a) {
-  typedef TileProduct<SplitOp, B, B, W, WJ, 2, GROUPS> Tile;
+  typedef TileProduct<SplitOp, B, B, W, WJ, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const uint32_t tiles = (uint32_t)ceil_div(a.s.r, B), each = tiles * (tiles + 1) / 2, at = place_of(blockIdx.x, gridDim.x);
   uint32_t i, j;
@@ -311,7 +311,7 @@ struct PartEpilogue {
 };
 
 __global__ __launch_bounds__(1024) void muon_gram_part_kernel(MuonArgs a, int splits) {
-  typedef TileProduct<SplitOp, 64, 64, 32, 32, 2, 4> Tile;
+  typedef TileProduct<SplitOp, 64, 64, 32, 32, 4> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   // the parts of a tile go to different XCDs, tiles of a part to the same
@@ -424,7 +424,7 @@ struct UpdateEpilogue {
 
 template <int BM, int BN, int WM, int WN, int GROUPS, int DEEP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * GROUPS * kWave) void muon_update_kernel(MuonArgs a, int from, int last) {
-  typedef TileProduct<SplitOp, BM, BN, WM, WN, 2, GROUPS> Tile;
+  typedef TileProduct<SplitOp, BM, BN, WM, WN, GROUPS> Tile;
   __shared__ __attribute__((aligned(128))) char lds0[Tile::kStage], lds1[Tile::kStage];
   const Shape& s = a.s;
   const uint32_t tiles_r = (uint32_t)ceil_div(s.r, BM), tiles_l = (uint32_t)ceil_div(s.l, BN), at = place_of(blockIdx.x, gridDim.x);

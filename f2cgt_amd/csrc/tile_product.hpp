@@ -63,23 +63,19 @@ __device__ __forceinline__ float word_of(int v) { return __builtin_bit_cast(floa
 __device__ __forceinline__ void add_word(fltx16& sums, int i, float word) { sums[i] += word; }
 __device__ __forceinline__ void add_word(intx16& sums, int i, float word) { sums[i] += __builtin_bit_cast(int, word); }
 
-// Waits until at most `loads` of this wave's copies into LDS are under way and its reads of LDS are done.
-template <int loads>
-__device__ __forceinline__ void wait_copies() {
-  __builtin_amdgcn_s_waitcnt((loads & 15) | (loads >> 4) << 14 | 7 << 4 | 0 << 8);
-}
+// Waits until this wave's copies into LDS and its reads of LDS are done.
+__device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(7 << 4); }
 
-// The pieces of a tile go from memory into LDS without a stop in registers, STAGES - 1 steps ahead of the one that is
-// multiplied; a step costs one barrier.  The stages are LDS arrays of their own (Buffers), which is how the compiler knows that a
-// read of one need not wait for the copies into the others.
+// The pieces of a tile go from memory into LDS without a stop in registers, a step ahead of the one that is multiplied; a step
+// costs one barrier.  The two stages are LDS arrays of their own (Buffers), which is how the compiler knows that a read of one need not
+// wait for the copies into the other.
 //
 // GROUPS > 1: groups of waves take the steps in turn, each into its own part of the stages, and add their sums in the end: for
 // tiles that are fewer than the chip's CUs (256 x 4096 x 4096 in 8 bits: four groups 12.8 us, two 14.3, one 20.6).
 //
-// Two stages are what all kernels use: with three or four the same tiles took as long or longer (fp16 planes, 1000 x 2051: 19.6 us with
-// two, 20.1 and 22.2), for the time of a step is the LDS's, which writes each byte once and reads it once for every wave beside or
+// With three stages or four the same tiles took as long or longer (fp16 planes, 1000 x 2051: 19.6 us with two, 20.1 and 22.2), for the time of a step is the LDS's, which writes each byte once and reads it once for every wave beside or
 // below, and a stage more is a workgroup less on a CU.
-template <class Op, int BM, int BN, int WM, int WN, int STAGES, int GROUPS = 1>
+template <class Op, int BM, int BN, int WM, int WN, int GROUPS = 1>
 struct TileProduct {
   static constexpr int kWaves = (BM / WM) * (BN / WN), kThreads = kWaves * kWave;      // of a group
   static constexpr int kBlock = kThreads * GROUPS;
@@ -91,9 +87,9 @@ struct TileProduct {
   static constexpr int kPieces = (BM + BN) * 8 / kThreads;             // copies of a thread in a step
   static_assert((BM + BN) * 8 % kThreads == 0 && BM * 8 % kThreads == 0, "whole pieces per thread");
   static constexpr int kStripsPerStage = kStage / kStrip;
-  static_assert(kStripsPerStage * STAGES >= kWaves * GROUPS, "a strip per wave");
+  static_assert(kStripsPerStage * 2 >= kWaves * GROUPS, "a strip per wave");
   typedef typename Op::Acc Acc;
-  typedef char* Buffers[STAGES];
+  typedef char* Buffers[2];
 
   // Rows [row0, row0 + BM) of a against rows [col0, col0 + BN) of b.  epilogue(strip, row, col, lane): strip [32][kLd] holds
   // the sums of 32 rows from `row` on and WN columns from `col` on.
@@ -182,21 +178,19 @@ struct TileProduct {
       }
     };
     if (steps > 0) {
-      // Step `step` from stage s: its copies are done when only those of the STAGES - 2 steps behind it are under way; then
-      // all waves have them, and nobody reads the stage of the step before any more, which the next copies overwrite.  (There
-      // are always as many copies under way: behind the last step it is copied again, into a stage that nobody reads.)
+      // Step `step` from stage s: this wave's copies are done, then all waves' are, and nobody reads the other stage any more, into
+      // which the next step's go.  (There always are some: behind the last step it is copied again, into a stage that nobody reads.)
       auto held = [&](int step) { return step < steps ? step : steps - 1; };
       const int part = group * kPart;
-#pragma unroll
-      for (int s = 0; s < STAGES - 1; ++s) copy(lds[s] + part, held(s * GROUPS + group));
+      copy(lds[0] + part, held(group));
       int step = group;
       while (true) {
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s) {
-          wait_copies<(STAGES - 2) * kPieces>();
+        for (int s = 0; s < 2; ++s) {
+          wait_copies();
           if (Op::kTrim && left < kLine && step == steps - 1) trim(lds[s] + part);
           __builtin_amdgcn_s_barrier();
-          copy(lds[(s + STAGES - 1) % STAGES] + part, held(step + (STAGES - 1) * GROUPS));
+          copy(lds[1 - s] + part, held(step + GROUPS));
           __builtin_amdgcn_sched_barrier(0);             // (the compiler would sink them to the step's end)
           if (GROUPS == 1 || step < steps) multiply(lds[s] + part);
           step += GROUPS;
@@ -205,14 +199,14 @@ struct TileProduct {
       }
     }
   done:
-    wait_copies<0>();
+    wait_copies();
     __builtin_amdgcn_s_barrier();
     // The columns' operand came first: a lane holds, of one row, four columns after four.
     auto strip_of = [&](int of) {
       const int n = of * kWaves + wave;
       char* at_stage = nullptr;
 #pragma unroll
-      for (int s = 0; s < STAGES; ++s)
+      for (int s = 0; s < 2; ++s)
         if (n / kStripsPerStage == s) at_stage = lds[s] + (n % kStripsPerStage) * kStrip;
       return reinterpret_cast<float*>(at_stage);
     };
