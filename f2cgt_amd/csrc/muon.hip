@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
 // ---- planes ----------------------------------------------------------------------------------------------------------------
 // v = hi + lo: a rounding, the exact rest rounded, and their sum.  The two ones are hidden from the compiler, so that it takes the
 // instruction that multiplies and adds fp16 and fp32 numbers and does not convert them first (two instructions a value instead of
-// three, one instead of three for the sum; same results: 48 of 128 x 128 46.8 -> 42.9 us then, with G kept in registers for P).
+// three, one instead of three for the sum; same results: two of 256 x 128 82.9 -> 78.6 us then, with G kept in registers for P).
 __device__ __forceinline__ float hidden(float one) {
   asm("" : "+s"(one));
   return one;
@@ -245,8 +245,9 @@ __device__ __forceinline__ void strip_passes(float* strip, int64_t row0, int64_t
 }
 
 // G from X, or P = b G + c G G from G (g not null): the tiles on and below the diagonal, each written on both sides of it.
-// At 4096 x 4096, where the card's power bounds them, G and P take 180 us each: 1.15e15 executed operations a second.  At 1000 x 2051 there are 136 tiles of 64 x 64 for 256 CUs, each of whose LDS is read and written for
-// most of the time (19.5 and 10.5 us); larger tiles leave more of the chip without one, and a third or fourth stage gained nothing.
+// At 4096 x 4096, where the card's power bounds them, G and P take 230 us each in a row of steps: 1.0e15 executed operations a second.
+// At 1000 x 2051 there are 136 tiles of 64 x 64 for 256 CUs, each of whose LDS is read and written for most of the time (19.6 and
+// 12.2 us); larger tiles leave more of the chip without one, and a third or fourth stage gained nothing.
 template <int WN>
 struct SymmetricEpilogue {
   const MuonArgs& a;
@@ -360,9 +361,9 @@ int gram_splits(int64_t n, const Shape& s) {
   return splits >= 2 && steps - steps / splits >= 20 ? (int)splits : 1;
 }
 
-// X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  At 4096 x 4096 300 us, 1.37e15 executed
-// operations a second, what the library's fp16 product of 8192 x 8192 x 8192 reaches when it runs as long (1.32e15); 22 us at 1000 x 2051.  (a X from its own planes: with a in
-// P's diagonal, which is rounded to 22 bits there, errors were half as much again.)
+// X = a X + P X in planes, both ways round, or the last one into the caller's matrix.  At 4096 x 4096 371 us in a row of steps, 1.1e15
+// executed operations a second at the 1.5 GHz that the card's power leaves (the library's fp16 product of 8192 x 8192 x 8192 in a long run 1.32e15);
+// 22 us at 1000 x 2051.  (a X from its own planes: with a in P's diagonal, which is rounded to 22 bits there, errors were half as much again.)
 template <int WN>
 struct UpdateEpilogue {
   const MuonArgs& a;
@@ -618,7 +619,9 @@ __device__ __forceinline__ void store_strips(const MuonArgs& a, int64_t z, float
     }
 }
 
-// Up to 32 rows, all in fp32 (32 x 32 x 2 instructions): a product of this size is latency, not rate.
+// Up to 32 rows, all in fp32 (32 x 32 x 2 instructions): a product of this size is latency, not rate.  32 x 256 19 us, 20 x 300 27,
+// 16 x 128 15, 48 of 32 x 128 16; of five steps, each three products that need each other, four barriers and a sum over the waves, 2.5 to 5
+// us a step.  P, 32 x 32, is one wave's.
 template <int S>
 __global__ __launch_bounds__(kOneWaves * kWave) void muon_narrow_kernel(MuonArgs a, int steps) {
   constexpr int kRow = 32 + 4;                             // floats of a row of 32 in LDS
@@ -715,10 +718,11 @@ __device__ __forceinline__ uint32_t beside(halfx2 rows, uint32_t turn) {
   return __builtin_amdgcn_perm(next, own, turn);
 }
 
-// 48 of 128 x 128 in bf16 40.5 us, two of 256 x 128 in fp32 74.  Of a step's 27 thousand clocks in the latter G takes 7500 and its planes
+// 48 of 128 x 128 in bf16 48 us, two of 256 x 128 in fp32 74.  Of a step's 27 thousand clocks in the latter G takes 7500 and its planes
 // 2200, P 5300, the update 8100 and the writing of X's lines 4100 (6000 value by value instead of by pairs); 15 400 of them issue matrix instructions on each SIMD,
 // the rest is the splitting of values, reads and writes of LDS, and the waits between three products that need each other.  Tiles over the whole chip would
-// be seventeen launches, 4 us and more each.
+// be seventeen launches, 4 us and more each.  Up to 128 columns there are four strips of them, and half of the waves have none in the
+// update and the writing of X's lines.
 //
 // From 33 to 32 RT rows: products of planes.  LDS: X's lines, a column tile of 32
 // after the other, while G is made; then G's and P's, of 32 RT rows by RT column tiles each, in the same place.  Where there is

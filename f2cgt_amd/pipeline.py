@@ -876,7 +876,9 @@ class Int8Linear(nn.Module):
 
 def int8_layers(module):
     """`module` for serving: every plain `nn.Linear` below it replaced by an `Int8Linear` of its weights, in place.  A
-    `MySAGEConv` then makes its dense part in 8 bits."""
+    `MySAGEConv` then makes its dense part in 8 bits: two products, their sum and the activation, one after the other.  That is for long
+    blocks and wide layers: 250 000 x (100 + 100) -> 128 takes 194 us, in fp32 262; 10 000 x (128 + 128) -> 256 31 and 45; 1024 x (1024 + 1024) -> 1024 33
+    and 47; but at 1024 x (128 + 128) -> 256 the host's four calls take 25 us, the one call in fp32 10."""
     for name, child in list(module.named_children()):
         if _plain_linear(child):
             setattr(module, name, Int8Linear(child))
