@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import numpy as np
 import torch
@@ -783,7 +784,7 @@ class Muon(torch.optim.Optimizer):
         if len(group["coefficients"]) != 3:
             raise ValueError("coefficients must be three numbers")
         # (a call for no matrix: the library's own check of steps and coefficients)
-        if c_abi.lib().f2cgt_orthogonalize(None, c_abi.DT_F32, None, 0, 0, 0, int(group["steps"]), (ctypes.c_float * 3)(*group["coefficients"]),
+        if c_abi.lib().f2cgt_orthogonalize(None, c_abi.DT_F32, None, 0, 0, 0, operator.index(group["steps"]), (ctypes.c_float * 3)(*group["coefficients"]),
                                            None, 0, None):
             raise ValueError(c_abi.lib().f2cgt_last_error().decode())
 

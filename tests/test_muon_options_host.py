@@ -27,6 +27,12 @@ def test_every_group(bad):
     assert opt.param_groups[1]["scale"] == "rms" and opt.param_groups[1]["momentum"] == 0.95
 
 
+def test_steps_are_a_whole_number():
+    with pytest.raises(TypeError):
+        pipeline.Muon([{"params": [_matrix()], "steps": 2.5}])
+    pipeline.Muon([{"params": [_matrix()], "steps": torch.tensor(3)}])
+
+
 def test_parameters():
     for bad in (torch.nn.Parameter(torch.zeros(3)), _matrix(torch.float64), _matrix(torch.complex64)):
         with pytest.raises(ValueError):
