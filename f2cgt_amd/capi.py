@@ -67,6 +67,16 @@ SIGNATURES = {
     "f2cgt_muon_workspace_bytes": ([L, L, L], c_int64),
     "f2cgt_orthogonalize": ([P, I, P, L, L, L, I, P, P, L, P], c_int),
     "f2cgt_muon_step": ([P, I, P, I, P, L, L, L, ctypes.c_float, ctypes.c_float, ctypes.c_float, I, I, P, P, L, P], c_int),
+    "f2cgt_layer_norm": ([P, I, L, P, P, I, P, P, P, P, L, P, L, L, ctypes.c_float, P], c_int),
+    "f2cgt_layer_norm_grad_workspace_bytes": ([I, L, L], c_int64),
+    "f2cgt_layer_norm_grad": ([P, I, L, P, L, P, L, P, P, P, P, I, P, P, P, I, P, L, L, L, P], c_int),
+    "f2cgt_pack_activations": ([P, I, L, P, L, P, L, L, P], c_int),
+    "f2cgt_unpack_activations": ([P, L, P, P, I, L, L, P], c_int),
+    "f2cgt_packed_linear_grad_workspace_bytes": ([I, L, L, L], c_int64),
+    "f2cgt_packed_linear_grad": ([P, I, L, P, L, P, P, P, I, P, L, L, L, L, P], c_int),
+    "f2cgt_embedding": ([P, I, L, P, I, P, ctypes.c_float, L, L, L, P], c_int),
+    "f2cgt_embedding_grad_workspace_bytes": ([L, L, L], c_int64),
+    "f2cgt_embedding_grad": ([P, I, L, P, I, P, ctypes.c_float, P, L, L, L, L, P], c_int),
     "f2cgt_kmeans_update_static": ([P, P, P, P, P, P, I, ctypes.c_float, L, L, L, P], c_int),
 }
 

@@ -1,0 +1,649 @@
+// Learnt rows: rows of a table by id, scaled, and the gradient of the table.
+//
+//   out_i = scale * table[id_i]                     dtable_r = scale * sum over i with id_i = r, in their order, of grad_i
+//
+// An id outside the table (a place of a padded batch) reads zeros and adds to no row.  Both are bound by memory.  The gradient
+// writes every row of the table once, those without ids as zeros, and adds in the order of the ids' places: no atomics on values, the
+// same bits each time.
+//
+// For that the ids are sorted, stable.  Up to kPickMost ids each workgroup, which owns a range of the table's rows, reads all ids,
+// keeps those of its range in LDS in their order and sorts them there: one launch.  More are sorted by digits first (a
+// histogram of each workgroup's ids, their prefixes, and a scatter that keeps the order, for every digit), and a workgroup finds its range in them.
+// Where a row has hundreds of ids, whole runs of kChunk of them are added up beforehand, all over the chip, and a workgroup's waves
+// share what is left.
+#include "rows.hpp"
+
+namespace f2cgt {
+namespace {
+
+__host__ __device__ constexpr int bits_of(uint32_t v) {        // of numbers up to v
+  int b = 0;
+  while (b < 32 && (v >> b) != 0) ++b;
+  return b;
+}
+
+// An id's row, or `rows` where it has none.
+template <typename Idx>
+__device__ __forceinline__ uint32_t key_of(Idx id, uint32_t rows) {
+  return (uint64_t)(int64_t)id < (uint64_t)rows ? (uint32_t)id : rows;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------
+struct LookupArgs {
+  const void* table;
+  const void* index;
+  void* out;
+  int64_t n, ld;
+  uint32_t rows;
+  int d, pieces, lanes;      // lanes: of a row, a power of two up to 64
+  float scale;
+};
+
+template <typename T, int V, typename Idx>
+__global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
+  constexpr int kUnroll = 4;
+  const int per_pass = 256 / a.lanes, sub = threadIdx.x & (a.lanes - 1);
+  const int64_t first = (int64_t)blockIdx.x * kUnroll * per_pass + threadIdx.x / a.lanes;
+  const T* from[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + (int64_t)u * per_pass;
+    from[u] = nullptr;
+    if (i < a.n) {
+      const uint32_t key = key_of(static_cast<const Idx*>(a.index)[i], a.rows);
+      if (key < a.rows) from[u] = static_cast<const T*>(a.table) + (int64_t)key * a.ld;
+    }
+  }
+  for (int p = sub; p < a.pieces; p += a.lanes) {
+    const int at = p * V + V > a.d ? a.d - V : p * V;        // (the last piece ends with the row)
+    float v[kUnroll][V];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[u][e] = 0.f;
+      if (from[u] != nullptr) load_piece<T, V>(from[u] + at, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = first + (int64_t)u * per_pass;
+      if (i >= a.n) continue;
+      if (from[u] != nullptr)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u][e] *= a.scale;
+      store_piece<T, V>(static_cast<T*>(a.out) + i * a.d + at, v[u]);
+    }
+  }
+}
+
+// ---- sorting by digits ------------------------------------------------------------------------------------
+constexpr int kSortThreads = 256, kSortItems = 16, kSortTile = kSortThreads * kSortItems, kSortWaves = kSortThreads / kWave;
+constexpr int kMostBits = 10;
+
+struct SortArgs {
+  const void* index;         // the first digit's keys are made of these
+  const uint32_t* keys;      // of the others: the last scatter's
+  const uint32_t* places;
+  uint32_t* keys_out;
+  uint32_t* places_out;
+  uint32_t* counts;          // [digits][blocks], then [digits] of the totals
+  int64_t n;
+  uint32_t rows, blocks;
+  int shift, bits;
+};
+
+// Key `i`; the widest beyond the end, which no digit counts.
+template <typename Idx, bool FIRST>
+__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i) {
+  if constexpr (FIRST) return key_of(static_cast<const Idx*>(a.index)[i], a.rows);
+  else return a.keys[i];
+}
+
+template <typename Idx, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
+  __shared__ uint32_t counts[1 << kMostBits];
+  const uint32_t digits = 1u << a.bits;
+  for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) counts[d] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
+  for (int u = 0; u < kSortItems; ++u) {
+    const int64_t i = first + u * kSortThreads + threadIdx.x;
+    if (i < a.n) atomicAdd(&counts[sort_key<Idx, FIRST>(a, i) >> a.shift & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) a.counts[(int64_t)d * a.blocks + blockIdx.x] = counts[d];
+}
+
+// A digit's counts become the sums of those before, its total goes behind them all.  One wave a digit.
+__global__ __launch_bounds__(kWave) void sort_prefix_kernel(SortArgs a) {
+  uint32_t* row = a.counts + (int64_t)blockIdx.x * a.blocks;
+  uint32_t before = 0;
+  for (uint32_t b = 0; b < a.blocks; b += kWave) {
+    const uint32_t i = b + threadIdx.x;
+    const uint32_t own = i < a.blocks ? row[i] : 0;
+    uint32_t upto = own;
+#pragma unroll
+    for (int by = 1; by < kWave; by *= 2) {
+      const uint32_t left = (uint32_t)__shfl_up((int)upto, by);
+      if ((int)threadIdx.x >= by) upto += left;
+    }
+    if (i < a.blocks) row[i] = before + upto - own;
+    before += (uint32_t)__shfl((int)upto, kWave - 1);
+  }
+  if (threadIdx.x == 0) a.counts[(int64_t)gridDim.x * a.blocks + blockIdx.x] = before;
+}
+
+// Lanes of the wave with the same digit as this one, among those that are `on`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on) {
+  uint64_t same = __ballot(on);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = digit >> b & 1;
+    const uint64_t with = __ballot(set);
+    same &= set ? with : ~with;
+  }
+  return same;
+}
+__device__ __forceinline__ uint32_t below(uint64_t lanes) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
+
+// Exclusive sums of values[0 .. count) in LDS, by the whole workgroup; `room` holds a word a wave.
+template <int THREADS>
+__device__ __forceinline__ void prefix_in_lds(uint32_t* values, uint32_t count, uint32_t* room) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  uint32_t before = 0;
+  for (uint32_t b = 0; b < count; b += THREADS) {
+    const uint32_t i = b + threadIdx.x;
+    const uint32_t own = i < count ? values[i] : 0;
+    uint32_t upto = own;
+#pragma unroll
+    for (int by = 1; by < kWave; by *= 2) {
+      const uint32_t left = (uint32_t)__shfl_up((int)upto, by);
+      if (lane >= by) upto += left;
+    }
+    if (lane == kWave - 1) room[wave] = upto;
+    __syncthreads();
+    uint32_t waves = before, all = 0;
+    for (int w = 0; w < THREADS / kWave; ++w) {
+      if (w < wave) waves += room[w];
+      all += room[w];
+    }
+    if (i < count) values[i] = waves + upto - own;
+    before += all;
+    __syncthreads();
+  }
+}
+
+template <typename Idx, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) {
+  __shared__ uint32_t base[1 << kMostBits];
+  __shared__ uint32_t own[kSortWaves][1 << kMostBits];
+  __shared__ uint32_t room[kSortWaves];
+  const uint32_t digits = 1u << a.bits;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) {
+    base[d] = a.counts[(int64_t)digits * a.blocks + d];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) own[w][d] = 0;
+  }
+  __syncthreads();
+  prefix_in_lds<kSortThreads>(base, digits, room);
+  // a wave has a run of the tile: counted, then placed in order
+  const int64_t first = (int64_t)blockIdx.x * kSortTile + wave * kWave * kSortItems + lane;
+  uint32_t key[kSortItems];
+#pragma unroll
+  for (int u = 0; u < kSortItems; ++u) {
+    const int64_t i = first + u * kWave;
+    key[u] = i < a.n ? sort_key<Idx, FIRST>(a, i) : 0;
+    if (i < a.n) atomicAdd(&own[wave][key[u] >> a.shift & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) {
+    uint32_t at = base[d] + a.counts[(int64_t)d * a.blocks + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t count = own[w][d];
+      own[w][d] = at;
+      at += count;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kSortItems; ++u) {
+    const int64_t i = first + u * kWave;
+    const bool on = i < a.n;
+    const uint32_t digit = key[u] >> a.shift & (digits - 1);
+    const uint64_t same = same_digit(digit, a.bits, on);
+    const uint32_t rank = below(same);
+    if (on) {
+      const uint32_t at = own[wave][digit] + rank;
+      a.keys_out[at] = key[u];
+      a.places_out[at] = FIRST ? (uint32_t)i : a.places[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (on && rank == 0) own[wave][digit] += (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---- sums over a row's gradients --------------------------------------------------------------------------
+constexpr int kChunk = 128;                  // ids of one row whose sum is made beforehand
+constexpr uint32_t kLong = 64;               // ids of a row above which a workgroup's waves share them
+
+struct SumArgs {
+  const void* grad;
+  const void* index;
+  const uint32_t* keys;      // sorted, with the places that they had
+  const uint32_t* places;
+  float* chunks;             // [n / kChunk][d]: sums of whole runs of one row
+  void* out;
+  int64_t n, ld;
+  uint32_t rows, range;      // range: rows of a workgroup
+  int d, pieces, slices;     // slices: parts of 64 pieces of a row, a workgroup each
+  float scale;
+};
+
+// Adds to v the piece at `at` of the gradients of places[first], places[first + 1], ... in order.
+template <typename T, int V, typename Place>
+__device__ __forceinline__ void add_rows(float (&v)[V], const SumArgs& a, const Place* places, uint32_t first, uint32_t last, int at) {
+  constexpr int kUnroll = 8;
+  typedef typename piece_words<T, V>::type words;
+  const T* grad = static_cast<const T*>(a.grad) + at;
+  uint32_t i = first;
+  for (; i + kUnroll <= last; i += kUnroll) {
+    words w[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) w[u] = *reinterpret_cast<const words*>(grad + (int64_t)places[i + u] * a.ld);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float g[V];
+      values_of<T, V>(w[u], g);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += g[e];
+    }
+  }
+  for (; i < last; ++i) {
+    float g[V];
+    load_piece<T, V>(grad + (int64_t)places[i] * a.ld, g);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += g[e];
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_chunks(float (&v)[V], const SumArgs& a, uint32_t first, uint32_t last, int at) {
+  for (uint32_t c = first; c < last; ++c) {
+    const float* from = a.chunks + (int64_t)c * a.d + at;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += from[e];
+  }
+}
+
+// Chunks of the sorted ids that are of one row: a wave a chunk and slice.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void chunk_sums_kernel(SumArgs a) {
+  const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  const int64_t chunk = item / a.slices;
+  const int slice = (int)(item - chunk * a.slices);
+  if (chunk >= a.n / kChunk) return;
+  const uint32_t first = (uint32_t)(chunk * kChunk);
+  if (a.keys[first] != a.keys[first + kChunk - 1] || a.keys[first] >= a.rows) return;
+  const int p = slice * kWave + (threadIdx.x & (kWave - 1));
+  if (p >= a.pieces) return;
+  const int at = p * V + V > a.d ? a.d - V : p * V;
+  float v[V] = {};
+  add_rows<T, V>(v, a, a.places, first, first + kChunk, at);
+  float* to = a.chunks + chunk * a.d + at;
+#pragma unroll
+  for (int e = 0; e < V; ++e) to[e] = v[e];
+}
+
+// Where keys of at least `key` begin in the sorted ones from lo to hi: by the 64 lanes of a wave, 64 parts at a time.
+__device__ __forceinline__ uint32_t begin_of(const uint32_t* keys, uint32_t lo, uint32_t hi, uint32_t key) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + kWave - 1) / kWave;
+    const uint64_t at = (uint64_t)lo + (uint64_t)lane * step;
+    const uint64_t less = __ballot(at < hi && keys[at] < key);
+    const uint32_t count = (uint32_t)__popcll(less);
+    if (count == 0) return lo;
+    const uint64_t next = (uint64_t)lo + (uint64_t)count * step;
+    lo = lo + (count - 1) * step + 1;
+    hi = next < hi ? (uint32_t)next : hi;
+  }
+  return lo;
+}
+
+// A workgroup's range of rows and slice of columns, the places of whose ids lie in order in places[start[r] .. start[r + 1]).
+template <typename T, int V, int THREADS, typename Place>
+__device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start,
+                                          const Place* places, bool chunked, uint32_t* long_rows, uint32_t* long_count, float* room) {
+  constexpr int kWaves = THREADS / kWave;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;       // pieces of the slice
+  int lanes = 1;
+  while (lanes < here) lanes *= 2;
+  const int groups = kWave / lanes, sub = lane & (lanes - 1);
+  const int p = slice * kWave + (sub < here ? sub : here - 1);
+  const int at = p * V + V > a.d ? a.d - V : p * V;
+  for (uint32_t r = (uint32_t)(wave * groups + lane / lanes); r < count; r += (uint32_t)(kWaves * groups)) {
+    const uint32_t s = start[r], e = start[r + 1];
+    if (e - s > kLong) {
+      if (sub == 0) long_rows[atomicAdd(long_count, 1u)] = r;         // (in any order: each is a sum of its own)
+      continue;
+    }
+    float v[V] = {};
+    add_rows<T, V>(v, a, places, s, e, at);
+    if (s != e)
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] *= a.scale;
+    if (sub < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + at, v);
+  }
+  __syncthreads();
+  const uint32_t longs = *long_count;
+  const int lp = slice * kWave + (lane < here ? lane : here - 1);
+  const int lat = lp * V + V > a.d ? a.d - V : lp * V;
+  for (uint32_t l = 0; l < longs; ++l) {
+    const uint32_t r = long_rows[l], s = start[r], e = start[r + 1];
+    uint32_t c0 = (s + kChunk - 1) / kChunk, c1 = e / kChunk;
+    if (!chunked || c0 >= c1) { c0 = 0; c1 = 0; }
+    const uint32_t head = c0 < c1 ? c0 * kChunk : e, tail = c0 < c1 ? c1 * kChunk : e;
+    auto part = [&](uint32_t from, uint32_t to, int w) { return from + (uint32_t)((uint64_t)(to - from) * w / kWaves); };
+    float v[V] = {};
+    add_rows<T, V>(v, a, places, part(s, head, wave), part(s, head, wave + 1), lat);
+    if (chunked) add_chunks<V>(v, a, part(c0, c1, wave), part(c0, c1, wave + 1), lat);
+    add_rows<T, V>(v, a, places, part(tail, e, wave), part(tail, e, wave + 1), lat);
+#pragma unroll
+    for (int x = 0; x < V; ++x) room[(wave * V + x) * kWave + lane] = v[x];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+        for (int x = 0; x < V; ++x) v[x] += room[(w * V + x) * kWave + lane];
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] *= a.scale;
+      if (lane < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + lat, v);
+    }
+    __syncthreads();
+  }
+}
+
+// From sorted ids.
+constexpr int kRangeSorted = 64;
+template <typename T, int V>
+__global__ __launch_bounds__(512) void sorted_sums_kernel(SumArgs a) {
+  __shared__ uint32_t start[kRangeSorted + 1], ends[2], long_rows[kRangeSorted], long_count;
+  __shared__ float room[512 * V];
+  const uint32_t range = blockIdx.x / a.slices, row0 = range * kRangeSorted;
+  const int slice = (int)(blockIdx.x - range * a.slices);
+  const uint32_t count = a.rows - row0 < kRangeSorted ? a.rows - row0 : kRangeSorted;
+  const int wave = threadIdx.x / kWave;
+  if (threadIdx.x == 0) long_count = 0;
+  if (wave < 2) {
+    const uint32_t at = begin_of(a.keys, 0, (uint32_t)a.n, row0 + (wave ? count : 0));
+    if (threadIdx.x % kWave == 0) ends[wave] = at;
+  }
+  __syncthreads();
+  for (uint32_t r = threadIdx.x; r <= count; r += 512) {
+    uint32_t lo = ends[0], hi = ends[1];
+    while (lo < hi) {
+      const uint32_t middle = lo + (hi - lo) / 2;
+      if (a.keys[middle] < row0 + r) lo = middle + 1;
+      else hi = middle;
+    }
+    start[r] = lo;
+  }
+  __syncthreads();
+  sum_range<T, V, 512>(a, row0, count, slice, start, a.places, true, long_rows, &long_count, room);
+}
+
+// From ids as they come: those of the range are kept in their order, then sorted by row.
+constexpr int kPickMost = 16384, kPickThreads = 1024, kPickWaves = kPickThreads / kWave, kRangePicked = 1024;
+
+// Where things lie in LDS, in bytes, which is as large as the call's ids and range ask for: two workgroups are to fit a CU.
+struct PickRoom {
+  uint32_t sorted, own, start, long_rows, all;
+  __host__ __device__ PickRoom(uint32_t n, uint32_t range, int values) {
+    const uint32_t kept = 4 * n, sums = (uint32_t)(kPickThreads * values * 4);      // (the waves' sums take the place of the kept ids)
+    sorted = ((kept > sums ? kept : sums) + 15) / 16 * 16;
+    own = sorted + (2 * n + 15) / 16 * 16;
+    start = own + kPickWaves * 2 * ((range + 1) / 2 * 2);
+    long_rows = start + 4 * (range + 1);
+    all = long_rows + 4 * range;
+  }
+};
+
+template <typename T, int V, typename Idx>
+__global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ uint32_t room_words[kPickWaves], long_count;
+  const PickRoom at_lds((uint32_t)a.n, a.range, V);
+  uint32_t* kept = reinterpret_cast<uint32_t*>(lds);                         // place | row in the range << 14, in the places' order
+  uint16_t* sorted = reinterpret_cast<uint16_t*>(lds + at_lds.sorted);       // places by row
+  uint32_t* start = reinterpret_cast<uint32_t*>(lds + at_lds.start);
+  uint32_t* long_rows = reinterpret_cast<uint32_t*>(lds + at_lds.long_rows);
+  const uint32_t part = blockIdx.x / a.slices, row0 = part * a.range;
+  const int slice = (int)(blockIdx.x - part * a.slices);
+  const uint32_t count = a.rows - row0 < a.range ? a.rows - row0 : a.range;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const uint32_t each = (a.range + 1) / 2 * 2;
+  uint16_t* all_own = reinterpret_cast<uint16_t*>(lds + at_lds.own);         // [waves][each]
+  uint16_t* own = all_own + wave * each;
+  const Idx* index = static_cast<const Idx*>(a.index);
+  if (threadIdx.x == 0) long_count = 0;
+  for (uint32_t r = threadIdx.x; r <= count; r += kPickThreads) start[r] = 0;
+  for (uint32_t r = lane; r < each; r += kWave) own[r] = 0;
+  // a wave reads a run of the ids: how many of them it keeps, then where
+  const uint32_t n = (uint32_t)a.n, run = (n + kPickWaves * kWave - 1) / (kPickWaves * kWave) * kWave;
+  const uint32_t first = wave * run, last = first + run < n ? first + run : n;
+  constexpr int kMost = kPickMost / kPickThreads;
+  uint32_t local[kMost], mine = 0;
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const uint32_t i = first + u * kWave + lane;
+    local[u] = ~0u;
+    if (u * kWave < (int)run && i < last) {
+      const uint32_t key = key_of(index[i], a.rows), in = key - row0;
+      if (key >= row0 && in < count) local[u] = in;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) mine += (uint32_t)__popcll(__ballot(local[u] != ~0u));
+  if (lane == 0) room_words[wave] = mine;
+  __syncthreads();
+  uint32_t at = 0, all = 0;
+  for (int w = 0; w < kPickWaves; ++w) {
+    if (w < wave) at += room_words[w];
+    all += room_words[w];
+  }
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const uint64_t with = __ballot(local[u] != ~0u);
+    if (local[u] != ~0u) {
+      kept[at + below(with)] = (first + u * kWave + lane) | local[u] << 14;
+      atomicAdd(&start[local[u]], 1u);
+    }
+    at += (uint32_t)__popcll(with);
+  }
+  __syncthreads();
+  // the kept ids by row: again a run of them to each wave
+  const uint32_t share = (all + kPickWaves * kWave - 1) / (kPickWaves * kWave) * kWave;
+  const uint32_t begin = wave * share < all ? wave * share : all, end = begin + share < all ? begin + share : all;
+  for (uint32_t i = begin + lane; i < end; i += kWave) {
+    // (16-bit counters, two to a word)
+    const uint32_t r = kept[i] >> 14;
+    atomicAdd(reinterpret_cast<uint32_t*>(own + (r & ~1u)), r & 1 ? 0x10000u : 1u);
+  }
+  prefix_in_lds<kPickThreads>(start, count + 1, room_words);
+  __syncthreads();
+  for (uint32_t r = threadIdx.x; r < count; r += kPickThreads) {
+    uint32_t before = 0;
+    for (int w = 0; w < kPickWaves; ++w) {
+      const uint32_t c = all_own[w * each + r];
+      all_own[w * each + r] = (uint16_t)before;    // (up to 16384: 16 bits hold it)
+      before += c;
+    }
+  }
+  __syncthreads();
+  const int bits = bits_of(count - 1);
+  for (uint32_t i = begin; i < end; i += kWave) {
+    const bool on = i + lane < end;
+    const uint32_t word = on ? kept[i + lane] : 0, r = word >> 14;
+    const uint64_t same = same_digit(r, bits, on);
+    const uint32_t rank = below(same);
+    if (on) sorted[start[r] + own[r] + rank] = (uint16_t)(word & (kPickMost - 1));
+    __builtin_amdgcn_wave_barrier();
+    if (on && rank == 0) own[r] += (uint16_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, false, long_rows, &long_count, reinterpret_cast<float*>(lds));
+}
+
+// Digits of the sort: as few as keys of rows + 1 values need, of one width.
+void digits_of(int64_t rows, int& passes, int& bits) {
+  const int all = bits_of((uint32_t)rows);
+  passes = (int)ceil_div(all, kMostBits);
+  bits = (int)ceil_div(all, passes);
+}
+
+struct Room {
+  int64_t sorted, counts, chunks;            // bytes: keys and places twice, counts of the digits, sums of chunks
+  explicit Room(int64_t n, int64_t rows, int64_t d) {
+    int passes, bits;
+    digits_of(rows, passes, bits);
+    sorted = ceil_div(n, 4) * 16 * 4;
+    counts = ceil_div((1ll << bits) * (ceil_div(n, kSortTile) + 1), 4) * 16;
+    chunks = n / kChunk * d * 4;
+  }
+};
+
+int check_embedding(const char* what, int64_t n, int64_t rows, int64_t d, int idx_dtype, int dtype) {
+  F2CGT_REQUIRE(n >= 0 && rows >= 0 && d >= 0, F2CGT_E_INVALID, "%s: sizes must not be negative", what);
+  F2CGT_REQUIRE(idx_dtype == F2CGT_DT_I32 || idx_dtype == F2CGT_DT_I64, F2CGT_E_UNSUPPORTED, "%s: ids must be int32 or int64", what);
+  F2CGT_REQUIRE(dtype == F2CGT_DT_F32 || dtype == F2CGT_DT_F16 || dtype == F2CGT_DT_BF16, F2CGT_E_UNSUPPORTED,
+                "%s: fp32, fp16 or bf16 rows only", what);
+  F2CGT_REQUIRE(n < (1ll << 31) && rows < (1ll << 31) && d < (1ll << 24), F2CGT_E_UNSUPPORTED,
+                "%s: at most 2^31 - 1 ids and rows and 2^24 - 1 columns", what);
+  return 0;
+}
+
+template <typename T, int V>
+int launch_lookup(LookupArgs a, int idx_dtype, hipStream_t st) {
+  a.pieces = (int)ceil_div(a.d, V);
+  a.lanes = a.pieces >= kWave ? kWave : pow2_ceil(a.pieces);
+  const int64_t blocks = ceil_div(a.n, 4 * (256 / a.lanes));
+  F2CGT_REQUIRE(blocks < (1ll << 24), F2CGT_E_UNSUPPORTED, "embedding: too many ids for a launch");
+  const dim3 grid((unsigned)blocks);
+  if (idx_dtype == F2CGT_DT_I64) lookup_kernel<T, V, int64_t><<<grid, dim3(256), 0, st>>>(a);
+  else lookup_kernel<T, V, int32_t><<<grid, dim3(256), 0, st>>>(a);
+  return launch_status("embedding");
+}
+
+template <typename T, int V>
+int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
+  const char* what = "embedding_grad";
+  a.pieces = (int)ceil_div(a.d, V);
+  a.slices = (int)ceil_div(a.pieces, kWave);
+  if (a.n <= kPickMost) {
+    // two workgroups' worth of ranges for each CU at least, of no more rows than LDS has counters for
+    const int64_t want = ceil_div((int64_t)a.rows * a.slices, 2 * num_cus());
+    a.range = (uint32_t)(want < 16 ? 16 : want > kRangePicked ? kRangePicked : want);
+    const int64_t blocks = ceil_div(a.rows, a.range) * a.slices;
+    F2CGT_REQUIRE(blocks < (1ll << 22), F2CGT_E_UNSUPPORTED, "%s: too many rows for a launch", what);
+    const uint32_t lds = PickRoom((uint32_t)a.n, a.range, V).all;
+    auto kernel = idx_dtype == F2CGT_DT_I64 ? picked_sums_kernel<T, V, int64_t> : picked_sums_kernel<T, V, int32_t>;
+    if (lds > 65536) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return fail((int)e, "%s: %s", what, hipGetErrorString(e));
+    }
+    kernel<<<dim3((unsigned)blocks), dim3(kPickThreads), lds, st>>>(a);
+    return launch_status(what);
+  }
+  const Room room(a.n, a.rows, a.d);
+  int passes, bits;
+  digits_of(a.rows, passes, bits);
+  const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div(a.rows, kRangeSorted) * a.slices;
+  const int64_t chunk_blocks = ceil_div(a.n / kChunk * a.slices, 4);
+  F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 24), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
+  uint32_t* words = reinterpret_cast<uint32_t*>(workspace);
+  const int64_t each = ceil_div(a.n, 4) * 4;
+  SortArgs s{a.index, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<uint32_t*>(workspace + room.sorted), a.n, a.rows, (uint32_t)blocks, 0, bits};
+  const dim3 grid((unsigned)blocks), digits(1u << bits);
+  for (int pass = 0; pass < passes; ++pass) {
+    s.shift = pass * bits;
+    s.keys = words + (pass & 1 ? 0 : 2) * each;
+    s.places = s.keys + each;
+    s.keys_out = words + (pass & 1 ? 2 : 0) * each;
+    s.places_out = s.keys_out + each;
+    if (pass > 0) {
+      sort_count_kernel<int32_t, false><<<grid, dim3(kSortThreads), 0, st>>>(s);
+      sort_prefix_kernel<<<digits, dim3(kWave), 0, st>>>(s);
+      sort_scatter_kernel<int32_t, false><<<grid, dim3(kSortThreads), 0, st>>>(s);
+    } else if (idx_dtype == F2CGT_DT_I64) {
+      sort_count_kernel<int64_t, true><<<grid, dim3(kSortThreads), 0, st>>>(s);
+      sort_prefix_kernel<<<digits, dim3(kWave), 0, st>>>(s);
+      sort_scatter_kernel<int64_t, true><<<grid, dim3(kSortThreads), 0, st>>>(s);
+    } else {
+      sort_count_kernel<int32_t, true><<<grid, dim3(kSortThreads), 0, st>>>(s);
+      sort_prefix_kernel<<<digits, dim3(kWave), 0, st>>>(s);
+      sort_scatter_kernel<int32_t, true><<<grid, dim3(kSortThreads), 0, st>>>(s);
+    }
+  }
+  a.keys = s.keys_out;
+  a.places = s.places_out;
+  a.chunks = reinterpret_cast<float*>(workspace + room.sorted + room.counts);
+  chunk_sums_kernel<T, V><<<dim3((unsigned)chunk_blocks), dim3(256), 0, st>>>(a);
+  sorted_sums_kernel<T, V><<<dim3((unsigned)sums), dim3(512), 0, st>>>(a);
+  return launch_status(what);
+}
+
+}  // namespace
+}  // namespace f2cgt
+
+using namespace f2cgt;
+
+extern "C" int f2cgt_embedding(const void* table, int dtype, int64_t ld, const void* index, int idx_dtype, void* out, float scale,
+                               int64_t n, int64_t rows, int64_t d, void* stream) {
+  const char* what = "embedding";
+  if (int rc = check_embedding(what, n, rows, d, idx_dtype, dtype)) return rc;
+  F2CGT_REQUIRE(rows <= 1 || ld >= d, F2CGT_E_INVALID, "%s: rows overlap", what);
+  if (n == 0 || d == 0) return 0;
+  F2CGT_REQUIRE((rows == 0 || table) && index && out, F2CGT_E_INVALID, "%s: null buffer", what);
+  const int size = dtype == F2CGT_DT_F32 ? 4 : 2;
+  F2CGT_REQUIRE(aligned(table, size) && aligned(out, size) && aligned(index, idx_dtype == F2CGT_DT_I64 ? 8 : 4), F2CGT_E_INVALID,
+                "%s: misaligned buffer", what);
+  const LookupArgs a{table, index, out, n, ld, (uint32_t)rows, (int)d, 0, 0, scale};
+  return with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (d >= kPieceOf<T>) return launch_lookup<T, kPieceOf<T>>(a, idx_dtype, as_stream(stream));
+    return launch_lookup<T, 1>(a, idx_dtype, as_stream(stream));
+  });
+}
+
+extern "C" int64_t f2cgt_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t d) {
+  if (n <= kPickMost || rows <= 0 || d <= 0 || n >= (1ll << 31) || rows >= (1ll << 31)) return 0;
+  const Room room(n, rows, d);
+  return room.sorted + room.counts + room.chunks;
+}
+
+extern "C" int f2cgt_embedding_grad(const void* grad, int dtype, int64_t ld, const void* index, int idx_dtype, void* dtable,
+                                    float scale, void* workspace, int64_t workspace_bytes, int64_t n, int64_t rows, int64_t d,
+                                    void* stream) {
+  const char* what = "embedding_grad";
+  if (int rc = check_embedding(what, n, rows, d, idx_dtype, dtype)) return rc;
+  F2CGT_REQUIRE(n <= 1 || ld >= d, F2CGT_E_INVALID, "%s: rows overlap", what);
+  if (rows == 0 || d == 0) return 0;
+  F2CGT_REQUIRE((n == 0 || (grad && index)) && dtable, F2CGT_E_INVALID, "%s: null buffer", what);
+  const int size = dtype == F2CGT_DT_F32 ? 4 : 2;
+  F2CGT_REQUIRE(aligned(grad, size) && aligned(dtable, size) && aligned(index, idx_dtype == F2CGT_DT_I64 ? 8 : 4), F2CGT_E_INVALID,
+                "%s: misaligned buffer", what);
+  const int64_t need = f2cgt_embedding_grad_workspace_bytes(n, rows, d);
+  F2CGT_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), F2CGT_E_INVALID,
+                "%s: workspace too small or misaligned", what);
+  const SumArgs a{grad, index, nullptr, nullptr, nullptr, dtable, n, ld, (uint32_t)rows, 0, (int)d, 0, 0, scale};
+  return with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (d >= kPieceOf<T>) return launch_grad<T, kPieceOf<T>>(a, idx_dtype, static_cast<char*>(workspace), as_stream(stream));
+    return launch_grad<T, 1>(a, idx_dtype, static_cast<char*>(workspace), as_stream(stream));
+  });
+}

@@ -1466,6 +1466,241 @@ void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torc
   }
 }
 
+// ---- layer norm, checkpoints in 8 bits, learnt rows --------------------------------------------------------
+// A vector beside rows of d values: fp32 or of their type.
+torch::Tensor norm_vector(const c10::optional<torch::Tensor>& v, const torch::Tensor& rows, const char* name) {
+  if (!v.has_value()) return torch::Tensor();
+  auto t = beside(v->defined() ? v->resolve_neg() : *v, rows, name);
+  TORCH_CHECK((t.scalar_type() == torch::kFloat32 || t.scalar_type() == rows.scalar_type()) && t.dim() == 1 && t.size(0) == rows.size(1),
+              name, " must be float32 or ", rows.scalar_type(), " [", rows.size(1), "]");
+  return t;
+}
+const void* data_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// A statistic for each row.
+torch::Tensor row_values(const torch::Tensor& v, const torch::Tensor& rows, const char* name) {
+  auto t = beside(v.defined() ? v.resolve_neg() : v, rows, name);
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.numel() == rows.size(0), name, " must be float32 with a value for each of the ",
+              rows.size(0), " rows");
+  return t;
+}
+
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+  auto shape = sizes.vec();
+  shape.back() = last;
+  return shape;
+}
+std::vector<int64_t> lead_of(at::IntArrayRef sizes) {
+  auto shape = sizes.vec();
+  shape.pop_back();
+  return shape;
+}
+
+// A checkpoint that a caller gives: codes [rows, k] as the kernels take them, exponents [rows, ceil(k / 32)].
+struct Checkpoint {
+  torch::Tensor codes, exponents;
+  Checkpoint(const torch::Tensor& codes_in, const torch::Tensor& exponents_in) {
+    TORCH_CHECK(codes_in.defined() && codes_in.device().is_cuda(), "codes must be a GPU tensor");
+    TORCH_CHECK(codes_in.dim() >= 1 && codes_in.scalar_type() == torch::kInt8, "codes must be int8 [..., columns]");
+    int64_t count = 1;
+    for (int64_t d = 0; d + 1 < codes_in.dim(); ++d) count *= codes_in.size(d);
+    codes = code_rows(codes_in.dim() == 2 ? codes_in : codes_in.reshape({count, codes_in.size(-1)}), "codes");
+    exponents = beside(exponents_in, codes, "exponents");
+    TORCH_CHECK(exponents.scalar_type() == torch::kUInt8 && exponents.sizes() == with_last(codes_in.sizes(), (codes.size(1) + 31) / 32),
+                "exponents must be uint8 with a value for each 32 columns of codes");
+  }
+  const int8_t* code_ptr() const { return codes.data_ptr<int8_t>(); }
+  int64_t stride() const { return codes.stride(0); }
+};
+
+struct Normed {
+  torch::Tensor out, mean, rstd, codes, exponents;
+};
+Normed norm_rows(const char* op, const torch::Tensor& x, const c10::optional<torch::Tensor>& weight_in,
+                 const c10::optional<torch::Tensor>& bias_in, double eps, bool statistics, bool pack) {
+  auto rows = value_rows(x, "x");
+  const int tag = dense_tag(rows.scalar_type(), "x");
+  undifferentiated(op, {x, weight_in.value_or(torch::Tensor()), bias_in.value_or(torch::Tensor())});
+  auto weight = norm_vector(weight_in, rows, "weight"), bias = norm_vector(bias_in, rows, "bias");
+  TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(), "weight and bias must be of one type");
+  const int weight_tag = weight.defined() ? dense_tag(weight.scalar_type(), "weight") : bias.defined() ? dense_tag(bias.scalar_type(), "bias") : tag;
+  c10::DeviceGuard guard(rows.device());
+  const int64_t m = rows.size(0), d = rows.size(1);
+  Normed r;
+  r.out = torch::empty(x.sizes(), rows.options());
+  if (statistics) {
+    r.mean = torch::empty(lead_of(x.sizes()), rows.options().dtype(torch::kFloat32));
+    r.rstd = torch::empty_like(r.mean);
+  }
+  if (pack) {
+    r.codes = room_for_codes(m, d, rows);
+    r.exponents = torch::empty(with_last(x.sizes(), (d + 31) / 32), rows.options().dtype(torch::kUInt8));
+  }
+  check_rc(f2cgt_layer_norm(rows.data_ptr(), tag, row_step(rows), data_or_null(weight), data_or_null(bias), weight_tag, r.out.data_ptr(),
+                            statistics ? r.mean.data_ptr<float>() : nullptr, statistics ? r.rstd.data_ptr<float>() : nullptr,
+                            pack ? r.codes.data_ptr<int8_t>() : nullptr, (d + 15) / 16 * 16,
+                            pack ? r.exponents.data_ptr<uint8_t>() : nullptr, m, d, (float)eps, current_stream()),
+           op);
+  if (pack && x.dim() != 2) r.codes = r.codes.view(x.sizes());
+  return r;
+}
+
+torch::Tensor layer_norm(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight, const c10::optional<torch::Tensor>& bias,
+                         double eps) {
+  return norm_rows("layer_norm", x, weight, bias, eps, false, false).out;
+}
+
+// -> (out, mean, rstd), and with `pack` the checkpoint of x: (.., codes, exponents).
+py::tuple layer_norm_train(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight, const c10::optional<torch::Tensor>& bias,
+                           double eps, bool pack) {
+  auto r = norm_rows("layer_norm_train", x, weight, bias, eps, true, pack);
+  if (pack) return py::make_tuple(r.out, r.mean, r.rstd, r.codes, r.exponents);
+  return py::make_tuple(r.out, r.mean, r.rstd);
+}
+
+typedef std::tuple<torch::Tensor, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> NormGrads;
+NormGrads norm_grads(const char* op, const torch::Tensor& grad_in, const torch::Tensor& x_in, const Checkpoint* kept,
+                     const torch::Tensor& mean_in, const torch::Tensor& rstd_in, const c10::optional<torch::Tensor>& weight_in,
+                     bool weight_grad, bool bias_grad) {
+  auto grad = value_rows(grad_in, "grad");
+  const int tag = dense_tag(grad.scalar_type(), "grad");
+  undifferentiated(op, {grad_in, x_in, mean_in, rstd_in, weight_in.value_or(torch::Tensor())});
+  torch::Tensor x;
+  if (kept == nullptr) {
+    x = value_rows(x_in, "x");
+    TORCH_CHECK(x.scalar_type() == grad.scalar_type() && x.device() == grad.device() && x_in.sizes() == grad_in.sizes(),
+                "grad and x must be of one type, shape and device");
+  } else {
+    TORCH_CHECK(kept->codes.device() == grad.device() && kept->codes.sizes() == grad.sizes(), "grad and codes must be of one shape and device");
+  }
+  auto mean = row_values(mean_in, grad, "mean"), rstd = row_values(rstd_in, grad, "rstd");
+  auto weight = norm_vector(weight_in, grad, "weight");
+  c10::DeviceGuard guard(grad.device());
+  const int64_t m = grad.size(0), d = grad.size(1);
+  const int weight_tag = weight.defined() ? dense_tag(weight.scalar_type(), "weight") : tag;
+  auto dx = torch::empty(grad_in.sizes(), grad.options());
+  const auto vector = grad.options().dtype(weight.defined() ? weight.scalar_type() : grad.scalar_type());
+  c10::optional<torch::Tensor> dw, db;
+  if (weight_grad) dw = torch::empty({d}, vector);
+  if (bias_grad) db = torch::empty({d}, vector);
+  const int64_t bytes = weight_grad || bias_grad ? f2cgt_layer_norm_grad_workspace_bytes(tag, m, d) : 0;
+  torch::Tensor ws;
+  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_layer_norm_grad(grad.data_ptr(), tag, row_step(grad), kept ? nullptr : x.data_ptr(), kept ? 0 : row_step(x),
+                                 kept ? kept->code_ptr() : nullptr, kept ? kept->stride() : 0,
+                                 kept ? kept->exponents.data_ptr<uint8_t>() : nullptr, mean.data_ptr<float>(), rstd.data_ptr<float>(),
+                                 data_or_null(weight), weight_tag, dx.data_ptr(), dw ? dw->data_ptr() : nullptr,
+                                 db ? db->data_ptr() : nullptr, weight_tag, bytes > 0 ? ws.data_ptr() : nullptr, bytes, m, d,
+                                 current_stream()),
+           op);
+  return {dx, dw, db};
+}
+NormGrads layer_norm_grad(const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& mean, const torch::Tensor& rstd,
+                          const c10::optional<torch::Tensor>& weight, bool weight_grad, bool bias_grad) {
+  return norm_grads("layer_norm_grad", grad, x, nullptr, mean, rstd, weight, weight_grad, bias_grad);
+}
+NormGrads layer_norm_packed_grad(const torch::Tensor& grad, const torch::Tensor& codes, const torch::Tensor& exponents,
+                                 const torch::Tensor& mean, const torch::Tensor& rstd, const c10::optional<torch::Tensor>& weight,
+                                 bool weight_grad, bool bias_grad) {
+  const Checkpoint kept(codes, exponents);
+  TORCH_CHECK(grad.defined() && codes.sizes() == grad.sizes(), "grad and codes must be of one shape and device");
+  return norm_grads("layer_norm_packed_grad", grad, torch::Tensor(), &kept, mean, rstd, weight, weight_grad, bias_grad);
+}
+
+// -> (codes int8 [..., k], exponents uint8 [..., ceil(k / 32)]).
+std::tuple<torch::Tensor, torch::Tensor> pack_activations(const torch::Tensor& x) {
+  auto rows = value_rows(x, "x");
+  const int tag = dense_tag(rows.scalar_type(), "x");
+  undifferentiated("pack_activations", {x});
+  c10::DeviceGuard guard(rows.device());
+  const int64_t m = rows.size(0), k = rows.size(1);
+  auto codes = room_for_codes(m, k, rows);
+  auto exponents = torch::empty(with_last(x.sizes(), (k + 31) / 32), rows.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_pack_activations(rows.data_ptr(), tag, row_step(rows), codes.data_ptr<int8_t>(), (k + 15) / 16 * 16,
+                                  exponents.data_ptr<uint8_t>(), m, k, current_stream()),
+           "pack_activations");
+  return {x.dim() == 2 ? codes : codes.view(x.sizes()), exponents};
+}
+
+torch::Tensor unpack_activations(const torch::Tensor& codes, const torch::Tensor& exponents, torch::ScalarType dtype) {
+  const Checkpoint kept(codes, exponents);
+  const int tag = dense_tag(dtype, "dtype");
+  c10::DeviceGuard guard(kept.codes.device());
+  auto out = torch::empty(codes.sizes(), kept.codes.options().dtype(dtype));
+  check_rc(f2cgt_unpack_activations(kept.code_ptr(), kept.stride(), kept.exponents.data_ptr<uint8_t>(), out.data_ptr(), tag,
+                                    kept.codes.size(0), kept.codes.size(1), current_stream()),
+           "unpack_activations");
+  return out;
+}
+
+// grad [..., n] and the checkpoint of a linear layer's input [..., k] -> (dweight [n, k], dbias [n] or None) of `dtype`.
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> packed_linear_grad(const torch::Tensor& grad_in, const torch::Tensor& codes,
+                                                                           const torch::Tensor& exponents, bool bias, torch::ScalarType dtype) {
+  const Checkpoint kept(codes, exponents);
+  auto grad = value_rows(grad_in, "grad");
+  const int tag = dense_tag(grad.scalar_type(), "grad"), out_tag = dense_tag(dtype, "dtype");
+  undifferentiated("packed_linear_grad", {grad_in});
+  TORCH_CHECK(grad.device() == kept.codes.device(), "grad is on ", grad.device(), ", the codes on ", kept.codes.device());
+  TORCH_CHECK(lead_of(grad_in.sizes()) == lead_of(codes.sizes()), "grad and codes must be of the same rows");
+  c10::DeviceGuard guard(grad.device());
+  const int64_t m = grad.size(0), n = grad.size(1), k = kept.codes.size(1);
+  auto dw = torch::empty({n, k}, grad.options().dtype(dtype));
+  c10::optional<torch::Tensor> db;
+  if (bias) db = torch::empty({n}, grad.options().dtype(dtype));
+  const int64_t bytes = f2cgt_packed_linear_grad_workspace_bytes(tag, m, n, k);
+  torch::Tensor ws;
+  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_packed_linear_grad(grad.data_ptr(), tag, row_step(grad), kept.code_ptr(), kept.stride(),
+                                    kept.exponents.data_ptr<uint8_t>(), dw.data_ptr(), db ? db->data_ptr() : nullptr, out_tag,
+                                    bytes > 0 ? ws.data_ptr() : nullptr, bytes, m, n, k, current_stream()),
+           "packed_linear_grad");
+  return {dw, db};
+}
+
+// Ids of either width.
+torch::Tensor ids_of(const torch::Tensor& index, const torch::Tensor& like) {
+  auto ids = beside(index, like, "index");
+  TORCH_CHECK(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "index must be int32 or int64");
+  return ids;
+}
+int id_tag(const torch::Tensor& ids) { return ids.scalar_type() == torch::kInt64 ? F2CGT_DT_I64 : F2CGT_DT_I32; }
+
+torch::Tensor embedding(const torch::Tensor& table, const torch::Tensor& index, double scale) {
+  TORCH_CHECK(table.defined() && table.dim() == 2, "table must be a matrix");
+  auto rows = value_rows(table, "table");
+  const int tag = dense_tag(rows.scalar_type(), "table");
+  undifferentiated("embedding", {table});
+  auto ids = ids_of(index, rows);
+  c10::DeviceGuard guard(rows.device());
+  const int64_t n = ids.numel(), d = rows.size(1);
+  auto shape = index.sizes().vec();
+  shape.push_back(d);
+  auto out = torch::empty(shape, rows.options());
+  check_rc(f2cgt_embedding(rows.data_ptr(), tag, row_step(rows), ids.data_ptr(), id_tag(ids), out.data_ptr(), (float)scale, n,
+                           rows.size(0), d, current_stream()),
+           "embedding");
+  return out;
+}
+
+torch::Tensor embedding_grad(const torch::Tensor& grad_in, const torch::Tensor& index, int64_t num_rows, double scale) {
+  auto grad = value_rows(grad_in, "grad");
+  const int tag = dense_tag(grad.scalar_type(), "grad");
+  undifferentiated("embedding_grad", {grad_in});
+  auto ids = ids_of(index, grad);
+  TORCH_CHECK(lead_of(grad_in.sizes()) == index.sizes().vec(), "grad must have a row for each id");
+  TORCH_CHECK(num_rows >= 0, "num_rows must not be negative");
+  c10::DeviceGuard guard(grad.device());
+  const int64_t n = ids.numel(), d = grad.size(1);
+  auto out = torch::empty({num_rows, d}, grad.options());
+  const int64_t bytes = f2cgt_embedding_grad_workspace_bytes(n, num_rows, d);
+  torch::Tensor ws;
+  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  check_rc(f2cgt_embedding_grad(grad.data_ptr(), tag, row_step(grad), ids.data_ptr(), id_tag(ids), out.data_ptr(), (float)scale,
+                                bytes > 0 ? ws.data_ptr() : nullptr, bytes, n, num_rows, d, current_stream()),
+           "embedding_grad");
+  return out;
+}
+
 }  // namespace
 
 // Output store policy of the SQ aggregation operators: "auto" (by output size), "stream"
@@ -1549,6 +1784,20 @@ PYBIND11_MODULE(F2CGTLib, m) {
       .def("muon_step", &muon_step, py::arg("weights"), py::arg("grads"), py::arg("momenta"), py::arg("step_size"),
            py::arg("decay") = 0.0, py::arg("momentum") = 0.95, py::arg("nesterov") = true, py::arg("steps") = 5,
            py::arg("coefficients") = std::array<double, 3>{3.4445, -4.7750, 2.0315})
+      .def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5)
+      .def("layer_norm_train", &layer_norm_train, py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+           py::arg("eps") = 1e-5, py::arg("pack") = false)
+      .def("layer_norm_grad", &layer_norm_grad, py::arg("grad"), py::arg("x"), py::arg("mean"), py::arg("rstd"),
+           py::arg("weight") = py::none(), py::arg("weight_grad") = true, py::arg("bias_grad") = true)
+      .def("layer_norm_packed_grad", &layer_norm_packed_grad, py::arg("grad"), py::arg("codes"), py::arg("exponents"),
+           py::arg("mean"), py::arg("rstd"), py::arg("weight") = py::none(), py::arg("weight_grad") = true, py::arg("bias_grad") = true)
+      .def("pack_activations", &pack_activations, py::arg("x"))
+      .def("unpack_activations", &unpack_activations, py::arg("codes"), py::arg("exponents"),
+           py::arg("dtype") = torch::ScalarType(torch::kFloat32))
+      .def("packed_linear_grad", &packed_linear_grad, py::arg("grad"), py::arg("codes"), py::arg("exponents"),
+           py::arg("bias") = false, py::arg("dtype") = torch::ScalarType(torch::kFloat32))
+      .def("embedding", &embedding, py::arg("table"), py::arg("index"), py::arg("scale") = 1.0)
+      .def("embedding_grad", &embedding_grad, py::arg("grad"), py::arg("index"), py::arg("num_rows"), py::arg("scale") = 1.0)
       .def("set_store_mode", &set_store_mode, py::arg("mode"));
   py::class_<PendingFlag, std::shared_ptr<PendingFlag>>(m, "PendingFlag").def("wait", &PendingFlag::wait);
   py::class_<KMeans>(m, "KMeans")

@@ -679,10 +679,10 @@ class CompressionManager:
 _MODULE_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
 
 
-def _plain_linear(layer):
-    """Whether calling `layer` is nn.Linear's own product and nothing else: no subclass or replaced forward, no
+def _plain_linear(layer, types=(nn.Linear,)):
+    """Whether calling `layer` is the own product of one of `types` and nothing else: no subclass or replaced forward, no
     parametrization (which is a subclass), no hook on it or on all modules."""
-    return (type(layer) is nn.Linear and "forward" not in layer.__dict__ and
+    return (type(layer) in types and "forward" not in layer.__dict__ and
             not any(getattr(layer, name) for name in _MODULE_HOOKS) and
             not any(getattr(_modules, "_global" + name) for name in _MODULE_HOOKS))
 
@@ -875,13 +875,147 @@ class Int8Linear(nn.Module):
         return _capi().quantized_linear(x, self.weight_codes[:, :self.in_features], self.weight_scales, self.bias)
 
 
+# ---- norms, 8-bit checkpoints and learnt rows for training -------------------------------------------
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, packed):
+        out, mean, rstd, *kept = _capi().layer_norm_train(x, weight, bias, eps, packed)
+        ctx.save_for_backward(weight, mean, rstd, *(kept or (x,)))
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        weight, mean, rstd, *kept = ctx.saved_tensors
+        wants = ctx.needs_input_grad
+        of = _capi().layer_norm_packed_grad if len(kept) == 2 else _capi().layer_norm_grad
+        dx, dw, db = of(grad, *kept, mean, rstd, weight, wants[1], wants[2])
+        return dx, dw, db, None, None
+
+
+class LayerNorm(nn.LayerNorm):
+    """`nn.LayerNorm` over the last dimension of rows on the GPU: one launch forward (and no statistics kept without gradients),
+    two backward.  With `packed` the backward pass keeps an 8-bit checkpoint of the input in place of the input itself, a
+    fourth of the memory (half for 16-bit inputs): its gradients are those at the decoded input, whose values are off by
+    up to 1/127 of the largest among the 32 columns around them.  Parameters in float32 or in the inputs' type; state as `nn.LayerNorm`'s."""
+
+    def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True, packed=False, device=None, dtype=None):
+        super().__init__(features, eps, elementwise_affine, bias, device=device, dtype=dtype)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("LayerNorm takes the last dimension only (got %s)" % (self.normalized_shape,))
+        self.packed = packed
+
+    def extra_repr(self):
+        return super().extra_repr() + (", packed=True" if self.packed else "")
+
+    def forward(self, x):
+        if x.shape[-1:] != self.normalized_shape:
+            raise ValueError("rows of %s do not fit a norm of %d" % (tuple(x.shape), self.normalized_shape[0]))
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias)):
+            return _LayerNorm.apply(x, self.weight, self.bias, self.eps, self.packed)
+        return _capi().layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class _PackedLinear(torch.autograd.Function):
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(weight, *_capi().pack_activations(x))
+        return nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @torch.amp.custom_bwd(device_type="cuda")
+    def backward(ctx, grad):
+        weight, codes, exponents = ctx.saved_tensors
+        wants = ctx.needs_input_grad
+        dx = torch.matmul(grad, weight) if wants[0] else None
+        dw = db = None
+        if wants[1]:
+            dw, db = _capi().packed_linear_grad(grad, codes, exponents, wants[2], weight.dtype)
+        elif wants[2]:
+            db = grad.reshape(-1, grad.shape[-1]).sum(dim=0, dtype=torch.float32).to(weight.dtype)
+        return dx, dw, db
+
+
+class PackedLinear(nn.Linear):
+    """An `nn.Linear` whose backward pass keeps its input as an 8-bit checkpoint (`pack_activations`): a fourth of the memory
+    of float32 inputs, half of 16-bit ones.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the one at the decoded
+    input.  `PackedLinear.of(linear)` shares a layer's parameters."""
+
+    @classmethod
+    def of(cls, linear):
+        self = cls.__new__(cls)
+        nn.Module.__init__(self)
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        self.register_parameter("weight", linear.weight)
+        self.register_parameter("bias", linear.bias)
+        self.train(linear.training)
+        return self
+
+    def forward(self, x):
+        if torch.is_grad_enabled() and self.weight.requires_grad:
+            return _PackedLinear.apply(x, self.weight, self.bias)
+        return super().forward(x)
+
+
+def packed_layers(module):
+    """`module` for training with less memory: every plain `nn.Linear` below it replaced by a `PackedLinear` of the same parameters, in
+    place, and the checkpoints of every `LayerNorm` packed.  What an optimiser holds stays what it trains."""
+    for name, child in list(module.named_children()):
+        if _plain_linear(child):
+            setattr(module, name, PackedLinear.of(child))
+        elif isinstance(child, LayerNorm):
+            child.packed = True
+        else:
+            packed_layers(child)
+    return module
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale = weight.shape[0], scale
+        return _capi().embedding(weight, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _capi().embedding_grad(grad, ctx.saved_tensors[0], ctx.rows, ctx.scale), None, None
+
+
+class NodeEmbedding(nn.Module):
+    """Learnt rows of nodes, next to `TensorCache`'s rows of given features: `rows(ids)` is `scale` times the rows of `weight`
+    [num_nodes, dim], zeros for an id outside the table (a place of a padded batch, -1).  The gradient is dense; a row's is the
+    sum over its ids in their order, so a step gives the same bits each time."""
+
+    def __init__(self, num_nodes, dim, scale=1.0, device=None, dtype=None):
+        super().__init__()
+        self.scale = float(scale)
+        self.weight = nn.Parameter(torch.empty((num_nodes, dim), device=device, dtype=dtype))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        """Rows whose scaled values have a variance of 1 / dim."""
+        nn.init.normal_(self.weight, std=1.0 / (abs(self.scale) or 1.0) / math.sqrt(max(1, self.weight.shape[1])))
+
+    def extra_repr(self):
+        return "%d, %d, scale=%g" % (*self.weight.shape, self.scale)
+
+    def forward(self, ids):
+        if torch.is_grad_enabled() and self.weight.requires_grad:
+            return _Embedding.apply(self.weight, ids, self.scale)
+        return _capi().embedding(self.weight, ids, self.scale)
+
+
 def int8_layers(module):
     """`module` for serving: every plain `nn.Linear` below it replaced by an `Int8Linear` of its weights, in place.  A
     `MySAGEConv` then makes its dense part in 8 bits: two products, their sum and the activation, one after the other.  That is for long
     blocks and wide layers: 250 000 x (100 + 100) -> 128 takes 194 us, in fp32 262; 10 000 x (128 + 128) -> 256 31 and 45; 1024 x (1024 + 1024) -> 1024 33
     and 47; but at 1024 x (128 + 128) -> 256 the host's four calls take 25 us, the one call in fp32 10."""
     for name, child in list(module.named_children()):
-        if _plain_linear(child):
+        if _plain_linear(child, (nn.Linear, PackedLinear)):
             setattr(module, name, Int8Linear(child))
         else:
             int8_layers(child)

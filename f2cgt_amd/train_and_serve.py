@@ -1,10 +1,12 @@
 """A GraphSAGE layer over compressed features, trained with orthogonalised updates and served with 8-bit weights:
 
-    python -m f2cgt_amd.train_and_serve [--nodes N] [--steps K] [--seed S]
+    python -m f2cgt_amd.train_and_serve [--nodes N] [--steps K] [--seed S] [--norm] [--packed] [--learnt]
 
 Features of a few classes are coded in 4 bits a value, a mean-aggregating layer (examples/conv.py:9-76) learns the classes
 with `pipeline.Muon` on its two weights (the bias goes to SGD), `pipeline.int8_layers` codes the trained weights, and the
-accuracies of both forms on blocks that were not trained on are printed.
+accuracies of both forms on blocks that were not trained on are printed.  `--norm` puts a `pipeline.LayerNorm` behind the layer,
+`--packed` keeps 8-bit checkpoints for the backward pass in place of activations (`pipeline.packed_layers`), and `--learnt` adds
+learnt rows (`pipeline.NodeEmbedding`) to the destination nodes' features.
 """
 from __future__ import annotations
 
@@ -27,7 +29,7 @@ def _block(nodes, rows, fanout, generator, labels):
     return seeds, torch.arange(0, rows * fanout + 1, fanout, device="cuda"), ids
 
 
-def run(nodes=20000, dim=100, classes=16, rows=1024, fanout=10, steps=60, seed=0):
+def run(nodes=20000, dim=100, classes=16, rows=1024, fanout=10, steps=60, seed=0, norm=False, packed=False, learnt=False):
     """-> (accuracy with fp32 weights, with 8-bit weights, share of equal answers, losses)."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     torch.manual_seed(seed)
@@ -37,14 +39,20 @@ def run(nodes=20000, dim=100, classes=16, rows=1024, fanout=10, steps=60, seed=0
     table, codebooks = pipeline.sq_compress(features, 4, 104, sample_index=torch.arange(nodes))
     manager = pipeline.CompressionManager({"methods": ["sq"], "feat_dim": dim, "configs": [(104, 4)], "codebooks": [codebooks],
                                            "compression_data": table}, fusion=True)
-    layer = pipeline.MySAGEConv(dim, classes, "mean", manager).cuda()
+    layer = pipeline.MySAGEConv(dim, classes, "mean", manager, norm=pipeline.LayerNorm(classes) if norm else None).cuda()
+    if packed:
+        pipeline.packed_layers(layer)
+    rows_of = pipeline.NodeEmbedding(nodes, dim, scale=0.1).cuda() if learnt else None
     weights = [layer.fc_self.weight, layer.fc_neigh.weight]
     muon = pipeline.Muon(weights, lr=0.05, weight_decay=0.01)
-    sgd = torch.optim.SGD([layer.fc_self.bias], lr=0.05)
+    sgd = torch.optim.SGD([layer.fc_self.bias] + (list(layer.norm.parameters()) if norm else []) +
+                          (list(rows_of.parameters()) if learnt else []), lr=0.05)
 
     def scores(of, block):
         seeds, indptr, ids = block
         h_self = manager._decompress(0, manager.data[seeds])
+        if learnt:
+            h_self = h_self + rows_of(seeds)
         return of((indptr, ids), (h_self, manager.data.data))
 
     losses = []
@@ -77,8 +85,11 @@ def main():
     p.add_argument("--nodes", type=int, default=20000)
     p.add_argument("--steps", type=int, default=60)
     p.add_argument("--seed", type=int, default=0)
+    p.add_argument("--norm", action="store_true")
+    p.add_argument("--packed", action="store_true")
+    p.add_argument("--learnt", action="store_true")
     a = p.parse_args()
-    full, few, equal, losses = run(nodes=a.nodes, steps=a.steps, seed=a.seed)
+    full, few, equal, losses = run(nodes=a.nodes, steps=a.steps, seed=a.seed, norm=a.norm, packed=a.packed, learnt=a.learnt)
     print("loss %.3f -> %.3f; accuracy fp32 %.3f, 8-bit weights %.3f, equal answers %.3f" %
           (losses[0], losses[-1], full, few, equal))
 

@@ -442,6 +442,69 @@ int f2cgt_muon_step(void* const* weights, int weight_dtype, const void* const* g
                     int64_t count, int64_t rows, int64_t cols, float step_size, float decay, float momentum, int nesterov,
                     int steps, const float* coefficients, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- layer norm --------------------------------------------------------------------- */
+
+/* No counterpart in the reference, whose layer calls whatever norm it is given (examples/conv.py:72-74).  Values: F2CGT_DT_F32,
+ * F2CGT_DT_F16, F2CGT_DT_BF16; weight and bias [d] (either may be NULL: ones, zeros) fp32 or of the rows' type.
+ *
+ * f2cgt_layer_norm: rows of x [m, d] (ld values apart) -> out [m, d] (dense, not x's buffer), (x - mean) * rstd * weight + bias
+ * with rstd = 1 / sqrt(mean((x - mean)^2) + eps); where mean and rstd (fp32 [m]) are not NULL, those too; where codes and exponents
+ * are not NULL, the checkpoint of x that f2cgt_pack_activations writes.
+ *
+ * f2cgt_layer_norm_grad: of grad [m, d] (grad_ld apart) and what the forward pass kept, x or its checkpoint (the other NULL):
+ * dx [m, d] (dense, no input's buffer), and where not NULL dweight and dbias [d] of grad_dtype.  The sums are made in a fixed order.
+ * workspace: f2cgt_layer_norm_grad_workspace_bytes (with neither sum: none), 16-byte aligned, contents irrelevant. */
+int f2cgt_layer_norm(const void* x, int dtype, int64_t ld, const void* weight, const void* bias, int weight_dtype, void* out,
+                     float* mean, float* rstd, int8_t* codes, int64_t code_stride, uint8_t* exponents, int64_t m, int64_t d,
+                     float eps, void* stream);
+int64_t f2cgt_layer_norm_grad_workspace_bytes(int dtype, int64_t m, int64_t d);
+int f2cgt_layer_norm_grad(const void* grad, int dtype, int64_t grad_ld, const void* x, int64_t ld, const int8_t* codes,
+                          int64_t code_stride, const uint8_t* exponents, const float* mean, const float* rstd, const void* weight,
+                          int weight_dtype, void* dx, void* dweight, void* dbias, int grad_dtype, void* workspace,
+                          int64_t workspace_bytes, int64_t m, int64_t d, void* stream);
+
+/* ---- activations kept in 8 bits for the backward pass --------------------------------- */
+
+/* No counterpart in the reference (it compresses features, not activations).
+ *
+ * f2cgt_pack_activations: x [m, k], rows ld values apart -> codes int8 [m, k], rows code_stride bytes apart (a multiple of 16, as is
+ * the buffer), and exponents uint8 [m, ceil(k / 32)]: of each 32 columns of a row, the last group of a row having fewer,
+ *   value = code * 2^(E - 127),  E - 127 the least whole number, -126 at least, with max|x| <= 127 * 2^(E - 127),
+ *   code = rint(x * 2^(127 - E)) (at E = 249, fp32's top, within +-63);
+ * a group with a NaN or an infinity has E = 255 and codes of zero, which stand for NaN.  The step is a power of two, so a value is a
+ * bf16 exactly.  Bytes behind a row's k are not written.
+ *
+ * f2cgt_unpack_activations: the values, out [m, k] dense; fp16 within +-65504.  The 16-byte piece with a row's last code must be
+ * readable, here and below.
+ *
+ * f2cgt_packed_linear_grad: dweight [n, k] = grad^T values and, where not NULL, dbias [n] = sums of grad's columns, dense, of out_dtype;
+ * grad [m, n] of dtype, rows ld apart.  Products are exact (parts
+ * of fp32 gradients below 2^-126 count as zeros), sums fp32 in a fixed order.  An infinity in grad gives NaN in its row
+ * of dweight.  workspace: f2cgt_packed_linear_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
+int f2cgt_pack_activations(const void* x, int dtype, int64_t ld, int8_t* codes, int64_t code_stride, uint8_t* exponents,
+                           int64_t m, int64_t k, void* stream);
+int f2cgt_unpack_activations(const int8_t* codes, int64_t code_stride, const uint8_t* exponents, void* out, int dtype, int64_t m,
+                             int64_t k, void* stream);
+int64_t f2cgt_packed_linear_grad_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld, const int8_t* codes, int64_t code_stride,
+                             const uint8_t* exponents, void* dweight, void* dbias, int out_dtype, void* workspace,
+                             int64_t workspace_bytes, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* ---- learnt rows ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose rows are features and are not trained.  index: F2CGT_DT_I32 or F2CGT_DT_I64 [n]; unlike
+ * elsewhere in this file an id outside [0, rows) is no row (a place of a padded batch): zeros, and no gradient.
+ *
+ * f2cgt_embedding: out [n, d] (dense) = scale * table[index], table [rows, d] with rows ld values apart.
+ * f2cgt_embedding_grad: dtable [rows, d] (dense, of grad's type), every row written: scale times the sum, in the order of their places and in
+ * fp32, of the rows of grad [n, d] (ld apart) whose id it is.  Rows with up to 64 ids are added one after the other, longer ones in
+ * parts that the sizes and ids fix.  workspace: f2cgt_embedding_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
+int f2cgt_embedding(const void* table, int dtype, int64_t ld, const void* index, int idx_dtype, void* out, float scale, int64_t n,
+                    int64_t rows, int64_t d, void* stream);
+int64_t f2cgt_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t d);
+int f2cgt_embedding_grad(const void* grad, int dtype, int64_t ld, const void* index, int idx_dtype, void* dtable, float scale,
+                         void* workspace, int64_t workspace_bytes, int64_t n, int64_t rows, int64_t d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
