@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(PackArgs a) {
 // ---- the weight's gradient -----------------------------------------------------------------------------
 typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
 
 struct GradArgs {
   const void* grad;          // [m, n], rows ld apart
@@ -156,32 +157,60 @@ struct GradArgs {
 
 template <typename T> constexpr int kPlanes = dtype_of<T>::tag == F2CGT_DT_F32 ? 3 : dtype_of<T>::tag == F2CGT_DT_F16 ? 2 : 1;
 
-// Eight numbers of T as bf16 planes, whose sum they are.  Each plane is the upper half of what is left: no rounding, 8 bits each.
-// (An infinity leaves a NaN, as it does in the sum of the product.)
-template <typename T>
-__device__ __forceinline__ void planes_of(const float (&v)[8], intx4 (&planes)[kPlanes<T>]) {
-  float left[8];
+// Eight numbers of T, as memory holds them.
+template <typename T> struct Eight {
+  static constexpr int kWords = 2 * (int)sizeof(T);
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const char* p) {
+    typedef typename piece_words<T, kPieceOf<T>>::type words;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) left[e] = v[e];
+    for (int i = 0; i < kWords; i += 4) {
+      const words v = reinterpret_cast<const words*>(p)[i / 4];
 #pragma unroll
-  for (int p = 0; p < kPlanes<T>; ++p) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      planes[p][e] = (int)__builtin_amdgcn_perm(__float_as_uint(left[2 * e + 1]), __float_as_uint(left[2 * e]), 0x07060302);
-    if (p + 1 < kPlanes<T>)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) left[e] -= __uint_as_float(__float_as_uint(left[e]) & 0xFFFF0000u);
+      for (int e = 0; e < 4; ++e) w[i + e] = v[e];
+    }
   }
-}
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else if constexpr (dtype_of<T>::tag == F2CGT_DT_BF16) return __uint_as_float(e % 2 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> 16 * (e % 2)));
+  }
+  __device__ __forceinline__ void set(int e, T v) {
+    if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(v);
+    else w[e / 2] = e % 2 ? w[e / 2] | (uint32_t)__builtin_bit_cast(uint16_t, v) << 16 : (uint32_t)__builtin_bit_cast(uint16_t, v);
+  }
+  // As bf16 planes, whose sum the numbers are.  Each plane is the upper half of what is left: no rounding, 8 bits each.  (An infinity
+  // leaves a NaN.)
+  __device__ __forceinline__ void planes(intx4 (&p)[kPlanes<T>]) const {
+    if constexpr (kPlanes<T> == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[0][e] = (int)w[e];
+    } else {
+      float left[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) left[e] = (*this)[e];
+#pragma unroll
+      for (int i = 0; i < kPlanes<T>; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[i][e] = (int)__builtin_amdgcn_perm(__float_as_uint(left[2 * e + 1]), __float_as_uint(left[2 * e]), 0x07060302);
+        if (i + 1 < kPlanes<T>)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) left[e] -= __uint_as_float(__float_as_uint(left[e]) & 0xFFFF0000u);
+      }
+    }
+  }
+};
 
-// A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step.  Rows lie in LDS as they do in memory, one line
-// of BN or BK bf16 a row, and matrix operands, which hold eight rows of one column a lane, are read through the transposing
-// LDS loads: sixteen lanes give the addresses of 4 rows x 16 columns in four pieces a row, and get a column each.  Units of 64 bytes of a
-// line change places by the row's last two bits, so the four rows of such a read lie in different banks.
-template <typename T, int BN, int BK, int WN, int WK, int BM>
+// A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step; GROUPS groups of waves take the steps in turn and
+// add their sums in the end.  Rows lie in LDS as they do in memory, one line of BN or BK bf16 a row, and matrix operands, which hold
+// eight rows of one column a lane, are read through the transposing LDS loads: sixteen lanes give the addresses of 4 rows x 16
+// columns in four pieces a row, and get a column each.  Units of 64 bytes of a line change places by the row's last two bits, so the four
+// rows of such a read lie in different banks.
+template <typename T, int BN, int BK, int WN, int WK, int BM, int GROUPS>
 struct GradTile {
   static constexpr int P = kPlanes<T>;
-  static constexpr int kThreads = (BN / WN) * (BK / WK) * kWave;
+  static constexpr int kThreads = (BN / WN) * (BK / WK) * kWave, kBlock = kThreads * GROUPS;
   static constexpr int TI = WN / 32, TJ = WK / 32;
   static constexpr int kLineG = BN * 2, kLineX = BK * 2;               // bytes
   static constexpr int kPlaneG = BM * kLineG;
@@ -190,21 +219,31 @@ struct GradTile {
   static_assert(kPiecesG * kThreads * 8 == BM * BN && kPiecesX * kThreads * 8 == BM * BK, "whole pieces per thread");
   static_assert(kThreads % (BN / 8) == 0 && kThreads % (BK / 8) == 0, "a thread's pieces are of the same columns");
   static constexpr int kRowsG = kThreads / (BN / 8), kRowsX = kThreads / (BK / 8);                // rows between a thread's pieces
-  static constexpr int kGroups = BM / 16;
+  static constexpr int kParts = BM / 16;
+  static_assert(kPiecesG % kParts == 0 || kPiecesG < kParts, "pieces in turn with products");
 
   // (64 banks hold one line of 256 bytes or half of a longer one, and two lines of 128)
   static __device__ __forceinline__ int line_at(int row, int byte, int line) {
     return row * line + (byte ^ (line == 128 ? (row >> 1 & 1) << 6 : (row & 3) << 6));
   }
+  struct Held {
+    Eight<T> g[kPiecesG];
+    uint2 x[kPiecesX];
+    uint32_t e[kPiecesX];
+  };
 };
 
-template <typename T, int BN, int BK, int WN, int WK, int BM>
-__global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave) void packed_linear_grad_kernel(GradArgs a) {
-  typedef GradTile<T, BN, BK, WN, WK, BM> Tile;
-  constexpr int P = Tile::P, TI = Tile::TI, TJ = Tile::TJ;
-  __shared__ __attribute__((aligned(16))) char stages[2 * Tile::kStage];
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+template <typename T, int BN, int BK, int WN, int WK, int BM, int GROUPS>
+__global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed_linear_grad_kernel(GradArgs a) {
+  typedef GradTile<T, BN, BK, WN, WK, BM, GROUPS> Tile;
+  constexpr int P = Tile::P, TI = Tile::TI, TJ = Tile::TJ, kThreads = Tile::kThreads;
+  constexpr int kAcross = (BN * BK * 4) * (GROUPS - 1);                 // the groups' sums on their way to the first one
+  constexpr int kLds = 2 * Tile::kStage * GROUPS > kAcross ? 2 * Tile::kStage * GROUPS : kAcross;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
+  const int t = threadIdx.x - group * kThreads, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int wi = (wave % (BN / WN)) * WN, wj = (wave / (BN / WN)) * WK;
+  char* stages = lds + group * 2 * Tile::kStage;
   // neighbours in time share rows: all tiles of a split are one XCD's
   const uint32_t tiles = a.tiles_n * a.tiles_k, place = place_of(blockIdx.x, tiles * a.splits);
   const uint32_t split = place / tiles;
@@ -216,76 +255,74 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave) void packed_linear_g
   // this thread's columns: those beyond the operand's end repeat its first ones (what they give is not kept)
   const int pg = t % (BN / 8) * 8, px = t % (BK / 8) * 8, rg = t / (BN / 8), rx = t / (BK / 8);
   const int cg = col_n + pg < a.n ? col_n + pg : 0, cx = col_k + px < a.k ? col_k + px : 0;
-  const T* grad = static_cast<const T*>(a.grad) + cg;
-  const int8_t* codes = a.codes + cx;
-  const uint8_t* exponents = a.exponents + cx / kCheckpointGroup;
+  // (32 bits from a step's first row: strides are below 2^24)
+  const uint32_t off_g = (uint32_t)(rg * (int)a.ld + cg) * (uint32_t)sizeof(T), off_x = (uint32_t)(rx * (int)a.code_stride + cx);
+  const uint32_t off_e = (uint32_t)(rx * a.groups + cx / kCheckpointGroup);
+  typedef typename Tile::Held Held;
 
-  float g[Tile::kPiecesG][8];
-  uint2 x[Tile::kPiecesX];
-  uint32_t ex[Tile::kPiecesX];
-  // A piece that runs over its row's end reads on in the next one; the last rows, which have none, are read value by value.
-  auto load = [&](int64_t step) {
-    const int64_t row0 = step * BM;
-    if (row0 + BM < a.m && a.n >= 8 && a.k > 0) {
+  // A piece that runs over its row's end reads on in the next one; the last rows, which have none, are read value by value.  Steps behind
+  // the last one read it again.
+  const bool pieces = a.n >= 8 && a.k > 0;
+  auto load = [&](Held& h, int64_t step) {
+    const int64_t row0 = (step < to ? step : to - 1) * BM;
+    const char* grad = static_cast<const char*>(a.grad) + row0 * a.ld * (int64_t)sizeof(T);
+    const int8_t* codes = a.codes + row0 * a.code_stride;
+    const uint8_t* exponents = a.exponents + row0 * a.groups;
+    if (row0 + BM < a.m && pieces) {
 #pragma unroll
-      for (int i = 0; i < Tile::kPiecesG; ++i) {
-        const T* p = grad + (row0 + rg + i * Tile::kRowsG) * a.ld;
-        if constexpr (sizeof(T) == 4) {
-          load_piece<T, 4>(p, *reinterpret_cast<float (*)[4]>(&g[i][0]));
-          load_piece<T, 4>(p + 4, *reinterpret_cast<float (*)[4]>(&g[i][4]));
-        } else {
-          load_piece<T, 8>(p, g[i]);
-        }
-      }
+      for (int i = 0; i < Tile::kPiecesG; ++i) h.g[i].load(grad + (int64_t)i * Tile::kRowsG * a.ld * (int64_t)sizeof(T) + off_g);
 #pragma unroll
       for (int i = 0; i < Tile::kPiecesX; ++i) {
-        const int64_t row = row0 + rx + i * Tile::kRowsX;
-        x[i] = *reinterpret_cast<const uint2*>(codes + row * a.code_stride);
-        ex[i] = exponents[row * a.groups];
+        h.x[i] = *reinterpret_cast<const uint2*>(codes + i * Tile::kRowsX * a.code_stride + off_x);
+        h.e[i] = exponents[(int64_t)i * Tile::kRowsX * a.groups + off_e];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < Tile::kPiecesG; ++i) {
-        const int64_t row = row0 + rg + i * Tile::kRowsG;
+        const bool in = row0 + rg + i * Tile::kRowsG < a.m;
+        const T* p = reinterpret_cast<const T*>(grad + (int64_t)i * Tile::kRowsG * a.ld * (int64_t)sizeof(T) + off_g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          g[i][e] = 0.f;
-          if (row < a.m && cg + e < a.n) g[i][e] = (float)grad[row * a.ld + e];
+          T v = (T)0.f;
+          if (in && cg + e < a.n) v = p[e];
+          h.g[i].set(e, v);
         }
       }
 #pragma unroll
       for (int i = 0; i < Tile::kPiecesX; ++i) {
-        const int64_t row = row0 + rx + i * Tile::kRowsX;
-        x[i] = uint2{0, 0};
-        ex[i] = 127;
-        if (row < a.m && a.k > 0) {
-          x[i] = *reinterpret_cast<const uint2*>(codes + row * a.code_stride);
-          ex[i] = exponents[row * a.groups];
+        h.x[i] = uint2{0, 0};
+        h.e[i] = 127;
+        if (row0 + rx + i * Tile::kRowsX < a.m && a.k > 0) {
+          h.x[i] = *reinterpret_cast<const uint2*>(codes + i * Tile::kRowsX * a.code_stride + off_x);
+          h.e[i] = exponents[(int64_t)i * Tile::kRowsX * a.groups + off_e];
         }
       }
     }
   };
   const bool sums = a.bias != nullptr && tj == 0;
   float db[8] = {};
-  auto place_held = [&](char* stage) {
+  // Pieces of one of kParts parts into a stage.
+  auto place_part = [&](const Held& h, char* stage, int part, bool count) {
 #pragma unroll
     for (int i = 0; i < Tile::kPiecesG; ++i) {
-      if (sums)
+      if (i % Tile::kParts != part) continue;
+      if (sums && count)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) db[e] += g[i][e];
+        for (int e = 0; e < 8; ++e) db[e] += h.g[i][e];
       intx4 planes[P];
-      planes_of<T>(g[i], planes);
+      h.g[i].planes(planes);
 #pragma unroll
       for (int p = 0; p < P; ++p)
         *reinterpret_cast<intx4*>(stage + p * Tile::kPlaneG + Tile::line_at(rg + i * Tile::kRowsG, pg * 2, Tile::kLineG)) = planes[p];
     }
 #pragma unroll
     for (int i = 0; i < Tile::kPiecesX; ++i) {
-      const float step = step_of(ex[i]);
+      if (i % Tile::kParts != part) continue;
+      const float step = step_of(h.e[i]);
       intx4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t word = e < 2 ? x[i].x : x[i].y;
+        const uint32_t word = e < 2 ? h.x[i].x : h.x[i].y;
         v[e] = (int)__builtin_amdgcn_perm(__float_as_uint(coded_value(word, 2 * (e % 2) + 1, step)),
                                           __float_as_uint(coded_value(word, 2 * (e % 2), step)), 0x07060302);
       }
@@ -302,77 +339,116 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave) void packed_linear_g
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
   // A lane's part of an operand: eight rows of column lane % 32, the rows 8 (lane / 32) on of a group of sixteen.
   const int tr_row = (lane >> 5) * 8 + (lane >> 2 & 3), tr_byte = ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
-  auto operand = [&](const char* plane, int group, int column, int line) {
+  auto operand = [&](const char* plane, int part, int column, int line) {
     shortx4 half[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) shortx4*)(plane + Tile::line_at(group * 16 + tr_row + 4 * h, column * 2 + tr_byte, line)));
-    typedef short shortx8 __attribute__((ext_vector_type(8)));
+          (__attribute__((address_space(3))) shortx4*)(plane + Tile::line_at(part * 16 + tr_row + 4 * h, column * 2 + tr_byte, line)));
     const shortx8 both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bfx8, both);
   };
-  auto multiply = [&](const char* stage) {
+  auto multiply_part = [&](const char* stage, int s) {
+    bfx8 fx[TJ];
 #pragma unroll
-    for (int s = 0; s < Tile::kGroups; ++s) {
-      bfx8 fx[TJ];
+    for (int j = 0; j < TJ; ++j) fx[j] = operand(stage + P * Tile::kPlaneG, s, wj + 32 * j, Tile::kLineX);
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) fx[j] = operand(stage + P * Tile::kPlaneG, s, wj + 32 * j, Tile::kLineX);
+    for (int p = P - 1; p >= 0; --p) {
+      bfx8 fg[TI];
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p) {
-        bfx8 fg[TI];
+      for (int i = 0; i < TI; ++i) fg[i] = operand(stage + p * Tile::kPlaneG, s, wi + 32 * i, Tile::kLineG);
 #pragma unroll
-        for (int i = 0; i < TI; ++i) fg[i] = operand(stage + p * Tile::kPlaneG, s, wi + 32 * i, Tile::kLineG);
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[i], fx[j], acc[i][j], 0, 0, 0);
+    }
+  };
+  // Two steps of each group are on their way from memory while one is multiplied: a round trip is longer than a step.
+  // Step s is multiplied out of stage s % 2 while the next one is placed in the other; then the registers of that take the step after the next two.
+  const int64_t rounds = (to - from + GROUPS - 1) / GROUPS;
+  Held held[2];
+  load(held[0], from + group);
+  load(held[1], from + group + GROUPS);
+#pragma unroll
+  for (int part = 0; part < Tile::kParts; ++part) place_part(held[0], stages, part, from + group < to);
+  load(held[0], from + group + 2 * GROUPS);
+  __syncthreads();
+  for (int64_t r = 0; r < rounds; r += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (r + u < rounds) {
+        const int64_t step = from + group + (r + u) * GROUPS;
+        char* now = stages + u * Tile::kStage;
+        char* next = stages + (u ^ 1) * Tile::kStage;
+        Held& h = held[u ^ 1];
+#pragma unroll
+        for (int part = 0; part < Tile::kParts; ++part) {
+          if (GROUPS == 1 || step < to) multiply_part(now, part);
+          place_part(h, next, part, step + GROUPS < to);
+        }
+        load(h, step + 3 * GROUPS);
+        __syncthreads();
+      }
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    // the other groups' sums, in their order
+    float* across = reinterpret_cast<float*>(lds);
+    if (group > 0) {
+      float* to_first = across + (group - 1) * BN * BK;
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) to_first[((i * TJ + j) * 16 + v) * kThreads + t] = acc[i][j][v];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 0; g < GROUPS - 1; ++g)
 #pragma unroll
         for (int i = 0; i < TI; ++i)
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[i], fx[j], acc[i][j], 0, 0, 0);
-      }
-    }
-  };
-  if (from < to) {
-    load(from);
-    place_held(stages);
-    __syncthreads();
-    for (int64_t step = from; step < to; ++step) {
-      const int turn = (int)(step - from) & 1;
-      char* now = stages + turn * Tile::kStage;
-      char* next = stages + (turn ^ 1) * Tile::kStage;
-      if (step + 1 < to) load(step + 1);
-      multiply(now);
-      if (step + 1 < to) place_held(next);
-      __syncthreads();
+          for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] += across[g * BN * BK + ((i * TJ + j) * 16 + v) * kThreads + t];
     }
   }
-
   // Sums out: a lane holds, of column lane % 32, rows 4 (lane / 32) to + 3 after every eight.
+  if (group == 0) {
 #pragma unroll
-  for (int i = 0; i < TI; ++i)
+    for (int i = 0; i < TI; ++i)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j)
+      for (int j = 0; j < TJ; ++j)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int row = col_n + wi + 32 * i + 8 * (v / 4) + 4 * (lane >> 5) + v % 4, column = col_k + wj + 32 * j + (lane & 31);
-        if (row < a.n && column < a.k) {
-          const int64_t at = (int64_t)row * a.k + column;
-          if (a.parts != nullptr) a.parts[(int64_t)split * a.n * a.k + at] = acc[i][j][v];
-          else store_value(a.out, a.out_tag, at, acc[i][j][v]);
+        for (int v = 0; v < 16; ++v) {
+          const int row = col_n + wi + 32 * i + 8 * (v / 4) + 4 * (lane >> 5) + v % 4, column = col_k + wj + 32 * j + (lane & 31);
+          if (row < a.n && column < a.k) {
+            const int64_t at = (int64_t)row * a.k + column;
+            if (a.parts != nullptr) a.parts[(int64_t)split * a.n * a.k + at] = acc[i][j][v];
+            else store_value(a.out, a.out_tag, at, acc[i][j][v]);
+          }
         }
-      }
+  }
   if (!sums) return;
-  float* room = reinterpret_cast<float*>(stages);
+  if constexpr (GROUPS > 1) __syncthreads();
+  constexpr int kRows = Tile::kRowsG * GROUPS;
+  static_assert(kRows * BN * 4 <= kLds, "the bias' sums fit");
+  float* room = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) room[rg * BN + pg + e] = db[e];
+  for (int e = 0; e < 8; ++e) room[(group * Tile::kRowsG + rg) * BN + pg + e] = db[e];
   __syncthreads();
-  if (t < BN && col_n + t < a.n) {
+  if (threadIdx.x < BN && col_n + (int)threadIdx.x < a.n) {
     float sum = 0.f;
-    for (int r = 0; r < Tile::kRowsG; ++r) sum += room[r * BN + t];
-    if (a.parts != nullptr) a.parts[(int64_t)a.splits * a.n * a.k + (int64_t)split * a.n + col_n + t] = sum;
-    else store_value(a.bias, a.out_tag, col_n + t, sum);
+    for (int r = 0; r < kRows; ++r) sum += room[r * BN + threadIdx.x];
+    if (a.parts != nullptr) a.parts[(int64_t)a.splits * a.n * a.k + (int64_t)split * a.n + col_n + threadIdx.x] = sum;
+    else store_value(a.bias, a.out_tag, col_n + threadIdx.x, sum);
   }
 }
 
-// Sums over the splits, in their order; the bias' in workgroups behind the weight's.  (No splits: zeros, of no rows.)
+// Sums over the splits: a workgroup has 256 outputs, each of its waves every fourth split, then the waves' sums in order; the bias' in
+// workgroups behind the weight's.  (No splits: zeros, of no rows.)
 struct JoinArgs {
   const float* parts;
   void* out;
@@ -382,27 +458,36 @@ struct JoinArgs {
   uint32_t splits, blocks;   // blocks: those of the weight
 };
 __global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
-  if (blockIdx.x < a.blocks) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at >= a.count) return;
-    if (a.whole) {
-      fltx4 sum = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t s = 0; s < a.splits; ++s) sum += *reinterpret_cast<const fltx4*>(a.parts + s * a.count + at);
-      store_four(a.out, a.tag, at, sum);
-    } else {
-      for (int e = 0; e < 4 && at + e < a.count; ++e) {
-        float sum = 0.f;
-        for (uint32_t s = 0; s < a.splits; ++s) sum += a.parts[s * a.count + at + e];
-        store_value(a.out, a.tag, at + e, sum);
+  __shared__ __attribute__((aligned(16))) float room[4][256];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const bool weight = blockIdx.x < a.blocks;
+  const int64_t count = weight ? a.count : a.n, first = (int64_t)(weight ? blockIdx.x : blockIdx.x - a.blocks) * 256;
+  const float* parts = weight ? a.parts : a.parts + (int64_t)a.splits * a.count;
+  void* out = weight ? a.out : a.bias;
+  const int64_t at = first + 4 * lane;
+  fltx4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (weight && a.whole) {
+    if (at < count) {
+      uint32_t s = wave;
+      for (; s + 12 < a.splits; s += 16) {
+        fltx4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const fltx4*>(parts + (int64_t)(s + 4 * u) * count + at);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum += v[u];
       }
+      for (; s < a.splits; s += 4) sum += *reinterpret_cast<const fltx4*>(parts + (int64_t)s * count + at);
     }
   } else {
-    const int64_t at = (int64_t)(blockIdx.x - a.blocks) * 256 + threadIdx.x;
-    if (at >= a.n) return;
-    float sum = 0.f;
-    for (uint32_t s = 0; s < a.splits; ++s) sum += a.parts[a.splits * a.count + (int64_t)s * a.n + at];
-    store_value(a.bias, a.tag, at, sum);
+    for (uint32_t s = wave; s < a.splits; s += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += at + e < count ? parts[(int64_t)s * count + at + e] : 0.f;
   }
+  *reinterpret_cast<fltx4*>(&room[wave][4 * lane]) = sum;
+  __syncthreads();
+  if (first + threadIdx.x >= count) return;
+  const float all = room[0][threadIdx.x] + room[1][threadIdx.x] + room[2][threadIdx.x] + room[3][threadIdx.x];
+  store_value(out, a.tag, first + threadIdx.x, all);
 }
 
 // How a product is cut: tiles of `size` squared, rows in `splits`.
@@ -414,11 +499,11 @@ Cut cut_of(int dtype, int64_t m, int64_t n, int64_t k) {
   const int64_t cus = num_cus();
   Cut c;
   auto tiles = [&](int size) { return ceil_div(n, size) * (k > 0 ? ceil_div(k, size) : 1); };     // (a bias has rows without columns too)
-  c.size = tiles(256) >= cus ? 256 : tiles(128) >= 8 || n * k >= 128 * 128 ? 128 : 64;
+  c.size = tiles(256) >= cus ? 256 : tiles(64) * ceil_div(m, 32) <= 4 * cus ? 64 : n * k > 64 * 64 ? 128 : 64;
   const int bm = dtype == F2CGT_DT_BF16 && c.size != 64 ? 64 : 32;
   c.tiles = tiles(c.size);
   c.steps = ceil_div(m, bm);
-  const int64_t most = ceil_div(c.steps, 4), want = c.size == 256 ? 1 : 2 * cus / c.tiles;
+  const int64_t most = c.steps, want = c.size == 256 ? 1 : c.size == 128 ? cus / c.tiles : 2 * cus / c.tiles;
   c.splits = want < 1 ? 1 : want > most ? most : want;
   return c;
 }
@@ -500,6 +585,7 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
   if (int rc = check_sizes(what, m, n, k)) return rc;
   F2CGT_REQUIRE(dense_type(dtype) && dense_type(out_dtype), F2CGT_E_UNSUPPORTED, "%s: fp32, fp16 or bf16 only", what);
   F2CGT_REQUIRE(m <= 1 || ld >= n, F2CGT_E_INVALID, "%s: rows overlap", what);
+  F2CGT_REQUIRE(m <= 1 || (ld < (1ll << 24) && code_stride < (1ll << 24)), F2CGT_E_UNSUPPORTED, "%s: rows 2^24 and more apart", what);
   if (n == 0 || (k == 0 && !dbias)) return 0;
   F2CGT_REQUIRE(dweight || k == 0, F2CGT_E_INVALID, "%s: null buffer", what);
   F2CGT_REQUIRE(aligned(grad, type_size(dtype)) && aligned(dweight, type_size(out_dtype)) && aligned(dbias, type_size(out_dtype)),
@@ -524,16 +610,16 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
     const int rc = with_type(dtype, [&](auto t) {
       typedef decltype(t) T;
       constexpr int BM = kPlanes<T> == 1 ? 64 : 32;
-      if (c.size == 256) packed_linear_grad_kernel<T, 256, 256, 128, 64, BM><<<grid, dim3(512), 0, st>>>(a);
-      else if (c.size == 128) packed_linear_grad_kernel<T, 128, 128, 64, 64, BM><<<grid, dim3(256), 0, st>>>(a);
-      else packed_linear_grad_kernel<T, 64, 64, 32, 32, 32><<<grid, dim3(256), 0, st>>>(a);
+      if (c.size == 256) packed_linear_grad_kernel<T, 256, 256, 128, 64, BM, 1><<<grid, dim3(512), 0, st>>>(a);
+      else if (c.size == 128) packed_linear_grad_kernel<T, 128, 128, 64, 64, BM, 2><<<grid, dim3(512), 0, st>>>(a);
+      else packed_linear_grad_kernel<T, 64, 64, 32, 32, 32, 1><<<grid, dim3(256), 0, st>>>(a);
       return launch_status(what);
     });
     if (rc || c.splits == 1) return rc;
   }
   JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype,
-             n * k % 4 == 0 && aligned(dweight, 4 * type_size(out_dtype)), (uint32_t)c.splits, (uint32_t)ceil_div(n * k, 1024)};
-  F2CGT_REQUIRE(ceil_div(n * k, 1024) < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
+             n * k % 4 == 0 && aligned(dweight, 4 * type_size(out_dtype)), (uint32_t)c.splits, (uint32_t)ceil_div(n * k, 256)};
+  F2CGT_REQUIRE(ceil_div(n * k, 256) < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
   join_splits_kernel<<<dim3(j.blocks + (dbias ? (unsigned)ceil_div(n, 256) : 0u)), dim3(256), 0, st>>>(j);
   return launch_status(what);
 }

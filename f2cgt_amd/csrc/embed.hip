@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs a) {
 }
 
 // ---- sorting by digits ------------------------------------------------------------------------------------
-constexpr int kSortThreads = 256, kSortItems = 16, kSortTile = kSortThreads * kSortItems, kSortWaves = kSortThreads / kWave;
+constexpr int kSortThreads = 1024, kSortItems = 4, kSortTile = kSortThreads * kSortItems, kSortWaves = kSortThreads / kWave;
 constexpr int kMostBits = 10;
 
 struct SortArgs {
@@ -243,80 +243,122 @@ struct SumArgs {
   float scale;
 };
 
-// Adds to v the piece at `at` of the gradients of places[first], places[first + 1], ... in order.
+// Adds to v the piece at `at` of the gradients of places[first], places[first + 1], ... in order, eight on their way at a time.
 template <typename T, int V, typename Place>
 __device__ __forceinline__ void add_rows(float (&v)[V], const SumArgs& a, const Place* places, uint32_t first, uint32_t last, int at) {
   constexpr int kUnroll = 8;
   typedef typename piece_words<T, V>::type words;
   const T* grad = static_cast<const T*>(a.grad) + at;
-  uint32_t i = first;
-  for (; i + kUnroll <= last; i += kUnroll) {
+  for (uint32_t i = first; i < last; i += kUnroll) {
     words w[kUnroll];
+    const uint32_t left = last - i;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u] = *reinterpret_cast<const words*>(grad + (int64_t)places[i + u] * a.ld);
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < left) w[u] = *reinterpret_cast<const words*>(grad + (int64_t)places[i + u] * a.ld);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+      if (u >= left) continue;
       float g[V];
       values_of<T, V>(w[u], g);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] += g[e];
     }
   }
-  for (; i < last; ++i) {
-    float g[V];
-    load_piece<T, V>(grad + (int64_t)places[i] * a.ld, g);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] += g[e];
-  }
 }
 template <int V>
 __device__ __forceinline__ void add_chunks(float (&v)[V], const SumArgs& a, uint32_t first, uint32_t last, int at) {
-  for (uint32_t c = first; c < last; ++c) {
-    const float* from = a.chunks + (int64_t)c * a.d + at;
+  constexpr int kUnroll = 4;
+  for (uint32_t c = first; c < last; c += kUnroll) {
+    float w[kUnroll][V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] += from[e];
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[u][e] = c + u < last ? a.chunks[(int64_t)(c + u) * a.d + at + e] : 0.f;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += w[u][e];
   }
 }
 
-// Chunks of the sorted ids that are of one row: a wave a chunk and slice.
+// Where each row's ids begin among the sorted ones (the last entry: where those outside the table do), by a search a row; and, in
+// the workgroups behind, sums of the chunks that are of one row: a wave a chunk and slice, whose lanes share the chunk where the slice has few pieces.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void chunk_sums_kernel(SumArgs a) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+__global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint32_t* starts, uint32_t search_blocks) {
+  if (blockIdx.x < search_blocks) {
+    const uint32_t r = blockIdx.x * 256 + threadIdx.x;
+    if (r > a.rows) return;
+    uint32_t lo = 0, hi = (uint32_t)a.n;
+    while (lo < hi) {
+      const uint32_t middle = lo + (hi - lo) / 2;
+      if (a.keys[middle] < r) lo = middle + 1;
+      else hi = middle;
+    }
+    starts[r] = lo;
+    return;
+  }
+  __shared__ float room[4][kWave * V];
+  const int64_t item = (int64_t)(blockIdx.x - search_blocks) * 4 + threadIdx.x / kWave;
   const int64_t chunk = item / a.slices;
-  const int slice = (int)(item - chunk * a.slices);
+  const int slice = (int)(item - chunk * a.slices), lane = threadIdx.x & (kWave - 1);
   if (chunk >= a.n / kChunk) return;
   const uint32_t first = (uint32_t)(chunk * kChunk);
   if (a.keys[first] != a.keys[first + kChunk - 1] || a.keys[first] >= a.rows) return;
-  const int p = slice * kWave + (threadIdx.x & (kWave - 1));
-  if (p >= a.pieces) return;
+  const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;
+  int lanes = 1;
+  while (lanes < here) lanes *= 2;
+  const int shares = kWave / lanes, share = lane / lanes, sub = lane & (lanes - 1);
+  const int p = slice * kWave + (sub < here ? sub : here - 1);
   const int at = p * V + V > a.d ? a.d - V : p * V;
   float v[V] = {};
-  add_rows<T, V>(v, a, a.places, first, first + kChunk, at);
+  const uint32_t each = kChunk / shares;
+  add_rows<T, V>(v, a, a.places, first + share * each, first + share * each + each, at);
+  float* mine = room[threadIdx.x / kWave];
+  if (shares > 1) {                            // (within a wave: LDS keeps its order)
+#pragma unroll
+    for (int e = 0; e < V; ++e) mine[e * kWave + lane] = v[e];
+    __builtin_amdgcn_wave_barrier();
+    for (int s = 1; s < shares; ++s)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += share == 0 ? mine[e * kWave + s * lanes + sub] : 0.f;
+  }
+  if (share != 0 || sub >= here) return;
+  // (a piece that was moved back leaves the columns of the one before to that: another slice may add in another order)
   float* to = a.chunks + chunk * a.d + at;
 #pragma unroll
-  for (int e = 0; e < V; ++e) to[e] = v[e];
+  for (int e = 0; e < V; ++e)
+    if (at + e >= p * V) to[e] = v[e];
 }
 
-// Where keys of at least `key` begin in the sorted ones from lo to hi: by the 64 lanes of a wave, 64 parts at a time.
-__device__ __forceinline__ uint32_t begin_of(const uint32_t* keys, uint32_t lo, uint32_t hi, uint32_t key) {
-  const uint32_t lane = threadIdx.x & (kWave - 1);
-  while (lo < hi) {
-    const uint32_t step = (hi - lo + kWave - 1) / kWave;
-    const uint64_t at = (uint64_t)lo + (uint64_t)lane * step;
-    const uint64_t less = __ballot(at < hi && keys[at] < key);
-    const uint32_t count = (uint32_t)__popcll(less);
-    if (count == 0) return lo;
-    const uint64_t next = (uint64_t)lo + (uint64_t)count * step;
-    lo = lo + (count - 1) * step + 1;
-    hi = next < hi ? (uint32_t)next : hi;
+// Rows of a workgroup's range, by how many ids they have: those without any are written as zeros at once, the others are listed
+// (in any order: each is a sum of its own).
+struct RowLists {
+  uint32_t* few;               // few[i]: rows with up to kLong ids from the front, those with more from the back
+  uint32_t* counts;            // of both
+};
+template <typename T, int V, int THREADS>
+__device__ __forceinline__ void list_rows(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start, const RowLists& lists) {
+  for (uint32_t r = threadIdx.x; r < count; r += THREADS) {
+    const uint32_t ids = start[r + 1] - start[r];
+    if (ids > kLong) lists.few[count - 1 - atomicAdd(&lists.counts[1], 1u)] = r;
+    else if (ids > 0) lists.few[atomicAdd(&lists.counts[0], 1u)] = r;
   }
-  return lo;
+  const int first = slice * kWave * V, width = a.d - first < kWave * V ? a.d - first : kWave * V;     // columns of the slice
+  typedef typename piece_words<T, V>::type words;
+  const words zero = {};
+  const int pieces = (width + V - 1) / V;
+  int lanes = 1;
+  while (lanes < pieces) lanes *= 2;
+  const int sub = threadIdx.x & (lanes - 1);
+  const int at = first + (sub * V + V > width ? (width < V ? 0 : width - V) : sub * V);
+  for (uint32_t r = threadIdx.x / lanes; r < count; r += THREADS / lanes)
+    if (start[r + 1] == start[r] && sub < pieces) *reinterpret_cast<words*>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + (at + V > a.d ? a.d - V : at)) = zero;
 }
 
-// A workgroup's range of rows and slice of columns, the places of whose ids lie in order in places[start[r] .. start[r + 1]).
+// Their sums: the places of row r's ids lie in order in places[start[r] .. start[r + 1]).  `room` holds a piece a lane.
 template <typename T, int V, int THREADS, typename Place>
 __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start,
-                                          const Place* places, bool chunked, uint32_t* long_rows, uint32_t* long_count, float* room) {
+                                          const Place* places, bool chunked, const RowLists& lists, float* room) {
   constexpr int kWaves = THREADS / kWave;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;       // pieces of the slice
@@ -325,25 +367,19 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
   const int groups = kWave / lanes, sub = lane & (lanes - 1);
   const int p = slice * kWave + (sub < here ? sub : here - 1);
   const int at = p * V + V > a.d ? a.d - V : p * V;
-  for (uint32_t r = (uint32_t)(wave * groups + lane / lanes); r < count; r += (uint32_t)(kWaves * groups)) {
-    const uint32_t s = start[r], e = start[r + 1];
-    if (e - s > kLong) {
-      if (sub == 0) long_rows[atomicAdd(long_count, 1u)] = r;         // (in any order: each is a sum of its own)
-      continue;
-    }
+  const uint32_t few = lists.counts[0], longs = lists.counts[1];
+  for (uint32_t l = (uint32_t)(wave * groups + lane / lanes); l < few; l += (uint32_t)(kWaves * groups)) {
+    const uint32_t r = lists.few[l];
     float v[V] = {};
-    add_rows<T, V>(v, a, places, s, e, at);
-    if (s != e)
+    add_rows<T, V>(v, a, places, start[r], start[r + 1], at);
 #pragma unroll
-      for (int x = 0; x < V; ++x) v[x] *= a.scale;
+    for (int x = 0; x < V; ++x) v[x] *= a.scale;
     if (sub < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + at, v);
   }
-  __syncthreads();
-  const uint32_t longs = *long_count;
   const int lp = slice * kWave + (lane < here ? lane : here - 1);
   const int lat = lp * V + V > a.d ? a.d - V : lp * V;
   for (uint32_t l = 0; l < longs; ++l) {
-    const uint32_t r = long_rows[l], s = start[r], e = start[r + 1];
+    const uint32_t r = lists.few[count - 1 - l], s = start[r], e = start[r + 1];
     uint32_t c0 = (s + kChunk - 1) / kChunk, c1 = e / kChunk;
     if (!chunked || c0 >= c1) { c0 = 0; c1 = 0; }
     const uint32_t head = c0 < c1 ? c0 * kChunk : e, tail = c0 < c1 ? c1 * kChunk : e;
@@ -352,6 +388,7 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
     add_rows<T, V>(v, a, places, part(s, head, wave), part(s, head, wave + 1), lat);
     if (chunked) add_chunks<V>(v, a, part(c0, c1, wave), part(c0, c1, wave + 1), lat);
     add_rows<T, V>(v, a, places, part(tail, e, wave), part(tail, e, wave + 1), lat);
+    __syncthreads();                           // (the row before is done with the room)
 #pragma unroll
     for (int x = 0; x < V; ++x) room[(wave * V + x) * kWave + lane] = v[x];
     __syncthreads();
@@ -363,37 +400,25 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
       for (int x = 0; x < V; ++x) v[x] *= a.scale;
       if (lane < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + lat, v);
     }
-    __syncthreads();
   }
 }
 
 // From sorted ids.
-constexpr int kRangeSorted = 64;
+constexpr int kRangeSorted = 64, kSumThreads = 256;
 template <typename T, int V>
-__global__ __launch_bounds__(512) void sorted_sums_kernel(SumArgs a) {
-  __shared__ uint32_t start[kRangeSorted + 1], ends[2], long_rows[kRangeSorted], long_count;
-  __shared__ float room[512 * V];
+__global__ __launch_bounds__(kSumThreads) void sorted_sums_kernel(SumArgs a, const uint32_t* starts) {
+  __shared__ uint32_t start[kRangeSorted + 1], few[kRangeSorted], counts[2];
+  __shared__ float room[kSumThreads * V];
   const uint32_t range = blockIdx.x / a.slices, row0 = range * kRangeSorted;
   const int slice = (int)(blockIdx.x - range * a.slices);
   const uint32_t count = a.rows - row0 < kRangeSorted ? a.rows - row0 : kRangeSorted;
-  const int wave = threadIdx.x / kWave;
-  if (threadIdx.x == 0) long_count = 0;
-  if (wave < 2) {
-    const uint32_t at = begin_of(a.keys, 0, (uint32_t)a.n, row0 + (wave ? count : 0));
-    if (threadIdx.x % kWave == 0) ends[wave] = at;
-  }
+  if (threadIdx.x < 2) counts[threadIdx.x] = 0;
+  if (threadIdx.x <= count) start[threadIdx.x] = starts[row0 + threadIdx.x];
   __syncthreads();
-  for (uint32_t r = threadIdx.x; r <= count; r += 512) {
-    uint32_t lo = ends[0], hi = ends[1];
-    while (lo < hi) {
-      const uint32_t middle = lo + (hi - lo) / 2;
-      if (a.keys[middle] < row0 + r) lo = middle + 1;
-      else hi = middle;
-    }
-    start[r] = lo;
-  }
+  const RowLists lists{few, counts};
+  list_rows<T, V, kSumThreads>(a, row0, count, slice, start, lists);
   __syncthreads();
-  sum_range<T, V, 512>(a, row0, count, slice, start, a.places, true, long_rows, &long_count, room);
+  sum_range<T, V, kSumThreads>(a, row0, count, slice, start, a.places, true, lists, room);
 }
 
 // From ids as they come: those of the range are kept in their order, then sorted by row.
@@ -401,26 +426,26 @@ constexpr int kPickMost = 16384, kPickThreads = 1024, kPickWaves = kPickThreads 
 
 // Where things lie in LDS, in bytes, which is as large as the call's ids and range ask for: two workgroups are to fit a CU.
 struct PickRoom {
-  uint32_t sorted, own, start, long_rows, all;
+  uint32_t sorted, own, start, few, all;
   __host__ __device__ PickRoom(uint32_t n, uint32_t range, int values) {
     const uint32_t kept = 4 * n, sums = (uint32_t)(kPickThreads * values * 4);      // (the waves' sums take the place of the kept ids)
     sorted = ((kept > sums ? kept : sums) + 15) / 16 * 16;
     own = sorted + (2 * n + 15) / 16 * 16;
     start = own + kPickWaves * 2 * ((range + 1) / 2 * 2);
-    long_rows = start + 4 * (range + 1);
-    all = long_rows + 4 * range;
+    few = start + 4 * (range + 1);
+    all = few + 4 * range;
   }
 };
 
 template <typename T, int V, typename Idx>
 __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ uint32_t room_words[kPickWaves], long_count;
+  __shared__ uint32_t room_words[kPickWaves], list_counts[2];
   const PickRoom at_lds((uint32_t)a.n, a.range, V);
   uint32_t* kept = reinterpret_cast<uint32_t*>(lds);                         // place | row in the range << 14, in the places' order
   uint16_t* sorted = reinterpret_cast<uint16_t*>(lds + at_lds.sorted);       // places by row
   uint32_t* start = reinterpret_cast<uint32_t*>(lds + at_lds.start);
-  uint32_t* long_rows = reinterpret_cast<uint32_t*>(lds + at_lds.long_rows);
+  const RowLists lists{reinterpret_cast<uint32_t*>(lds + at_lds.few), list_counts};
   const uint32_t part = blockIdx.x / a.slices, row0 = part * a.range;
   const int slice = (int)(blockIdx.x - part * a.slices);
   const uint32_t count = a.rows - row0 < a.range ? a.rows - row0 : a.range;
@@ -429,7 +454,7 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   uint16_t* all_own = reinterpret_cast<uint16_t*>(lds + at_lds.own);         // [waves][each]
   uint16_t* own = all_own + wave * each;
   const Idx* index = static_cast<const Idx*>(a.index);
-  if (threadIdx.x == 0) long_count = 0;
+  if (threadIdx.x < 2) list_counts[threadIdx.x] = 0;
   for (uint32_t r = threadIdx.x; r <= count; r += kPickThreads) start[r] = 0;
   for (uint32_t r = lane; r < each; r += kWave) own[r] = 0;
   // a wave reads a run of the ids: how many of them it keeps, then where
@@ -475,6 +500,7 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   }
   prefix_in_lds<kPickThreads>(start, count + 1, room_words);
   __syncthreads();
+  list_rows<T, V, kPickThreads>(a, row0, count, slice, start, lists);
   for (uint32_t r = threadIdx.x; r < count; r += kPickThreads) {
     uint32_t before = 0;
     for (int w = 0; w < kPickWaves; ++w) {
@@ -496,7 +522,7 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, false, long_rows, &long_count, reinterpret_cast<float*>(lds));
+  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, false, lists, reinterpret_cast<float*>(lds));
 }
 
 // Digits of the sort: as few as keys of rows + 1 values need, of one width.
@@ -507,12 +533,13 @@ void digits_of(int64_t rows, int& passes, int& bits) {
 }
 
 struct Room {
-  int64_t sorted, counts, chunks;            // bytes: keys and places twice, counts of the digits, sums of chunks
+  int64_t sorted, counts, starts, chunks;    // bytes: keys and places twice, counts of the digits, the rows' starts, sums of chunks
   explicit Room(int64_t n, int64_t rows, int64_t d) {
     int passes, bits;
     digits_of(rows, passes, bits);
     sorted = ceil_div(n, 4) * 16 * 4;
     counts = ceil_div((1ll << bits) * (ceil_div(n, kSortTile) + 1), 4) * 16;
+    starts = ceil_div(rows + 1, 4) * 16;
     chunks = n / kChunk * d * 4;
   }
 };
@@ -564,7 +591,7 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   digits_of(a.rows, passes, bits);
   const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div(a.rows, kRangeSorted) * a.slices;
   const int64_t chunk_blocks = ceil_div(a.n / kChunk * a.slices, 4);
-  F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 24), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
+  F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
   uint32_t* words = reinterpret_cast<uint32_t*>(workspace);
   const int64_t each = ceil_div(a.n, 4) * 4;
   SortArgs s{a.index, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<uint32_t*>(workspace + room.sorted), a.n, a.rows, (uint32_t)blocks, 0, bits};
@@ -591,9 +618,11 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   }
   a.keys = s.keys_out;
   a.places = s.places_out;
-  a.chunks = reinterpret_cast<float*>(workspace + room.sorted + room.counts);
-  chunk_sums_kernel<T, V><<<dim3((unsigned)chunk_blocks), dim3(256), 0, st>>>(a);
-  sorted_sums_kernel<T, V><<<dim3((unsigned)sums), dim3(512), 0, st>>>(a);
+  uint32_t* starts = reinterpret_cast<uint32_t*>(workspace + room.sorted + room.counts);
+  a.chunks = reinterpret_cast<float*>(workspace + room.sorted + room.counts + room.starts);
+  const int64_t search_blocks = ceil_div((int64_t)a.rows + 1, 256);
+  starts_and_chunks_kernel<T, V><<<dim3((unsigned)(search_blocks + chunk_blocks)), dim3(256), 0, st>>>(a, starts, (uint32_t)search_blocks);
+  sorted_sums_kernel<T, V><<<dim3((unsigned)sums), dim3(kSumThreads), 0, st>>>(a, starts);
   return launch_status(what);
 }
 
@@ -623,7 +652,7 @@ extern "C" int f2cgt_embedding(const void* table, int dtype, int64_t ld, const v
 extern "C" int64_t f2cgt_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t d) {
   if (n <= kPickMost || rows <= 0 || d <= 0 || n >= (1ll << 31) || rows >= (1ll << 31)) return 0;
   const Room room(n, rows, d);
-  return room.sorted + room.counts + room.chunks;
+  return room.sorted + room.counts + room.starts + room.chunks;
 }
 
 extern "C" int f2cgt_embedding_grad(const void* grad, int dtype, int64_t ld, const void* index, int idx_dtype, void* dtable,

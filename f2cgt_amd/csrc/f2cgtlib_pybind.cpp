@@ -1642,6 +1642,7 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> packed_linear_grad(const
   undifferentiated("packed_linear_grad", {grad_in});
   TORCH_CHECK(grad.device() == kept.codes.device(), "grad is on ", grad.device(), ", the codes on ", kept.codes.device());
   TORCH_CHECK(lead_of(grad_in.sizes()) == lead_of(codes.sizes()), "grad and codes must be of the same rows");
+  if (row_step(grad) >= 1 << 24) grad = grad.contiguous();
   c10::DeviceGuard guard(grad.device());
   const int64_t m = grad.size(0), n = grad.size(1), k = kept.codes.size(1);
   auto dw = torch::empty({n, k}, grad.options().dtype(dtype));

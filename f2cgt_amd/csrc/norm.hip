@@ -218,6 +218,56 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(NormArgs a) {
   }
 }
 
+// What a lane holds of a row of the backward pass, as memory has it.
+template <typename T, int V, int C, bool PACKED>
+struct GradRow {
+  typedef typename piece_words<T, V>::type words;
+  words g[C], x[PACKED ? 1 : C];
+  uint32_t codes[PACKED ? C : 1][(V + 3) / 4], first[PACKED ? C : 1], last[PACKED ? C : 1];
+  float mean, rstd;
+
+  template <int LANES>
+  __device__ __forceinline__ void load(const NormGradArgs& a, const Columns<V, LANES, C>& col, int64_t row) {
+    const T* grad = static_cast<const T*>(a.grad) + row * a.grad_ld;
+#pragma unroll
+    for (int c = 0; c < C; ++c) g[c] = *reinterpret_cast<const words*>(grad + col.at[c]);
+    if constexpr (PACKED) {
+      const int8_t* from = a.codes + row * a.code_stride;
+      const uint8_t* exponents = a.exponents + row * ((a.d + kCheckpointGroup - 1) / kCheckpointGroup);
+      typedef uint32_t word_any __attribute__((aligned(1)));
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if constexpr (V == 1) {
+          codes[c][0] = (uint8_t)from[col.at[c]];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) codes[c][i] = reinterpret_cast<const word_any*>(from + col.at[c])[i];
+        }
+        // (a piece that was moved back may lie in two groups)
+        first[c] = exponents[col.at[c] / kCheckpointGroup];
+        last[c] = exponents[(col.at[c] + V - 1) / kCheckpointGroup];
+      }
+    } else {
+      const T* from = static_cast<const T*>(a.x) + row * a.ld;
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = *reinterpret_cast<const words*>(from + col.at[c]);
+    }
+    mean = a.mean[row];
+    rstd = a.rstd[row];
+  }
+  __device__ __forceinline__ void values(int c, int at, float (&v)[V]) const {
+    if constexpr (PACKED) {
+      const int border = (at + V - 1) / kCheckpointGroup * kCheckpointGroup - at;
+      const float step0 = step_of(first[c]), step1 = step_of(last[c]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = coded_value(codes[c][e / 4], e % 4, e < border ? step0 : step1);
+    } else {
+      values_of<T, V>(x[c], v);
+    }
+  }
+};
+
+// A row's loads are issued a row ahead: what a workgroup has under way covers the latency of the sums over its lanes.
 template <typename T, int V, int LANES, int C, bool PACKED>
 __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGradArgs a) {
   constexpr int kBlock = block_of(LANES), kRows = kBlock / LANES, kWaves = LANES > kWave ? LANES / kWave : 1;
@@ -226,57 +276,40 @@ __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGr
   __shared__ float room[2][2 * kWaves];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const Columns<V, LANES, C> col(lane, a.d);
+  constexpr bool kAhead = LANES < 1024 || C * V <= 8;                 // (128 registers hold no second row of sixteen values a lane)
   float w[C][V], dw[C][V], db[C][V];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
+  for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       w[c][e] = 1.f;
       dw[c][e] = db[c][e] = 0.f;
     }
+#pragma unroll
+  for (int c = 0; c < C; ++c)
     if (a.weight != nullptr) load_weight<T, V>(a.weight, a.wide_weight, col.at[c], w[c]);
-  }
   const float d = (float)a.d;
+  const int64_t stride = (int64_t)gridDim.x * kRows, first_row = (int64_t)blockIdx.x * kRows + group;
+  auto held = [&](int64_t row) { return row < a.m ? row : a.m - 1; };          // (lanes without a row repeat the last one and write nothing)
+  GradRow<T, V, C, PACKED> now, next;
+  if (kAhead) next.load(a, col, held(first_row));
   int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.m; base += (int64_t)gridDim.x * kRows, turn ^= 1) {
-    const bool live = base + group < a.m;
-    const int64_t row = live ? base + group : a.m - 1;
-    const T* grad = static_cast<const T*>(a.grad) + row * a.grad_ld;
-    float g[C][V], n[C][V];
-#pragma unroll
-    for (int c = 0; c < C; ++c) load_piece<T, V>(grad + col.at[c], g[c]);
-    if constexpr (PACKED) {
-      const int8_t* codes = a.codes + row * a.code_stride;
-      const uint8_t* exponents = a.exponents + row * ((a.d + kCheckpointGroup - 1) / kCheckpointGroup);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        // (a piece that was moved back may lie in two groups)
-        const int first = col.at[c] / kCheckpointGroup, last = (col.at[c] + V - 1) / kCheckpointGroup;
-        const int border = last * kCheckpointGroup - col.at[c];
-        const float step0 = step_of(exponents[first]), step1 = step_of(exponents[last]);
-        uint32_t words[(V + 3) / 4];
-        if constexpr (V == 1) {
-          words[0] = (uint8_t)codes[col.at[c]];
-        } else {
-          typedef uint32_t word_any __attribute__((aligned(1)));
-#pragma unroll
-          for (int i = 0; i < V / 4; ++i) words[i] = reinterpret_cast<const word_any*>(codes + col.at[c])[i];
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) n[c][e] = coded_value(words[e / 4], e % 4, e < border ? step0 : step1);
-      }
+  for (int64_t row = first_row; row - group < a.m; row += stride, turn ^= 1) {
+    const bool live = row < a.m;
+    if constexpr (kAhead) {
+      now = next;
+      next.load(a, col, held(row + stride));
     } else {
-      const T* x = static_cast<const T*>(a.x) + row * a.ld;
-#pragma unroll
-      for (int c = 0; c < C; ++c) load_piece<T, V>(x + col.at[c], n[c]);
+      now.load(a, col, held(row));
     }
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float s[2] = {0.f, 0.f};
+    float s[2] = {0.f, 0.f}, g[C][V], n[C][V];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      values_of<T, V>(now.g[c], g[c]);
+      now.values(c, col.at[c], n[c]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        n[c][e] = (n[c][e] - mean) * rstd;
+        n[c][e] = (n[c][e] - now.mean) * now.rstd;
         const bool own = e >= col.skip[c];
         const float u = own ? g[c][e] * w[c][e] : 0.f;
         s[0] += u;
@@ -284,6 +317,7 @@ __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGr
         dw[c][e] += live ? g[c][e] * n[c][e] : 0.f;
         db[c][e] += live ? g[c][e] : 0.f;
       }
+    }
     sum_group<LANES>(s, room[turn]);
     const float first = s[0] / d, second = s[1] / d;
     T* dx = static_cast<T*>(a.dx) + row * a.d;
@@ -291,7 +325,7 @@ __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGr
     for (int c = 0; c < C; ++c) {
       float y[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = rstd * (g[c][e] * w[c][e] - first - n[c][e] * second);
+      for (int e = 0; e < V; ++e) y[e] = now.rstd * (g[c][e] * w[c][e] - first - n[c][e] * second);
       if (live && col.on[c]) store_piece<T, V>(dx + col.at[c], y);
     }
   }
@@ -307,16 +341,16 @@ __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGr
         sums[(e * 2 + 1) * kBlock + threadIdx.x] = db[c][e];
       }
       __syncthreads();
-      if (group == 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          for (int r = 1; r < kRows; ++r) {
-            dw[c][e] += sums[(e * 2) * kBlock + r * LANES + lane];
-            db[c][e] += sums[(e * 2 + 1) * kBlock + r * LANES + lane];
-          }
+      for (int o = threadIdx.x; o < LANES * 2 * V; o += kBlock) {
+        const int l = o % LANES, e = o / LANES / 2, which = o / LANES % 2, start = (l + c * LANES) * V;
+        const int at = start + V > a.d ? a.d - V : start;
+        if (start >= a.d || e < start - at) continue;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < kRows; ++r) sum += sums[(e * 2 + which) * kBlock + r * LANES + l];
+        parts[which * a.d + at + e] = sum;
       }
-    }
-    if (group == 0 && col.on[c]) {
+    } else if (col.on[c]) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (e >= col.skip[c]) {
@@ -431,6 +465,7 @@ bool with_geometry(int64_t d, const F& f) {
   else if (pieces <= 32) f(count_of<V>{}, count_of<32>{}, count_of<1>{});
   else if (pieces <= 64) f(count_of<V>{}, count_of<64>{}, count_of<1>{});
   else if (pieces <= 128) f(count_of<V>{}, count_of<64>{}, count_of<2>{});
+  else if (V == 4 && pieces <= 192) f(count_of<V>{}, count_of<64>{}, count_of<3>{});
   else if (pieces <= 256) f(count_of<V>{}, count_of<256>{}, count_of<1>{});
   else if (pieces <= 512) f(count_of<V>{}, count_of<512>{}, count_of<1>{});
   else if (pieces <= 1024) f(count_of<V>{}, count_of<1024>{}, count_of<1>{});
