@@ -10,6 +10,8 @@
 #include "rows.hpp"
 #include "tile_product.hpp"
 
+#include <type_traits>
+
 namespace f2cgt {
 namespace {
 
@@ -202,6 +204,8 @@ template <typename T> struct Eight {
   }
 };
 
+typedef uint32_t word_any __attribute__((aligned(1)));
+
 // A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step; GROUPS groups of waves take the steps in turn and
 // add their sums in the end.  Rows lie in LDS as they do in memory, one line of BN or BK bf16 a row, and matrix operands, which hold
 // eight rows of one column a lane, are read through the transposing LDS loads: sixteen lanes give the addresses of 4 rows x 16
@@ -229,7 +233,7 @@ struct GradTile {
   struct Held {
     Eight<T> g[kPiecesG];
     uint2 x[kPiecesX];
-    uint32_t e[kPiecesX];
+    uint32_t e[kPiecesX];      // exponents, each the lowest byte of four
   };
 };
 
@@ -237,8 +241,8 @@ template <typename T, int BN, int BK, int WN, int WK, int BM, int GROUPS>
 __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed_linear_grad_kernel(GradArgs a) {
   typedef GradTile<T, BN, BK, WN, WK, BM, GROUPS> Tile;
   constexpr int P = Tile::P, TI = Tile::TI, TJ = Tile::TJ, kThreads = Tile::kThreads;
-  constexpr int kAcross = (BN * BK * 4) * (GROUPS - 1);                 // the groups' sums on their way to the first one
-  constexpr int kLds = 2 * Tile::kStage * GROUPS > kAcross ? 2 * Tile::kStage * GROUPS : kAcross;
+  constexpr int kLd = WK + 1, kStrips = 32 * kLd * 4 * (kThreads / kWave) * GROUPS;      // a strip of sums for each wave on its way out
+  constexpr int kStages = 2 * Tile::kStage * GROUPS, kLds = kStages > kStrips ? kStages : kStrips;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
   const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads) : 0;
   const int t = threadIdx.x - group * kThreads, lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
@@ -250,7 +254,9 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   uint32_t ti, tj;
   tile_of(place - split * tiles, a.tiles_n, a.tiles_k, 4, ti, tj);
   const int col_n = (int)ti * BN, col_k = (int)tj * BK;
-  const int64_t from = a.steps * split / a.splits, to = a.steps * (split + 1) / a.splits;
+  // (whole rounds to every split but the last)
+  const int64_t shares = (a.steps + GROUPS - 1) / GROUPS, from = shares * split / a.splits * GROUPS;
+  const int64_t ahead = shares * (split + 1) / a.splits * GROUPS, to = ahead < a.steps ? ahead : a.steps;
 
   // this thread's columns: those beyond the operand's end repeat its first ones (what they give is not kept)
   const int pg = t % (BN / 8) * 8, px = t % (BK / 8) * 8, rg = t / (BN / 8), rx = t / (BK / 8);
@@ -260,73 +266,83 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   const uint32_t off_e = (uint32_t)(rx * a.groups + cx / kCheckpointGroup);
   typedef typename Tile::Held Held;
 
-  // A piece that runs over its row's end reads on in the next one; the last rows, which have none, are read value by value.  Steps behind
-  // the last one read it again.
-  const bool pieces = a.n >= 8 && a.k > 0;
-  auto load = [&](Held& h, int64_t step) {
-    const int64_t row0 = (step < to ? step : to - 1) * BM;
+  // A piece that runs over its row's end reads on in the next one, and four exponents at a time, of which the first counts, in the next ones: the
+  // steps of the last four rows are not among these.  (Of a single exponent's byte the compiler makes a word where the loop ends, behind a wait.)
+  const int64_t whole = a.n >= 8 && a.m > 4 ? (a.m - 4) / BM : 0;
+  const int64_t rounds = (whole < to ? (whole > from ? whole - from : 0) : to - from) / GROUPS, end = from + rounds * GROUPS;
+  // Pieces of one of kParts parts of a step into registers.
+  auto load_part = [&](Held& h, int64_t step, int part) {
+    const int64_t row0 = step * BM;
     const char* grad = static_cast<const char*>(a.grad) + row0 * a.ld * (int64_t)sizeof(T);
     const int8_t* codes = a.codes + row0 * a.code_stride;
     const uint8_t* exponents = a.exponents + row0 * a.groups;
-    if (row0 + BM < a.m && pieces) {
+    uint32_t og = off_g, ox = off_x, oe = off_e;
+    asm("" : "+v"(og), "+v"(ox), "+v"(oe));       // (32 bits beside a scalar base, which the compiler would widen ahead of the loop)
 #pragma unroll
-      for (int i = 0; i < Tile::kPiecesG; ++i) h.g[i].load(grad + (int64_t)i * Tile::kRowsG * a.ld * (int64_t)sizeof(T) + off_g);
+    for (int i = 0; i < Tile::kPiecesG; ++i)
+      if (i % Tile::kParts == part) h.g[i].load(grad + (int64_t)i * Tile::kRowsG * a.ld * (int64_t)sizeof(T) + og);
 #pragma unroll
-      for (int i = 0; i < Tile::kPiecesX; ++i) {
-        h.x[i] = *reinterpret_cast<const uint2*>(codes + i * Tile::kRowsX * a.code_stride + off_x);
-        h.e[i] = exponents[(int64_t)i * Tile::kRowsX * a.groups + off_e];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < Tile::kPiecesG; ++i) {
-        const bool in = row0 + rg + i * Tile::kRowsG < a.m;
-        const T* p = reinterpret_cast<const T*>(grad + (int64_t)i * Tile::kRowsG * a.ld * (int64_t)sizeof(T) + off_g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          T v = (T)0.f;
-          if (in && cg + e < a.n) v = p[e];
-          h.g[i].set(e, v);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < Tile::kPiecesX; ++i) {
-        h.x[i] = uint2{0, 0};
-        h.e[i] = 127;
-        if (row0 + rx + i * Tile::kRowsX < a.m && a.k > 0) {
-          h.x[i] = *reinterpret_cast<const uint2*>(codes + i * Tile::kRowsX * a.code_stride + off_x);
-          h.e[i] = exponents[(int64_t)i * Tile::kRowsX * a.groups + off_e];
-        }
-      }
+    for (int i = 0; i < Tile::kPiecesX; ++i) {
+      if (i % Tile::kParts != part) continue;
+      h.x[i] = *reinterpret_cast<const uint2*>(codes + i * Tile::kRowsX * a.code_stride + ox);
+      h.e[i] = *reinterpret_cast<const word_any*>(exponents + (int64_t)i * Tile::kRowsX * a.groups + oe);
     }
   };
   const bool sums = a.bias != nullptr && tj == 0;
   float db[8] = {};
-  // Pieces of one of kParts parts into a stage.
-  auto place_part = [&](const Held& h, char* stage, int part, bool count) {
+  auto place_g = [&](auto with_sums, const Eight<T>& g, char* stage, int row, bool count) {
+    if constexpr (decltype(with_sums)::value)
 #pragma unroll
-    for (int i = 0; i < Tile::kPiecesG; ++i) {
-      if (i % Tile::kParts != part) continue;
-      if (sums && count)
+      for (int e = 0; e < 8; ++e) db[e] += count ? g[e] : 0.f;
+    intx4 planes[P];
+    g.planes(planes);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) db[e] += h.g[i][e];
-      intx4 planes[P];
-      h.g[i].planes(planes);
+    for (int p = 0; p < P; ++p)
+      *reinterpret_cast<intx4*>(stage + p * Tile::kPlaneG + Tile::line_at(row, pg * 2, Tile::kLineG)) = planes[p];
+  };
+  auto place_x = [&](const uint2& x, uint32_t exponent, char* stage, int row) {
+    const float step = __uint_as_float(exponent << 24 >> 1);
+    intx4 v;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-        *reinterpret_cast<intx4*>(stage + p * Tile::kPlaneG + Tile::line_at(rg + i * Tile::kRowsG, pg * 2, Tile::kLineG)) = planes[p];
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t word = e < 2 ? x.x : x.y;
+      v[e] = (int)__builtin_amdgcn_perm(__float_as_uint(coded_value(word, 2 * (e % 2) + 1, step)),
+                                        __float_as_uint(coded_value(word, 2 * (e % 2), step)), 0x07060302);
     }
+    *reinterpret_cast<intx4*>(stage + P * Tile::kPlaneG + Tile::line_at(row, px * 2, Tile::kLineX)) = v;
+  };
+  // What load_part loaded into a stage.
+  auto place_part = [&](auto with_sums, const Held& h, char* stage, int part, bool count) {
 #pragma unroll
+    for (int i = 0; i < Tile::kPiecesG; ++i)
+      if (i % Tile::kParts == part) place_g(with_sums, h.g[i], stage, rg + i * Tile::kRowsG, count);
+#pragma unroll
+    for (int i = 0; i < Tile::kPiecesX; ++i)
+      if (i % Tile::kParts == part) place_x(h.x[i], h.e[i], stage, rx + i * Tile::kRowsX);
+  };
+  // The matrix's last rows, value by value, at places that exist, into a stage; what is not theirs is made zero.
+  auto place_last = [&](auto with_sums, int64_t step, char* stage) {
+    const int64_t row0 = step * BM;
+    constexpr int kAtOnce = BN > 128 ? 1 : 4;      // (large tiles have no registers for more)
+#pragma unroll kAtOnce
     for (int i = 0; i < Tile::kPiecesX; ++i) {
-      if (i % Tile::kParts != part) continue;
-      const float step = step_of(h.e[i]);
-      intx4 v;
+      const int64_t row = row0 + rx + i * Tile::kRowsX, held_row = row < a.m ? row : a.m - 1;
+      uint2 x = *reinterpret_cast<const uint2*>(a.codes + held_row * a.code_stride + cx);
+      const uint32_t exponent = a.exponents[held_row * a.groups + cx / kCheckpointGroup];
+      if (row >= a.m) x = uint2{0, 0};
+      place_x(x, row < a.m ? exponent : 127, stage, rx + i * Tile::kRowsX);
+    }
+#pragma unroll kAtOnce
+    for (int i = 0; i < Tile::kPiecesG; ++i) {
+      const int64_t row = row0 + rg + i * Tile::kRowsG;
+      const T* p = static_cast<const T*>(a.grad) + (row < a.m ? row : a.m - 1) * a.ld;
+      T v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t word = e < 2 ? h.x[i].x : h.x[i].y;
-        v[e] = (int)__builtin_amdgcn_perm(__float_as_uint(coded_value(word, 2 * (e % 2) + 1, step)),
-                                          __float_as_uint(coded_value(word, 2 * (e % 2), step)), 0x07060302);
-      }
-      *reinterpret_cast<intx4*>(stage + P * Tile::kPlaneG + Tile::line_at(rx + i * Tile::kRowsX, px * 2, Tile::kLineX)) = v;
+      for (int e = 0; e < 8; ++e) v[e] = p[cg + e < a.n ? cg + e : a.n - 1];
+      Eight<T> g;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g.set(e, row < a.m && cg + e < a.n ? v[e] : (T)0.f);
+      place_g(with_sums, g, stage, rg + i * Tile::kRowsG, true);
     }
   };
 
@@ -348,91 +364,104 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
     const shortx8 both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bfx8, both);
   };
-  auto multiply_part = [&](const char* stage, int s) {
-    bfx8 fx[TJ];
+  // Operands of a part of a stage; those of the next part are read while one is multiplied.
+  bfx8 fx[2][TJ], fg[2][P][TI];
+  auto read_part = [&](const char* stage, int s) {
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) fx[j] = operand(stage + P * Tile::kPlaneG, s, wj + 32 * j, Tile::kLineX);
+    for (int j = 0; j < TJ; ++j) fx[s & 1][j] = operand(stage + P * Tile::kPlaneG, s, wj + 32 * j, Tile::kLineX);
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p) {
-      bfx8 fg[TI];
+    for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-      for (int i = 0; i < TI; ++i) fg[i] = operand(stage + p * Tile::kPlaneG, s, wi + 32 * i, Tile::kLineG);
+      for (int i = 0; i < TI; ++i) fg[s & 1][p][i] = operand(stage + p * Tile::kPlaneG, s, wi + 32 * i, Tile::kLineG);
+  };
+  auto multiply_part = [&](int s) {
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p)
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[i], fx[j], acc[i][j], 0, 0, 0);
-    }
+        for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[s & 1][p][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
   };
-  // Two steps of each group are on their way from memory while one is multiplied: a round trip is longer than a step.
-  // Step s is multiplied out of stage s % 2 while the next one is placed in the other; then the registers of that take the step after the next two.
-  const int64_t rounds = (to - from + GROUPS - 1) / GROUPS;
-  Held held[2];
-  load(held[0], from + group);
-  load(held[1], from + group + GROUPS);
+  // A group's step s is multiplied out of stage s % 2 while its next one goes from registers into the other stage, a part at a time, and the
+  // registers of each part take the step after that: its loads have a whole round for their way.  (One copy of the round, and no branch in
+  // it: what a short call waits for is the kernel's code, and where paths meet the compiler would wait for every load.)
+  auto go = [&](auto with_sums) {
+    auto held_step = [&](int64_t step) { return step < end ? step : from; };       // (behind the last one: the first one again)
+    if (rounds > 0) {
+      Held h;
 #pragma unroll
-  for (int part = 0; part < Tile::kParts; ++part) place_part(held[0], stages, part, from + group < to);
-  load(held[0], from + group + 2 * GROUPS);
-  __syncthreads();
-  for (int64_t r = 0; r < rounds; r += 2) {
+      for (int part = 0; part < Tile::kParts; ++part) load_part(h, from + group, part);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (r + u < rounds) {
-        const int64_t step = from + group + (r + u) * GROUPS;
-        char* now = stages + u * Tile::kStage;
-        char* next = stages + (u ^ 1) * Tile::kStage;
-        Held& h = held[u ^ 1];
+      for (int part = 0; part < Tile::kParts; ++part) {
+        place_part(with_sums, h, stages, part, true);
+        load_part(h, held_step(from + group + GROUPS), part);
+      }
+      __syncthreads();
+      int turn = 0;
+      for (int64_t step = from + group; step < end; step += GROUPS, turn ^= 1) {
+        const char* now = stages + turn * Tile::kStage;
+        char* next = stages + (turn ^ 1) * Tile::kStage;
+        const int64_t after = held_step(step + 2 * GROUPS);
+        read_part(now, 0);
 #pragma unroll
         for (int part = 0; part < Tile::kParts; ++part) {
-          if (GROUPS == 1 || step < to) multiply_part(now, part);
-          place_part(h, next, part, step + GROUPS < to);
+          if (part + 1 < Tile::kParts) read_part(now, part + 1);
+          multiply_part(part);
+          place_part(with_sums, h, next, part, step + GROUPS < end);
+          load_part(h, after, part);
         }
-        load(h, step + 3 * GROUPS);
         __syncthreads();
       }
     }
-  }
-  if constexpr (GROUPS > 1) {
-    // the other groups' sums, in their order
-    float* across = reinterpret_cast<float*>(lds);
-    if (group > 0) {
-      float* to_first = across + (group - 1) * BN * BK;
+    for (int64_t at = end; at < to; at += GROUPS) {          // what is left of the steps, a few at most
+      const int64_t step = at + group;
+      if (step < to) place_last(with_sums, step, stages);
+      __syncthreads();
+      if (step < to)
 #pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) to_first[((i * TJ + j) * 16 + v) * kThreads + t] = acc[i][j][v];
-    }
-    __syncthreads();
-    if (group == 0) {
-#pragma unroll
-      for (int g = 0; g < GROUPS - 1; ++g)
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int j = 0; j < TJ; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] += across[g * BN * BK + ((i * TJ + j) * 16 + v) * kThreads + t];
-    }
-  }
-  // Sums out: a lane holds, of column lane % 32, rows 4 (lane / 32) to + 3 after every eight.
-  if (group == 0) {
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-      for (int j = 0; j < TJ; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int row = col_n + wi + 32 * i + 8 * (v / 4) + 4 * (lane >> 5) + v % 4, column = col_k + wj + 32 * j + (lane & 31);
-          if (row < a.n && column < a.k) {
-            const int64_t at = (int64_t)row * a.k + column;
-            if (a.parts != nullptr) a.parts[(int64_t)split * a.n * a.k + at] = acc[i][j][v];
-            else store_value(a.out, a.out_tag, at, acc[i][j][v]);
-          }
+        for (int part = 0; part < Tile::kParts; ++part) {
+          read_part(stages, part);
+          multiply_part(part);
         }
+      __syncthreads();
+    }
+  };
+  if (sums) go(std::true_type{});
+  else go(std::false_type{});
+
+  // Sums out, 32 rows of each wave's tile at a time by way of LDS, where the groups' sums are added in their order; a row of WK columns to a
+  // store.  (A lane holds, of column lane % 32, rows 4 (lane / 32) to + 3 after every eight.)
+  constexpr int kWaves = kThreads / kWave, kStrip = 32 * kLd;
+  float* strips = reinterpret_cast<float*>(lds);
+  float* strip = strips + (group * kWaves + wave) * kStrip;
+#pragma unroll
+  for (int i = 0; i < TI; ++i) {
+    if (GROUPS > 1 && i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) strip[(8 * (v / 4) + 4 * (lane >> 5) + v % 4) * kLd + 32 * j + (lane & 31)] = acc[i][j][v];
+    if (GROUPS > 1) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+    // (each group stores a share of the strip's rows)
+    const int row0 = col_n + wi + 32 * i, column0 = col_k + wj;
+    const int rows = a.n - row0 < 32 ? a.n - row0 : 32;
+    constexpr int kWide = WK < kWave ? WK : kWave, kAtOnce = kWave / kWide;       // columns and rows to a pass of the lanes
+    for (int r = group * kAtOnce + lane / kWide; r < rows; r += GROUPS * kAtOnce)
+#pragma unroll
+      for (int c = lane % kWide; c < WK; c += kWide)
+        if (column0 + c < a.k) {
+          float sum = strips[wave * kStrip + r * kLd + c];
+#pragma unroll
+          for (int o = 1; o < GROUPS; ++o) sum += strips[(o * kWaves + wave) * kStrip + r * kLd + c];
+          const int64_t at = (int64_t)(row0 + r) * a.k + column0 + c;
+          if (a.parts != nullptr) a.parts[(int64_t)split * a.n * a.k + at] = sum;
+          else store_value(a.out, a.out_tag, at, sum);
+        }
+    if (GROUPS == 1) __builtin_amdgcn_wave_barrier();
   }
   if (!sums) return;
-  if constexpr (GROUPS > 1) __syncthreads();
+  __syncthreads();
   constexpr int kRows = Tile::kRowsG * GROUPS;
   static_assert(kRows * BN * 4 <= kLds, "the bias' sums fit");
   float* room = reinterpret_cast<float*>(lds);
@@ -447,47 +476,73 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   }
 }
 
-// Sums over the splits: a workgroup has 256 outputs, each of its waves every fourth split, then the waves' sums in order; the bias' in
-// workgroups behind the weight's.  (No splits: zeros, of no rows.)
+// Sums of a gradient's columns alone, of a layer without inputs.
+struct ColumnArgs {
+  const void* grad;
+  void* bias;
+  int64_t m, ld;
+  int n, out_tag;
+};
+template <typename T>
+__global__ __launch_bounds__(64) void column_sums_kernel(ColumnArgs a) {
+  const int column = blockIdx.x * 64 + threadIdx.x;
+  if (column >= a.n) return;
+  const T* from = static_cast<const T*>(a.grad) + column;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int64_t row = 0; row < a.m; ++row) sum += (float)from[row * a.ld];
+  store_value(a.bias, a.out_tag, column, sum);
+}
+
+// Sums over the splits: a workgroup has 64 E outputs, each of its sixteen waves every sixteenth split, then the waves' sums in order; the
+// bias' in workgroups behind the weight's.  (No splits: zeros, of no rows.)
 struct JoinArgs {
   const float* parts;
   void* out;
   void* bias;
   int64_t count;             // n k
-  int n, tag, whole;         // whole: four values at a time
+  int n, tag;
   uint32_t splits, blocks;   // blocks: those of the weight
 };
-__global__ __launch_bounds__(256) void join_splits_kernel(JoinArgs a) {
-  __shared__ __attribute__((aligned(16))) float room[4][256];
+constexpr int kJoinWaves = 16;
+template <int E>
+__global__ __launch_bounds__(kJoinWaves * kWave) void join_splits_kernel(JoinArgs a) {
+  constexpr int kOuts = 64 * E;
+  __shared__ float room[kJoinWaves][kOuts];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const bool weight = blockIdx.x < a.blocks;
-  const int64_t count = weight ? a.count : a.n, first = (int64_t)(weight ? blockIdx.x : blockIdx.x - a.blocks) * 256;
-  const float* parts = weight ? a.parts : a.parts + (int64_t)a.splits * a.count;
+  const int64_t count = weight ? a.count : a.n, first = (int64_t)(weight ? blockIdx.x : blockIdx.x - a.blocks) * kOuts;
+  const float* parts = (weight ? a.parts : a.parts + (int64_t)a.splits * a.count) + first;
   void* out = weight ? a.out : a.bias;
-  const int64_t at = first + 4 * lane;
-  fltx4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (weight && a.whole) {
-    if (at < count) {
-      uint32_t s = wave;
-      for (; s + 12 < a.splits; s += 16) {
-        fltx4 v[4];
+  const int64_t left = count - first;
+  constexpr int kAtOnce = 16 / E;
+  float sum[E] = {};
+  for (uint32_t s = wave; s < a.splits; s += kAtOnce * kJoinWaves) {
+    float v[kAtOnce][E];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const fltx4*>(parts + (int64_t)(s + 4 * u) * count + at);
+    for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sum += v[u];
+      for (int e = 0; e < E; ++e) {
+        v[u][e] = 0.f;
+        if (s + u * kJoinWaves < a.splits && lane + 64 * e < left) v[u][e] = parts[(int64_t)(s + u * kJoinWaves) * count + lane + 64 * e];
       }
-      for (; s < a.splits; s += 4) sum += *reinterpret_cast<const fltx4*>(parts + (int64_t)s * count + at);
-    }
-  } else {
-    for (uint32_t s = wave; s < a.splits; s += 4)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += at + e < count ? parts[(int64_t)s * count + at + e] : 0.f;
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] += v[u][e];
   }
-  *reinterpret_cast<fltx4*>(&room[wave][4 * lane]) = sum;
+#pragma unroll
+  for (int e = 0; e < E; ++e) room[wave][lane + 64 * e] = sum[e];
   __syncthreads();
-  if (first + threadIdx.x >= count) return;
-  const float all = room[0][threadIdx.x] + room[1][threadIdx.x] + room[2][threadIdx.x] + room[3][threadIdx.x];
+  if (threadIdx.x >= kOuts || (int64_t)threadIdx.x >= left) return;
+  float all = room[0][threadIdx.x];
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) all += room[w][threadIdx.x];
   store_value(out, a.tag, first + threadIdx.x, all);
+}
+
+constexpr int rows_of_step(int dtype, int size) {
+  return size > 64 && dtype == F2CGT_DT_BF16 ? 64 : 32;
 }
 
 // How a product is cut: tiles of `size` squared, rows in `splits`.
@@ -498,9 +553,9 @@ struct Cut {
 Cut cut_of(int dtype, int64_t m, int64_t n, int64_t k) {
   const int64_t cus = num_cus();
   Cut c;
-  auto tiles = [&](int size) { return ceil_div(n, size) * (k > 0 ? ceil_div(k, size) : 1); };     // (a bias has rows without columns too)
+  auto tiles = [&](int size) { return ceil_div(n, size) * ceil_div(k, size); };
   c.size = tiles(256) >= cus ? 256 : tiles(64) * ceil_div(m, 32) <= 4 * cus ? 64 : n * k > 64 * 64 ? 128 : 64;
-  const int bm = dtype == F2CGT_DT_BF16 && c.size != 64 ? 64 : 32;
+  const int bm = rows_of_step(dtype, c.size);
   c.tiles = tiles(c.size);
   c.steps = ceil_div(m, bm);
   const int64_t most = c.steps, want = c.size == 256 ? 1 : c.size == 128 ? cus / c.tiles : 2 * cus / c.tiles;
@@ -573,7 +628,7 @@ extern "C" int f2cgt_unpack_activations(const int8_t* codes, int64_t code_stride
 }
 
 extern "C" int64_t f2cgt_packed_linear_grad_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k < 0 || !dense_type(dtype)) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || !dense_type(dtype)) return 0;
   const Cut c = cut_of(dtype, m, n, k);
   return c.splits > 1 ? c.splits * n * (k + 1) * 4 : 0;
 }
@@ -596,6 +651,13 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
       if (int rc = check_codes(what, codes, code_stride, exponents, k)) return rc;
   }
   hipStream_t st = as_stream(stream);
+  if (k == 0) {
+    const ColumnArgs a{grad, dbias, m, ld, (int)n, out_dtype};
+    return with_type(dtype, [&](auto t) {
+      column_sums_kernel<decltype(t)><<<dim3((unsigned)ceil_div(n, 64)), dim3(64), 0, st>>>(a);
+      return launch_status(what);
+    });
+  }
   Cut c{};
   if (m > 0) {
     c = cut_of(dtype, m, n, k);
@@ -605,21 +667,24 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
     F2CGT_REQUIRE(c.tiles * c.splits < (1ll << 22), F2CGT_E_UNSUPPORTED, "%s: too many tiles", what);
     const GradArgs a{grad, codes, exponents, c.splits > 1 ? static_cast<float*>(workspace) : nullptr, dweight, dbias, m, ld,
                      code_stride, (int)n, (int)k, (int)ceil_div(k, kCheckpointGroup), out_dtype, c.steps, (uint32_t)c.splits,
-                     (uint32_t)ceil_div(n, c.size), (uint32_t)(k > 0 ? ceil_div(k, c.size) : 1)};
+                     (uint32_t)ceil_div(n, c.size), (uint32_t)ceil_div(k, c.size)};
     const dim3 grid((unsigned)(c.tiles * c.splits));
     const int rc = with_type(dtype, [&](auto t) {
       typedef decltype(t) T;
-      constexpr int BM = kPlanes<T> == 1 ? 64 : 32;
-      if (c.size == 256) packed_linear_grad_kernel<T, 256, 256, 128, 64, BM, 1><<<grid, dim3(512), 0, st>>>(a);
-      else if (c.size == 128) packed_linear_grad_kernel<T, 128, 128, 64, 64, BM, 2><<<grid, dim3(512), 0, st>>>(a);
-      else packed_linear_grad_kernel<T, 64, 64, 32, 32, 32, 1><<<grid, dim3(256), 0, st>>>(a);
+      constexpr int tag = dtype_of<T>::tag;
+      if (c.size == 256) packed_linear_grad_kernel<T, 256, 256, 128, 64, rows_of_step(tag, 256), 1><<<grid, dim3(512), 0, st>>>(a);
+      else if (c.size == 128) packed_linear_grad_kernel<T, 128, 128, 64, 64, rows_of_step(tag, 128), 2><<<grid, dim3(512), 0, st>>>(a);
+      else packed_linear_grad_kernel<T, 64, 64, 32, 32, rows_of_step(tag, 64), 1><<<grid, dim3(256), 0, st>>>(a);
       return launch_status(what);
     });
     if (rc || c.splits == 1) return rc;
   }
-  JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype,
-             n * k % 4 == 0 && aligned(dweight, 4 * type_size(out_dtype)), (uint32_t)c.splits, (uint32_t)ceil_div(n * k, 256)};
-  F2CGT_REQUIRE(ceil_div(n * k, 256) < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
-  join_splits_kernel<<<dim3(j.blocks + (dbias ? (unsigned)ceil_div(n, 256) : 0u)), dim3(256), 0, st>>>(j);
+  // 64 outputs to a workgroup until there is one for each CU (128 x 128 of 255 splits 8 us in 64 workgroups, 6 in 256; 256 x 128 of 32 splits 2.5 in 128, 4.5 in 512)
+  const int outs = n * k <= 64 * (int64_t)num_cus() ? 64 : 256;
+  F2CGT_REQUIRE(ceil_div(n * k, outs) < (1ll << 21), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
+  const JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype, (uint32_t)c.splits, (uint32_t)ceil_div(n * k, outs)};
+  const dim3 join_grid(j.blocks + (dbias ? (unsigned)ceil_div(n, outs) : 0u)), join_block(kJoinWaves * kWave);
+  if (outs == 64) join_splits_kernel<1><<<join_grid, join_block, 0, st>>>(j);
+  else join_splits_kernel<4><<<join_grid, join_block, 0, st>>>(j);
   return launch_status(what);
 }

@@ -81,21 +81,19 @@ constexpr int kMostBits = 10;
 
 struct SortArgs {
   const void* index;         // the first digit's keys are made of these
-  const uint32_t* keys;      // of the others: the last scatter's
-  const uint32_t* places;
-  uint32_t* keys_out;
-  uint32_t* places_out;
+  const uint2* pairs;        // of the others: (key, place), the last scatter's
+  uint2* pairs_out;
   uint32_t* counts;          // [digits][blocks], then [digits] of the totals
   int64_t n;
   uint32_t rows, blocks;
   int shift, bits;
 };
 
-// Key `i`; the widest beyond the end, which no digit counts.
+// Key and place of the ids as they stand before a digit.
 template <typename Idx, bool FIRST>
-__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i) {
-  if constexpr (FIRST) return key_of(static_cast<const Idx*>(a.index)[i], a.rows);
-  else return a.keys[i];
+__device__ __forceinline__ uint2 sort_pair(const SortArgs& a, int64_t i) {
+  if constexpr (FIRST) return uint2{key_of(static_cast<const Idx*>(a.index)[i], a.rows), (uint32_t)i};
+  else return a.pairs[i];
 }
 
 template <typename Idx, bool FIRST>
@@ -108,26 +106,35 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
 #pragma unroll
   for (int u = 0; u < kSortItems; ++u) {
     const int64_t i = first + u * kSortThreads + threadIdx.x;
-    if (i < a.n) atomicAdd(&counts[sort_key<Idx, FIRST>(a, i) >> a.shift & (digits - 1)], 1u);
+    if (i < a.n) atomicAdd(&counts[sort_pair<Idx, FIRST>(a, i).x >> a.shift & (digits - 1)], 1u);
   }
   __syncthreads();
   for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) a.counts[(int64_t)d * a.blocks + blockIdx.x] = counts[d];
 }
 
-// A digit's counts become the sums of those before, its total goes behind them all.  One wave a digit.
+// A digit's counts become the sums of those before, its total goes behind them all.  One wave a digit, four workgroups' counts a lane.
 __global__ __launch_bounds__(kWave) void sort_prefix_kernel(SortArgs a) {
   uint32_t* row = a.counts + (int64_t)blockIdx.x * a.blocks;
   uint32_t before = 0;
-  for (uint32_t b = 0; b < a.blocks; b += kWave) {
-    const uint32_t i = b + threadIdx.x;
-    const uint32_t own = i < a.blocks ? row[i] : 0;
-    uint32_t upto = own;
+  for (uint32_t b = 0; b < a.blocks; b += 4 * kWave) {
+    const uint32_t i = b + 4 * threadIdx.x;
+    uint32_t own[4], all = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[e] = i + e < a.blocks ? row[i + e] : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) all += own[e];
+    uint32_t upto = all;
 #pragma unroll
     for (int by = 1; by < kWave; by *= 2) {
       const uint32_t left = (uint32_t)__shfl_up((int)upto, by);
       if ((int)threadIdx.x >= by) upto += left;
     }
-    if (i < a.blocks) row[i] = before + upto - own;
+    uint32_t at = before + upto - all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i + e < a.blocks) row[i + e] = at;
+      at += own[e];
+    }
     before += (uint32_t)__shfl((int)upto, kWave - 1);
   }
   if (threadIdx.x == 0) a.counts[(int64_t)gridDim.x * a.blocks + blockIdx.x] = before;
@@ -190,12 +197,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
   prefix_in_lds<kSortThreads>(base, digits, room);
   // a wave has a run of the tile: counted, then placed in order
   const int64_t first = (int64_t)blockIdx.x * kSortTile + wave * kWave * kSortItems + lane;
-  uint32_t key[kSortItems];
+  uint2 pair[kSortItems];
 #pragma unroll
   for (int u = 0; u < kSortItems; ++u) {
     const int64_t i = first + u * kWave;
-    key[u] = i < a.n ? sort_key<Idx, FIRST>(a, i) : 0;
-    if (i < a.n) atomicAdd(&own[wave][key[u] >> a.shift & (digits - 1)], 1u);
+    pair[u] = uint2{0, 0};
+    if (i < a.n) {
+      pair[u] = sort_pair<Idx, FIRST>(a, i);
+      atomicAdd(&own[wave][pair[u].x >> a.shift & (digits - 1)], 1u);
+    }
   }
   __syncthreads();
   for (uint32_t d = threadIdx.x; d < digits; d += kSortThreads) {
@@ -212,14 +222,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
   for (int u = 0; u < kSortItems; ++u) {
     const int64_t i = first + u * kWave;
     const bool on = i < a.n;
-    const uint32_t digit = key[u] >> a.shift & (digits - 1);
+    const uint32_t digit = pair[u].x >> a.shift & (digits - 1);
     const uint64_t same = same_digit(digit, a.bits, on);
     const uint32_t rank = below(same);
-    if (on) {
-      const uint32_t at = own[wave][digit] + rank;
-      a.keys_out[at] = key[u];
-      a.places_out[at] = FIRST ? (uint32_t)i : a.places[i];
-    }
+    if (on) a.pairs_out[own[wave][digit] + rank] = pair[u];
     __builtin_amdgcn_wave_barrier();
     if (on && rank == 0) own[wave][digit] += (uint32_t)__popcll(same);
     __builtin_amdgcn_wave_barrier();
@@ -233,20 +239,22 @@ constexpr uint32_t kLong = 64;               // ids of a row above which a workg
 struct SumArgs {
   const void* grad;
   const void* index;
-  const uint32_t* keys;      // sorted, with the places that they had
-  const uint32_t* places;
+  const uint2* pairs;        // sorted: key, and the place that it had
   float* chunks;             // [n / kChunk][d]: sums of whole runs of one row
   void* out;
   int64_t n, ld;
   uint32_t rows, range;      // range: rows of a workgroup
   int d, pieces, slices;     // slices: parts of 64 pieces of a row, a workgroup each
+  int sparse;                // most rows have no ids: zeros into all of them before anything else
   float scale;
 };
 
-// Adds to v the piece at `at` of the gradients of places[first], places[first + 1], ... in order, eight on their way at a time.
-template <typename T, int V, typename Place>
+__device__ __forceinline__ uint32_t place_in(uint2 pair) { return pair.y; }
+__device__ __forceinline__ uint32_t place_in(uint32_t place) { return place; }
+
+// Adds to v the piece at `at` of the gradients of places[first], places[first + 1], ... in order, some on their way at a time.
+template <typename T, int V, int kUnroll, typename Place>
 __device__ __forceinline__ void add_rows(float (&v)[V], const SumArgs& a, const Place* places, uint32_t first, uint32_t last, int at) {
-  constexpr int kUnroll = 8;
   typedef typename piece_words<T, V>::type words;
   const T* grad = static_cast<const T*>(a.grad) + at;
   for (uint32_t i = first; i < last; i += kUnroll) {
@@ -254,7 +262,7 @@ __device__ __forceinline__ void add_rows(float (&v)[V], const SumArgs& a, const 
     const uint32_t left = last - i;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (u < left) w[u] = *reinterpret_cast<const words*>(grad + (int64_t)places[i + u] * a.ld);
+      if (u < left) w[u] = *reinterpret_cast<const words*>(grad + (int64_t)place_in(places[i + u]) * a.ld);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       if (u >= left) continue;
@@ -267,7 +275,7 @@ __device__ __forceinline__ void add_rows(float (&v)[V], const SumArgs& a, const 
 }
 template <int V>
 __device__ __forceinline__ void add_chunks(float (&v)[V], const SumArgs& a, uint32_t first, uint32_t last, int at) {
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 8;
   for (uint32_t c = first; c < last; c += kUnroll) {
     float w[kUnroll][V];
 #pragma unroll
@@ -281,20 +289,37 @@ __device__ __forceinline__ void add_chunks(float (&v)[V], const SumArgs& a, uint
   }
 }
 
-// Where each row's ids begin among the sorted ones (the last entry: where those outside the table do), by a search a row; and, in
-// the workgroups behind, sums of the chunks that are of one row: a wave a chunk and slice, whose lanes share the chunk where the slice has few pieces.
+// Where keys of at least `key` begin in the sorted ones from lo to hi, by the 64 lanes of a wave: 64 parts at a time.
+__device__ __forceinline__ uint32_t begin_of(const uint2* pairs, uint32_t lo, uint32_t hi, uint32_t key) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + kWave - 1) / kWave;
+    const uint64_t at = (uint64_t)lo + (uint64_t)lane * step;
+    const uint32_t count = (uint32_t)__popcll(__ballot(at < hi && pairs[at < hi ? at : lo].x < key));
+    if (count == 0) return lo;
+    const uint64_t next = (uint64_t)lo + (uint64_t)count * step;
+    lo = lo + (count - 1) * step + 1;
+    hi = next < hi ? (uint32_t)next : hi;
+  }
+  return lo;
+}
+
+// Where each row's ids begin among the sorted ones (the last entry: where those outside the table do): a wave looks for the first of its
+// 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the chunks that are of
+// one row: a wave a chunk and slice, whose lanes share the chunk where the slice has few pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint32_t* starts, uint32_t search_blocks) {
   if (blockIdx.x < search_blocks) {
-    const uint32_t r = blockIdx.x * 256 + threadIdx.x;
-    if (r > a.rows) return;
-    uint32_t lo = 0, hi = (uint32_t)a.n;
+    const uint32_t r0 = blockIdx.x * 256 + threadIdx.x / kWave * kWave, r = r0 + (threadIdx.x & (kWave - 1));
+    if (r0 > a.rows) return;
+    uint32_t lo = begin_of(a.pairs, 0, (uint32_t)a.n, r0);
+    uint32_t hi = r0 + kWave > a.rows ? (uint32_t)a.n : begin_of(a.pairs, lo, (uint32_t)a.n, r0 + kWave);
     while (lo < hi) {
       const uint32_t middle = lo + (hi - lo) / 2;
-      if (a.keys[middle] < r) lo = middle + 1;
+      if (a.pairs[middle].x < r) lo = middle + 1;
       else hi = middle;
     }
-    starts[r] = lo;
+    if (r <= a.rows) starts[r] = lo;
     return;
   }
   __shared__ float room[4][kWave * V];
@@ -303,7 +328,7 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   const int slice = (int)(item - chunk * a.slices), lane = threadIdx.x & (kWave - 1);
   if (chunk >= a.n / kChunk) return;
   const uint32_t first = (uint32_t)(chunk * kChunk);
-  if (a.keys[first] != a.keys[first + kChunk - 1] || a.keys[first] >= a.rows) return;
+  if (a.pairs[first].x != a.pairs[first + kChunk - 1].x || a.pairs[first].x >= a.rows) return;
   const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;
   int lanes = 1;
   while (lanes < here) lanes *= 2;
@@ -312,7 +337,7 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   const int at = p * V + V > a.d ? a.d - V : p * V;
   float v[V] = {};
   const uint32_t each = kChunk / shares;
-  add_rows<T, V>(v, a, a.places, first + share * each, first + share * each + each, at);
+  add_rows<T, V, 8>(v, a, a.pairs, first + share * each, first + share * each + each, at);
   float* mine = room[threadIdx.x / kWave];
   if (shares > 1) {                            // (within a wave: LDS keeps its order)
 #pragma unroll
@@ -323,42 +348,45 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
       for (int e = 0; e < V; ++e) v[e] += share == 0 ? mine[e * kWave + s * lanes + sub] : 0.f;
   }
   if (share != 0 || sub >= here) return;
-  // (a piece that was moved back leaves the columns of the one before to that: another slice may add in another order)
   float* to = a.chunks + chunk * a.d + at;
 #pragma unroll
   for (int e = 0; e < V; ++e)
-    if (at + e >= p * V) to[e] = v[e];
+    if (at + e >= p * V) to[e] = v[e];         // (a piece that was moved back: its own columns)
 }
 
-// Rows of a workgroup's range, by how many ids they have: those without any are written as zeros at once, the others are listed
-// (in any order: each is a sum of its own).
+// Zeros into rows of a workgroup's range and slice: those that wanted(row) is true of.
+template <typename T, int V, int THREADS, typename Wanted>
+__device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const Wanted& wanted) {
+  const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;       // pieces of the slice
+  int lanes = 1;
+  while (lanes < here) lanes *= 2;
+  const int sub = threadIdx.x & (lanes - 1), p = slice * kWave + sub;
+  if (sub >= here) return;
+  const int at = p * V + V > a.d ? a.d - V : p * V;
+  const float zero[V] = {};
+  T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.d + at;
+  for (uint32_t r = threadIdx.x / lanes; r < count; r += THREADS / lanes)
+    if (wanted(r)) store_piece<T, V>(out + (int64_t)r * a.d, zero);
+}
+
+// Rows of a workgroup's range that have ids, few and many (in any order: each is a sum of its own).
 struct RowLists {
-  uint32_t* few;               // few[i]: rows with up to kLong ids from the front, those with more from the back
+  uint32_t* rows;              // those with up to kLong ids from the front, those with more from the back
   uint32_t* counts;            // of both
 };
-template <typename T, int V, int THREADS>
-__device__ __forceinline__ void list_rows(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start, const RowLists& lists) {
+template <int THREADS>
+__device__ __forceinline__ void list_rows(uint32_t count, const uint32_t* start, const RowLists& lists) {
   for (uint32_t r = threadIdx.x; r < count; r += THREADS) {
     const uint32_t ids = start[r + 1] - start[r];
-    if (ids > kLong) lists.few[count - 1 - atomicAdd(&lists.counts[1], 1u)] = r;
-    else if (ids > 0) lists.few[atomicAdd(&lists.counts[0], 1u)] = r;
+    if (ids > kLong) lists.rows[count - 1 - atomicAdd(&lists.counts[1], 1u)] = r;
+    else if (ids > 0) lists.rows[atomicAdd(&lists.counts[0], 1u)] = r;
   }
-  const int first = slice * kWave * V, width = a.d - first < kWave * V ? a.d - first : kWave * V;     // columns of the slice
-  typedef typename piece_words<T, V>::type words;
-  const words zero = {};
-  const int pieces = (width + V - 1) / V;
-  int lanes = 1;
-  while (lanes < pieces) lanes *= 2;
-  const int sub = threadIdx.x & (lanes - 1);
-  const int at = first + (sub * V + V > width ? (width < V ? 0 : width - V) : sub * V);
-  for (uint32_t r = threadIdx.x / lanes; r < count; r += THREADS / lanes)
-    if (start[r + 1] == start[r] && sub < pieces) *reinterpret_cast<words*>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + (at + V > a.d ? a.d - V : at)) = zero;
 }
 
-// Their sums: the places of row r's ids lie in order in places[start[r] .. start[r + 1]).  `room` holds a piece a lane.
+// Their sums: the places of row r's ids lie in order in places[start[r] - skipped .. start[r + 1] - skipped).  `room` holds a piece a lane.
 template <typename T, int V, int THREADS, typename Place>
 __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start,
-                                          const Place* places, bool chunked, const RowLists& lists, float* room) {
+                                          const Place* places, uint32_t skipped, bool chunked, const RowLists& lists, float* room) {
   constexpr int kWaves = THREADS / kWave;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;       // pieces of the slice
@@ -369,36 +397,48 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
   const int at = p * V + V > a.d ? a.d - V : p * V;
   const uint32_t few = lists.counts[0], longs = lists.counts[1];
   for (uint32_t l = (uint32_t)(wave * groups + lane / lanes); l < few; l += (uint32_t)(kWaves * groups)) {
-    const uint32_t r = lists.few[l];
+    const uint32_t r = lists.rows[l];
     float v[V] = {};
-    add_rows<T, V>(v, a, places, start[r], start[r + 1], at);
+    add_rows<T, V, 8>(v, a, places, start[r] - skipped, start[r + 1] - skipped, at);
 #pragma unroll
     for (int x = 0; x < V; ++x) v[x] *= a.scale;
     if (sub < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + at, v);
   }
-  const int lp = slice * kWave + (lane < here ? lane : here - 1);
-  const int lat = lp * V + V > a.d ? a.d - V : lp * V;
+  // Of a row with many ids each group of lanes has a share, in the groups' order.
+  const int shares = kWaves * groups, share = wave * groups + lane / lanes;
   for (uint32_t l = 0; l < longs; ++l) {
-    const uint32_t r = lists.few[count - 1 - l], s = start[r], e = start[r + 1];
+    const uint32_t r = lists.rows[count - 1 - l], s = start[r], e = start[r + 1];
     uint32_t c0 = (s + kChunk - 1) / kChunk, c1 = e / kChunk;
     if (!chunked || c0 >= c1) { c0 = 0; c1 = 0; }
     const uint32_t head = c0 < c1 ? c0 * kChunk : e, tail = c0 < c1 ? c1 * kChunk : e;
-    auto part = [&](uint32_t from, uint32_t to, int w) { return from + (uint32_t)((uint64_t)(to - from) * w / kWaves); };
+    auto part = [&](uint32_t from, uint32_t to, int w) { return from + (uint32_t)((uint64_t)(to - from) * w / shares); };
     float v[V] = {};
-    add_rows<T, V>(v, a, places, part(s, head, wave), part(s, head, wave + 1), lat);
-    if (chunked) add_chunks<V>(v, a, part(c0, c1, wave), part(c0, c1, wave + 1), lat);
-    add_rows<T, V>(v, a, places, part(tail, e, wave), part(tail, e, wave + 1), lat);
+    add_rows<T, V, 16>(v, a, places, part(s, head, share) - skipped, part(s, head, share + 1) - skipped, at);
+    if (chunked) {
+      add_chunks<V>(v, a, part(c0, c1, share), part(c0, c1, share + 1), at);
+      add_rows<T, V, 16>(v, a, places, part(tail, e, share) - skipped, part(tail, e, share + 1) - skipped, at);
+    }
     __syncthreads();                           // (the row before is done with the room)
 #pragma unroll
     for (int x = 0; x < V; ++x) room[(wave * V + x) * kWave + lane] = v[x];
     __syncthreads();
-    if (wave == 0) {
-      for (int w = 1; w < kWaves; ++w)
+    if (wave == 0 && lane < here) {
+      // (piece `lane` in each share)
 #pragma unroll
-        for (int x = 0; x < V; ++x) v[x] += room[(w * V + x) * kWave + lane];
+      for (int x = 0; x < V; ++x) v[x] = 0.f;
+      for (int w = 0; w < kWaves; ++w)
+        for (int g = 0; g < groups; ++g)
+#pragma unroll
+          for (int x = 0; x < V; ++x) v[x] += room[(w * V + x) * kWave + g * lanes + lane];
 #pragma unroll
       for (int x = 0; x < V; ++x) v[x] *= a.scale;
-      if (lane < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + lat, v);
+      // (a piece that was moved back leaves the columns of the one before to that: another slice may share the row otherwise)
+      T* out = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + at;
+      if (at == p * V) store_piece<T, V>(out, v);
+      else
+#pragma unroll
+        for (int x = 0; x < V; ++x)
+          if (at + x >= p * V) out[x] = (T)v[x];
     }
   }
 }
@@ -407,7 +447,8 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
 constexpr int kRangeSorted = 64, kSumThreads = 256;
 template <typename T, int V>
 __global__ __launch_bounds__(kSumThreads) void sorted_sums_kernel(SumArgs a, const uint32_t* starts) {
-  __shared__ uint32_t start[kRangeSorted + 1], few[kRangeSorted], counts[2];
+  constexpr uint32_t kNear = 1024;             // places of the range, brought near where they fit: a round trip less for each row
+  __shared__ uint32_t start[kRangeSorted + 1], few[kRangeSorted], counts[2], near[kNear];
   __shared__ float room[kSumThreads * V];
   const uint32_t range = blockIdx.x / a.slices, row0 = range * kRangeSorted;
   const int slice = (int)(blockIdx.x - range * a.slices);
@@ -416,9 +457,14 @@ __global__ __launch_bounds__(kSumThreads) void sorted_sums_kernel(SumArgs a, con
   if (threadIdx.x <= count) start[threadIdx.x] = starts[row0 + threadIdx.x];
   __syncthreads();
   const RowLists lists{few, counts};
-  list_rows<T, V, kSumThreads>(a, row0, count, slice, start, lists);
+  const uint32_t first = start[0], ids = start[count] - first;
+  if (ids <= kNear)
+    for (uint32_t i = threadIdx.x; i < ids; i += kSumThreads) near[i] = a.pairs[first + i].y;
+  list_rows<kSumThreads>(count, start, lists);
+  zero_rows<T, V, kSumThreads>(a, row0, count, slice, [&](uint32_t r) { return start[r + 1] == start[r]; });
   __syncthreads();
-  sum_range<T, V, kSumThreads>(a, row0, count, slice, start, a.places, true, lists, room);
+  if (ids <= kNear) sum_range<T, V, kSumThreads>(a, row0, count, slice, start, near, first, true, lists, room);
+  else sum_range<T, V, kSumThreads>(a, row0, count, slice, start, a.pairs, 0, true, lists, room);
 }
 
 // From ids as they come: those of the range are kept in their order, then sorted by row.
@@ -461,15 +507,20 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   const uint32_t n = (uint32_t)a.n, run = (n + kPickWaves * kWave - 1) / (kPickWaves * kWave) * kWave;
   const uint32_t first = wave * run, last = first + run < n ? first + run : n;
   constexpr int kMost = kPickMost / kPickThreads;
+  Idx raw[kMost];
   uint32_t local[kMost], mine = 0;
 #pragma unroll
   for (int u = 0; u < kMost; ++u) {
     const uint32_t i = first + u * kWave + lane;
-    local[u] = ~0u;
-    if (u * kWave < (int)run && i < last) {
-      const uint32_t key = key_of(index[i], a.rows), in = key - row0;
-      if (key >= row0 && in < count) local[u] = in;
-    }
+    raw[u] = -1;
+    if (u * kWave < (int)run && i < last) raw[u] = index[i];
+  }
+  // (while the ids are on their way; done at the latest before the sums)
+  if (a.sparse) zero_rows<T, V, kPickThreads>(a, row0, count, slice, [](uint32_t) { return true; });
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const uint32_t key = key_of(raw[u], a.rows), in = key - row0;
+    local[u] = key < a.rows && key >= row0 && in < count ? in : ~0u;
   }
 #pragma unroll
   for (int u = 0; u < kMost; ++u) mine += (uint32_t)__popcll(__ballot(local[u] != ~0u));
@@ -500,7 +551,8 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   }
   prefix_in_lds<kPickThreads>(start, count + 1, room_words);
   __syncthreads();
-  list_rows<T, V, kPickThreads>(a, row0, count, slice, start, lists);
+  list_rows<kPickThreads>(count, start, lists);
+  if (!a.sparse) zero_rows<T, V, kPickThreads>(a, row0, count, slice, [&](uint32_t r) { return start[r + 1] == start[r]; });
   for (uint32_t r = threadIdx.x; r < count; r += kPickThreads) {
     uint32_t before = 0;
     for (int w = 0; w < kPickWaves; ++w) {
@@ -521,8 +573,9 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
     if (on && rank == 0) own[r] += (uint16_t)__popcll(same);
     __builtin_amdgcn_wave_barrier();
   }
+  if (a.sparse) __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);      // this wave's zeros are written, before any wave writes sums
   __syncthreads();
-  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, false, lists, reinterpret_cast<float*>(lds));
+  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, 0, false, lists, reinterpret_cast<float*>(lds));
 }
 
 // Digits of the sort: as few as keys of rows + 1 values need, of one width.
@@ -533,11 +586,11 @@ void digits_of(int64_t rows, int& passes, int& bits) {
 }
 
 struct Room {
-  int64_t sorted, counts, starts, chunks;    // bytes: keys and places twice, counts of the digits, the rows' starts, sums of chunks
+  int64_t sorted, counts, starts, chunks;    // bytes: pairs twice, counts of the digits, the rows' starts, sums of chunks
   explicit Room(int64_t n, int64_t rows, int64_t d) {
     int passes, bits;
     digits_of(rows, passes, bits);
-    sorted = ceil_div(n, 4) * 16 * 4;
+    sorted = ceil_div(n, 2) * 16 * 2;
     counts = ceil_div((1ll << bits) * (ceil_div(n, kSortTile) + 1), 4) * 16;
     starts = ceil_div(rows + 1, 4) * 16;
     chunks = n / kChunk * d * 4;
@@ -592,16 +645,14 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div(a.rows, kRangeSorted) * a.slices;
   const int64_t chunk_blocks = ceil_div(a.n / kChunk * a.slices, 4);
   F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
-  uint32_t* words = reinterpret_cast<uint32_t*>(workspace);
-  const int64_t each = ceil_div(a.n, 4) * 4;
-  SortArgs s{a.index, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<uint32_t*>(workspace + room.sorted), a.n, a.rows, (uint32_t)blocks, 0, bits};
+  uint2* pairs = reinterpret_cast<uint2*>(workspace);
+  const int64_t each = ceil_div(a.n, 2) * 2;
+  SortArgs s{a.index, nullptr, nullptr, reinterpret_cast<uint32_t*>(workspace + room.sorted), a.n, a.rows, (uint32_t)blocks, 0, bits};
   const dim3 grid((unsigned)blocks), digits(1u << bits);
   for (int pass = 0; pass < passes; ++pass) {
     s.shift = pass * bits;
-    s.keys = words + (pass & 1 ? 0 : 2) * each;
-    s.places = s.keys + each;
-    s.keys_out = words + (pass & 1 ? 2 : 0) * each;
-    s.places_out = s.keys_out + each;
+    s.pairs = pairs + (pass & 1 ? 0 : each);
+    s.pairs_out = pairs + (pass & 1 ? each : 0);
     if (pass > 0) {
       sort_count_kernel<int32_t, false><<<grid, dim3(kSortThreads), 0, st>>>(s);
       sort_prefix_kernel<<<digits, dim3(kWave), 0, st>>>(s);
@@ -616,8 +667,7 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
       sort_scatter_kernel<int32_t, true><<<grid, dim3(kSortThreads), 0, st>>>(s);
     }
   }
-  a.keys = s.keys_out;
-  a.places = s.places_out;
+  a.pairs = s.pairs_out;
   uint32_t* starts = reinterpret_cast<uint32_t*>(workspace + room.sorted + room.counts);
   a.chunks = reinterpret_cast<float*>(workspace + room.sorted + room.counts + room.starts);
   const int64_t search_blocks = ceil_div((int64_t)a.rows + 1, 256);
@@ -669,7 +719,7 @@ extern "C" int f2cgt_embedding_grad(const void* grad, int dtype, int64_t ld, con
   const int64_t need = f2cgt_embedding_grad_workspace_bytes(n, rows, d);
   F2CGT_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), F2CGT_E_INVALID,
                 "%s: workspace too small or misaligned", what);
-  const SumArgs a{grad, index, nullptr, nullptr, nullptr, dtable, n, ld, (uint32_t)rows, 0, (int)d, 0, 0, scale};
+  const SumArgs a{grad, index, nullptr, nullptr, dtable, n, ld, (uint32_t)rows, 0, (int)d, 0, 0, rows > n, scale};
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     if (d >= kPieceOf<T>) return launch_grad<T, kPieceOf<T>>(a, idx_dtype, static_cast<char*>(workspace), as_stream(stream));

@@ -474,19 +474,26 @@ bool with_geometry(int64_t d, const F& f) {
   return true;
 }
 
-int64_t rows_of_block(int64_t d, int size) {
-  int64_t rows = 0;
-  auto count = [&](auto, auto lanes, auto) { rows = block_of(decltype(lanes)::value) / decltype(lanes)::value; };
+struct BlockOf {
+  int64_t block, rows;                     // threads, rows at a time (0: long rows)
+};
+BlockOf block_for(int64_t d, int size) {
+  BlockOf b{0, 0};
+  auto count = [&](auto, auto lanes, auto) {
+    b.block = block_of(decltype(lanes)::value);
+    b.rows = b.block / decltype(lanes)::value;
+  };
   if (size == 4) with_geometry<float>(d, count);
   else with_geometry<__bf16>(d, count);
-  return rows;                             // 0: long rows
+  return b;
 }
 
 // Workgroups of the backward pass: each writes 2 d sums.
 int64_t grad_blocks(int64_t m, int64_t d, int size) {
-  const int64_t rows = rows_of_block(d, size);
-  if (rows == 0) return m < 64 ? m : 64;         // (rows of the columns' kernel)
-  const int64_t all = ceil_div(m, rows), most = 4 * (int64_t)num_cus();
+  const BlockOf rows = block_for(d, size);
+  if (rows.rows == 0) return m < 64 ? m : 64;         // (rows of the columns' kernel)
+  // (as many as are on the chip at once: more only write and read more sums, at 16384 x 8192 64 MB of them beside 805)
+  const int64_t all = ceil_div(m, rows.rows), most = (int64_t)num_cus() * 1024 / rows.block;
   return all < most ? all : most;
 }
 

@@ -205,7 +205,8 @@ def test_gradients_at_views_and_of_nothing():
     assert dw.shape == (70, 89) and not dw.any() and not db.any()
     none, ex0 = lib.pack_activations(torch.empty((500, 0), device="cuda"))
     dw, db = lib.packed_linear_grad(grad, none, ex0, True)
-    assert dw.shape == (70, 0) and torch.equal(db, want[1])
+    # (no columns: another order of the same 500 additions, each off by half a step of a sum that Σ|g| bounds)
+    assert dw.shape == (70, 0) and bool(((db - want[1]).double().abs() <= 2 * 500 * U * grad.double().abs().sum(0)).all())
     assert lib.packed_linear_grad(empty.new_empty((500, 0)), codes, ex, True)[0].shape == (0, 89)
     assert lib.unpack_activations(none, ex0).shape == (500, 0)
 
