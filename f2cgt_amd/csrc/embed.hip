@@ -323,12 +323,20 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
     return;
   }
   __shared__ float room[4][kWave * V];
+  __shared__ uint32_t near[4][kChunk];
   const int64_t item = (int64_t)(blockIdx.x - search_blocks) * 4 + threadIdx.x / kWave;
   const int64_t chunk = item / a.slices;
   const int slice = (int)(item - chunk * a.slices), lane = threadIdx.x & (kWave - 1);
   if (chunk >= a.n / kChunk) return;
   const uint32_t first = (uint32_t)(chunk * kChunk);
-  if (a.pairs[first].x != a.pairs[first + kChunk - 1].x || a.pairs[first].x >= a.rows) return;
+  static_assert(kChunk == 2 * kWave, "two places a lane");
+  const uint2 mine_low = a.pairs[first + lane], mine_high = a.pairs[first + kWave + lane];
+  const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine_low.x);
+  if (key != (uint32_t)__builtin_amdgcn_readlane((int)mine_high.x, kWave - 1) || key >= a.rows) return;
+  uint32_t* places = near[threadIdx.x / kWave];              // (within a wave: LDS keeps its order)
+  places[lane] = mine_low.y;
+  places[kWave + lane] = mine_high.y;
+  __builtin_amdgcn_wave_barrier();
   const int here = a.pieces - slice * kWave < kWave ? a.pieces - slice * kWave : kWave;
   int lanes = 1;
   while (lanes < here) lanes *= 2;
@@ -337,9 +345,9 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   const int at = p * V + V > a.d ? a.d - V : p * V;
   float v[V] = {};
   const uint32_t each = kChunk / shares;
-  add_rows<T, V, 8>(v, a, a.pairs, first + share * each, first + share * each + each, at);
+  add_rows<T, V, 8>(v, a, places, share * each, share * each + each, at);
   float* mine = room[threadIdx.x / kWave];
-  if (shares > 1) {                            // (within a wave: LDS keeps its order)
+  if (shares > 1) {
 #pragma unroll
     for (int e = 0; e < V; ++e) mine[e * kWave + lane] = v[e];
     __builtin_amdgcn_wave_barrier();
@@ -384,7 +392,7 @@ __device__ __forceinline__ void list_rows(uint32_t count, const uint32_t* start,
 }
 
 // Their sums: the places of row r's ids lie in order in places[start[r] - skipped .. start[r + 1] - skipped).  `room` holds a piece a lane.
-template <typename T, int V, int THREADS, typename Place>
+template <typename T, int V, int THREADS, int ROWS, int LONG_UNROLL, typename Place>
 __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint32_t count, int slice, const uint32_t* start,
                                           const Place* places, uint32_t skipped, bool chunked, const RowLists& lists, float* room) {
   constexpr int kWaves = THREADS / kWave;
@@ -396,13 +404,35 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
   const int p = slice * kWave + (sub < here ? sub : here - 1);
   const int at = p * V + V > a.d ? a.d - V : p * V;
   const uint32_t few = lists.counts[0], longs = lists.counts[1];
-  for (uint32_t l = (uint32_t)(wave * groups + lane / lanes); l < few; l += (uint32_t)(kWaves * groups)) {
-    const uint32_t r = lists.rows[l];
-    float v[V] = {};
-    add_rows<T, V, 8>(v, a, places, start[r] - skipped, start[r + 1] - skipped, at);
+  // Some rows to a group of lanes at a time, whose first two ids are all on their way at once: most rows have no more.
+  constexpr int kRows = ROWS, kFirst = 2;
+  typedef typename piece_words<T, V>::type words;
+  for (uint32_t l0 = (uint32_t)(wave * groups + lane / lanes) * kRows; l0 < few; l0 += (uint32_t)(kWaves * groups * kRows)) {
+    uint32_t r[kRows], s[kRows], e[kRows];
+    words w[kRows][kFirst];
 #pragma unroll
-    for (int x = 0; x < V; ++x) v[x] *= a.scale;
-    if (sub < here) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.d + at, v);
+    for (int q = 0; q < kRows; ++q) {
+      r[q] = lists.rows[l0 + q < few ? l0 + q : few - 1];
+      s[q] = start[r[q]] - skipped;
+      e[q] = start[r[q] + 1] - skipped;
+#pragma unroll
+      for (int u = 0; u < kFirst; ++u)          // (the first one twice where there is no second)
+        w[q][u] = *reinterpret_cast<const words*>(static_cast<const T*>(a.grad) + at + (int64_t)place_in(places[s[q] + u < e[q] ? s[q] + u : s[q]]) * a.ld);
+    }
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      float v[V] = {}, g[V];
+#pragma unroll
+      for (int u = 0; u < kFirst; ++u) {
+        values_of<T, V>(w[q][u], g);
+#pragma unroll
+        for (int x = 0; x < V; ++x) v[x] = s[q] + u < e[q] ? v[x] + g[x] : v[x];
+      }
+      if (s[q] + kFirst < e[q]) add_rows<T, V, 8>(v, a, places, s[q] + kFirst, e[q], at);
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] *= a.scale;
+      if (sub < here && l0 + q < few) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r[q]) * a.d + at, v);
+    }
   }
   // Of a row with many ids each group of lanes has a share, in the groups' order.
   const int shares = kWaves * groups, share = wave * groups + lane / lanes;
@@ -413,10 +443,10 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
     const uint32_t head = c0 < c1 ? c0 * kChunk : e, tail = c0 < c1 ? c1 * kChunk : e;
     auto part = [&](uint32_t from, uint32_t to, int w) { return from + (uint32_t)((uint64_t)(to - from) * w / shares); };
     float v[V] = {};
-    add_rows<T, V, 16>(v, a, places, part(s, head, share) - skipped, part(s, head, share + 1) - skipped, at);
+    add_rows<T, V, LONG_UNROLL>(v, a, places, part(s, head, share) - skipped, part(s, head, share + 1) - skipped, at);
     if (chunked) {
       add_chunks<V>(v, a, part(c0, c1, share), part(c0, c1, share + 1), at);
-      add_rows<T, V, 16>(v, a, places, part(tail, e, share) - skipped, part(tail, e, share + 1) - skipped, at);
+      add_rows<T, V, LONG_UNROLL>(v, a, places, part(tail, e, share) - skipped, part(tail, e, share + 1) - skipped, at);
     }
     __syncthreads();                           // (the row before is done with the room)
 #pragma unroll
@@ -463,8 +493,8 @@ __global__ __launch_bounds__(kSumThreads) void sorted_sums_kernel(SumArgs a, con
   list_rows<kSumThreads>(count, start, lists);
   zero_rows<T, V, kSumThreads>(a, row0, count, slice, [&](uint32_t r) { return start[r + 1] == start[r]; });
   __syncthreads();
-  if (ids <= kNear) sum_range<T, V, kSumThreads>(a, row0, count, slice, start, near, first, true, lists, room);
-  else sum_range<T, V, kSumThreads>(a, row0, count, slice, start, a.pairs, 0, true, lists, room);
+  if (ids <= kNear) sum_range<T, V, kSumThreads, 4, 8>(a, row0, count, slice, start, near, first, true, lists, room);
+  else sum_range<T, V, kSumThreads, 4, 8>(a, row0, count, slice, start, a.pairs, 0, true, lists, room);
 }
 
 // From ids as they come: those of the range are kept in their order, then sorted by row.
@@ -484,7 +514,7 @@ struct PickRoom {
 };
 
 template <typename T, int V, typename Idx>
-__global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
+__global__ __launch_bounds__(kPickThreads, 8) void picked_sums_kernel(SumArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint32_t room_words[kPickWaves], list_counts[2];
   const PickRoom at_lds((uint32_t)a.n, a.range, V);
@@ -575,7 +605,7 @@ __global__ __launch_bounds__(kPickThreads) void picked_sums_kernel(SumArgs a) {
   }
   if (a.sparse) __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);      // this wave's zeros are written, before any wave writes sums
   __syncthreads();
-  sum_range<T, V, kPickThreads>(a, row0, count, slice, start, sorted, 0, false, lists, reinterpret_cast<float*>(lds));
+  sum_range<T, V, kPickThreads, 1, 8>(a, row0, count, slice, start, sorted, 0, false, lists, reinterpret_cast<float*>(lds));
 }
 
 // Digits of the sort: as few as keys of rows + 1 values need, of one width.
