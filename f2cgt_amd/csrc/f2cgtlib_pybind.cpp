@@ -1217,6 +1217,9 @@ void undifferentiated(const char* op, std::initializer_list<torch::Tensor> tenso
   }
 }
 
+// A lazily negated view as the values that it stands for; any other tensor as it is, without a dispatch.
+torch::Tensor with_sign(const torch::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // Rows of values that a kernel can take one after the other: x itself, or a copy where columns lie apart, rows overlap or x is
 // a lazily negated view, which holds the values' opposites (here and below: contiguous() keeps it one).
 torch::Tensor value_rows(const torch::Tensor& x, const char* name) {
@@ -1224,7 +1227,7 @@ torch::Tensor value_rows(const torch::Tensor& x, const char* name) {
   TORCH_CHECK(x.dim() >= 1, name, " must have rows");
   int64_t count = 1;
   for (int64_t d = 0; d + 1 < x.dim(); ++d) count *= x.size(d);
-  auto rows = (x.dim() == 2 ? x : x.reshape({count, x.size(-1)})).resolve_neg();
+  auto rows = with_sign(x.dim() == 2 ? x : x.reshape({count, x.size(-1)}));
   const bool plain = (rows.size(1) <= 1 || rows.stride(1) == 1) && (rows.size(0) <= 1 || rows.stride(0) >= rows.size(1));
   return plain ? rows : rows.contiguous();
 }
@@ -1238,7 +1241,7 @@ torch::Tensor room_for_codes(int64_t rows, int64_t k, const torch::Tensor& like)
 // The same of codes that a caller gives: themselves, or a copy where they are not laid out so.
 torch::Tensor code_rows(const torch::Tensor& codes_in, const char* name) {
   TORCH_CHECK(codes_in.defined() && codes_in.device().is_cuda(), name, " must be a GPU tensor");
-  const auto codes = codes_in.resolve_neg();
+  const auto codes = with_sign(codes_in);
   TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == torch::kInt8, name, " must be int8 [rows, columns]");
   const int64_t step = codes.stride(0), whole = (codes.size(1) + 15) / 16 * 16;
   // (the kernels read whole pieces, the last row's last one too)
@@ -1467,10 +1470,20 @@ void muon_step(const std::vector<torch::Tensor>& weights, const std::vector<torc
 }
 
 // ---- layer norm, checkpoints in 8 bits, learnt rows --------------------------------------------------------
+// Device memory for the length of a call, from torch's allocator, in the order of the current stream.
+struct Workspace {
+  c10::DataPtr held;
+  int64_t bytes;
+  explicit Workspace(int64_t size) : bytes(size) {
+    if (size > 0) held = c10::GetAllocator(c10::DeviceType::CUDA)->allocate((size_t)size);
+  }
+  void* get() const { return held.get(); }
+};
+
 // A vector beside rows of d values: fp32 or of their type.
 torch::Tensor norm_vector(const c10::optional<torch::Tensor>& v, const torch::Tensor& rows, const char* name) {
   if (!v.has_value()) return torch::Tensor();
-  auto t = beside(v->defined() ? v->resolve_neg() : *v, rows, name);
+  auto t = beside(with_sign(*v), rows, name);
   TORCH_CHECK((t.scalar_type() == torch::kFloat32 || t.scalar_type() == rows.scalar_type()) && t.dim() == 1 && t.size(0) == rows.size(1),
               name, " must be float32 or ", rows.scalar_type(), " [", rows.size(1), "]");
   return t;
@@ -1479,7 +1492,7 @@ const void* data_or_null(const torch::Tensor& t) { return t.defined() ? t.data_p
 
 // A statistic for each row.
 torch::Tensor row_values(const torch::Tensor& v, const torch::Tensor& rows, const char* name) {
-  auto t = beside(v.defined() ? v.resolve_neg() : v, rows, name);
+  auto t = beside(with_sign(v), rows, name);
   TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.numel() == rows.size(0), name, " must be float32 with a value for each of the ",
               rows.size(0), " rows");
   return t;
@@ -1583,14 +1596,12 @@ NormGrads norm_grads(const char* op, const torch::Tensor& grad_in, const torch::
   c10::optional<torch::Tensor> dw, db;
   if (weight_grad) dw = torch::empty({d}, vector);
   if (bias_grad) db = torch::empty({d}, vector);
-  const int64_t bytes = weight_grad || bias_grad ? f2cgt_layer_norm_grad_workspace_bytes(tag, m, d) : 0;
-  torch::Tensor ws;
-  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  const Workspace ws(weight_grad || bias_grad ? f2cgt_layer_norm_grad_workspace_bytes(tag, m, d) : 0);
   check_rc(f2cgt_layer_norm_grad(grad.data_ptr(), tag, row_step(grad), kept ? nullptr : x.data_ptr(), kept ? 0 : row_step(x),
                                  kept ? kept->code_ptr() : nullptr, kept ? kept->stride() : 0,
                                  kept ? kept->exponents.data_ptr<uint8_t>() : nullptr, mean.data_ptr<float>(), rstd.data_ptr<float>(),
                                  data_or_null(weight), weight_tag, dx.data_ptr(), dw ? dw->data_ptr() : nullptr,
-                                 db ? db->data_ptr() : nullptr, weight_tag, bytes > 0 ? ws.data_ptr() : nullptr, bytes, m, d,
+                                 db ? db->data_ptr() : nullptr, weight_tag, ws.get(), ws.bytes, m, d,
                                  current_stream()),
            op);
   return {dx, dw, db};
@@ -1648,12 +1659,10 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> packed_linear_grad(const
   auto dw = torch::empty({n, k}, grad.options().dtype(dtype));
   c10::optional<torch::Tensor> db;
   if (bias) db = torch::empty({n}, grad.options().dtype(dtype));
-  const int64_t bytes = f2cgt_packed_linear_grad_workspace_bytes(tag, m, n, k);
-  torch::Tensor ws;
-  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  const Workspace ws(f2cgt_packed_linear_grad_workspace_bytes(tag, m, n, k));
   check_rc(f2cgt_packed_linear_grad(grad.data_ptr(), tag, row_step(grad), kept.code_ptr(), kept.stride(),
                                     kept.exponents.data_ptr<uint8_t>(), dw.data_ptr(), db ? db->data_ptr() : nullptr, out_tag,
-                                    bytes > 0 ? ws.data_ptr() : nullptr, bytes, m, n, k, current_stream()),
+                                    ws.get(), ws.bytes, m, n, k, current_stream()),
            "packed_linear_grad");
   return {dw, db};
 }
@@ -1693,11 +1702,9 @@ torch::Tensor embedding_grad(const torch::Tensor& grad_in, const torch::Tensor& 
   c10::DeviceGuard guard(grad.device());
   const int64_t n = ids.numel(), d = grad.size(1);
   auto out = torch::empty({num_rows, d}, grad.options());
-  const int64_t bytes = f2cgt_embedding_grad_workspace_bytes(n, num_rows, d);
-  torch::Tensor ws;
-  if (bytes > 0) ws = torch::empty({bytes}, grad.options().dtype(torch::kUInt8));
+  const Workspace ws(f2cgt_embedding_grad_workspace_bytes(n, num_rows, d));
   check_rc(f2cgt_embedding_grad(grad.data_ptr(), tag, row_step(grad), ids.data_ptr(), id_tag(ids), out.data_ptr(), (float)scale,
-                                bytes > 0 ? ws.data_ptr() : nullptr, bytes, n, num_rows, d, current_stream()),
+                                ws.get(), ws.bytes, n, num_rows, d, current_stream()),
            "embedding_grad");
   return out;
 }
