@@ -494,8 +494,8 @@ __global__ __launch_bounds__(64) void column_sums_kernel(ColumnArgs a) {
   store_value(a.bias, a.out_tag, column, sum);
 }
 
-// Sums over the splits: a workgroup has 64 E outputs, each of its sixteen waves every sixteenth split, then the waves' sums in order; the
-// bias' in workgroups behind the weight's.  (No splits: zeros, of no rows.)
+// Sums over the splits: SHARE waves have 64 E outputs, each of them every SHAREth split, then the waves' sums are added in order; the bias' in
+// workgroups behind the weight's.  (No splits: zeros, of no rows.)
 struct JoinArgs {
   const float* parts;
   void* out;
@@ -504,41 +504,48 @@ struct JoinArgs {
   int n, tag;
   uint32_t splits, blocks;   // blocks: those of the weight
 };
-constexpr int kJoinWaves = 16;
-template <int E>
-__global__ __launch_bounds__(kJoinWaves * kWave) void join_splits_kernel(JoinArgs a) {
+template <int WAVES, int SHARE, int E>
+__global__ __launch_bounds__(WAVES * kWave) void join_splits_kernel(JoinArgs a) {
   constexpr int kOuts = 64 * E;
-  __shared__ float room[kJoinWaves][kOuts];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  __shared__ float room[SHARE > 1 ? WAVES : 1][kOuts];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, share = wave % SHARE;
   const bool weight = blockIdx.x < a.blocks;
-  const int64_t count = weight ? a.count : a.n, first = (int64_t)(weight ? blockIdx.x : blockIdx.x - a.blocks) * kOuts;
+  const int64_t count = weight ? a.count : a.n;
+  const int64_t first = ((int64_t)(weight ? blockIdx.x : blockIdx.x - a.blocks) * (WAVES / SHARE) + wave / SHARE) * kOuts;
   const float* parts = (weight ? a.parts : a.parts + (int64_t)a.splits * a.count) + first;
   void* out = weight ? a.out : a.bias;
   const int64_t left = count - first;
   constexpr int kAtOnce = 16 / E;
   float sum[E] = {};
-  for (uint32_t s = wave; s < a.splits; s += kAtOnce * kJoinWaves) {
+  for (uint32_t s = share; s < a.splits; s += kAtOnce * SHARE) {
     float v[kAtOnce][E];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         v[u][e] = 0.f;
-        if (s + u * kJoinWaves < a.splits && lane + 64 * e < left) v[u][e] = parts[(int64_t)(s + u * kJoinWaves) * count + lane + 64 * e];
+        if (s + u * SHARE < a.splits && lane + 64 * e < left) v[u][e] = parts[(int64_t)(s + u * SHARE) * count + lane + 64 * e];
       }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) sum[e] += v[u][e];
   }
+  if constexpr (SHARE > 1) {
+    static_assert(WAVES == SHARE, "one set of outputs to a workgroup");
 #pragma unroll
-  for (int e = 0; e < E; ++e) room[wave][lane + 64 * e] = sum[e];
-  __syncthreads();
-  if (threadIdx.x >= kOuts || (int64_t)threadIdx.x >= left) return;
-  float all = room[0][threadIdx.x];
+    for (int e = 0; e < E; ++e) room[wave][lane + 64 * e] = sum[e];
+    __syncthreads();
+    if (threadIdx.x >= kOuts || (int64_t)threadIdx.x >= left) return;
+    float all = room[0][threadIdx.x];
 #pragma unroll
-  for (int w = 1; w < kJoinWaves; ++w) all += room[w][threadIdx.x];
-  store_value(out, a.tag, first + threadIdx.x, all);
+    for (int w = 1; w < SHARE; ++w) all += room[w][threadIdx.x];
+    store_value(out, a.tag, first + threadIdx.x, all);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (lane + 64 * e < left) store_value(out, a.tag, first + lane + 64 * e, sum[e]);
+  }
 }
 
 constexpr int rows_of_step(int dtype, int size) {
@@ -550,17 +557,44 @@ struct Cut {
   int size;
   int64_t tiles, steps, splits;
 };
+// The shortest of the cuts that are tried, by times that were measured (us; planes of one, two and three): a launch with the begin and
+// end of a tile of 64, 128 and 256 squared 2.5, 7 and 9; 32 rows of a tile of 64 squared 0.45, 0.55 and 0.65 where it is alone on its CU, 0.17, 0.20 and 0.275 for each of many, of 128 squared 0.43, 0.62 and 0.78, of
+// 256 squared 0.95, 1.8 and 2.45, those alone on their CUs; splits' sums a launch more, 3.5, and 5 MB a us both ways.  What it decides, bf16 and fp32:
+// 1000 x 1000 -> 1000 64 squared 18.5 and 24, 128 squared 22.8 and 25.1; 8192 x 2048 -> 2048 256 squared in four splits 94 and 187, 128 squared
+// 120 and 207; 60 001 x 602 -> 128 128 squared 33.7 and 46.2, 64 squared 35.7 and 56.0; 30 000 x 64 -> 1024 64 squared in 48 or 64 splits 24.3
+// and 31.6, in 32 26.9 and 33.1, 128 squared 28.9 and 38.9.
 Cut cut_of(int dtype, int64_t m, int64_t n, int64_t k) {
+  static constexpr float kAlone[3][3] = {{0.45f, 0.55f, 0.65f}, {0.43f, 0.62f, 0.78f}, {0.95f, 1.8f, 2.45f}};
+  static constexpr float kShared[3] = {0.17f, 0.20f, 0.275f}, kBegin[3] = {2.5f, 7.f, 9.f};
+  const int planes = dtype == F2CGT_DT_BF16 ? 0 : dtype == F2CGT_DT_F16 ? 1 : 2;
   const int64_t cus = num_cus();
-  Cut c;
-  auto tiles = [&](int size) { return ceil_div(n, size) * ceil_div(k, size); };
-  c.size = tiles(256) >= cus ? 256 : tiles(64) * ceil_div(m, 32) <= 4 * cus ? 64 : n * k > 64 * 64 ? 128 : 64;
-  const int bm = rows_of_step(dtype, c.size);
-  c.tiles = tiles(c.size);
-  c.steps = ceil_div(m, bm);
-  const int64_t most = c.steps, want = c.size == 256 ? 1 : c.size == 128 ? cus / c.tiles : 2 * cus / c.tiles;
-  c.splits = want < 1 ? 1 : want > most ? most : want;
-  return c;
+  Cut best{};
+  float least = 0.f;
+  for (int i = 0; i < 3; ++i) {
+    const int size = 64 << i;
+    if (i == 2 && (n <= 128 || k <= 128)) continue;
+    const int64_t tiles = ceil_div(n, size) * ceil_div(k, size), steps = ceil_div(m, rows_of_step(dtype, size));
+    const float each = (float)rows_of_step(dtype, size) / 32;
+    auto take = [&](int64_t splits) {
+      if (splits < 1 || splits > steps || splits > 1024 || (splits > 1 && (splits * tiles > 8 * cus || splits * n * k > (1ll << 28)))) return;
+      const int64_t rounds = ceil_div(tiles * splits, cus);
+      float step = kAlone[i][planes] * (i == 0 ? 1.f : (float)rounds);
+      if (i == 0 && kShared[planes] * (float)rounds > step) step = kShared[planes] * (float)rounds;
+      float time = kBegin[i] + (float)ceil_div(steps, splits) * each * step;
+      if (splits > 1) time += 3.5f + (float)(splits * n * k) * 8e-6f / 5.f;
+      if (best.size != 0 && time >= least) return;
+      least = time;
+      best = Cut{size, tiles, steps, splits};
+    };
+    // one, two and three to the power of two, and as many as fill the chip
+    take(1);
+    for (int64_t s = 2; s <= 1024; s *= 2) {
+      take(s);
+      take(s + s / 2);
+    }
+    for (int64_t s = 1; s <= 4; s *= 2) take(s * cus / tiles);
+  }
+  return best;
 }
 
 int check_codes(const char* what, const int8_t* codes, int64_t stride, const uint8_t* exponents, int64_t k) {
@@ -679,12 +713,15 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
     });
     if (rc || c.splits == 1) return rc;
   }
-  // 64 outputs to a workgroup until there is one for each CU (128 x 128 of 255 splits 8 us in 64 workgroups, 6 in 256; 256 x 128 of 32 splits 2.5 in 128, 4.5 in 512)
-  const int outs = n * k <= 64 * (int64_t)num_cus() ? 64 : 256;
+  // Few splits: a wave for 256 outputs.  Many: sixteen waves for 256, or for 64 until there is a workgroup for each CU (128 x 128 of 255 splits 8 us in
+  // 64 workgroups, 6 in 256).
+  const bool few = c.splits <= 8;
+  const int outs = few ? 1024 : n * k <= 64 * (int64_t)num_cus() ? 64 : 256;
   F2CGT_REQUIRE(ceil_div(n * k, outs) < (1ll << 21), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
   const JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype, (uint32_t)c.splits, (uint32_t)ceil_div(n * k, outs)};
-  const dim3 join_grid(j.blocks + (dbias ? (unsigned)ceil_div(n, outs) : 0u)), join_block(kJoinWaves * kWave);
-  if (outs == 64) join_splits_kernel<1><<<join_grid, join_block, 0, st>>>(j);
-  else join_splits_kernel<4><<<join_grid, join_block, 0, st>>>(j);
+  const dim3 join_grid(j.blocks + (dbias ? (unsigned)ceil_div(n, outs) : 0u));
+  if (few) join_splits_kernel<4, 1, 4><<<join_grid, dim3(256), 0, st>>>(j);
+  else if (outs == 64) join_splits_kernel<16, 16, 1><<<join_grid, dim3(1024), 0, st>>>(j);
+  else join_splits_kernel<16, 16, 4><<<join_grid, dim3(1024), 0, st>>>(j);
   return launch_status(what);
 }
