@@ -373,8 +373,15 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t row0, uint3
   const int at = p * V + V > a.d ? a.d - V : p * V;
   const float zero[V] = {};
   T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.d + at;
-  for (uint32_t r = threadIdx.x / lanes; r < count; r += THREADS / lanes)
-    if (wanted(r)) store_piece<T, V>(out + (int64_t)r * a.d, zero);
+  for (uint32_t r = threadIdx.x / lanes; r < count; r += THREADS / lanes) {
+    if (!wanted(r)) continue;
+    // (a piece that was moved back: its own columns, for those before may hold another slice's sums by now)
+    if (at == p * V) store_piece<T, V>(out + (int64_t)r * a.d, zero);
+    else
+#pragma unroll
+      for (int x = 0; x < V; ++x)
+        if (at + x >= p * V) out[(int64_t)r * a.d + x] = (T)0.f;
+  }
 }
 
 // Rows of a workgroup's range that have ids, few and many (in any order: each is a sum of its own).

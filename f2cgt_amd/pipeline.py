@@ -930,12 +930,7 @@ class _PackedLinear(torch.autograd.Function):
         weight, codes, exponents = ctx.saved_tensors
         wants = ctx.needs_input_grad
         dx = torch.matmul(grad, weight) if wants[0] else None
-        dw = db = None
-        if wants[1]:
-            dw, db = _capi().packed_linear_grad(grad, codes, exponents, wants[2], weight.dtype)
-        elif wants[2]:
-            db = grad.reshape(-1, grad.shape[-1]).sum(dim=0, dtype=torch.float32).to(weight.dtype)
-        return dx, dw, db
+        return (dx, *_capi().packed_linear_grad(grad, codes, exponents, wants[2], weight.dtype))      # (the weight's is always wanted)
 
 
 class PackedLinear(nn.Linear):
