@@ -494,8 +494,8 @@ __global__ __launch_bounds__(64) void column_sums_kernel(ColumnArgs a) {
   store_value(a.bias, a.out_tag, column, sum);
 }
 
-// Sums over the splits: SHARE waves have 64 E outputs, each of them every SHAREth split, then the waves' sums are added in order; the bias' in
-// workgroups behind the weight's.  (No splits: zeros, of no rows.)
+// Sums over the splits: SHARE waves have 64 E outputs, each of them every SHAREth split, then the waves' sums are added in order; the bias'
+// in workgroups behind the weight's.  (No splits: zeros, of no rows.)
 struct JoinArgs {
   const float* parts;
   void* out;
@@ -557,12 +557,13 @@ struct Cut {
   int size;
   int64_t tiles, steps, splits;
 };
-// The shortest of the cuts that are tried, by times that were measured (us; planes of one, two and three): a launch with the begin and
-// end of a tile of 64, 128 and 256 squared 2.5, 7 and 9; 32 rows of a tile of 64 squared 0.45, 0.55 and 0.65 where it is alone on its CU, 0.17, 0.20 and 0.275 for each of many, of 128 squared 0.43, 0.62 and 0.78, of
-// 256 squared 0.95, 1.8 and 2.45, those alone on their CUs; splits' sums a launch more, 3.5, and 5 MB a us both ways.  What it decides, bf16 and fp32:
-// 1000 x 1000 -> 1000 64 squared 18.5 and 24, 128 squared 22.8 and 25.1; 8192 x 2048 -> 2048 256 squared in four splits 94 and 187, 128 squared
-// 120 and 207; 60 001 x 602 -> 128 128 squared 33.7 and 46.2, 64 squared 35.7 and 56.0; 30 000 x 64 -> 1024 64 squared in 48 or 64 splits 24.3
-// and 31.6, in 32 26.9 and 33.1, 128 squared 28.9 and 38.9.
+// The shortest of the cuts that are tried, by times that were measured (us; planes of one, two and three): a launch with the begin and end
+// of a tile of 64, 128 and 256 squared 2.5, 7 and 9; 32 rows of a tile of 64 squared 0.45, 0.55 and 0.65 where it is alone on its CU, 0.17,
+// 0.20 and 0.275 for each of many, of 128 squared 0.43, 0.62 and 0.78, of 256 squared 0.95, 1.8 and 2.45, those alone on their CUs; splits'
+// sums a launch more, 3.5, and 5 MB a us both ways.  What it decides, bf16 and fp32: 1000 x 1000 -> 1000 64 squared 18.5 and 24, 128 squared
+// 22.8 and 25.1; 8192 x 2048 -> 2048 256 squared in four splits 94 and 187, 128 squared 120 and 207; 60 001 x 602 -> 128 128 squared 33.7 and
+// 46.2, 64 squared 35.7 and 56.0; 30 000 x 64 -> 1024 64 squared in 48 or 64 splits 24.3 and 31.6, in 32 26.9 and 33.1, 128 squared 28.9 and
+// 38.9.
 Cut cut_of(int dtype, int64_t m, int64_t n, int64_t k) {
   static constexpr float kAlone[3][3] = {{0.45f, 0.55f, 0.65f}, {0.43f, 0.62f, 0.78f}, {0.95f, 1.8f, 2.45f}};
   static constexpr float kShared[3] = {0.17f, 0.20f, 0.275f}, kBegin[3] = {2.5f, 7.f, 9.f};
@@ -713,8 +714,8 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
     });
     if (rc || c.splits == 1) return rc;
   }
-  // Few splits: a wave for 256 outputs.  Many: sixteen waves for 256, or for 64 until there is a workgroup for each CU (128 x 128 of 255 splits 8 us in
-  // 64 workgroups, 6 in 256).
+  // Few splits: a wave for 256 outputs.  Many: sixteen waves for 256, or for 64 until there is a workgroup for each CU (128 x 128 of 255
+  // splits 8 us in 64 workgroups, 6 in 256).
   const bool few = c.splits <= 8;
   const int outs = few ? 1024 : n * k <= 64 * (int64_t)num_cus() ? 64 : 256;
   F2CGT_REQUIRE(ceil_div(n * k, outs) < (1ll << 21), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);

@@ -73,21 +73,19 @@ __device__ __forceinline__ void sum_group(float (&v)[N], float* room) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = sum_lanes<(LANES < kWave ? LANES : kWave)>(v[i]);
   if constexpr (LANES > kWave) {
-    constexpr int kWaves = LANES / kWave;
-    const int wave = threadIdx.x / kWave;
+    constexpr int kWaves = LANES / kWave, kSpread = kWaves <= 4 ? 4 : kWaves <= 8 ? 8 : 16;
+    const int wave = threadIdx.x / kWave, at = threadIdx.x % kSpread;
     if (threadIdx.x % kWave == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) room[i * kWaves + wave] = v[i];
     __syncthreads();
+    // (every lane one wave's sum, then as over lanes)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      // (every lane one wave's sum, then as over lanes)
-      v[i] = sum_lanes<kWaves>(room[i * kWaves + threadIdx.x % kWaves]);
-    }
+    for (int i = 0; i < N; ++i) v[i] = sum_lanes<kSpread>(at < kWaves ? room[i * kWaves + at] : 0.f);
   }
 }
 
-constexpr int block_of(int lanes) { return lanes > 256 ? lanes : 256; }
+constexpr int block_of(int lanes) { return lanes > kWave ? lanes : 256; }     // (threads of a workgroup)
 
 template <typename T, int V, int LANES, int C, bool PACK>
 __global__ __launch_bounds__(block_of(LANES)) void layer_norm_kernel(NormArgs a) {
@@ -452,25 +450,38 @@ __global__ __launch_bounds__(1024) void join_sums_kernel(JoinArgs a) {
   else static_cast<__bf16*>(a.to[which])[at] = (__bf16)sum;
 }
 
-// f(piece values, lanes, pieces a lane) for the width d: few lanes to a short row, so that a workgroup has several; as many as a row has
-// pieces to a long one.  -> false: longer than a workgroup's registers hold.
+// f(piece values, lanes, pieces a lane) for the width d: few lanes to a short row, so that a workgroup has several rows; as many as a row
+// has pieces to a long one.  Measured, GB/s of what is read and written, forward and backward: 32 lanes with three pieces rather than 64
+// with two up to 96 pieces (111476 x 602 in bf16 5470 and 4300 against 4760 and 3530), 4 rather than 8 up to four (1048576 x 16 in fp32
+// 5830 and 5000 against 4400 and 4880), 192 rather than 256 in 16 bits (65154 x 1030 in bf16 3850 and 3840 against 3270 and 3465); 384 and
+// 768 lose to the powers of two, since a CU holds two or one (22369 x 1500 in fp32 4850 and 4400 against 5300 and 4820).  Four pieces to
+// each of 1024 lanes rather than the kernels for long rows (2048 x 16384 in fp32 5560 and 4000 against 3290 and 2530); with 16 bits that
+// would be 32 values a lane, beyond the registers of the backward pass.
 template <int N> struct count_of { static constexpr int value = N; };
 template <typename T, typename F>
 bool with_geometry(int64_t d, const F& f) {
   constexpr int V = kPieceOf<T>;
   const int64_t pieces = ceil_div(d, V);
   if (d < V) f(count_of<1>{}, count_of<8>{}, count_of<1>{});
+  else if (pieces <= 4) f(count_of<V>{}, count_of<4>{}, count_of<1>{});
   else if (pieces <= 8) f(count_of<V>{}, count_of<8>{}, count_of<1>{});
   else if (pieces <= 16) f(count_of<V>{}, count_of<16>{}, count_of<1>{});
   else if (pieces <= 32) f(count_of<V>{}, count_of<32>{}, count_of<1>{});
   else if (pieces <= 64) f(count_of<V>{}, count_of<64>{}, count_of<1>{});
+  else if (pieces <= 96) f(count_of<V>{}, count_of<32>{}, count_of<3>{});
   else if (pieces <= 128) f(count_of<V>{}, count_of<64>{}, count_of<2>{});
   else if (V == 4 && pieces <= 192) f(count_of<V>{}, count_of<64>{}, count_of<3>{});
+  else if (pieces <= 192) f(count_of<V>{}, count_of<192>{}, count_of<1>{});
   else if (pieces <= 256) f(count_of<V>{}, count_of<256>{}, count_of<1>{});
   else if (pieces <= 512) f(count_of<V>{}, count_of<512>{}, count_of<1>{});
   else if (pieces <= 1024) f(count_of<V>{}, count_of<1024>{}, count_of<1>{});
   else if (pieces <= 2048) f(count_of<V>{}, count_of<1024>{}, count_of<2>{});
-  else return false;
+  else if constexpr (V == 4) {
+    if (pieces > 4096) return false;
+    f(count_of<V>{}, count_of<1024>{}, count_of<4>{});
+  } else {
+    return false;
+  }
   return true;
 }
 
@@ -492,8 +503,9 @@ BlockOf block_for(int64_t d, int size) {
 int64_t grad_blocks(int64_t m, int64_t d, int size) {
   const BlockOf rows = block_for(d, size);
   if (rows.rows == 0) return m < 64 ? m : 64;         // (rows of the columns' kernel)
-  // (as many as are on the chip at once: more only write and read more sums, at 16384 x 8192 64 MB of them beside 805)
-  const int64_t all = ceil_div(m, rows.rows), most = (int64_t)num_cus() * 1024 / rows.block;
+  // (as many as are on the chip at once, the same number on each CU: more only write and read more sums, at 16384 x 8192 64 MB of them
+  // beside 805)
+  const int64_t all = ceil_div(m, rows.rows), most = (int64_t)num_cus() * (1024 / rows.block);
   return all < most ? all : most;
 }
 
