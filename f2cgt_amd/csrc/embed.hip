@@ -2,15 +2,18 @@
 //
 //   out_i = scale * table[id_i]                     dtable_r = scale * sum over i with id_i = r, in their order, of grad_i
 //
-// An id outside the table (a place of a padded batch) reads zeros and adds to no row.  Both are bound by memory.  The gradient
-// writes every row of the table once, those without ids as zeros, and adds in the order of the ids' places: no atomics on values, the
-// same bits each time.
+// An id outside the table (a place of a padded batch) reads zeros and adds to no row.  The gradient writes every row of the table, those
+// without ids as zeros, and adds in the order of the ids' places (a row of more than kLong ids in parts of that order): no atomics on
+// values, the same bits each time.
 //
 // For that the ids are sorted, stable.  Up to kPickMost ids each workgroup, which owns a range of the table's rows, reads all ids,
-// keeps those of its range in LDS in their order and sorts them there: one launch.  More are sorted by digits first (a
-// histogram of each workgroup's ids, their prefixes, and a scatter that keeps the order, for every digit), and a workgroup finds its range in them.
-// Where a row has hundreds of ids, whole runs of kChunk of them are added up beforehand, all over the chip, and a workgroup's waves
-// share what is left.
+// keeps those of its range in LDS in their order and sorts them there: one launch.  More are sorted by digits first (a histogram of each workgroup's ids, their prefixes, and a scatter that keeps the
+// order, for every digit), and a workgroup finds its range in them.  Where a row has hundreds of ids, whole runs of kChunk of them are
+// added up beforehand, all over the chip, and a workgroup's waves share what is left.
+//
+// Memory bounds the lookup: 109 074 of 2.4 million rows of 100 in fp32, 87 MB both ways, in 19.5 us.  The gradient of a million ids of
+// 250 000 rows of 256 in bf16, 512 MB read and 128 written: digits 45 us, runs 85, sums and zeros 102 to 122 (rows of 512 bytes at random
+// places: latency, and few bytes at a time).
 #include "rows.hpp"
 
 namespace f2cgt {
@@ -304,8 +307,8 @@ __device__ __forceinline__ uint32_t begin_of(const uint2* pairs, uint32_t lo, ui
   return lo;
 }
 
-// Where each row's ids begin among the sorted ones (the last entry: where those outside the table do): a wave looks for the first of its
-// 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the chunks that are of
+// Where each row's ids begin among the sorted ones (the last entry: where those outside the table do): a wave looks for the first of
+// its 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the chunks that are of
 // one row: a wave a chunk and slice, whose lanes share the chunk where the slice has few pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint32_t* starts, uint32_t search_blocks) {
@@ -414,17 +417,20 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
   // Some rows to a group of lanes at a time, whose first two ids are all on their way at once: most rows have no more.
   constexpr int kRows = ROWS, kFirst = 2;
   typedef typename piece_words<T, V>::type words;
-  for (uint32_t l0 = (uint32_t)(wave * groups + lane / lanes) * kRows; l0 < few; l0 += (uint32_t)(kWaves * groups * kRows)) {
+  const uint32_t apart = (uint32_t)(kWaves * groups);
+  for (uint32_t l0 = (uint32_t)(wave * groups + lane / lanes); l0 < few; l0 += apart * kRows) {
     uint32_t r[kRows], s[kRows], e[kRows];
     words w[kRows][kFirst];
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
-      r[q] = lists.rows[l0 + q < few ? l0 + q : few - 1];
+      const uint32_t l = l0 + q * apart;
+      r[q] = lists.rows[l < few ? l : few - 1];
       s[q] = start[r[q]] - skipped;
-      e[q] = start[r[q] + 1] - skipped;
+      e[q] = l < few ? start[r[q] + 1] - skipped : s[q];
 #pragma unroll
       for (int u = 0; u < kFirst; ++u)          // (the first one twice where there is no second)
-        w[q][u] = *reinterpret_cast<const words*>(static_cast<const T*>(a.grad) + at + (int64_t)place_in(places[s[q] + u < e[q] ? s[q] + u : s[q]]) * a.ld);
+        w[q][u] = *reinterpret_cast<const words*>(static_cast<const T*>(a.grad) + at +
+                                                  (int64_t)place_in(places[s[q] + u < e[q] ? s[q] + u : s[q]]) * a.ld);
     }
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
@@ -438,7 +444,7 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
       if (s[q] + kFirst < e[q]) add_rows<T, V, 8>(v, a, places, s[q] + kFirst, e[q], at);
 #pragma unroll
       for (int x = 0; x < V; ++x) v[x] *= a.scale;
-      if (sub < here && l0 + q < few) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r[q]) * a.d + at, v);
+      if (sub < here && l0 + q * apart < few) store_piece<T, V>(static_cast<T*>(a.out) + (int64_t)(row0 + r[q]) * a.d + at, v);
     }
   }
   // Of a row with many ids each group of lanes has a share, in the groups' order.
@@ -481,15 +487,16 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
 }
 
 // From sorted ids.
-constexpr int kRangeSorted = 64, kSumThreads = 256;
+constexpr uint32_t kRangeSorted = 64;        // rows of a workgroup, at most
+constexpr int kSumThreads = 256;
 template <typename T, int V>
 __global__ __launch_bounds__(kSumThreads) void sorted_sums_kernel(SumArgs a, const uint32_t* starts) {
   constexpr uint32_t kNear = 1024;             // places of the range, brought near where they fit: a round trip less for each row
   __shared__ uint32_t start[kRangeSorted + 1], few[kRangeSorted], counts[2], near[kNear];
   __shared__ float room[kSumThreads * V];
-  const uint32_t range = blockIdx.x / a.slices, row0 = range * kRangeSorted;
+  const uint32_t range = blockIdx.x / a.slices, row0 = range * a.range;
   const int slice = (int)(blockIdx.x - range * a.slices);
-  const uint32_t count = a.rows - row0 < kRangeSorted ? a.rows - row0 : kRangeSorted;
+  const uint32_t count = a.rows - row0 < a.range ? a.rows - row0 : a.range;
   if (threadIdx.x < 2) counts[threadIdx.x] = 0;
   if (threadIdx.x <= count) start[threadIdx.x] = starts[row0 + threadIdx.x];
   __syncthreads();
@@ -615,6 +622,10 @@ __global__ __launch_bounds__(kPickThreads, 8) void picked_sums_kernel(SumArgs a)
   sum_range<T, V, kPickThreads, 1, 8>(a, row0, count, slice, start, sorted, 0, false, lists, reinterpret_cast<float*>(lds));
 }
 
+// Whether ids are picked rather than sorted: up to as many as LDS is laid out for (11264 of 100000 x 128 in fp32 18 us, sorted 39), but not
+// thousands of one to three rows, which are a workgroup's each (16384 of one row of 128 113 us, sorted 33; 4000 31 and 31).
+bool picks(int64_t n, int64_t rows) { return n <= kPickMost && (n <= 4096 || rows >= 4); }
+
 // Digits of the sort: as few as keys of rows + 1 values need, of one width.
 void digits_of(int64_t rows, int& passes, int& bits) {
   const int all = bits_of((uint32_t)rows);
@@ -661,10 +672,16 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   const char* what = "embedding_grad";
   a.pieces = (int)ceil_div(a.d, V);
   a.slices = (int)ceil_div(a.pieces, kWave);
-  if (a.n <= kPickMost) {
-    // two workgroups' worth of ranges for each CU at least, of no more rows than LDS has counters for
-    const int64_t want = ceil_div((int64_t)a.rows * a.slices, 2 * num_cus());
-    a.range = (uint32_t)(want < 16 ? 16 : want > kRangePicked ? kRangePicked : want);
+  if (picks(a.n, a.rows)) {
+    // A workgroup for each CU, since each reads all ids: 16384 ids of 20000 x 128 in fp32 12.3 us, with two for each 19.7, 1000 of them 10.4
+    // and 14.0.  Two where zeros are most of it (11264 of 300000 x 128 in fp32, 600 KB a CU, 34.5 us, with one 44.2; of 100000 x 128 with
+    // hot ids 21.3 and 22.8, but where LDS has no room for both, 16384 of them, 31.2 and 27.1), and where LDS has no counters for a
+    // CU's rows.
+    const int64_t cus = num_cus(), one = ceil_div((int64_t)a.rows * a.slices, cus), two = ceil_div((int64_t)a.rows * a.slices, 2 * cus);
+    const uint32_t range = (uint32_t)(two > kRangePicked ? kRangePicked : two);
+    const bool both = 2 * PickRoom((uint32_t)a.n, range, V).all <= 160 * 1024;
+    const bool alone = one <= kRangePicked && (int64_t)a.rows * a.d * (int64_t)sizeof(T) <= cus * (both ? 131072 : 262144);
+    a.range = alone ? (uint32_t)one : range;
     const int64_t blocks = ceil_div(a.rows, a.range) * a.slices;
     F2CGT_REQUIRE(blocks < (1ll << 22), F2CGT_E_UNSUPPORTED, "%s: too many rows for a launch", what);
     const uint32_t lds = PickRoom((uint32_t)a.n, a.range, V).all;
@@ -679,7 +696,10 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   const Room room(a.n, a.rows, a.d);
   int passes, bits;
   digits_of(a.rows, passes, bits);
-  const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div(a.rows, kRangeSorted) * a.slices;
+  // fewer rows to a workgroup until there are four for each CU: 40000 ids of 1000 x 128 in fp32 29 us, of 64 rows each 104
+  a.range = kRangeSorted;
+  while (a.range > 4 && ceil_div((int64_t)a.rows, a.range) * a.slices < 4 * num_cus()) a.range /= 2;
+  const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div((int64_t)a.rows, a.range) * a.slices;
   const int64_t chunk_blocks = ceil_div(a.n / kChunk * a.slices, 4);
   F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
   uint2* pairs = reinterpret_cast<uint2*>(workspace);
@@ -737,7 +757,7 @@ extern "C" int f2cgt_embedding(const void* table, int dtype, int64_t ld, const v
 }
 
 extern "C" int64_t f2cgt_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t d) {
-  if (n <= kPickMost || rows <= 0 || d <= 0 || n >= (1ll << 31) || rows >= (1ll << 31)) return 0;
+  if (rows <= 0 || picks(n, rows) || d <= 0 || n >= (1ll << 31) || rows >= (1ll << 31)) return 0;
   const Room room(n, rows, d);
   return room.sorted + room.counts + room.starts + room.chunks;
 }

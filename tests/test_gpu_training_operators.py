@@ -172,3 +172,21 @@ def test_a_captured_training_step():
         seed.mul_(-0.5)
         with torch.no_grad():
             rows.weight.add_(0.125)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 17, 63, 65, 255, 257, 300, 511, 513, 700, 4100])
+@pytest.mark.parametrize("n", [1, 90, 4096, 4097, 16384, 16385, 40000])
+def test_tables_of_each_size(n, rows):
+    """Ranges of a workgroup from one row up, and the sizes at which ids are sorted rather than picked."""
+    lib = f2cgt_amd.load()
+    g = _gen(n + rows)
+    for d, dtype in ((36, torch.float32), (300, torch.bfloat16)):
+        ids = torch.randint(-1, rows, (n,), generator=g, device="cuda")
+        grad = torch.randint(-3, 4, (n, d), generator=g, device="cuda")
+        grad[ids < 0] = 0
+        order = torch.argsort(ids)
+        lengths = torch.bincount(ids[ids >= 0], minlength=rows)
+        keep = order[int((ids < 0).sum()):]
+        want = torch.segment_reduce(grad[keep].double(), "sum", lengths=lengths, axis=0, initial=0.0)
+        # (sums of whole numbers below 2^24, rounded once)
+        assert torch.equal(lib.embedding_grad(grad.to(dtype), ids, rows), want.to(dtype))
