@@ -4,9 +4,13 @@
 // unpack: code 2^(E - 127)
 // grad:   dW = g^T v, db = sum of g's rows, for a layer out = v W^T + b whose input v is held as codes
 //
-// Pack and unpack are bound by memory.  The product goes through bf16 matrix instructions: every v is a bf16 exactly, and g is one
-// bf16 plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the other, exactly), so all
-// products are exact and only the fp32 sums round.
+// Pack and unpack are bound by memory: 250 000 x 100 in fp32 31 to 33 us (126 MB, 4 TB/s) and 20.5 (6.1 TB/s), 262 144 x 128 5.8 TB/s
+// either way, in 16 bits 4.8 and 6.1.  The product goes through bf16 matrix instructions: every v is a
+// bf16 exactly, and g is one bf16 plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the
+// other, exactly), so all products are exact and only the fp32 sums round.  Large ones are bound by the matrix instructions at the card's
+// power cap (16 384 x 4096 -> 4096 in bf16 500 to 550 us, 1.0 to 1.1e15 operations a second, 56 % of the clocks in which the CUs have waves; a
+// library's product of bf16 operands in this layout 558), long sums for few outputs by splitting into planes and placing them (60 001 x
+// 602 -> 128 in fp32 41 us, of which its matrix instructions are 41 %), small ones by a launch and latency (1024 x 128 -> 256 6.8 us).
 #include "rows.hpp"
 #include "tile_product.hpp"
 
@@ -207,7 +211,7 @@ template <typename T> struct Eight {
 typedef uint32_t word_any __attribute__((aligned(1)));
 
 // A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step; GROUPS groups of waves take the steps in turn and
-// add their sums in the end.  Rows lie in LDS as they do in memory, one line of BN or BK bf16 a row, and matrix operands, which hold
+// add their sums in the end (two groups on 128 squared, for eight waves on a CU).  Rows lie in LDS as they do in memory, one line of BN or BK bf16 a row, and matrix operands, which hold
 // eight rows of one column a lane, are read through the transposing LDS loads: sixteen lanes give the addresses of 4 rows x 16
 // columns in four pieces a row, and get a column each.  Units of 64 bytes of a line change places by the row's last two bits, so the four
 // rows of such a read lie in different banks.
@@ -266,8 +270,9 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   const uint32_t off_e = (uint32_t)(rx * a.groups + cx / kCheckpointGroup);
   typedef typename Tile::Held Held;
 
-  // A piece that runs over its row's end reads on in the next one, and four exponents at a time, of which the first counts, in the next ones: the
-  // steps of the last four rows are not among these.  (Of a single exponent's byte the compiler makes a word where the loop ends, behind a wait.)
+  // A piece that runs over its row's end reads on in the next one, and four exponents at a time, of which the first counts, in the next
+  // ones: the steps of the last four rows are not among these.  (Of a single exponent's byte the compiler makes a word where the loop
+  // ends, behind a wait.)
   const int64_t whole = a.n >= 8 && a.m > 4 ? (a.m - 4) / BM : 0;
   const int64_t rounds = (whole < to ? (whole > from ? whole - from : 0) : to - from) / GROUPS, end = from + rounds * GROUPS;
   // Pieces of one of kParts parts of a step into registers.
@@ -380,7 +385,8 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[s & 1][p][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TJ; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fg[s & 1][p][i], fx[s & 1][j], acc[i][j], 0, 0, 0);
   };
   // A group's step s is multiplied out of stage s % 2 while its next one goes from registers into the other stage, a part at a time, and the
   // registers of each part take the step after that: its loads have a whole round for their way.  (One copy of the round, and no branch in
@@ -719,7 +725,8 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
   const bool few = c.splits <= 8;
   const int outs = few ? 1024 : n * k <= 64 * (int64_t)num_cus() ? 64 : 256;
   F2CGT_REQUIRE(ceil_div(n * k, outs) < (1ll << 21), F2CGT_E_UNSUPPORTED, "%s: too many outputs", what);
-  const JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype, (uint32_t)c.splits, (uint32_t)ceil_div(n * k, outs)};
+  const JoinArgs j{static_cast<const float*>(workspace), dweight, dbias, n * k, (int)n, out_dtype, (uint32_t)c.splits,
+                   (uint32_t)ceil_div(n * k, outs)};
   const dim3 join_grid(j.blocks + (dbias ? (unsigned)ceil_div(n, outs) : 0u));
   if (few) join_splits_kernel<4, 1, 4><<<join_grid, dim3(256), 0, st>>>(j);
   else if (outs == 64) join_splits_kernel<16, 16, 1><<<join_grid, dim3(1024), 0, st>>>(j);

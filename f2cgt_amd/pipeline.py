@@ -9,7 +9,9 @@ place of DGL blocks, ShmTensor and torch.distributed (one process, one GPU):
   * `CompressionManager` (examples/compress.py:8-106): keeps the code tables and codebooks,
     serves seed rows (first level) and neighbour rows (second level);
   * `MySAGEConv` (examples/conv.py:9-76): GraphSAGE mean layer whose neighbour aggregation is the
-    fused decompress + mean operator.
+    fused decompress + mean operator;
+  * beyond the reference, for training and serving what is built on these: `Muon`, `LayerNorm`, `PackedLinear`
+    (activations kept in 8 bits for the backward pass), `NodeEmbedding` (learnt rows) and `Int8Linear`.
 
 Everything numerical happens in `F2CGTLib` (f2cgt_amd.load()); this module only moves tensors.
 """
@@ -897,7 +899,8 @@ class LayerNorm(nn.LayerNorm):
     """`nn.LayerNorm` over the last dimension of rows on the GPU: one launch forward (and no statistics kept without gradients),
     two backward.  With `packed` the backward pass keeps an 8-bit checkpoint of the input in place of the input itself, a
     fourth of the memory (half for 16-bit inputs): its gradients are those at the decoded input, whose values are off by
-    up to 1/127 of the largest among the 32 columns around them.  Parameters in float32 or in the inputs' type; state as `nn.LayerNorm`'s."""
+    up to 1/127 of the largest among the 32 columns around them.  Parameters in float32 or in the inputs' type; state as
+    `nn.LayerNorm`'s.  Once differentiable."""
 
     def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True, packed=False, device=None, dtype=None):
         super().__init__(features, eps, elementwise_affine, bias, device=device, dtype=dtype)
@@ -935,8 +938,8 @@ class _PackedLinear(torch.autograd.Function):
 
 class PackedLinear(nn.Linear):
     """An `nn.Linear` whose backward pass keeps its input as an 8-bit checkpoint (`pack_activations`): a fourth of the memory
-    of float32 inputs, half of 16-bit ones.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the one at the decoded
-    input.  `PackedLinear.of(linear)` shares a layer's parameters."""
+    of float32 inputs, half of 16-bit ones.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the
+    one at the decoded input.  `PackedLinear.of(linear)` shares a layer's parameters.  Once differentiable."""
 
     @classmethod
     def of(cls, linear):

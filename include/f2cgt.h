@@ -478,9 +478,8 @@ int f2cgt_layer_norm_grad(const void* grad, int dtype, int64_t grad_ld, const vo
  * readable, here and below.
  *
  * f2cgt_packed_linear_grad: dweight [n, k] = grad^T values and, where not NULL, dbias [n] = sums of grad's columns, dense, of out_dtype;
- * grad [m, n] of dtype, rows ld apart.  Products are exact (parts
- * of fp32 gradients below 2^-126 count as zeros), sums fp32 in a fixed order.  An infinity in grad gives NaN in its row
- * of dweight.  workspace: f2cgt_packed_linear_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
+ * grad [m, n] of dtype, rows ld (below 2^24) apart.  Products are exact (parts of fp32 gradients below 2^-126 count as zeros), sums
+ * fp32 in a fixed order.  An infinity in an fp16 or fp32 grad gives NaN in its row of dweight.  workspace: f2cgt_packed_linear_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
 int f2cgt_pack_activations(const void* x, int dtype, int64_t ld, int8_t* codes, int64_t code_stride, uint8_t* exponents,
                            int64_t m, int64_t k, void* stream);
 int f2cgt_unpack_activations(const int8_t* codes, int64_t code_stride, const uint8_t* exponents, void* out, int dtype, int64_t m,
@@ -496,9 +495,9 @@ int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld, const int8
  * elsewhere in this file an id outside [0, rows) is no row (a place of a padded batch): zeros, and no gradient.
  *
  * f2cgt_embedding: out [n, d] (dense) = scale * table[index], table [rows, d] with rows ld values apart.
- * f2cgt_embedding_grad: dtable [rows, d] (dense, of grad's type), every row written: scale times the sum, in the order of their places and in
- * fp32, of the rows of grad [n, d] (ld apart) whose id it is.  Rows with up to 64 ids are added one after the other, longer ones in
- * parts that the sizes and ids fix.  workspace: f2cgt_embedding_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
+ * f2cgt_embedding_grad: dtable [rows, d] (dense, of grad's type), every row written: scale times the sum, in the order of their places
+ * and in fp32, of the rows of grad [n, d] (ld apart) whose id it is.  Rows with up to 64 ids are added one after the other, longer ones
+ * in parts that the sizes and ids fix.  workspace: f2cgt_embedding_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
 int f2cgt_embedding(const void* table, int dtype, int64_t ld, const void* index, int idx_dtype, void* out, float scale, int64_t n,
                     int64_t rows, int64_t d, void* stream);
 int64_t f2cgt_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t d);
