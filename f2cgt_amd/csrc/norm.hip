@@ -458,14 +458,19 @@ __global__ __launch_bounds__(1024) void join_sums_kernel(JoinArgs a) {
 }
 
 // f(piece values, lanes, pieces a lane) for the width d: few lanes to a short row, so that a workgroup has several rows; as many as a row
-// has pieces to a long one.  Measured, GB/s of what is read and written, forward and backward: 32 lanes with three pieces rather than 64
-// with two up to 96 pieces (111476 x 602 in bf16 5470 and 4300 against 4760 and 3530), 4 rather than 8 up to four (1048576 x 16 in fp32
-// 5830 and 5000 against 4400 and 4880), 192 rather than 256 in 16 bits (65154 x 1030 in bf16 3850 and 3840 against 3270 and 3465); 384 and
-// 768 lose to the powers of two, since a CU holds two or one (22369 x 1500 in fp32 4850 and 4400 against 5300 and 4820).  Four pieces to
-// each of 1024 lanes rather than the kernels for long rows (2048 x 16384 in fp32 5560 and 4000 against 3290 and 2530); with 16 bits that
-// would be 32 values a lane, beyond the registers of the backward pass.
+// has pieces to a long one.  Where those would be a power of two of which many have no piece, three pieces a lane.  Measured, GB/s of
+// what is read and written, forward and backward:
+//   up to four pieces 4 lanes rather than 8: 1048576 x 16 in fp32 5830 and 5000 against 4400 and 4880;
+//   up to 96 32 x 3 rather than 64 x 2: 111476 x 602 in bf16 5470 and 4300 against 4760 and 3530;
+//   up to 192 64 x 3 forward (65154 x 1030 in bf16 5250, with 192 lanes 3850, with 256 3270), backward the same in fp32, in 16 bits, where
+//   three pieces are 24 values a lane, 192 lanes (3840, with 256 3465);
+//   up to 384 and 768 128 x 3 and 256 x 3 forward (32577 x 1030 in fp32 5800 against 4090, 31956 x 2100 in bf16 5020 against 3250), but
+//   not backward, where rows and sums of three pieces leave a CU few waves (22369 x 1500 in fp32 3930 against 4820); workgroups of 384
+//   and 768 lanes lose to both, since a CU holds two or one;
+//   up to 4096 in fp32 1024 x 4 rather than the kernels for long rows: 2048 x 16384 5560 and 4000 against 3290 and 2530 (in 16 bits that
+//   would be 32 values a lane, beyond the registers of the backward pass).
 template <int N> struct count_of { static constexpr int value = N; };
-template <typename T, typename F>
+template <typename T, bool FORWARD, typename F>
 bool with_geometry(int64_t d, const F& f) {
   constexpr int V = kPieceOf<T>;
   const int64_t pieces = ceil_div(d, V);
@@ -477,11 +482,18 @@ bool with_geometry(int64_t d, const F& f) {
   else if (pieces <= 64) f(count_of<V>{}, count_of<64>{}, count_of<1>{});
   else if (pieces <= 96) f(count_of<V>{}, count_of<32>{}, count_of<3>{});
   else if (pieces <= 128) f(count_of<V>{}, count_of<64>{}, count_of<2>{});
-  else if (V == 4 && pieces <= 192) f(count_of<V>{}, count_of<64>{}, count_of<3>{});
-  else if (pieces <= 192) f(count_of<V>{}, count_of<192>{}, count_of<1>{});
-  else if (pieces <= 256) f(count_of<V>{}, count_of<256>{}, count_of<1>{});
-  else if (pieces <= 512) f(count_of<V>{}, count_of<512>{}, count_of<1>{});
-  else if (pieces <= 1024) f(count_of<V>{}, count_of<1024>{}, count_of<1>{});
+  else if (pieces <= 192) {
+    if constexpr (V == 4 || FORWARD) f(count_of<V>{}, count_of<64>{}, count_of<3>{});
+    else f(count_of<V>{}, count_of<192>{}, count_of<1>{});
+  } else if (pieces <= 256) f(count_of<V>{}, count_of<256>{}, count_of<1>{});
+  else if (pieces <= 384) {
+    if constexpr (FORWARD) f(count_of<V>{}, count_of<128>{}, count_of<3>{});
+    else f(count_of<V>{}, count_of<512>{}, count_of<1>{});
+  } else if (pieces <= 512) f(count_of<V>{}, count_of<512>{}, count_of<1>{});
+  else if (pieces <= 768) {
+    if constexpr (FORWARD) f(count_of<V>{}, count_of<256>{}, count_of<3>{});
+    else f(count_of<V>{}, count_of<1024>{}, count_of<1>{});
+  } else if (pieces <= 1024) f(count_of<V>{}, count_of<1024>{}, count_of<1>{});
   else if (pieces <= 2048) f(count_of<V>{}, count_of<1024>{}, count_of<2>{});
   else if constexpr (V == 4) {
     if (pieces > 4096) return false;
@@ -501,8 +513,8 @@ BlockOf block_for(int64_t d, int size) {
     b.block = block_of(decltype(lanes)::value);
     b.rows = b.block / decltype(lanes)::value;
   };
-  if (size == 4) with_geometry<float>(d, count);
-  else with_geometry<__bf16>(d, count);
+  if (size == 4) with_geometry<float, false>(d, count);
+  else with_geometry<__bf16, false>(d, count);
   return b;
 }
 
@@ -561,7 +573,7 @@ extern "C" int f2cgt_layer_norm(const void* x, int dtype, int64_t ld, const void
       if (codes) layer_norm_kernel<T, V, L, C, true><<<grid, block, 0, st>>>(a);
       else layer_norm_kernel<T, V, L, C, false><<<grid, block, 0, st>>>(a);
     };
-    if (!with_geometry<T>(d, launch)) {
+    if (!with_geometry<T, true>(d, launch)) {
       const dim3 grid((unsigned)(m < 2 * num_cus() ? m : 2 * num_cus()));
       if (codes) layer_norm_long_kernel<T, true><<<grid, dim3(1024), 0, st>>>(a);
       else layer_norm_long_kernel<T, false><<<grid, dim3(1024), 0, st>>>(a);
@@ -610,7 +622,7 @@ extern "C" int f2cgt_layer_norm_grad(const void* grad, int dtype, int64_t grad_l
         if (codes) layer_norm_grad_kernel<T, V, L, C, true><<<grid, block, 0, st>>>(a);
         else layer_norm_grad_kernel<T, V, L, C, false><<<grid, block, 0, st>>>(a);
       };
-      if (!with_geometry<T>(d, launch)) {
+      if (!with_geometry<T, false>(d, launch)) {
         const dim3 grid((unsigned)(m < 2 * num_cus() ? m : 2 * num_cus())), columns((unsigned)ceil_div(d, 256), (unsigned)blocks);
         if (codes) layer_norm_grad_long_kernel<T, true><<<grid, dim3(1024), 0, st>>>(a);
         else layer_norm_grad_long_kernel<T, false><<<grid, dim3(1024), 0, st>>>(a);
