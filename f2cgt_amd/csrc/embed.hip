@@ -292,6 +292,15 @@ __device__ __forceinline__ void add_chunks(float (&v)[V], const SumArgs& a, uint
   }
 }
 
+// Sums over the groups of `lanes` lanes of a wave, in all of them.  (One group after the other, by way of LDS, a workgroup's 256
+// took 23 us.)
+template <int V>
+__device__ __forceinline__ void sum_shares(float (&v)[V], int lanes) {
+  for (int by = lanes; by < kWave; by *= 2)
+#pragma unroll
+    for (int x = 0; x < V; ++x) v[x] += __shfl_xor(v[x], by);
+}
+
 // Where keys of at least `key` begin in the sorted ones from lo to hi, by the 64 lanes of a wave: 64 parts at a time.
 __device__ __forceinline__ uint32_t begin_of(const uint2* pairs, uint32_t lo, uint32_t hi, uint32_t key) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
@@ -325,7 +334,6 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
     if (r <= a.rows) starts[r] = lo;
     return;
   }
-  __shared__ float room[4][kWave * V];
   __shared__ uint32_t near[4][kChunk];
   const int64_t item = (int64_t)(blockIdx.x - search_blocks) * 4 + threadIdx.x / kWave;
   const int64_t chunk = item / a.slices;
@@ -349,15 +357,7 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   float v[V] = {};
   const uint32_t each = kChunk / shares;
   add_rows<T, V, 8>(v, a, places, share * each, share * each + each, at);
-  float* mine = room[threadIdx.x / kWave];
-  if (shares > 1) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) mine[e * kWave + lane] = v[e];
-    __builtin_amdgcn_wave_barrier();
-    for (int s = 1; s < shares; ++s)
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] += share == 0 ? mine[e * kWave + s * lanes + sub] : 0.f;
-  }
+  sum_shares<V>(v, lanes);
   if (share != 0 || sub >= here) return;
   float* to = a.chunks + chunk * a.d + at;
 #pragma unroll
@@ -461,18 +461,19 @@ __device__ __forceinline__ void sum_range(const SumArgs& a, uint32_t row0, uint3
       add_chunks<V>(v, a, part(c0, c1, share), part(c0, c1, share + 1), at);
       add_rows<T, V, LONG_UNROLL>(v, a, places, part(tail, e, share) - skipped, part(tail, e, share + 1) - skipped, at);
     }
+    sum_shares<V>(v, lanes);
     __syncthreads();                           // (the row before is done with the room)
+    if (lane < lanes)
 #pragma unroll
-    for (int x = 0; x < V; ++x) room[(wave * V + x) * kWave + lane] = v[x];
+      for (int x = 0; x < V; ++x) room[(wave * V + x) * kWave + lane] = v[x];
     __syncthreads();
     if (wave == 0 && lane < here) {
-      // (piece `lane` in each share)
 #pragma unroll
       for (int x = 0; x < V; ++x) v[x] = 0.f;
+#pragma unroll 4
       for (int w = 0; w < kWaves; ++w)
-        for (int g = 0; g < groups; ++g)
 #pragma unroll
-          for (int x = 0; x < V; ++x) v[x] += room[(w * V + x) * kWave + g * lanes + lane];
+        for (int x = 0; x < V; ++x) v[x] += room[(w * V + x) * kWave + lane];
 #pragma unroll
       for (int x = 0; x < V; ++x) v[x] *= a.scale;
       // (a piece that was moved back leaves the columns of the one before to that: another slice may share the row otherwise)
