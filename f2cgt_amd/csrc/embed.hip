@@ -236,7 +236,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortArgs a) 
 }
 
 // ---- sums over a row's gradients --------------------------------------------------------------------------
-constexpr int kChunk = 128;                  // ids of one row whose sum is made beforehand
+// ids of one row whose sum is made beforehand (64 are faster for few ids, but not where a chunk is four waves', and slower for many: the
+// million above 293 us)
+constexpr int kChunk = 128;
 constexpr uint32_t kLong = 64;               // ids of a row above which a workgroup's waves share them
 
 struct SumArgs {
@@ -248,6 +250,7 @@ struct SumArgs {
   int64_t n, ld;
   uint32_t rows, range;      // range: rows of a workgroup
   int d, pieces, slices;     // slices: parts of 64 pieces of a row, a workgroup each
+  int spread;                // waves of a chunk and slice, 1 or 4
   int sparse;                // most rows have no ids: zeros into all of them before anything else
   float scale;
 };
@@ -318,7 +321,7 @@ __device__ __forceinline__ uint32_t begin_of(const uint2* pairs, uint32_t lo, ui
 
 // Where each row's ids begin among the sorted ones (the last entry: where those outside the table do): a wave looks for the first of
 // its 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the chunks that are of
-// one row: a wave a chunk and slice, whose lanes share the chunk where the slice has few pieces.
+// one row: a wave a chunk and slice (or four), whose lanes share the chunk where the slice has few pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint32_t* starts, uint32_t search_blocks) {
   if (blockIdx.x < search_blocks) {
@@ -335,7 +338,9 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
     return;
   }
   __shared__ uint32_t near[4][kChunk];
-  const int64_t item = (int64_t)(blockIdx.x - search_blocks) * 4 + threadIdx.x / kWave;
+  __shared__ float room[4][V][kWave];
+  const int wave = threadIdx.x / kWave, quarter = a.spread == 4 ? wave : 0;
+  const int64_t item = (int64_t)(blockIdx.x - search_blocks) * (4 / a.spread) + (a.spread == 4 ? 0 : wave);
   const int64_t chunk = item / a.slices;
   const int slice = (int)(item - chunk * a.slices), lane = threadIdx.x & (kWave - 1);
   if (chunk >= a.n / kChunk) return;
@@ -344,7 +349,7 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   const uint2 mine_low = a.pairs[first + lane], mine_high = a.pairs[first + kWave + lane];
   const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine_low.x);
   if (key != (uint32_t)__builtin_amdgcn_readlane((int)mine_high.x, kWave - 1) || key >= a.rows) return;
-  uint32_t* places = near[threadIdx.x / kWave];              // (within a wave: LDS keeps its order)
+  uint32_t* places = near[wave];               // (within a wave: LDS keeps its order)
   places[lane] = mine_low.y;
   places[kWave + lane] = mine_high.y;
   __builtin_amdgcn_wave_barrier();
@@ -355,9 +360,19 @@ __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint3
   const int p = slice * kWave + (sub < here ? sub : here - 1);
   const int at = p * V + V > a.d ? a.d - V : p * V;
   float v[V] = {};
-  const uint32_t each = kChunk / shares;
-  add_rows<T, V, 8>(v, a, places, share * each, share * each + each, at);
+  const uint32_t all = shares * a.spread, mine = quarter * shares + share;      // (up to 256 shares of the 128)
+  add_rows<T, V, 8>(v, a, places, kChunk * mine / all, kChunk * (mine + 1) / all, at);
   sum_shares<V>(v, lanes);
+  if (a.spread == 4) {                         // (the workgroup has one item: all of it is here)
+#pragma unroll
+    for (int e = 0; e < V; ++e) room[wave][e][lane] = v[e];
+    __syncthreads();
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += room[w][e][lane];
+    if (wave != 0) return;
+  }
   if (share != 0 || sub >= here) return;
   float* to = a.chunks + chunk * a.d + at;
 #pragma unroll
@@ -701,7 +716,10 @@ int launch_grad(SumArgs a, int idx_dtype, char* workspace, hipStream_t st) {
   a.range = kRangeSorted;
   while (a.range > 4 && ceil_div((int64_t)a.rows, a.range) * a.slices < 4 * num_cus()) a.range /= 2;
   const int64_t blocks = ceil_div(a.n, kSortTile), sums = ceil_div((int64_t)a.rows, a.range) * a.slices;
-  const int64_t chunk_blocks = ceil_div(a.n / kChunk * a.slices, 4);
+  // Four waves to a chunk where the chunks alone are few: 26 906 hot ids of 82 859 x 152 in fp32 62 us, with one 98.
+  const int64_t items = a.n / kChunk * a.slices;
+  a.spread = items < 16 * num_cus() ? 4 : 1;
+  const int64_t chunk_blocks = ceil_div(items * a.spread, 4);
   F2CGT_REQUIRE(sums < (1ll << 23) && chunk_blocks < (1ll << 23), F2CGT_E_UNSUPPORTED, "%s: too many values for a launch", what);
   uint2* pairs = reinterpret_cast<uint2*>(workspace);
   const int64_t each = ceil_div(a.n, 2) * 2;
@@ -777,7 +795,7 @@ extern "C" int f2cgt_embedding_grad(const void* grad, int dtype, int64_t ld, con
   const int64_t need = f2cgt_embedding_grad_workspace_bytes(n, rows, d);
   F2CGT_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), F2CGT_E_INVALID,
                 "%s: workspace too small or misaligned", what);
-  const SumArgs a{grad, index, nullptr, nullptr, dtable, n, ld, (uint32_t)rows, 0, (int)d, 0, 0, rows > n, scale};
+  const SumArgs a{grad, index, nullptr, nullptr, dtable, n, ld, (uint32_t)rows, 0, (int)d, 0, 0, 1, rows > n, scale};
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     if (d >= kPieceOf<T>) return launch_grad<T, kPieceOf<T>>(a, idx_dtype, static_cast<char*>(workspace), as_stream(stream));
