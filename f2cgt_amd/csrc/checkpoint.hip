@@ -5,12 +5,12 @@
 // grad:   dW = g^T v, db = sum of g's rows, for a layer out = v W^T + b whose input v is held as codes
 //
 // Pack and unpack are bound by memory: 250 000 x 100 in fp32 31 to 33 us (126 MB, 4 TB/s) and 20.5 (6.1 TB/s), 262 144 x 128 5.8 TB/s
-// either way, in 16 bits 4.8 and 6.1.  The product goes through bf16 matrix instructions: every v is a
-// bf16 exactly, and g is one bf16 plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the
-// other, exactly), so all products are exact and only the fp32 sums round.  Large ones are bound by the matrix instructions at the card's
-// power cap (16 384 x 4096 -> 4096 in bf16 500 to 550 us, 1.0 to 1.1e15 operations a second, 56 % of the clocks in which the CUs have waves; a
-// library's product of bf16 operands in this layout 558), long sums for few outputs by splitting into planes and placing them (60 001 x
-// 602 -> 128 in fp32 41 us, of which its matrix instructions are 41 %), small ones by a launch and latency (1024 x 128 -> 256 6.8 us).
+// either way, in 16 bits 4.8 and 6.1.  The product goes through bf16 matrix instructions: every v is a bf16 exactly, and g is one bf16
+// plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the other, exactly), so all
+// products are exact and only the fp32 sums round.  Large ones are bound by the matrix instructions at the card's power cap (16 384 x
+// 4096 -> 4096 in bf16 500 to 550 us, 1.0 to 1.1e15 operations a second, 56 % of the clocks in which the CUs have waves; a library's
+// product of bf16 operands in this layout 558), long sums for few outputs by splitting into planes and placing them (60 001 x 602 ->
+// 128 in fp32 41 us, of which its matrix instructions are 41 %), small ones by a launch and latency (1024 x 128 -> 256 6.8 us).
 #include "rows.hpp"
 #include "tile_product.hpp"
 
@@ -210,11 +210,11 @@ template <typename T> struct Eight {
 
 typedef uint32_t word_any __attribute__((aligned(1)));
 
-// A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step; GROUPS groups of waves take the steps in turn and
-// add their sums in the end (two groups on 128 squared, for eight waves on a CU).  Rows lie in LDS as they do in memory, one line of BN or BK bf16 a row, and matrix operands, which hold
-// eight rows of one column a lane, are read through the transposing LDS loads: sixteen lanes give the addresses of 4 rows x 16
-// columns in four pieces a row, and get a column each.  Units of 64 bytes of a line change places by the row's last two bits, so the four
-// rows of such a read lie in different banks.
+// A tile of dW: BN outputs by BK inputs, WN x WK to a wave, BM rows of g and v a step; GROUPS groups of waves take the steps in turn
+// and add their sums in the end (two groups on 128 squared, for eight waves on a CU).  Rows lie in LDS as they do in memory, one line
+// of BN or BK bf16 a row, and matrix operands, which hold eight rows of one column a lane, are read through the transposing LDS loads:
+// sixteen lanes give the addresses of 4 rows x 16 columns in four pieces a row, and get a column each.  Units of 64 bytes of a line
+// change places by the row's last two bits, so the four rows of such a read lie in different banks.
 template <typename T, int BN, int BK, int WN, int WK, int BM, int GROUPS>
 struct GradTile {
   static constexpr int P = kPlanes<T>;

@@ -2,18 +2,19 @@
 //
 //   out_i = scale * table[id_i]                     dtable_r = scale * sum over i with id_i = r, in their order, of grad_i
 //
-// An id outside the table (a place of a padded batch) reads zeros and adds to no row.  The gradient writes every row of the table, those
-// without ids as zeros, and adds in the order of the ids' places (a row of more than kLong ids in parts of that order): no atomics on
-// values, the same bits each time.
+// An id outside the table (a place of a padded batch) reads zeros and adds to no row.  The gradient writes every row of the table,
+// those without ids as zeros, and adds in the order of the ids' places (a row of more than kLong ids in parts of that order): no
+// atomics on values, the same bits each time.
 //
 // For that the ids are sorted, stable.  Up to kPickMost ids each workgroup, which owns a range of the table's rows, reads all ids,
-// keeps those of its range in LDS in their order and sorts them there: one launch.  More are sorted by digits first (a histogram of each workgroup's ids, their prefixes, and a scatter that keeps the
-// order, for every digit), and a workgroup finds its range in them.  Where a row has hundreds of ids, whole runs of kChunk of them are
-// added up beforehand, all over the chip, and a workgroup's waves share what is left.
+// keeps those of its range in LDS in their order and sorts them there: one launch.  More are sorted by digits first (a histogram of
+// each workgroup's ids, their prefixes, and a scatter that keeps the order, for every digit), and a workgroup finds its range in them.
+// Where a row has hundreds of ids, whole runs of kChunk of them are added up beforehand, all over the chip, and a workgroup's waves
+// share what is left.
 //
 // Memory bounds the lookup: 109 074 of 2.4 million rows of 100 in fp32, 87 MB both ways, in 19.5 us.  The gradient of a million ids of
-// 250 000 rows of 256 in bf16, 512 MB read and 128 written: digits 45 us, runs 85, sums and zeros 102 to 122 (rows of 512 bytes at random
-// places: latency, and few bytes at a time).
+// 250 000 rows of 256 in bf16, 512 MB read and 128 written: digits 45 us, runs 85, sums and zeros 102 to 122 (rows of 512 bytes at
+// random places: latency, and few bytes at a time).
 #include "rows.hpp"
 
 namespace f2cgt {
@@ -320,8 +321,8 @@ __device__ __forceinline__ uint32_t begin_of(const uint2* pairs, uint32_t lo, ui
 }
 
 // Where each row's ids begin among the sorted ones (the last entry: where those outside the table do): a wave looks for the first of
-// its 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the chunks that are of
-// one row: a wave a chunk and slice (or four), whose lanes share the chunk where the slice has few pieces.
+// its 64 rows and the end of the last one, then each lane for its own row in between.  And, in the workgroups behind, sums of the
+// chunks that are of one row: a wave a chunk and slice (or four), whose lanes share the chunk where the slice has few pieces.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void starts_and_chunks_kernel(SumArgs a, uint32_t* starts, uint32_t search_blocks) {
   if (blockIdx.x < search_blocks) {
