@@ -9,8 +9,8 @@
 // workgroups; every order is fixed by the sizes.
 //
 // Memory bounds both.  Where a copy of 4 GB makes 4.8 TB/s: 250 000 x 128 in fp32 forward 46 us (5.6 TB/s of what is read and written;
-// with the call 52), 16 384 x 8192 in bf16 backward 150 us (5.4 TB/s), 60 001 x 602 in fp32 from its checkpoint 69 us (4.7 TB/s); rows
-// longer than that, which are read once a pass, 1.1 to 3.  Few rows are bound by latency: 1 x 4096 takes 2.4 us, 1024 x 256 backward 3.3
+// with the call 52), 16 384 x 8192 in bf16 backward 150 us (5.4 TB/s), 60 001 x 602 in fp32 from its checkpoint 69 us (4.7 TB/s);
+// longer rows, which are read once a pass, 1.1 to 3 TB/s.  Few rows are bound by latency: 1 x 4096 takes 2.4 us, 1024 x 256 backward 3.3
 // and 2.4 for the second kernel.
 #include "rows.hpp"
 
