@@ -482,21 +482,36 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   }
 }
 
-// Sums of a gradient's columns alone, of a layer without inputs.
+// Sums of a gradient's columns alone, of a layer without inputs: sixteen waves with every sixteenth row of 64 columns, a thousand rows of a
+// wave to a part and the parts to a sum.  (One sum for all rows stands still at 2^24 equal values.)
 struct ColumnArgs {
   const void* grad;
   void* bias;
   int64_t m, ld;
   int n, out_tag;
 };
+constexpr int kColumnWaves = 16, kColumnPart = 1024;
 template <typename T>
-__global__ __launch_bounds__(64) void column_sums_kernel(ColumnArgs a) {
-  const int column = blockIdx.x * 64 + threadIdx.x;
-  if (column >= a.n) return;
-  const T* from = static_cast<const T*>(a.grad) + column;
+__global__ __launch_bounds__(kColumnWaves * kWave) void column_sums_kernel(ColumnArgs a) {
+  __shared__ float room[kColumnWaves][kWave];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, column = blockIdx.x * kWave + lane;
   float sum = 0.f;
+  if (column < a.n) {
+    const T* from = static_cast<const T*>(a.grad) + column;
+    for (int64_t row = wave; row < a.m;) {
+      const int64_t left = (a.m - row + kColumnWaves - 1) / kColumnWaves;
+      const int rows = left < kColumnPart ? (int)left : kColumnPart;
+      float part = 0.f;
 #pragma unroll 8
-  for (int64_t row = 0; row < a.m; ++row) sum += (float)from[row * a.ld];
+      for (int r = 0; r < rows; ++r, row += kColumnWaves) part += (float)from[row * a.ld];
+      sum += part;
+    }
+  }
+  room[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || column >= a.n) return;
+#pragma unroll
+  for (int w = 1; w < kColumnWaves; ++w) sum += room[w][lane];
   store_value(a.bias, a.out_tag, column, sum);
 }
 
@@ -695,7 +710,7 @@ extern "C" int f2cgt_packed_linear_grad(const void* grad, int dtype, int64_t ld,
   if (k == 0) {
     const ColumnArgs a{grad, dbias, m, ld, (int)n, out_dtype};
     return with_type(dtype, [&](auto t) {
-      column_sums_kernel<decltype(t)><<<dim3((unsigned)ceil_div(n, 64)), dim3(64), 0, st>>>(a);
+      column_sums_kernel<decltype(t)><<<dim3((unsigned)ceil_div(n, kWave)), dim3(kColumnWaves * kWave), 0, st>>>(a);
       return launch_status(what);
     });
   }
