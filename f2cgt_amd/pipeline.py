@@ -743,6 +743,8 @@ class MySAGEConv(nn.Module):
             rst = capi.sage_linear(h_self, h_neigh, self.fc_self.weight, self.fc_neigh.weight, self.fc_self.bias, relu)
         if rst is None:
             rst, relu = self.fc_self(h_self) + self.fc_neigh(h_neigh), False
+        elif relu and rst.grad_fn is not None and getattr(self.norm, "packed", False):
+            rst.grad_fn.metadata[_KEEPS_RESULT] = True                # (its backward pass masks by what is positive in it)
         if self.activation is not None and not relu:
             rst = self.activation(rst)
         if self.norm is not None:
@@ -878,6 +880,16 @@ class Int8Linear(nn.Module):
 
 
 # ---- norms, 8-bit checkpoints and learnt rows for training -------------------------------------------
+_KEEPS_RESULT = "f2cgt_keeps_its_result"
+
+
+def _kept_by_its_maker(x):
+    """Whether the operation that made x (or whose result x is a view of) keeps that result for its own backward pass, as a ReLU, a tanh
+    or a softmax does: x itself then costs no memory, and a checkpoint beside it would."""
+    maker = (x if x._base is None else x._base).grad_fn
+    return maker is not None and (hasattr(type(maker), "_saved_result") or _KEEPS_RESULT in maker.metadata)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
@@ -899,8 +911,8 @@ class LayerNorm(nn.LayerNorm):
     """`nn.LayerNorm` over the last dimension of rows on the GPU: one launch forward (and no statistics kept without gradients),
     two backward.  With `packed` the backward pass keeps an 8-bit checkpoint of the input in place of the input itself, a
     fourth of the memory (half for 16-bit inputs): its gradients are those at the decoded input, whose values are off by
-    up to 1/127 of the largest among the 32 columns around them.  Parameters in float32 or in the inputs' type; state as
-    `nn.LayerNorm`'s.  Once differentiable."""
+    up to 1/127 of the largest among the 32 columns around them.  An input that its maker keeps anyway (a ReLU's result) is
+    kept as it is.  Parameters in float32 or in the inputs' type; state as `nn.LayerNorm`'s.  Once differentiable."""
 
     def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True, packed=False, device=None, dtype=None):
         super().__init__(features, eps, elementwise_affine, bias, device=device, dtype=dtype)
@@ -915,7 +927,7 @@ class LayerNorm(nn.LayerNorm):
         if x.shape[-1:] != self.normalized_shape:
             raise ValueError("rows of %s do not fit a norm of %d" % (tuple(x.shape), self.normalized_shape[0]))
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias)):
-            return _LayerNorm.apply(x, self.weight, self.bias, self.eps, self.packed)
+            return _LayerNorm.apply(x, self.weight, self.bias, self.eps, self.packed and not _kept_by_its_maker(x))
         return _capi().layer_norm(x, self.weight, self.bias, self.eps)
 
 
@@ -939,7 +951,8 @@ class _PackedLinear(torch.autograd.Function):
 class PackedLinear(nn.Linear):
     """An `nn.Linear` whose backward pass keeps its input as an 8-bit checkpoint (`pack_activations`): a fourth of the memory
     of float32 inputs, half of 16-bit ones.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the
-    one at the decoded input.  `PackedLinear.of(linear)` shares a layer's parameters.  Once differentiable."""
+    one at the decoded input.  An input that its maker keeps anyway (a ReLU's result) is kept as it is, and the call is
+    `nn.Linear`'s.  `PackedLinear.of(linear)` shares a layer's parameters.  Once differentiable."""
 
     @classmethod
     def of(cls, linear):
@@ -953,7 +966,10 @@ class PackedLinear(nn.Linear):
 
     def forward(self, x):
         if torch.is_grad_enabled() and self.weight.requires_grad:
-            return _PackedLinear.apply(x, self.weight, self.bias)
+            # (autocast's product keeps a copy of its own where it changes the type)
+            copied = torch.is_autocast_enabled("cuda") and x.dtype != torch.get_autocast_dtype("cuda")
+            if copied or not _kept_by_its_maker(x):
+                return _PackedLinear.apply(x, self.weight, self.bias)
         return super().forward(x)
 
 
