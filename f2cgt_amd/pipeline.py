@@ -935,7 +935,9 @@ class _PackedLinear(torch.autograd.Function):
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias):
-        ctx.save_for_backward(weight, *_capi().pack_activations(x))
+        # (the weight for the input's gradient alone: behind given features it may change between the passes)
+        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None, *_capi().pack_activations(x))
+        ctx.dtype = weight.dtype
         return nn.functional.linear(x, weight, bias)
 
     @staticmethod
@@ -945,7 +947,7 @@ class _PackedLinear(torch.autograd.Function):
         weight, codes, exponents = ctx.saved_tensors
         wants = ctx.needs_input_grad
         dx = torch.matmul(grad, weight) if wants[0] else None
-        return (dx, *_capi().packed_linear_grad(grad, codes, exponents, wants[2], weight.dtype))      # (the weight's is always wanted)
+        return (dx, *_capi().packed_linear_grad(grad, codes, exponents, wants[2], ctx.dtype))      # (the weight's is always wanted)
 
 
 class PackedLinear(nn.Linear):
