@@ -696,7 +696,8 @@ class MySAGEConv(nn.Module):
 
     The two products, their sum, the bias and a ReLU are one call (`sage_linear`) where the two layers are plain
     `nn.Linear`s on dense fp32 device tensors and the inputs are not differentiated; the layers' own operators otherwise,
-    also under transforms, modes, autocast and tracing.  The values are the operators' own, and so is the ReLU's mask: a
+    also under transforms, modes, autocast and tracing, and for the step of `PackedLinear`s, which are plain layers without
+    gradients only.  The values are the operators' own, and so is the ReLU's mask: a
     kernel makes them at the sizes at which it adds in the library's order (a minibatch's, up to 128 columns), the
     library's products at all others.  The gradients are one or two launches up to 4096 rows, beyond which the
     pass is the operators'.  A step at 1024 x (128 + 128) -> 256 takes the host 65 us where the operators take 187, the
@@ -739,7 +740,10 @@ class MySAGEConv(nn.Module):
                                                       sm.configs[level][1], sm.configs[level][0], sm.feat_dim)
         relu = self.activation is torch.relu or self.activation is nn.functional.relu
         rst = None
-        if _plain_linear(self.fc_self) and _plain_linear(self.fc_neigh) and self.fc_neigh.bias is None:
+        layers = self.fc_self, self.fc_neigh
+        # (a PackedLinear is an nn.Linear where no gradient asks for its checkpoint)
+        types = (nn.Linear,) if torch.is_grad_enabled() and any(f.weight.requires_grad for f in layers) else (nn.Linear, PackedLinear)
+        if all(_plain_linear(f, types) for f in layers) and self.fc_neigh.bias is None:
             rst = capi.sage_linear(h_self, h_neigh, self.fc_self.weight, self.fc_neigh.weight, self.fc_self.bias, relu)
         if rst is None:
             rst, relu = self.fc_self(h_self) + self.fc_neigh(h_neigh), False
