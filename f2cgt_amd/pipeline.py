@@ -981,15 +981,22 @@ class PackedLinear(nn.Linear):
 
 def packed_layers(module):
     """`module` for training with less memory: every plain `nn.Linear` below it replaced by a `PackedLinear` of the same parameters, in
-    place, and the checkpoints of every `LayerNorm` packed.  What an optimiser holds stays what it trains."""
-    for name, child in list(module.named_children()):
-        if _plain_linear(child):
-            setattr(module, name, PackedLinear.of(child))
-        elif isinstance(child, LayerNorm):
-            child.packed = True
-        else:
-            packed_layers(child)
-    return module
+    place, and the checkpoints of every `LayerNorm` packed.  A layer under several names stays one.  What an optimiser holds
+    stays what it trains.  (A plain `nn.Linear` itself has no place: its `PackedLinear` is returned.)"""
+    return _packed_layers(module, {})
+
+
+def _packed_layers(module, done):
+    if module not in done:
+        done[module] = PackedLinear.of(module) if _plain_linear(module) else module
+        if isinstance(module, LayerNorm):
+            module.packed = True
+        for name, child in list(module._modules.items()):
+            if child is not None:
+                packed = _packed_layers(child, done)
+                if packed is not child:
+                    setattr(module, name, packed)
+    return done[module]
 
 
 class _Embedding(torch.autograd.Function):
