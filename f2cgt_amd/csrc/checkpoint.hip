@@ -6,8 +6,8 @@
 //
 // Pack and unpack are bound by memory: 250 000 x 100 in fp32 31 to 33 us (126 MB, 4 TB/s) and 20.5 (6.1 TB/s), 262 144 x 128 5.8 TB/s
 // either way, in 16 bits 4.8 and 6.1.  The product goes through bf16 matrix instructions: every v is a bf16 exactly, and g is one bf16
-// plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the other, exactly), so all
-// products are exact and only the fp32 sums round.  Large ones are bound by the matrix instructions at the card's power cap (16 384 x
+// plane (bf16), two (fp16: 11 bits in 8 + 8) or three (fp32: 24 bits in 8 + 8 + 8, cut off one after the other, exactly but for bits
+// below 2^-133, bf16's least number), so all products are exact and only the fp32 sums round.  Large ones are bound by the matrix instructions at the card's power cap (16 384 x
 // 4096 -> 4096 in bf16 500 to 550 us, 1.0 to 1.1e15 operations a second, 56 % of the clocks in which the CUs have waves; a library's
 // product of bf16 operands in this layout 558), long sums for few outputs by splitting into planes and placing them (60 001 x 602 ->
 // 128 in fp32 41 us, of which its matrix instructions are 41 %), small ones by a launch and latency (1024 x 128 -> 256 6.8 us).
@@ -271,8 +271,9 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
   typedef typename Tile::Held Held;
 
   // A piece that runs over its row's end reads on in the next one, and four exponents at a time, of which the first counts, in the next
-  // ones: the steps of the last four rows are not among these.  (Of a single exponent's byte the compiler makes a word where the loop
-  // ends, behind a wait.)
+  // ones: the steps of the last four rows are not among these, and with fewer than eight outputs, whose pieces run over more rows, no step
+  // is (250 000 x 128 -> 1 to 7 in fp32 32 us, -> 8 26; in bf16 27 and 19).  (Of a single exponent's byte the compiler makes a word where
+  // the loop ends, behind a wait.)
   const int64_t whole = a.n >= 8 && a.m > 4 ? (a.m - 4) / BM : 0;
   const int64_t rounds = (whole < to ? (whole > from ? whole - from : 0) : to - from) / GROUPS, end = from + rounds * GROUPS;
   // Pieces of one of kParts parts of a step into registers.
@@ -419,7 +420,7 @@ __global__ __launch_bounds__((BN / WN) * (BK / WK) * kWave * GROUPS) void packed
         __syncthreads();
       }
     }
-    for (int64_t at = end; at < to; at += GROUPS) {          // what is left of the steps, a few at most
+    for (int64_t at = end; at < to; at += GROUPS) {          // what is left of the steps: a few, or all with fewer than eight outputs
       const int64_t step = at + group;
       if (step < to) place_last(with_sums, step, stages);
       __syncthreads();
@@ -584,7 +585,7 @@ struct Cut {
 // sums a launch more, 3.5, and 5 MB a us both ways.  What it decides, bf16 and fp32: 1000 x 1000 -> 1000 64 squared 18.5 and 24, 128 squared
 // 22.8 and 25.1; 8192 x 2048 -> 2048 256 squared in four splits 94 and 187, 128 squared 120 and 207; 60 001 x 602 -> 128 128 squared 33.7 and
 // 46.2, 64 squared 35.7 and 56.0; 30 000 x 64 -> 1024 64 squared in 48 or 64 splits 24.3 and 31.6, in 32 26.9 and 33.1, 128 squared 28.9 and
-// 38.9.
+// 38.9.  (Fewer than eight outputs, whose steps are not on their way ahead, are cut by the same times.)
 Cut cut_of(int dtype, int64_t m, int64_t n, int64_t k) {
   static constexpr float kAlone[3][3] = {{0.45f, 0.55f, 0.65f}, {0.43f, 0.62f, 0.78f}, {0.95f, 1.8f, 2.45f}};
   static constexpr float kShared[3] = {0.17f, 0.20f, 0.275f}, kBegin[3] = {2.5f, 7.f, 9.f};

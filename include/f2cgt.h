@@ -451,7 +451,8 @@ int f2cgt_muon_step(void* const* weights, int weight_dtype, const void* const* g
  * with rstd = 1 / sqrt(mean((x - mean)^2) + eps); where mean and rstd (fp32 [m]) are not NULL, those too; where codes and exponents
  * are not NULL, the checkpoint of x that f2cgt_pack_activations writes.
  *
- * f2cgt_layer_norm_grad: of grad [m, d] (grad_ld apart) and what the forward pass kept, x or its checkpoint (the other NULL):
+ * f2cgt_layer_norm_grad: of grad [m, d] (grad_ld apart) and what the forward pass kept, x or its checkpoint (the other NULL), and
+ * x's mean and rstd (those of the decoded rows, which differ a little, are not made):
  * dx [m, d] (dense, no input's buffer), and where not NULL dweight and dbias [d] of grad_dtype.  The sums are made in a fixed order.
  * workspace: f2cgt_layer_norm_grad_workspace_bytes (with neither sum: none), 16-byte aligned, contents irrelevant. */
 int f2cgt_layer_norm(const void* x, int dtype, int64_t ld, const void* weight, const void* bias, int weight_dtype, void* out,
@@ -478,8 +479,9 @@ int f2cgt_layer_norm_grad(const void* grad, int dtype, int64_t grad_ld, const vo
  * readable, here and below.
  *
  * f2cgt_packed_linear_grad: dweight [n, k] = grad^T values and, where not NULL, dbias [n] = sums of grad's columns, dense, of out_dtype;
- * grad [m, n] of dtype, rows ld (below 2^24) apart.  Products are exact (parts of fp32 gradients below 2^-126 count as zeros), sums
- * fp32 in a fixed order.  An infinity in an fp16 or fp32 grad gives NaN in its row of dweight.  workspace: f2cgt_packed_linear_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
+ * grad [m, n] of dtype, rows ld (below 2^24) apart.  Products are exact (bits of fp32 gradients below 2^-133 count as zeros), sums
+ * fp32 in a fixed order.  An infinity in an fp16 or fp32 grad gives NaN in its row of dweight.
+ * workspace: f2cgt_packed_linear_grad_workspace_bytes, 16-byte aligned, contents irrelevant. */
 int f2cgt_pack_activations(const void* x, int dtype, int64_t ld, int8_t* codes, int64_t code_stride, uint8_t* exponents,
                            int64_t m, int64_t k, void* stream);
 int f2cgt_unpack_activations(const int8_t* codes, int64_t code_stride, const uint8_t* exponents, void* out, int dtype, int64_t m,
