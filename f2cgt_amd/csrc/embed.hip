@@ -576,7 +576,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void picked_sums_kernel(SumArgs a)
     raw[u] = -1;
     if (u * kWave < (int)run && i < last) raw[u] = index[i];
   }
-  // (while the ids are on their way; done at the latest before the sums)
+  // (their stores are waited for with the ids, in front of the first key: they hide the ids' way and nothing behind it)
   if (a.sparse) zero_rows<T, V, kPickThreads>(a, row0, count, slice, [](uint32_t) { return true; });
 #pragma unroll
   for (int u = 0; u < kMost; ++u) {
@@ -634,7 +634,8 @@ __global__ __launch_bounds__(kPickThreads, 8) void picked_sums_kernel(SumArgs a)
     if (on && rank == 0) own[r] += (uint16_t)__popcll(same);
     __builtin_amdgcn_wave_barrier();
   }
-  if (a.sparse) __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);      // this wave's zeros are written, before any wave writes sums
+  // This wave's zeros are written, before any wave writes sums: said here, whatever was waited for on the way.
+  if (a.sparse) __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);
   __syncthreads();
   sum_range<T, V, kPickThreads, 1, 8>(a, row0, count, slice, start, sorted, 0, false, lists, reinterpret_cast<float*>(lds));
 }

@@ -4,7 +4,8 @@
 //   u = grad w     dx = rstd (u - sum(u) / d - n sum(u n) / d)     dw = sum over rows of grad n     db = sum over rows of grad
 //
 // Everything is fp32 until the one rounding of a result.  A row of up to 16384 columns stays in registers from its load to its store, so
-// the squares are of differences from the mean (a second pass that costs no memory).  The backward pass takes x or its 8-bit checkpoint.
+// the squares are of differences from the mean (a second pass that costs no memory).  The backward pass takes x or its 8-bit checkpoint;
+// with that, n is (decoded x - mean) rstd with the statistics of x itself, as the forward pass kept them.
 // dw and db: a workgroup adds the rows that it takes in registers, its sums go to memory, and a second kernel adds those of all
 // workgroups; every order is fixed by the sizes.
 //
@@ -281,7 +282,8 @@ __global__ __launch_bounds__(block_of(LANES)) void layer_norm_grad_kernel(NormGr
   __shared__ float room[2][2 * kWaves];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const Columns<V, LANES, C> col(lane, a.d);
-  constexpr bool kAhead = LANES < 1024 || C * V <= 8;                 // (128 registers hold no second row of sixteen values a lane)
+  // (128 registers hold no second row of sixteen values a lane, nor all of one from a checkpoint: 24 of them lie in scratch in fp32, 3 in 16 bits)
+  constexpr bool kAhead = LANES < 1024 || C * V <= 8;
   float w[C][V], dw[C][V], db[C][V];
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -474,7 +476,7 @@ __global__ __launch_bounds__(1024) void join_sums_kernel(JoinArgs a) {
 //   up to 384 and 768 128 x 3 and 256 x 3 forward (32577 x 1030 in fp32 5800 against 4090, 31956 x 2100 in bf16 5020 against 3250), but
 //   not backward, where rows and sums of three pieces leave a CU few waves (22369 x 1500 in fp32 3930 against 4820); workgroups of 384
 //   and 768 lanes lose to both, since a CU holds two or one;
-//   up to 4096 in fp32 1024 x 4 rather than the kernels for long rows: 2048 x 16384 5560 and 4000 against 3290 and 2530 (in 16 bits that
+//   up to 4096 in fp32 1024 x 4 rather than the kernels for long rows: 2048 x 16384 5560 and 4500 against 3290 and 2530 (in 16 bits that
 //   would be 32 values a lane, beyond the registers of the backward pass).
 template <int N> struct count_of { static constexpr int value = N; };
 template <typename T, bool FORWARD, typename F>

@@ -913,10 +913,14 @@ class _LayerNorm(torch.autograd.Function):
 
 class LayerNorm(nn.LayerNorm):
     """`nn.LayerNorm` over the last dimension of rows on the GPU: one launch forward (and no statistics kept without gradients),
-    two backward.  With `packed` the backward pass keeps an 8-bit checkpoint of the input in place of the input itself, a
-    fourth of the memory (half for 16-bit inputs): its gradients are those at the decoded input, whose values are off by
-    up to 1/127 of the largest among the 32 columns around them.  An input that its maker keeps anyway (a ReLU's result) is
-    kept as it is.  Parameters in float32 or in the inputs' type; state as `nn.LayerNorm`'s.  Once differentiable."""
+    two backward.  Parameters in float32 or in the inputs' type, and outputs in the inputs' type, also under autocast (where
+    `nn.LayerNorm` makes float32 of 16 bits); state as `nn.LayerNorm`'s.  Once differentiable.
+
+    With `packed` an 8-bit checkpoint of the input is kept for the backward pass in place of the input itself, 33 bytes for 128 of
+    float32 or 64 of 16 bits: the formula's gradients with the decoded input, whose values are off by up to 1/127 of the largest among
+    the 32 columns around them, and the mean and deviation of the input itself.  An input that its maker keeps anyway (the result of a ReLU, a
+    tanh, a softmax) is kept as it is; one that something else holds (another layer of the same input, a sum around the norm, the
+    program itself) is not known here, and its checkpoint comes on top."""
 
     def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True, packed=False, device=None, dtype=None):
         super().__init__(features, eps, elementwise_affine, bias, device=device, dtype=dtype)
@@ -955,10 +959,15 @@ class _PackedLinear(torch.autograd.Function):
 
 
 class PackedLinear(nn.Linear):
-    """An `nn.Linear` whose backward pass keeps its input as an 8-bit checkpoint (`pack_activations`): a fourth of the memory
-    of float32 inputs, half of 16-bit ones.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the
-    one at the decoded input.  An input that its maker keeps anyway (a ReLU's result) is kept as it is, and the call is
-    `nn.Linear`'s.  `PackedLinear.of(linear)` shares a layer's parameters.  Once differentiable."""
+    """An `nn.Linear` that keeps its input for the backward pass as an 8-bit checkpoint (`pack_activations`): 33 bytes for 128 of
+    float32 or 64 of 16 bits.  The output and the input's gradient are `nn.Linear`'s, the weight's gradient is the one at the
+    decoded input, whose values are off by up to 1/127 of the largest among the 32 columns around them (all 32 are NaN where one is no
+    finite number); an infinity in a float32 or float16 gradient makes NaN of its output's weights, and bits of float32 gradients below 2^-133 are
+    lost.  `PackedLinear.of(linear)` shares a layer's parameters.  Once differentiable.
+
+    An input that its maker keeps anyway (the result of a ReLU, a tanh, a softmax) is kept as it is, and the call is `nn.Linear`'s.  One that
+    something else holds (another layer of the same input, a sum around the layer, the program itself) is not known here, and its
+    checkpoint comes on top: it saves behind a norm, dropout, an aggregation or a GELU."""
 
     @classmethod
     def of(cls, linear):
@@ -982,7 +991,8 @@ class PackedLinear(nn.Linear):
 def packed_layers(module):
     """`module` for training with less memory: every plain `nn.Linear` below it replaced by a `PackedLinear` of the same parameters, in
     place, and the checkpoints of every `LayerNorm` packed.  A layer under several names stays one.  What an optimiser holds
-    stays what it trains.  (A plain `nn.Linear` itself has no place: its `PackedLinear` is returned.)"""
+    stays what it trains.  (A plain `nn.Linear` itself has no place: its `PackedLinear` is returned.)  What is saved is said at the two; a
+    `MySAGEConv` trains packed layers by its operators, and answers by its one call where no gradient asks for a checkpoint."""
     return _packed_layers(module, {})
 
 
