@@ -689,6 +689,12 @@ def _plain_linear(layer, types=(nn.Linear,)):
             not any(getattr(_modules, "_global" + name) for name in _MODULE_HOOKS))
 
 
+def _plain_product(layer):
+    """Whether calling `layer` now is nn.Linear's own product: also a `PackedLinear`'s call that keeps no checkpoint of its input."""
+    return _plain_linear(layer) or (type(layer) is PackedLinear and not (torch.is_grad_enabled() and layer.weight.requires_grad) and
+                                    _plain_linear(layer, (PackedLinear,)))
+
+
 class MySAGEConv(nn.Module):
     """examples/conv.py:9-76.  `forward(csc, feat)`: `csc = (indptr, indices)` of the block
     (destination rows x source rows), `feat = (h_self, h_neigh)`; with a fusing manager `h_neigh`
@@ -740,10 +746,7 @@ class MySAGEConv(nn.Module):
                                                       sm.configs[level][1], sm.configs[level][0], sm.feat_dim)
         relu = self.activation is torch.relu or self.activation is nn.functional.relu
         rst = None
-        layers = self.fc_self, self.fc_neigh
-        # (a PackedLinear is an nn.Linear where no gradient asks for its checkpoint)
-        types = (nn.Linear,) if torch.is_grad_enabled() and any(f.weight.requires_grad for f in layers) else (nn.Linear, PackedLinear)
-        if all(_plain_linear(f, types) for f in layers) and self.fc_neigh.bias is None:
+        if _plain_product(self.fc_self) and _plain_product(self.fc_neigh) and self.fc_neigh.bias is None:
             rst = capi.sage_linear(h_self, h_neigh, self.fc_self.weight, self.fc_neigh.weight, self.fc_self.bias, relu)
         if rst is None:
             rst, relu = self.fc_self(h_self) + self.fc_neigh(h_neigh), False
